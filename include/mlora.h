@@ -391,6 +391,81 @@ int mlora_merge_adapter(void *stream, void *const *w, const int32_t *slots, int3
                         int64_t h_in, int64_t h_out, const mlora_pool *pool_a, const mlora_pool *pool_b,
                         int64_t adapter, int64_t max_rank, float scaling, int32_t sign, mlora_dtype dtype);
 
+/* ---------------------------------------------------------------------------------------------
+ * The attention block of a serving step: rotary positions written into the paged cache, attention of the new tokens
+ * over it, eviction from it.  The cache's rows are pool rows (a token's k or v of all key heads,
+ * valora/common/mem_allocator.py:243-258): page p of size s holds rows p * s .. p * s + s - 1, and request b's token j is
+ * row table[b][j / s] * s + j % s.  With s = 1 a page is a row as the pool's allocator hands it out.
+ * ------------------------------------------------------------------------------------------- */
+#define MLORA_ROTARY_PARTS 3
+enum {
+  MLORA_ROTARY_TURN = 1,      /* the part's heads are rotated (q, k); without it they are copied (v)     */
+  MLORA_ROTARY_TO_ROWS = 2    /* dst is the pool: token t goes to row loc[t]; without it to row t         */
+};
+/* One tensor of the call: [T, heads, head_dim], elements of a head contiguous, strides in elements.  dst may be src
+ * (same strides); other overlaps are not allowed.                                               */
+typedef struct {
+  const void *src;
+  void *dst;
+  int64_t src_token_stride, src_head_stride, dst_token_stride, dst_head_stride;
+  int32_t heads;
+  int32_t flags;
+} mlora_rotary_part;
+
+/* Pair i of a head's first rotary_dim elements -- (2 i, 2 i + 1) if interleaved, else (i, i + rotary_dim / 2) -- is turned
+ * by positions[t] * freqs[i] turns and multiplied by gain; the other elements are copied.  freqs: device double
+ * [rotary_dim / 2].  loc: device int64 [T], pool rows, each at most once; tokens whose row is outside [0, n_rows) are not
+ * written to the pool.                                                                          */
+int mlora_rotary(void *stream, const mlora_rotary_part *parts, int32_t n_parts, const int64_t *positions,
+                 const int64_t *loc, int64_t n_rows, int64_t T, int32_t head_dim, int32_t rotary_dim,
+                 int32_t interleaved, const double *freqs, float gain, mlora_dtype dtype);
+
+/* A batch as the attention calls of its layers see it.  Request b's new tokens are rows b_start_loc[b] .. + b_seq_len[b] - 1
+ * of q and out, and the last b_seq_len[b] of its b_kv_len[b] cached tokens: token i sees the cache indices up to its own,
+ * b_kv_len[b] - b_seq_len[b] + i, and of those the last `window` only where window > 0.  Requests without new tokens, and
+ * those whose rows lie outside [0, n_tokens) or are more than max_seq_len, are left out; a b_kv_len above max_kv_len counts
+ * as max_kv_len, one below 0 as 0.  The caller fills everything but the buffer's contents.       */
+typedef struct {
+  void *dev;                /* mlora_attention_plan_bytes() bytes, 16-byte aligned                     */
+  size_t bytes;
+  int64_t n_req, n_tokens;  /* rows of q                                                               */
+  int64_t max_seq_len;      /* no request has more new tokens, nor                                     */
+  int64_t max_kv_len;       /* more cached ones; the grids, the table and the workspace go by these    */
+  int32_t q_heads, kv_heads;/* q_heads is a multiple of kv_heads: query head h reads key head
+                               h / (q_heads / kv_heads)                                                */
+  int32_t head_dim;         /* 32, 64, 96, 128 or 256                                                  */
+  int32_t page_size;        /* a power of two up to 256                                                */
+  int32_t window;           /* 0: no bound                                                             */
+} mlora_attention_plan;
+size_t mlora_attention_plan_bytes(const mlora_attention_plan *plan);
+/* Bytes of workspace a call needs, 256-byte aligned; calls that share it must not overlap in time.   */
+size_t mlora_attention_workspace_bytes(const mlora_attention_plan *plan, int32_t weights);
+/* Cuts the batch's work on the device, in one launch (b_start_loc, b_seq_len, b_kv_len: device int32 [n_req]).  Once for
+ * the layers of a forward pass; again, in place, when the lengths have changed.                  */
+int mlora_build_attention_plan(void *stream, const mlora_attention_plan *plan, const int32_t *b_start_loc,
+                               const int32_t *b_seq_len, const int32_t *b_kv_len);
+/* out[t][h] = sum over the cached tokens j that t sees of softmax_j(scale * q[t][h] . k_j) v_j.  q, out: [n_tokens][q_heads]
+ * [head_dim], strides in elements between tokens, rows of 16-byte multiples; key_buffer / value_buffer: n_rows pool rows
+ * [kv_heads][head_dim] of the layer; table: device int32 [n_req][table_width] page numbers.  A cached token whose page is not
+ * in the pool is not seen by anyone.  Rows that see nothing become zeros; rows of out that belong to no request keep their
+ * contents.  weights (float [n_req][>= max_kv_len], or null): weights[b][j] += what request b's rows give to cached token j,
+ * over all heads.  out must not overlap an input.                                                */
+int mlora_paged_attention(void *stream, const mlora_attention_plan *plan, void *workspace, size_t workspace_bytes,
+                          void *out, int64_t out_stride, const void *q, int64_t q_stride, const void *key_buffer,
+                          int64_t key_stride, const void *value_buffer, int64_t value_stride, int64_t n_rows,
+                          const int32_t *table, int64_t table_stride, int64_t table_width, float scale, float *weights,
+                          int64_t weights_stride, mlora_dtype dtype);
+
+/* Requests that hold more than `budget` pages keep the first `sinks`, the last `recent` (at least 1) and, of those
+ * between, the ones whose tokens' weights add up to most (ties: the page that comes first; not a number counts
+ * least), in their order.  table: int32 [n_req][width] (table_stride between rows), weights: float [n_req][width * page_size].
+ * All outputs are dense and written whole: new_table [n_req][width] and freed [n_req][width], -1 behind their entries,
+ * new_weights [n_req][width * page_size], 0 behind, new_kv_len [n_req].  Outputs must not overlap inputs.  */
+int mlora_cache_evict(void *stream, const int32_t *table, int64_t table_stride, const int32_t *kv_len,
+                      const float *weights, int64_t weights_stride, int64_t n_req, int64_t width, int32_t page_size,
+                      int64_t budget, int64_t recent, int64_t sinks, int32_t *new_table, int32_t *new_kv_len,
+                      float *new_weights, int32_t *freed);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,151 @@
+"""GPU: eviction by accumulated attention weight against the definition, element for element."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from valora_amd.kv_cache import evict
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(table, lens, weights, budget, recent, sinks, page):
+    table, weights = table.cpu().numpy(), weights.cpu().numpy()
+    n, width = table.shape
+    new_table, freed = np.full_like(table, -1), np.full_like(table, -1)
+    new_w, new_len = np.zeros((n, width * page), dtype=np.float32), []
+    for b, length in enumerate(lens):
+        length = min(max(length, 0), width * page)
+        pages = -(-length // page)
+        stay, go = list(range(pages)), []
+        if pages > budget:
+            mass = weights[b, :pages * page].astype(np.float64).reshape(pages, page).sum(1).astype(np.float32)
+            middle = range(sinks, pages - recent)
+            rank = lambda i: (math.isnan(mass[i]), -mass[i] if not math.isnan(mass[i]) else 0.0, i)  # noqa: E731
+            kept = sorted(middle, key=rank)[:budget - sinks - recent]
+            stay = sorted([*range(sinks), *kept, *range(pages - recent, pages)])
+            go = sorted(set(range(pages)) - set(stay))
+        new_table[b, :len(stay)], freed[b, :len(go)] = table[b, stay], table[b, go]
+        left = length - len(go) * page
+        tokens = (np.array(stay, dtype=np.int64)[:, None] * page + np.arange(page)).reshape(-1)[:left]
+        new_w[b, :left] = weights[b, tokens]
+        new_len.append(left)
+    return new_table, np.array(new_len, dtype=np.int32), new_w, freed
+
+
+def check(dev, table, lens, weights, budget, recent, sinks=0, page=1):
+    kv = torch.tensor(lens, dtype=torch.int32, device=dev)
+    got = evict(table.to(dev), kv, weights.to(dev), budget, recent, sinks, page)
+    torch.cuda.synchronize()
+    for g, w, name in zip(got, reference(table, lens, weights, budget, recent, sinks, page), ("table", "len", "weights", "freed")):
+        assert np.array_equal(g.cpu().numpy(), w, equal_nan=True), name
+    return got
+
+
+def make(lens, page=1, extra=3, seed=0, kind="heavy"):
+    g = torch.Generator().manual_seed(seed)
+    width = max([-(-l // page) for l in lens] + [0]) + extra
+    table = torch.randperm(max(1, len(lens) * width), generator=g)[:len(lens) * width].view(len(lens), width).to(torch.int32)
+    u = torch.rand(len(lens), width * page, generator=g)
+    w = {"heavy": u.pow(8) * 100, "zeros": (u > 0.9).float(), "equal": torch.full_like(u, 0.25), "negative": u - 0.5,
+         "few": torch.randint(0, 4, u.shape, generator=g).float(), "tiny": u * 1e-42, "huge": u * 3e38}[kind]
+    return table, w
+
+
+@pytest.mark.parametrize("kind", ["heavy", "zeros", "equal", "negative", "few", "tiny", "huge"])
+@pytest.mark.parametrize("budget,recent,sinks", [(1, 1, 0), (64, 16, 4), (65, 1, 64), (100, 100, 0), (1000, 1, 0), (7, 3, 4)])
+def test_budgets(dev, kind, budget, recent, sinks):
+    lens = [0, 1, 2, 63, 64, 65, 100, 101, 1000, 1001, 1023, 1024, 1025, 2500, budget, budget + 1]
+    table, w = make(lens, seed=budget, kind=kind)
+    check(dev, table, lens, w, budget, recent, sinks)
+
+
+@pytest.mark.parametrize("page", [2, 16, 64, 256])
+def test_pages_of_several_tokens(dev, page):
+    lens = [1, page - 1, page, page + 1, 5 * page, 9 * page + 1, 12 * page - 1, 30 * page + page // 2]
+    for kind in ("heavy", "few", "zeros"):
+        table, w = make(lens, page, seed=page, kind=kind)
+        check(dev, table, lens, w, 6, 2, 1, page)
+
+
+def test_values_that_are_not_finite(dev):
+    lens = [200, 300]
+    table, w = make(lens, seed=1, kind="few")
+    w[0, 5:60], w[0, 70], w[0, 71], w[0, 72:80] = math.nan, math.inf, -math.inf, -0.0
+    w[1, ::2] = math.nan
+    for budget in (10, 60, 150, 199):
+        check(dev, table, lens, w, budget, 3, 2)
+    table, w = make([160, 160], 16, seed=2)
+    w[0, 40] = math.nan
+    w[1, 17], w[1, 18] = math.inf, -math.inf
+    check(dev, table, [160, 160], w, 4, 1, 1, 16)
+
+
+def test_more_pages_than_stay_in_shared_memory(dev):
+    lens = [36864, 36865, 60000, 5]
+    table, w = make(lens, extra=1, seed=3)
+    check(dev, table, lens, w, 5000, 100, 4)
+    table, w = make([36864 - 7], extra=7, seed=4, kind="zeros")      # the last size that does
+    check(dev, table, [36864 - 7], w, 20000, 64, 4)
+
+
+def test_what_is_behind_a_request_does_not_matter(dev):
+    """Lengths outside the table count as its ends; weights and pages behind a request's last token are not looked at."""
+    table, w = make([50, 50, 50], seed=5)
+    w[:, 40:] = math.nan
+    check(dev, table, [40, 33, 12], w, 16, 4, 1)
+    check(dev, table, [-5, 10**9, -2**31], torch.nan_to_num(w), 16, 4, 1)
+
+
+def test_slices(dev):
+    lens = [90, 20, 70]
+    table, w = make(lens, seed=6)
+    width = table.shape[1]
+    wide_t, wide_w = torch.full((3, width + 50), 7, dtype=torch.int32, device=dev), torch.full((3, width + 31), math.nan, device=dev)
+    wide_t[:, 20:20 + width], wide_w[:, 11:11 + width] = table.to(dev), w.to(dev)
+    got = evict(wide_t[:, 20:20 + width], torch.tensor(lens, dtype=torch.int32, device=dev), wide_w[:, 11:11 + width], 30, 8, 2)
+    torch.cuda.synchronize()
+    for g, want in zip(got, reference(table, lens, w, 30, 8, 2, 1)):
+        assert np.array_equal(g.cpu().numpy(), want)
+
+
+def test_nothing_to_do(dev):
+    for n, width in ((0, 0), (0, 5), (3, 0)):
+        got = evict(torch.empty(n, width, dtype=torch.int32, device=dev), torch.zeros(n, dtype=torch.int32, device=dev),
+                    torch.empty(n, width, device=dev), 4, 1)
+        torch.cuda.synchronize()
+        assert [tuple(g.shape) for g in got] == [(n, width), (n,), (n, width), (n, width)] and not got[1].any()
+
+
+def test_replayed_graph(dev):
+    lens = [300, 90, 64, 10]
+    table, w = make(lens, seed=7)
+    td, wd, kv = table.to(dev), w.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+    evict(td, kv, wd, 64, 8, 2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = evict(td, kv, wd, 64, 8, 2)
+    g = torch.Generator().manual_seed(8)
+    for step in range(3):
+        w = torch.rand(w.shape, generator=g)
+        wd.copy_(w)
+        kv.add_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, reference(table, kv.cpu().tolist(), w, 64, 8, 2, 1)):
+            assert np.array_equal(a.cpu().numpy(), b)
+
+
+def test_refusals(dev):
+    table, w = make([20, 30])
+    t, wd, kv = table.to(dev), w.to(dev), torch.tensor([20, 30], dtype=torch.int32, device=dev)
+    cases = [(lambda: evict(t, kv, wd, 4, 0), "at least 1"), (lambda: evict(t, kv, wd, 4, 3, 2), "budget=4"), (lambda: evict(t, kv, wd, 4, 1, -1), "sinks"),
+             (lambda: evict(t, kv, wd, 4, 1, 0, 3), "shape|power of two|page"), (lambda: evict(t.long(), kv, wd, 4, 1), "Int"),
+             (lambda: evict(t, kv.long(), wd, 4, 1), "Int"), (lambda: evict(t, kv, wd.half(), 4, 1), "Float"), (lambda: evict(t, kv[:1], wd, 4, 1), "b_kv_len"),
+             (lambda: evict(t, kv, wd[:, :5], 4, 1), "weights"), (lambda: evict(t.cpu(), kv, wd, 4, 1), "CUDA"), (lambda: evict(t, kv.cpu(), wd, 4, 1), "CUDA"),
+             (lambda: evict(t.t().contiguous().t(), kv, wd, 4, 1), "contiguous"), (lambda: evict(t, kv, wd, 4, 1, 0, 512), "page_size=512")]
+    for call, message in cases:
+        with pytest.raises(RuntimeError, match=message):
+            call()

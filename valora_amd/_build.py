@@ -16,11 +16,12 @@ from typing import List
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ["api.hip", "tiles.hip", "plan.hip", "shrink.hip", "expand.hip", "decode.hip", "pool.hip", "merge.hip"]
+SOURCES = ["api.hip", "tiles.hip", "plan.hip", "shrink.hip", "expand.hip", "decode.hip", "pool.hip", "merge.hip",
+           "rotary.hip", "attention_plan.hip", "attention.hip", "evict.hip"]
 TABLE_JSON = os.path.join(HERE, "tile_table.json")
 TABLE_INC = os.path.join(CSRC, "tile_table_gen.inc")
 LIB_PATH = os.path.join(HERE, "libmlora.so")
-BINDING_SRC = os.path.join(CSRC, "binding.cpp")
+BINDING_SRCS = [os.path.join(CSRC, s) for s in ("binding.cpp", "binding_attention.cpp")]
 BINDING_PATH = os.path.join(HERE, "_binding.so")
 
 HIPCC_FLAGS = [
@@ -83,7 +84,7 @@ def binding_command() -> List[str]:
     return ([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
              "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_binding",
              f"-D_GLIBCXX_USE_CXX11_ABI={abi}"] +
-            [a for d in inc for a in ("-isystem", d)] + [BINDING_SRC] +
+            [a for d in inc for a in ("-isystem", d)] + BINDING_SRCS +
             [f"-L{d}" for d in libdirs] + [f"-L{HERE}", "-lmlora", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",
                                            "-ltorch_python", "-L/opt/rocm/lib", "-lamdhip64", "-Wl,-rpath,$ORIGIN"] +
             [f"-Wl,-rpath,{d}" for d in libdirs] + ["-Wl,-rpath,/opt/rocm/lib", "-o", BINDING_PATH])

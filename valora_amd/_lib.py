@@ -29,7 +29,8 @@ SYMBOLS = [
     "mlora_pool_alloc", "mlora_pool_alloc_contiguous", "mlora_pool_free", "mlora_pool_fill",
     "mlora_pool_scatter_rows", "mlora_pool_gather_rows", "mlora_index_compact", "mlora_merge_adapter",
     "mlora_build_compensation_plan", "mlora_lora_compensate", "mlora_runs_in_one_launch",
-    "mlora_targets_together",
+    "mlora_targets_together", "mlora_rotary", "mlora_cache_evict", "mlora_attention_plan_bytes",
+    "mlora_attention_workspace_bytes", "mlora_build_attention_plan", "mlora_paged_attention",
 ]
 
 
@@ -49,6 +50,20 @@ MAX_TARGETS = 4
 class Plan(ctypes.Structure):
     _fields_ = [("dev", c_void_p), ("bytes", c_size_t), ("T", c_int64), ("n_adapters", c_int64),
                 ("bm_shrink", c_int32), ("bm_expand", c_int32), ("n_slots", c_int32)]
+
+
+class RotaryPart(ctypes.Structure):
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("src_token_stride", c_int64), ("src_head_stride", c_int64),
+                ("dst_token_stride", c_int64), ("dst_head_stride", c_int64), ("heads", c_int32), ("flags", c_int32)]
+
+
+class AttentionPlan(ctypes.Structure):
+    _fields_ = [("dev", c_void_p), ("bytes", c_size_t), ("n_req", c_int64), ("n_tokens", c_int64), ("max_seq_len", c_int64),
+                ("max_kv_len", c_int64), ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("page_size", c_int32), ("window", c_int32)]
+
+
+ROTARY_PARTS, ROTARY_TURN, ROTARY_TO_ROWS = 3, 1, 2
 
 
 class TileConfig(ctypes.Structure):
@@ -122,8 +137,20 @@ def lib():
                                       c_void_p]
     L.mlora_merge_adapter.argtypes = [c_void_p, POINTER(c_void_p), POINTER(c_int32), c_int32, c_int64, c_int64, c_int64,
                                       POINTER(Pool), POINTER(Pool), c_int64, c_int64, ctypes.c_float, c_int32, c_int]
-    for n in SYMBOLS[6:]:  # everything after the size queries returns a status (the last one a truth value)
+    L.mlora_rotary.argtypes = [c_void_p, POINTER(RotaryPart), c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
+                               c_int32, c_void_p, ctypes.c_float, c_int]
+    L.mlora_cache_evict.argtypes = [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int32,
+                                    c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]
+    L.mlora_attention_plan_bytes.argtypes = [POINTER(AttentionPlan)]
+    L.mlora_attention_workspace_bytes.argtypes = [POINTER(AttentionPlan), c_int32]
+    L.mlora_build_attention_plan.argtypes = [c_void_p, POINTER(AttentionPlan), c_void_p, c_void_p, c_void_p]
+    L.mlora_paged_attention.argtypes = [c_void_p, POINTER(AttentionPlan), c_void_p, c_size_t, c_void_p, c_int64, c_void_p, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                        ctypes.c_float, c_void_p, c_int64, c_int]
+    for n in SYMBOLS[6:]:  # everything after the size queries returns a status (or a truth value)
         getattr(L, n).restype = c_int
+    for n in ("mlora_attention_plan_bytes", "mlora_attention_workspace_bytes"):
+        getattr(L, n).restype = c_size_t
     _lib = L
     return L
 

@@ -1,0 +1,45 @@
+// Layouts and arguments that the attention kernels (attention.hip) and their plan (attention_plan.hip) share.
+#pragma once
+
+#include "mlora_internal.h"
+
+namespace mlora {
+
+// A call's work is cut into tiles of packed rows: row r of a request and key head is (new token r / group, query head
+// r % group of the key head's `group`), so the heads of a group share what is read of the cache.  Requests of up to FEW_ROWS rows
+// (decoding ones) are one tile of the few-rows kernel, the others tiles of TALL_ROWS rows of the tall kernel.  A tile's span of
+// the cache is cut into pieces where there are too few tiles to fill the device; a piece leaves its rows' sums, not yet
+// divided, in a slot of the workspace, and the combining kernel joins them.
+constexpr int FEW_ROWS = 16, TALL_ROWS = 128;
+constexpr int AT_PIECE_STEP = 64;            // a piece's length is a multiple of this
+
+// plan buffer (int32 words): hdr[32] | few[max_few][8] | tall[max_tall][8] | joins[max_joins][8] | requests[n_req + 1][4]
+// record: {request, first row, rows, begin, end, slot (-1: the tile's only piece), first new token in q, position of the
+// request's new token 0}; the piece covers cache indices [begin, end)
+// join:   {first slot, pieces, rows, first row, first new token in q, 1 in the tall list, 0, 0}
+// request: {blocks of WEIGHT_TOKENS cached tokens of the requests before, first new token in q, new tokens, cached tokens};
+// the last one holds the count of all blocks only
+constexpr int AT_HDR = 32, AT_REC = 8, AT_REQ = 4;
+enum AttnHdr { AH_FEW = 0, AH_TALL = 1, AH_JOINS = 2, AH_BLOCKS = 3 };
+constexpr int WEIGHT_TOKENS = 256;
+
+struct AttnLayout {
+  int64_t group;
+  int64_t max_few, max_tall, max_joins;      // records
+  int64_t slots_few, slots_tall;
+  int64_t off_few, off_tall, off_joins, off_requests, words;
+  int few_items, tall_items;                 // (piece, key head) pairs the lists are cut for
+  int few_least, tall_least;                 // a piece is no shorter than this
+};
+
+AttnLayout attention_layout(const mlora_attention_plan &p);
+int check_attention_plan(const mlora_attention_plan *p, const char *who);
+
+// workspace: sums of the slots [slot][key head][rows][head_dim] floats, their references and
+// sums [slot][key head][rows][4], and with weights the logarithm of each row's sum [token][query head]
+struct AttnWorkspace {
+  int64_t few_o, tall_o, few_ml, tall_ml, lse, bytes;
+};
+AttnWorkspace attention_workspace(const mlora_attention_plan &p, const AttnLayout &L, bool weights);
+
+}  // namespace mlora

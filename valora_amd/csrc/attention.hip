@@ -1,0 +1,883 @@
+// Attention of new tokens over the paged cache.
+//
+// A row (new token i, query head h) of a request sees the cache indices j of [max(0, p - window + 1), p], p = kv_len - n + i:
+//
+//     out = sum_j exp(scale q.k_j - m) v_j / sum_j exp(scale q.k_j - m)
+//
+// in one pass over the row's part of the cache, with the running maximum m and the running sum in 32 bits (csrc/attention.h
+// says how the work is cut).  Rows that see nothing, and rows all of whose scores are -infinity, come out as zeros.
+//
+// Both matrix products keep the rows on the columns of the accumulators: S^T = K Q^T and O^T = V^T P^T.  A lane then holds scores
+// of one row only, the running maximum and sum are one register each, and the exponentials are the second product's
+// operand as they stand: its contraction may run over the cached tokens in any order, so it runs in the order in which the first
+// product left them, and V^T is read from LDS to fit (ds_read_b64_tr_b16 hands a lane four tokens of one column).
+// K and V go from memory into LDS without passing through registers, each 16 bytes to a place that keeps the reads free of bank
+// conflicts.  The page numbers of a tile go ahead of it the same way, so the only waits of the loop are the counted ones
+// written in it.
+//
+// The maximum is followed lazily: a row's scores are taken relative to a reference that stays as long as no score of the wave
+// has grown 2^8 times above the maximum it was set by, and neither sums nor accumulators are scaled meanwhile.  In fp16 the
+// reference is that maximum: weights go up to 2^8, and the small ones keep what bits fp16 has for them.  In bf16, whose values may
+// be as large as the accumulators hold, it lies 2^8 above: weights go up to 1.
+#include "attention.h"
+#include "kernel_common.h"
+
+namespace mlora {
+
+namespace {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
+constexpr float GROWTH = 8.0f;         // in powers of two
+
+struct AttnArgs {
+  const int32_t *plan;
+  const int32_t *records;              // of the launch's list
+  uint16_t *out;
+  const uint16_t *q, *k, *v;
+  const int32_t *table;
+  float *part_o;                       // of the launch's list
+  float4 *part_ml;                     // {reference, sum of the rounded weights, sum of the weights, -}
+  float *lse;                          // null: not wanted
+  float *weights;
+  int64_t out_stride, q_stride, table_stride, weights_stride, n_rows;
+  uint32_t k_stride, v_stride;         // bytes
+  float c;                             // scale * log2(e)
+  int count_at, q_heads, kv_heads, group, page_shift, window, n_req, n_pages;
+};
+
+template <typename T>
+struct Wide;
+template <>
+struct Wide<_Float16> {
+  static __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ float add2(uint32_t p, float l) { return __builtin_amdgcn_fdot2(as<f16x2>(p), f16x2{1, 1}, l, false); }
+  static constexpr uint32_t EXPONENT = 0x7c00;
+  static constexpr float AHEAD = 0.0f;         // the reference above the maximum
+};
+template <>
+struct Wide<__bf16> {
+  static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ float add2(uint32_t p, float l) { return __builtin_amdgcn_fdot2_f32_bf16(as<bf16x2>(p), bf16x2{1, 1}, l, false); }
+  static constexpr uint32_t EXPONENT = 0x7f80;
+  static constexpr float AHEAD = GROWTH;
+};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// What is made of x below is made there
+__device__ __forceinline__ void here(uint32_t &x) { asm volatile("" : "+v"(x)); }
+// Bits lo to hi, of the 64 that there are
+__device__ __forceinline__ uint64_t run(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 63);
+  return lo <= hi ? (~0ull >> (63 - hi)) & (~0ull << lo) : 0;
+}
+// All ones where the bit is set.  (Flags kept as such would fill the scalar registers.)
+__device__ __forceinline__ uint32_t bit(uint32_t bits, int at) { return (uint32_t)((int32_t)(bits << (31 - at)) >> 31); }
+// x, or -infinity unless the bit is set
+__device__ __forceinline__ float unless(float x, uint32_t ones) { return as<float>((as<uint32_t>(x) & ones) | (0xff800000u & ~ones)); }
+template <typename T>
+__device__ __forceinline__ uint32_t ones2(uint32_t lo, uint32_t hi) {
+  const uint32_t one = Traits<T>::from_float(1.0f);
+  return (lo & one) | (hi & one << 16);
+}
+// What is written below stays below, loads among it: the steps of the rare paths are not interleaved, which would take registers from
+// the common one
+__device__ __forceinline__ void one_by_one() {
+  requested();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// ---- memory to LDS: lane l's 16 (4) bytes go to base + 16 l (4 l); base is the wave's --------------------------------------
+// (M0 holds the base; nothing else here uses it.  Waits are the caller's: the compiler does not know of these loads.)
+__device__ __forceinline__ void to_lds16(const void *p, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
+}
+__device__ __forceinline__ void to_lds4(const void *p, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(p) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_offset(const void *p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+
+__device__ __forceinline__ u32x4 lds16(uint32_t at) { return *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)at; }
+__device__ __forceinline__ int32_t lds_word(uint32_t at) { return *(const __attribute__((address_space(3))) int32_t *)(uintptr_t)at; }
+__device__ __forceinline__ s16x4 lds_turned(uint32_t at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)at);
+}
+
+// ---- a tile in LDS: rows of D elements, 16-byte pieces of a row exchanged so that what is read together lies in different banks --
+// K is read 16 bytes of 16 or 32 rows at a time, V 32 bytes of 8 rows.
+template <int D>
+struct Tile {
+  static constexpr int P = D / 8, ROW = D * 2;
+  static __device__ __forceinline__ int k_turn(int t) {
+    return D >= 128 ? t & 15 : D == 64 ? (t >> 1) & 7 : D == 32 ? (t >> 2) & 3 : (t >> 2) & 3;
+  }
+  static __device__ __forceinline__ int v_turn(int t) {
+    return D >= 128 ? (t & 7) << 1 : D == 64 ? ((t >> 1) & 3) << 1 : ((t >> 2) & 1) << 1;
+  }
+  // 12 pieces (D = 96) are no power of two: they are rotated, where the others are exchanged
+  static __device__ __forceinline__ int place(int piece, int turn) {
+    if (D != 96) return piece ^ turn;
+    const int s = piece + turn;
+    return s >= P ? s - P : s;
+  }
+  static __device__ __forceinline__ int piece(int place, int turn) {
+    if (D != 96) return place ^ turn;
+    const int s = place - turn;
+    return s < 0 ? s + P : s;
+  }
+  // Address of piece `low + high` of row t of a tile at `base`; `low` is the lane's, `high`, a multiple of a power of two above
+  // it, the instruction's: one exchange of bits behind what a lane keeps for all of its reads.
+  static __device__ __forceinline__ uint32_t at(uint32_t base, int t, int turn, int low, int high) {
+    if (D != 96) return (base + t * ROW + (low ^ turn) * 16) ^ high * 16;
+    return base + t * ROW + place(low + high, turn) * 16;
+  }
+  static __device__ __forceinline__ uint32_t k_at(uint32_t base, int t, int low, int high) { return at(base, t, k_turn(t), low, high); }
+  static __device__ __forceinline__ uint32_t v_at(uint32_t base, int t, int low, int high) { return at(base, t, v_turn(t), low, high); }
+};
+
+// The request's pages and what a piece covers of its cache
+struct Cache {
+  const int32_t *table;
+  const char *k, *v;          // of the key head
+  uint32_t k_stride, v_stride;
+  int begin, end, shift, n_pages;
+};
+
+// page numbers of tokens [base, base + 64), token base + l by lane l
+__device__ __forceinline__ void load_pages(const Cache &c, int base, uint32_t slice, int lane) {
+  const int t = min(base + lane, c.end - 1);
+  to_lds4(c.table + (t >> c.shift), slice);
+}
+
+__device__ __forceinline__ bool bad_page(const Cache &c, int32_t page) { return (uint32_t)page >= (uint32_t)c.n_pages; }
+
+// Pool row of token base + t, whose page number is in the slice; row 0 where the page is none of the pool
+__device__ __forceinline__ uint32_t row_of(const Cache &c, int base, int t, uint32_t slice) {
+  const int32_t page = lds_word(slice + t * 4);
+  const int tok = min(base + t, c.end - 1);
+  return bad_page(c, page) ? 0 : ((uint32_t)page << c.shift) + (tok & ((1 << c.shift) - 1));
+}
+
+// K and V of tokens [base, base + N) into LDS, by WAVES waves together
+template <int D, int N, int WAVES>
+__device__ __forceinline__ void load_tile(const Cache &c, int base, uint32_t slice, uint32_t kt, uint32_t vt, int wave, int lane) {
+  using L = Tile<D>;
+  constexpr int EACH = N * L::P / 64 / WAVES;
+  static_assert(EACH * 64 * WAVES == N * L::P, "whole loads");
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int first = (i * WAVES + wave) * 64, unit = first + lane;
+    const int t = unit / L::P, place = unit - t * L::P;
+    const uint64_t row = row_of(c, base, t, slice);
+    to_lds16(c.k + row * c.k_stride + L::piece(place, L::k_turn(t)) * 16, uniform(kt + first * 16));
+    to_lds16(c.v + row * c.v_stride + L::piece(place, L::v_turn(t)) * 16, uniform(vt + first * 16));
+  }
+}
+
+// ---- running maximum and sum of a lane's row ---------------------------------------------------------------------------------
+template <typename T>
+struct Softmax {
+  float m = -INFINITY;       // reference, in powers of two; -infinity: nothing seen yet
+  float minus = 0.0f;        // -m, or 0
+  float limit = -INFINITY;   // a score this much above m moves it
+  float l = 0.0f;            // sum of the weights as the product takes them
+  float sum = 0.0f;          // and of the weights before they are rounded (where the row's logarithm is wanted)
+
+  // the reference goes by the highest score seen; returns what accumulators are scaled by
+  __device__ __forceinline__ float move(float highest) {
+    const float to = fmaxf(m, highest + Wide<T>::AHEAD);
+    const float alpha = m == -INFINITY ? 0.0f : exp2_(m - to);
+    const bool none = to == -INFINITY;
+    m = to;
+    minus = none ? 0.0f : -to;
+    limit = none ? -INFINITY : GROWTH - Wide<T>::AHEAD;
+    l *= alpha;
+    sum *= alpha;
+    return alpha;
+  }
+};
+
+// Logarithm of a row's sum, in powers of two; -infinity: the row sees nothing
+__device__ __forceinline__ float row_log(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
+
+// ---- V that is not finite -----------------------------------------------------------------------------------------------------
+// A token that a row does not see has weight 0, and 0 times an infinity is not 0.  Where a tile holds tokens that some row does not
+// see and values that are not finite, the product runs over the finite ones alone, and a second one counts for each row and
+// column the others it does see: +infinity as 1, -infinity as 128, not a number as 16384 (at most 64 tokens a sum).
+// Bits 15 and 31 of `finite` stay set while the values are finite: 0x7fff added to what an exponent lacks of all ones carries
+template <typename T>
+__device__ __forceinline__ void check_finite(u32x4 v, uint32_t &finite) {
+  constexpr uint32_t E = Wide<T>::EXPONENT, E2 = E << 16 | E;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) finite &= (~v[i] & E2) + 0x7fff7fffu;
+}
+__device__ __forceinline__ bool all_finite(uint32_t finite) { return !__any((finite & 0x80008000u) != 0x80008000u); }
+template <typename T>
+__device__ __forceinline__ void split_not_finite(u32x4 &v, u32x4 &code) {
+  constexpr uint32_t E = Wide<T>::EXPONENT;
+  const uint32_t one = Traits<T>::from_float(1.0f), low = Traits<T>::from_float(128.0f), odd = Traits<T>::from_float(16384.0f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t fin = 0, cod = 0;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      const uint32_t x = v[i] >> h & 0xffffu;
+      const uint32_t which = x & (0x7fffu ^ E) ? odd : x & 0x8000u ? low : one;
+      fin |= ((x & E) == E ? 0u : x) << h;
+      cod |= ((x & E) == E ? which : 0u) << h;
+    }
+    v[i] = fin;
+    code[i] = cod;
+  }
+}
+__device__ __forceinline__ float not_finite(float code) {
+  const int n = (int)code;
+  const float plus = n & 127 ? INFINITY : 0.0f, minus = n & 16256 ? -INFINITY : 0.0f;
+  return n >> 14 ? NAN : plus + minus;
+}
+
+// ---- few rows: up to 16, every wave on tokens of its own ------------------------------------------------------------------------
+// Decoding: bound by the bytes of K and V.  Each wave streams tiles of 32 tokens through a double buffer of its own, without
+// barriers; at the end the waves' sums are joined through LDS.
+constexpr int FEW_TOKENS = 32;
+template <int D>
+struct Few {
+  static constexpr int WAVES = D <= 128 ? 4 : 2;
+  static constexpr uint32_t TILE = FEW_TOKENS * D * 2, BUFFER = 2 * TILE, SLICES = 4, WAVE = 2 * BUFFER + SLICES * 256;
+  static constexpr int O_STRIDE = D + 4;     // floats of a row of a wave's sums
+  static_assert(WAVES * FEW_ROWS * (O_STRIDE + 4) * 4 <= WAVES * WAVE, "the sums fit where the tiles were");
+};
+
+template <typename T, int D, bool SUMS>
+__global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs a) {
+  using F = Few<D>;
+  using L = Tile<D>;
+  constexpr int WAVES = F::WAVES, CH = D / 32, DB = D / 16;
+  using vec8 = typename Traits<T>::vec8;
+  __shared__ __align__(256) char lds[WAVES * F::WAVE];
+  const int rec_i = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x - (unsigned)rec_i * a.kv_heads);
+  if (rec_i >= a.plan[a.count_at]) return;
+  const int32_t *rec = a.records + (int64_t)rec_i * AT_REC;
+  const int req = rec[0], row0 = rec[1], rows = rec[2], slot = rec[5], tok0 = rec[6], pos0 = rec[7];
+  if (rows <= 0) return;
+  const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
+  const int lrow = lane & 15, kg = lane >> 4;
+  Cache c{a.table + (int64_t)req * a.table_stride, reinterpret_cast<const char *>(a.k) + head * D * 2,
+          reinterpret_cast<const char *>(a.v) + head * D * 2, a.k_stride, a.v_stride, rec[3], rec[4], a.page_shift, a.n_pages};
+  const uint32_t mem = lds_offset(lds) + wave * F::WAVE, slices = mem + 2 * F::BUFFER;
+
+  const int tiles = (c.end - c.begin + FEW_TOKENS - 1) / FEW_TOKENS;
+  const int mine = tiles > wave ? (tiles - wave + WAVES - 1) / WAVES : 0;
+  auto base_of = [&](int k) { return c.begin + (wave + k * WAVES) * FEW_TOKENS; };
+
+  // the lane's row: q, and what it sees
+  const int row = row0 + min(lrow, rows - 1);
+  const int tok = row / a.group, hq = head * a.group + row - tok * a.group;
+  const int last = pos0 + tok, from = a.window > 0 ? last - a.window + 1 : 0;
+  const int sure_from = a.window > 0 ? pos0 + (row0 + rows - 1) / a.group - a.window + 1 : 0, sure_last = pos0 + row0 / a.group;
+  const uint16_t *qp = a.q + (int64_t)(tok0 + tok) * a.q_stride + hq * D;
+  vec8 q[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 32 + kg * 8));
+
+  f32x4 o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
+  Softmax<T> sm;
+
+  auto compute = [&](int k) {
+    const int base = base_of(k);
+    const uint32_t kt = mem + (k & 1) * F::BUFFER, vt = kt + F::TILE;
+    f32x4 s[2];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      s[tt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < CH; ++i) s[tt] = Traits<T>::mfma(as<vec8>(lds16(L::k_at(kt, lrow, kg, i * 4) + tt * 16 * L::ROW)), q[i], s[tt]);
+    }
+    const int32_t page = lds_word(slices + (k & 3) * 256 + (lane & 31) * 4);
+    const uint32_t bad = (uint32_t)__ballot(bad_page(c, page));
+    const bool masked = base < sure_from || base + FEW_TOKENS - 1 > sure_last || base + FEW_TOKENS > c.end || bad;
+    uint32_t seen = 0;                                          // bit tt * 16 + i: the lane's row sees token tt * 16 + kg * 4 + i
+    if (masked) {
+      seen = (uint32_t)(run(from - base, min(last, c.end - 1) - base) & ~(uint64_t)bad) >> kg * 4;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = unless(s[i >> 2][i & 3], bit(seen, (i >> 2) * 16 + (i & 3)));
+    }
+    float hi = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) hi = fmaxf(hi, s[i >> 2][i & 3]);
+    if (__any(fmaf(hi, a.c, sm.minus) > sm.limit)) {
+      hi = fmaxf(hi, __shfl_xor(hi, 16));
+      hi = fmaxf(hi, __shfl_xor(hi, 32));
+      const float alpha = sm.move(hi * a.c);
+#pragma unroll
+      for (int i = 0; i < DB; ++i) o[i] *= alpha;
+    }
+    u32x4 p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // (the sum is that of the rounded weights, which the product takes: a row that looks at one token gets exactly its v)
+      const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
+      const float ex = exp2_(fmaf(x, a.c, sm.minus)), ey = exp2_(fmaf(y, a.c, sm.minus));
+      p[i] = Traits<T>::pack2(ex, ey);
+      sm.l = Wide<T>::add2(p[i], sm.l);
+      if constexpr (SUMS) sm.sum += ex + ey;
+    }
+    const int vtok = kg * 4 + (lrow >> 2);
+    auto values = [&](int db) {
+      const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane & 3) >> 1, 2 * db);
+      struct { s16x4 lo, hi; } v{lds_turned(at), lds_turned(at + 16 * L::ROW)};
+      return as<u32x4>(v);
+    };
+    bool plain = true;
+    if (masked) {
+      uint32_t finite = ~0u;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) check_finite<T>(values(db), finite);
+      plain = all_finite(finite);
+      one_by_one();     // (the values are read again: to keep them would take the registers of the whole tile)
+    }
+    if (plain) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = Traits<T>::mfma(as<vec8>(values(db)), as<vec8>(p), o[db]);
+    } else {
+      u32x4 ones;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ones[i] = ones2<T>(bit(seen, (i >> 1) * 16 + (i & 1) * 2), bit(seen, (i >> 1) * 16 + (i & 1) * 2 + 1));
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        u32x4 v = values(db), code;
+        split_not_finite<T>(v, code);
+        o[db] = Traits<T>::mfma(as<vec8>(v), as<vec8>(p), o[db]);
+        const f32x4 n = Traits<T>::mfma(as<vec8>(code), as<vec8>(ones), f32x4{0, 0, 0, 0});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[db][i] += not_finite(n[i]);
+        one_by_one();
+      }
+    }
+  };
+
+  if (mine > 0) {
+    constexpr int GROUP = 2 * FEW_TOKENS * L::P / 64 + 1;      // loads of one tile: K, V, the page numbers of a later one
+    load_pages(c, base_of(0), slices, lane & 31);
+    load_pages(c, base_of(1), slices + 256, lane & 31);
+    wait_vmcnt<0>();
+    load_tile<D, FEW_TOKENS, 1>(c, base_of(0), slices, mem, mem + F::TILE, 0, lane);
+    load_pages(c, base_of(2), slices + 2 * 256, lane & 31);
+    for (int k = 0; k < mine; ++k) {
+      wait_lgkmcnt0();                                          // the buffer of tile k - 1 has been read
+      if (k + 1 < mine) {
+        const uint32_t kt = mem + ((k + 1) & 1) * F::BUFFER;
+        load_tile<D, FEW_TOKENS, 1>(c, base_of(k + 1), slices + ((k + 1) & 3) * 256, kt, kt + F::TILE, 0, lane);
+        load_pages(c, base_of(k + 3), slices + ((k + 3) & 3) * 256, lane & 31);
+        wait_vmcnt<GROUP>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      compute(k);
+    }
+  }
+
+  // ---- the waves' sums
+  sm.l += __shfl_xor(sm.l, 16);
+  sm.l += __shfl_xor(sm.l, 32);
+  if constexpr (SUMS) {
+    sm.sum += __shfl_xor(sm.sum, 16);
+    sm.sum += __shfl_xor(sm.sum, 32);
+  }
+  float *so = reinterpret_cast<float *>(lds);                   // [wave][row][O_STRIDE]
+  float4 *ml = reinterpret_cast<float4 *>(so + WAVES * FEW_ROWS * F::O_STRIDE);
+  __syncthreads();
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+    *reinterpret_cast<f32x4 *>(so + (wave * FEW_ROWS + lrow) * F::O_STRIDE + db * 16 + kg * 4) = o[db];
+  if (kg == 0) ml[wave * FEW_ROWS + lrow] = float4{sm.m, sm.l, sm.sum, 0.0f};
+  __syncthreads();
+  constexpr int PER_ROW = WAVES * 64 / FEW_ROWS;                // threads of a row, four columns at a time
+  const int r = threadIdx.x / PER_ROW, part = threadIdx.x % PER_ROW;
+  if (r >= rows) return;
+  float m = -INFINITY, l = 0.0f, sum = 0.0f, f[WAVES];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, ml[w * FEW_ROWS + r].x);
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const float4 x = ml[w * FEW_ROWS + r];
+    f[w] = x.x == -INFINITY ? 0.0f : exp2_(x.x - m);
+    l += f[w] * x.y;
+    sum += f[w] * x.z;
+  }
+  const int t = (row0 + r) / a.group, h = head * a.group + row0 + r - t * a.group;
+  const float inv = slot >= 0 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  for (int d = part * 4; d < D; d += PER_ROW * 4) {
+    f32x4 x{0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      if (ml[w * FEW_ROWS + r].x != -INFINITY) x += *reinterpret_cast<const f32x4 *>(so + (w * FEW_ROWS + r) * F::O_STRIDE + d) * f[w];
+    x *= inv;
+    if (slot >= 0) {
+      *reinterpret_cast<f32x4 *>(a.part_o + (((int64_t)slot * a.kv_heads + head) * FEW_ROWS + r) * D + d) = x;
+    } else {
+      uint2 y{Traits<T>::pack2(x[0], x[1]), Traits<T>::pack2(x[2], x[3])};
+      *reinterpret_cast<uint2 *>(a.out + (int64_t)(tok0 + t) * a.out_stride + h * D + d) = y;
+    }
+  }
+  if (part == 0) {
+    if (slot >= 0) a.part_ml[((int64_t)slot * a.kv_heads + head) * FEW_ROWS + r] = float4{m, l, sum, 0.0f};
+    else if (SUMS) a.lse[(int64_t)(tok0 + t) * a.q_heads + h] = row_log(m, sum);
+  }
+}
+
+// ---- tall tiles: 32 rows a wave, K and V shared by the workgroup ------------------------------------------------------------------
+constexpr int TALL_WAVES = TALL_ROWS / 32;
+template <int D>
+struct Tall {
+  static constexpr int TOKENS = D <= 128 ? 64 : 32;          // of a tile (scores and accumulators have to fit the registers)
+  static constexpr uint32_t TILE = TOKENS * D * 2, BUFFER = 2 * TILE, SLICES = 4, TOTAL = 2 * BUFFER + TALL_WAVES * SLICES * 256;
+};
+
+template <typename T, int D, bool SUMS>
+__global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall_kernel(AttnArgs a) {
+  using F = Tall<D>;
+  using L = Tile<D>;
+  constexpr int CH = D / 16, DB = D / 32, TOKENS = F::TOKENS, BL = TOKENS / 32;
+  using vec8 = typename Traits<T>::vec8;
+  __shared__ __align__(256) char lds[F::TOTAL];
+  const int rec_i = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x - (unsigned)rec_i * a.kv_heads);
+  if (rec_i >= a.plan[a.count_at]) return;
+  const int32_t *rec = a.records + (int64_t)rec_i * AT_REC;
+  const int req = rec[0], row0 = rec[1], rows = rec[2], slot = rec[5], tok0 = rec[6], pos0 = rec[7];
+  if (rows <= 0) return;
+  const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
+  const int lrow = lane & 31, half = lane >> 5;
+  Cache c{a.table + (int64_t)req * a.table_stride, reinterpret_cast<const char *>(a.k) + head * D * 2,
+          reinterpret_cast<const char *>(a.v) + head * D * 2, a.k_stride, a.v_stride, rec[3], rec[4], a.page_shift, a.n_pages};
+  const uint32_t mem = lds_offset(lds), slices = mem + 2 * F::BUFFER + wave * F::SLICES * 256;
+  const int tiles = (c.end - c.begin + TOKENS - 1) / TOKENS;
+  auto base_of = [&](int k) { return c.begin + k * TOKENS; };
+
+  const int wrow = wave * 32;                                   // the wave's rows: [wrow, wrow + wrows) of the tile
+  const int wrows = min(32, rows - wrow);
+  const bool works = wrows > 0;
+  const int row = row0 + (works ? wrow + min(lrow, wrows - 1) : 0);
+  const int tok = row / a.group, hq = head * a.group + row - tok * a.group;
+  const int last = pos0 + tok, from = a.window > 0 ? last - a.window + 1 : 0;
+  const int first_tok = (row0 + wrow) / a.group, last_tok = (row0 + wrow + (works ? wrows : 1) - 1) / a.group;
+  const int sure_from = a.window > 0 ? pos0 + last_tok - a.window + 1 : 0, sure_last = pos0 + first_tok;   // all its rows see these,
+  const int any_from = a.window > 0 ? pos0 + first_tok - a.window + 1 : 0, any_last = pos0 + last_tok;     // and some row these
+  const uint16_t *qp = a.q + (int64_t)(tok0 + tok) * a.q_stride + hq * D;
+  vec8 q[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 16 + half * 8));
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+  Softmax<T> sm;
+
+  auto compute = [&](int k) {
+    const int base = base_of(k);
+    const uint32_t kt = mem + (k & 1) * F::BUFFER, vt = kt + F::TILE;
+    f32x16 s[BL];
+#pragma unroll
+    for (int b = 0; b < BL; ++b) {
+      s[b] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < CH; ++i) s[b] = Wide<T>::mfma(as<vec8>(lds16(L::k_at(kt, lrow, half, i * 2) + b * 32 * L::ROW)), q[i], s[b]);
+    }
+    const uint64_t bad = __ballot(bad_page(c, lds_word(slices + (k & 3) * 256 + lane * 4)));   // (lanes behind the tile: of later tokens)
+    const bool masked = base < sure_from || base + TOKENS - 1 > sure_last || base + TOKENS > c.end || bad;
+    uint32_t seen[BL] = {};                                     // bit 8 x + i of b: the lane's row sees token 32 b + 8 x + 4 half + i
+    if (masked) {
+      const uint64_t sees = (run(from - base, min(last, c.end - 1) - base) & ~bad) >> half * 4;
+#pragma unroll
+      for (int b = 0; b < BL; ++b) {
+        seen[b] = (uint32_t)(sees >> 32 * b);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = unless(s[b][i], bit(seen[b], (i >> 2) * 8 + (i & 3)));
+      }
+    }
+    float hi = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 16 * BL; ++i) hi = fmaxf(hi, s[i >> 4][i & 15]);
+    if (__any(fmaf(hi, a.c, sm.minus) > sm.limit)) {
+      hi = fmaxf(hi, __shfl_xor(hi, 32));
+      const float alpha = sm.move(hi * a.c);
+#pragma unroll
+      for (int i = 0; i < DB; ++i) o[i] *= alpha;
+    }
+    u32x4 p[2 * BL];
+#pragma unroll
+    for (int g = 0; g < 2 * BL; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = s[g >> 1][(g & 1) * 8 + 2 * i], y = s[g >> 1][(g & 1) * 8 + 2 * i + 1];
+        const float ex = exp2_(fmaf(x, a.c, sm.minus)), ey = exp2_(fmaf(y, a.c, sm.minus));
+        p[g][i] = Traits<T>::pack2(ex, ey);
+        sm.l = Wide<T>::add2(p[g][i], sm.l);
+        if constexpr (SUMS) sm.sum += ex + ey;
+      }
+    // tokens 16 g + 4 half .. + 3 and 8 further, of the lane's column of 32 from 32 db on
+    const int vtok = half * 4 + ((lane & 15) >> 2);
+    auto values = [&](int g, int db) {
+      const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane >> 4 & 1) * 2 + ((lane & 3) >> 1), 4 * db) + g * 16 * L::ROW;
+      struct { s16x4 lo, hi; } v{lds_turned(at), lds_turned(at + 8 * L::ROW)};
+      return as<u32x4>(v);
+    };
+    bool plain = true;
+    if (masked) {
+      uint32_t finite = ~0u;
+#pragma unroll
+      for (int g = 0; g < 2 * BL; ++g) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) check_finite<T>(values(g, db), finite);
+        one_by_one();     // (the values are read again: to keep them would take the registers of the whole tile)
+      }
+      plain = all_finite(finite);
+    }
+    // (a branch for each 32 columns: over all of them at once the two ways would keep the accumulators twice)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      if (plain) {
+#pragma unroll
+        for (int g = 0; g < 2 * BL; ++g) o[db] = Wide<T>::mfma(as<vec8>(values(g, db)), as<vec8>(p[g]), o[db]);
+      } else {
+        f32x16 n{};
+#pragma unroll
+        for (int g = 0; g < 2 * BL; ++g) {
+          u32x4 ones, v = values(g, db), code;
+          uint32_t sees = seen[g >> 1];
+          here(sees);      // (the flags are made again for each 32 columns: kept, they would take registers from the common way)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = (g & 1) * 16 + (i >> 1) * 8 + (i & 1) * 2;
+            ones[i] = ones2<T>(bit(sees, at), bit(sees, at + 1));
+          }
+          split_not_finite<T>(v, code);
+          o[db] = Wide<T>::mfma(as<vec8>(v), as<vec8>(p[g]), o[db]);
+          n = Wide<T>::mfma(as<vec8>(code), as<vec8>(ones), n);
+          one_by_one();
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] += not_finite(n[i]);
+        one_by_one();
+      }
+    }
+  };
+
+  if (tiles > 0) {
+    load_pages(c, base_of(0), slices, lane);
+    load_pages(c, base_of(1), slices + 256, lane);
+    wait_vmcnt<0>();
+    load_tile<D, TOKENS, TALL_WAVES>(c, base_of(0), slices, mem, mem + F::TILE, wave, lane);
+    load_pages(c, base_of(2), slices + 2 * 256, lane);
+    for (int k = 0; k < tiles; ++k) {
+      // tile k has come, and every wave is through with the other buffer
+      wait_vmcnt<0>();
+      wait_lgkmcnt0();
+      __syncthreads();
+      if (k + 1 < tiles) {
+        const uint32_t kt = mem + ((k + 1) & 1) * F::BUFFER;
+        load_tile<D, TOKENS, TALL_WAVES>(c, base_of(k + 1), slices + ((k + 1) & 3) * 256, kt, kt + F::TILE, wave, lane);
+        load_pages(c, base_of(k + 3), slices + ((k + 3) & 3) * 256, lane);
+      }
+      const int base = base_of(k);
+      if (!works || base > any_last || base + TOKENS <= any_from) continue;
+      compute(k);
+    }
+  }
+
+  if (!works) return;
+  sm.l += __shfl_xor(sm.l, 32);
+  if constexpr (SUMS) sm.sum += __shfl_xor(sm.sum, 32);
+  if (lrow >= wrows) return;
+  if (slot >= 0) {
+    const int64_t at = ((int64_t)slot * a.kv_heads + head) * TALL_ROWS + wrow + lrow;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4 *>(a.part_o + at * D + db * 32 + i * 8 + half * 4) =
+            f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+    if (half == 0) a.part_ml[at] = float4{sm.m, sm.l, sm.sum, 0.0f};
+    return;
+  }
+  const float inv = sm.l == 0.0f ? 0.0f : 1.0f / sm.l;
+  uint16_t *op = a.out + (int64_t)(tok0 + tok) * a.out_stride + hq * D;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint2 y{Traits<T>::pack2(o[db][4 * i] * inv, o[db][4 * i + 1] * inv),
+                    Traits<T>::pack2(o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv)};
+      *reinterpret_cast<uint2 *>(op + db * 32 + i * 8 + half * 4) = y;
+    }
+  if (SUMS && half == 0) a.lse[(int64_t)(tok0 + tok) * a.q_heads + hq] = row_log(sm.m, sm.sum);
+}
+
+// ---- joining the pieces of a tile ---------------------------------------------------------------------------------------------------
+// One workgroup per tile, key head and 16 rows; always in the order of the pieces.
+struct JoinArgs {
+  AttnArgs a;
+  const int32_t *joins;
+  const float *few_o, *tall_o;
+  const float4 *few_ml, *tall_ml;
+};
+constexpr int JOIN_ROWS = 16, JOIN_THREADS = 256, JOIN_PER_ROW = JOIN_THREADS / JOIN_ROWS;
+
+template <typename T, int D>
+__global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(JoinArgs j) {
+  const AttnArgs &a = j.a;
+  const int join_i = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x - (unsigned)join_i * a.kv_heads);
+  if (join_i >= a.plan[AH_JOINS]) return;
+  const int32_t *join = j.joins + (int64_t)join_i * AT_REC;
+  const int slot0 = join[0], pieces = join[1], rows = join[2], row0 = join[3], tok0 = join[4];
+  const bool tall = join[5];
+  const int r = blockIdx.y * JOIN_ROWS + threadIdx.x / JOIN_PER_ROW, part = threadIdx.x % JOIN_PER_ROW;
+  if (pieces <= 0 || r >= rows) return;
+  const int height = tall ? TALL_ROWS : FEW_ROWS;
+  const int64_t step = (int64_t)a.kv_heads * height, at = ((int64_t)slot0 * a.kv_heads + head) * height + r;
+  const float4 *ml = (tall ? j.tall_ml : j.few_ml) + at;
+  const float *po = (tall ? j.tall_o : j.few_o) + at * D;
+  float m = -INFINITY;
+  for (int i = 0; i < pieces; ++i) m = fmaxf(m, ml[i * step].x);
+  constexpr int N = (D + 4 * JOIN_PER_ROW - 1) / (4 * JOIN_PER_ROW);
+  f32x4 x[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = f32x4{0, 0, 0, 0};
+  float l = 0.0f, sum = 0.0f;
+#pragma unroll 2
+  for (int i = 0; i < pieces; ++i) {
+    const float4 p = ml[i * step];
+    const float f = p.x == -INFINITY ? 0.0f : exp2_(p.x - m);
+    l += f * p.y;
+    sum += f * p.z;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int d = (n * JOIN_PER_ROW + part) * 4;
+      if (d < D && p.x != -INFINITY) x[n] += *reinterpret_cast<const f32x4 *>(po + i * step * D + d) * f;
+    }
+  }
+  const int t = (row0 + r) / a.group, h = head * a.group + row0 + r - t * a.group;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int d = (n * JOIN_PER_ROW + part) * 4;
+    if (d >= D) continue;
+    const uint2 y{Traits<T>::pack2(x[n][0] * inv, x[n][1] * inv), Traits<T>::pack2(x[n][2] * inv, x[n][3] * inv)};
+    *reinterpret_cast<uint2 *>(a.out + (int64_t)(tok0 + t) * a.out_stride + h * D + d) = y;
+  }
+  if (a.lse && part == 0) a.lse[(int64_t)(tok0 + t) * a.q_heads + h] = row_log(m, sum);
+}
+
+// ---- weights: how much attention each cached token got ---------------------------------------------------------------------------
+//     weights[b][j] += sum over the call's rows of exp(scale q.k_j - log sum)
+// A wave owns 64 cached tokens and goes over all key heads and rows, so a weight is one thread's sum in a fixed order.  K is
+// read a second time (the sum of a row is not known before its last token).
+constexpr int WEIGHT_WAVES = WEIGHT_TOKENS / 64;
+
+template <typename T, int D>
+__global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(AttnArgs a) {
+  constexpr int CH = D / 32;
+  using vec8 = typename Traits<T>::vec8;
+  __shared__ int found;
+  const int32_t *requests = a.records;
+  const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6), lrow = lane & 15, kg = lane >> 4;
+  const int total = a.plan[AH_BLOCKS];
+  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    // the request whose run of blocks holds the item
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.n_req; b += WEIGHT_WAVES * 64)
+      if (requests[b * AT_REQ] <= item && item < requests[(b + 1) * AT_REQ]) found = b;
+    __syncthreads();
+    const int b = (int)uniform((uint32_t)found);
+    const int32_t *rq = requests + (int64_t)b * AT_REQ;
+    const int tok0 = rq[1], n = rq[2], kv = rq[3], pos0 = kv - n, rows = n * a.group;
+    const int begin = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
+    const int base = begin + (item - rq[0]) * WEIGHT_TOKENS + wave * 64;
+    if (base >= kv) continue;
+    // rows that see any of the tokens
+    const int row_lo = base > pos0 ? (base - pos0) * a.group & ~15 : 0;
+    const int64_t hi = a.window > 0 ? ((int64_t)base + 63 - pos0 + a.window) * a.group : rows;
+    const int row_hi = hi < rows ? (int)hi : rows;
+
+    const int32_t *table = a.table + (int64_t)b * a.table_stride;
+    int64_t at[4];                                              // this lane's token of each 16: pool row
+    uint64_t bad = 0;                                           // tokens whose page is none of the pool
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      const int j = min(base + tt * 16 + lrow, kv - 1);
+      const int32_t page = table[j >> a.page_shift];
+      const bool none = (uint32_t)page >= (uint32_t)a.n_pages;
+      at[tt] = none ? 0 : ((int64_t)page << a.page_shift) + (j & ((1 << a.page_shift) - 1));
+      bad |= (uint64_t)(__ballot(none) & 0xffffu) << tt * 16;
+    }
+    float w[4][4] = {};
+    for (int head = 0; head < a.kv_heads; ++head) {
+      const char *kp = reinterpret_cast<const char *>(a.k) + head * D * 2 + kg * 16;
+      vec8 kf[4][CH];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int i = 0; i < CH; ++i) kf[tt][i] = as<vec8>(*reinterpret_cast<const u32x4 *>(kp + at[tt] * a.k_stride + i * 64));
+      for (int r0 = row_lo; r0 < row_hi; r0 += 16) {
+        const int row = r0 + lrow < rows ? r0 + lrow : rows - 1;
+        const int tok = row / a.group, h = head * a.group + row - tok * a.group;
+        const float lse = r0 + lrow < rows ? a.lse[(int64_t)(tok0 + tok) * a.q_heads + h] : -INFINITY;
+        const uint16_t *qp = a.q + (int64_t)(tok0 + tok) * a.q_stride + h * D + kg * 8;
+        vec8 q[CH];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 32));
+        const int last = pos0 + tok, from = a.window > 0 ? last - a.window + 1 : 0;
+        const uint64_t sees = lse == -INFINITY ? 0 : (run(from - base, last - base) & ~bad) >> kg * 4;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          f32x4 s{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < CH; ++i) s = Traits<T>::mfma(kf[tt][i], q[i], s);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[tt][i] += as<float>(as<uint32_t>(exp2_(fmaf(s[i], a.c, -lse))) & bit((uint32_t)(sees >> (tt >> 1) * 32), (tt & 1) * 16 + i));
+        }
+      }
+    }
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = w[tt][i];
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
+        const int j = base + tt * 16 + kg * 4 + i;
+        if (lrow == 0 && j < kv) a.weights[(int64_t)b * a.weights_stride + j] += x;
+      }
+  }
+}
+
+template <typename T, int D>
+int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, AttnArgs a, char *ws, const AttnWorkspace &w) {
+  const auto *few_o = reinterpret_cast<float *>(ws + w.few_o);
+  const auto *tall_o = reinterpret_cast<float *>(ws + w.tall_o);
+  const auto *few_ml = reinterpret_cast<float4 *>(ws + w.few_ml);
+  const auto *tall_ml = reinterpret_cast<float4 *>(ws + w.tall_ml);
+  const int32_t *plan = a.plan;
+  if (L.max_tall > 0) {
+    a.records = plan + L.off_tall;
+    a.count_at = AH_TALL;
+    a.part_o = const_cast<float *>(tall_o);
+    a.part_ml = const_cast<float4 *>(tall_ml);
+    hipLaunchKernelGGL((a.lse ? attend_tall_kernel<T, D, true> : attend_tall_kernel<T, D, false>), dim3((unsigned)(L.max_tall * a.kv_heads)), dim3(TALL_WAVES * 64), 0, st, a);
+    if (int rc = check_launch("attend_tall_kernel")) return rc;
+  }
+  if (L.max_few > 0) {
+    a.records = plan + L.off_few;
+    a.count_at = AH_FEW;
+    a.part_o = const_cast<float *>(few_o);
+    a.part_ml = const_cast<float4 *>(few_ml);
+    hipLaunchKernelGGL((a.lse ? attend_few_kernel<T, D, true> : attend_few_kernel<T, D, false>), dim3((unsigned)(L.max_few * a.kv_heads)), dim3(Few<D>::WAVES * 64), 0, st, a);
+    if (int rc = check_launch("attend_few_kernel")) return rc;
+  }
+  if (L.max_joins > 0) {
+    const JoinArgs j{a, plan + L.off_joins, few_o, tall_o, few_ml, tall_ml};
+    hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3((unsigned)(L.max_joins * a.kv_heads), L.slots_tall ? TALL_ROWS / JOIN_ROWS : 1),
+                       dim3(JOIN_THREADS), 0, st, j);
+    if (int rc = check_launch("attend_join_kernel")) return rc;
+  }
+  if (a.weights && p.max_kv_len > 0) {
+    a.records = plan + L.off_requests;
+    // as many workgroups as the device holds at once: how many blocks there are it knows
+    const int64_t most = p.n_req * ((p.max_kv_len + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS);
+    hipLaunchKernelGGL((attend_weights_kernel<T, D>), dim3((unsigned)(most < 1024 ? most : 1024)), dim3(WEIGHT_WAVES * 64), 0, st, a);
+    if (int rc = check_launch("attend_weights_kernel")) return rc;
+  }
+  return MLORA_OK;
+}
+
+template <typename T>
+int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, const AttnArgs &a, char *ws, const AttnWorkspace &w) {
+  switch (p.head_dim) {
+    case 32: return launch<T, 32>(st, p, L, a, ws, w);
+    case 64: return launch<T, 64>(st, p, L, a, ws, w);
+    case 96: return launch<T, 96>(st, p, L, a, ws, w);
+    case 128: return launch<T, 128>(st, p, L, a, ws, w);
+    default: return launch<T, 256>(st, p, L, a, ws, w);
+  }
+}
+
+}  // namespace
+
+}  // namespace mlora
+
+using namespace mlora;
+
+extern "C" int mlora_paged_attention(void *stream, const mlora_attention_plan *plan, void *workspace, size_t workspace_bytes,
+                                     void *out, int64_t out_stride, const void *q, int64_t q_stride, const void *key_buffer,
+                                     int64_t key_stride, const void *value_buffer, int64_t value_stride, int64_t n_rows,
+                                     const int32_t *table, int64_t table_stride, int64_t table_width, float scale, float *weights,
+                                     int64_t weights_stride, mlora_dtype dtype) {
+  const char *who = "paged_attention";
+  if (int rc = check_attention_plan(plan, who)) return rc;
+  if (!(scale > 0.0f) || scale > 1e30f) return fail(MLORA_ERR_INVALID, "%s: scale=%g must be positive", who, (double)scale);
+  if (dtype != MLORA_F16 && dtype != MLORA_BF16) return fail(MLORA_ERR_NO_KERNEL, "No suitable kernel. %s: dtype=%d", who, (int)dtype);
+  const AttnLayout L = attention_layout(*plan);
+  if (!plan->dev || plan->bytes < (size_t)L.words * 4) return fail(MLORA_ERR_WORKSPACE, "%s: the plan's buffer is too small", who);
+  const int64_t qw = (int64_t)plan->q_heads * plan->head_dim, kw = (int64_t)plan->kv_heads * plan->head_dim;
+  if (q_stride < qw || out_stride < qw || key_stride < kw || value_stride < kw)
+    return fail(MLORA_ERR_INVALID, "%s: a row of q, out or the pool is shorter than its heads", who);
+  if ((q_stride | out_stride | key_stride | value_stride) & 7 ||
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(key_buffer) |
+        reinterpret_cast<uintptr_t>(value_buffer)) & 15))
+    return fail(MLORA_ERR_INVALID, "%s: rows of q, out and the pool must be multiples of 16 bytes and 16-byte aligned", who);
+  if (key_stride > 0x3fffffff || value_stride > 0x3fffffff) return fail(MLORA_ERR_NO_KERNEL, "%s: pool rows above 2 GB", who);
+  if (n_rows < 0 || n_rows > 0x7fffffff) return fail(MLORA_ERR_NO_KERNEL, "%s: more than 2^31 - 1 pool rows", who);
+  const int64_t pages = (plan->max_kv_len + plan->page_size - 1) / plan->page_size;
+  if (table_width < pages || table_stride < table_width)
+    return fail(MLORA_ERR_INVALID, "%s: a row of the table has %lld pages, max_kv_len=%lld needs %lld", who, (long long)table_width,
+                (long long)plan->max_kv_len, (long long)pages);
+  if (weights && weights_stride < plan->max_kv_len)
+    return fail(MLORA_ERR_INVALID, "%s: a row of the weights is shorter than max_kv_len=%lld", who, (long long)plan->max_kv_len);
+  if (plan->n_req == 0 || plan->n_tokens == 0 || plan->max_seq_len == 0) return MLORA_OK;
+  // a pool without a whole page has no row to stand in for the ones that are not there
+  const int64_t n_pages = n_rows / plan->page_size;
+  if (!out || !q || (plan->max_kv_len > 0 && !table)) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
+  if (!key_buffer || !value_buffer || n_pages == 0) return fail(MLORA_ERR_INVALID, "%s: the pool holds no page", who);
+  const AttnWorkspace w = attention_workspace(*plan, L, weights != nullptr);
+  if (w.bytes > 0 && (!workspace || (int64_t)workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return fail(MLORA_ERR_WORKSPACE, "%s: workspace has %zu bytes (256-byte aligned), needs %lld", who, workspace ? workspace_bytes : 0,
+                (long long)w.bytes);
+  int shift = 0;
+  while ((1 << shift) < plan->page_size) ++shift;
+  AttnArgs a{};
+  a.plan = static_cast<const int32_t *>(plan->dev);
+  a.out = static_cast<uint16_t *>(out);
+  a.q = static_cast<const uint16_t *>(q);
+  a.k = static_cast<const uint16_t *>(key_buffer);
+  a.v = static_cast<const uint16_t *>(value_buffer);
+  a.table = table;
+  a.lse = weights ? reinterpret_cast<float *>(static_cast<char *>(workspace) + w.lse) : nullptr;
+  a.weights = weights;
+  a.out_stride = out_stride;
+  a.q_stride = q_stride;
+  a.table_stride = table_stride;
+  a.weights_stride = weights_stride;
+  a.k_stride = (uint32_t)key_stride * 2;
+  a.v_stride = (uint32_t)value_stride * 2;
+  a.c = scale * 1.44269504088896340736f;
+  a.q_heads = plan->q_heads;
+  a.kv_heads = plan->kv_heads;
+  a.group = (int)L.group;
+  a.page_shift = shift;
+  a.window = plan->window;
+  a.n_req = (int)plan->n_req;
+  a.n_pages = (int)n_pages;
+  char *ws = static_cast<char *>(workspace);
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == MLORA_F16 ? launch<_Float16>(st, *plan, L, a, ws, w) : launch<__bf16>(st, *plan, L, a, ws, w);
+}

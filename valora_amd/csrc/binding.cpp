@@ -32,20 +32,10 @@
 #include <string>
 #include <vector>
 
-#include "mlora.h"
+#include "binding_common.h"
 #include "one_call_tiles.h"
 
-namespace py = pybind11;
-
 namespace {
-
-[[noreturn]] void raise(const std::string &msg) { throw std::runtime_error(msg); }
-
-void check_rc(int rc) {
-  if (rc == MLORA_OK) return;
-  const char *m = mlora_last_error();
-  raise((m && *m) ? std::string(m) : "libmlora call failed with status " + std::to_string(rc));
-}
 
 // ---- the cache ------------------------------------------------------------------------------------
 // Module state without locks: every entry point is called from Python with the GIL held.
@@ -150,14 +140,6 @@ Entry *insert(std::unique_ptr<Entry> e) {
 }
 
 // ---- operand checks shared by the entry points --------------------------------------------------------
-mlora_dtype dtype_code(const at::Tensor &t) {
-  if (t.scalar_type() == at::kHalf) return MLORA_F16;
-  if (t.scalar_type() == at::kBFloat16) return MLORA_BF16;
-  return (mlora_dtype)-1;
-}
-
-std::string dtype_name(const at::Tensor &t) { return std::string("torch.") + c10::toString(t.scalar_type()); }
-
 [[noreturn]] void no_kernel(int64_t h_in, int64_t h_out, const at::Tensor &x) {
   // valora/csrc/lora_ops.cc:122-125
   raise("No suitable kernel. h_in=" + std::to_string(h_in) + " h_out=" + std::to_string(h_out) + " dtype=" +
@@ -503,18 +485,7 @@ void lora_get_qkvo_fwd_expand(const at::Tensor &x, const at::Tensor &w, const at
 // What a LoraPlan holds on the native side: the plan, the index tensors it was cut from and the scratch of its calls.
 // A call checks its operands and goes straight to the C ABI.  Through ctypes a call cost 9-12 us of host time, more than
 // the GPU needs for a small decode batch (7 us); here it is the argument conversion plus the launches.
-// The C calls run without the interpreter lock (a launch waits where the device's queue is full, and other Python threads
-// go on meanwhile), on copies of what another thread's rebuild may replace.
-template <typename F>
-void check_unlocked(F call) {
-  int rc;
-  {
-    py::gil_scoped_release unlocked;
-    rc = call();
-  }
-  check_rc(rc);   // (the message belongs to this thread)
-}
-
+// The C calls run without the interpreter lock, on copies of what another thread's rebuild may replace.
 struct NativePlan {
   mlora_plan plan{};
   at::Tensor buf, scratch, ids, a_start, a_len;
@@ -749,6 +720,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_readonly("buf", &NativePlan::buf)
       .def_readonly("scratch", &NativePlan::scratch)
       .def_readonly("scratch_per_target", &NativePlan::scratch_per_target);
+  bind_attention(m);
   m.def("tile_lookup", &tile_lookup);
   m.def("one_call_tile", &mlora::one_call_tile);
   m.def("cache_lookup", &cache_lookup);

@@ -13,7 +13,8 @@ extends the reference's: three (key, value) buffer pairs that share one row numb
 
 -- so an adapter still owns ``4 * r`` pool rows and every index tensor of the reference keeps its
 meaning.  The base projections, normalisation, rotary embedding and attention are stock PyTorch
-(`torch.mm`, `scaled_dot_product_attention`): they are the caller's side of the boundary; the LoRA
+(`torch.mm`, `scaled_dot_product_attention`), unless the caller's attention is that of the paged cache
+(``valora_amd.kv_cache``), which has its own kernels for rotation, storing and attention; the LoRA
 deltas go through ``LoraPlan``: q, k, v in one multi-target call, gate and up in another, o and
 down in single calls -- four LoRA calls (8 to 12 launches) per layer for seven projections, where the
 reference issues 8 calls (16 launches, each followed by a synchronize) for its four
@@ -84,7 +85,9 @@ def layer_forward(x: torch.Tensor, w: LayerWeights, pools: Optional[LayerPools],
                   attention: Callable[[torch.Tensor, torch.Tensor, torch.Tensor], torch.Tensor], heads: int,
                   cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [T, H]`` -> ``[T, H]``.  ``pools`` / ``plans`` None runs the base model only.  ``attention(q, k, v)``
-    takes and returns ``[T, H]`` matrices (it owns the KV cache and the request boundaries)."""
+    takes and returns ``[T, H]`` matrices (it owns the KV cache and the request boundaries): ``segment_attention`` for whole
+    prompts without a cache, ``valora_amd.kv_cache.KVCache.step(...).attention(layer)`` for new tokens over the paged cache, which
+    rotates q and k itself (``cos`` / ``sin`` None)."""
     lora = pools is not None and plans is not None
     idx = (pools.a_start, pools.a_len, pools.a_loc) if lora else None
     h = rmsnorm(x, w.ln1)
