@@ -19,6 +19,8 @@
 // has grown 2^8 times above the maximum it was set by, and neither sums nor accumulators are scaled meanwhile.  In fp16 the
 // reference is that maximum: weights go up to 2^8, and the small ones keep what bits fp16 has for them.  In bf16, whose values may
 // be as large as the accumulators hold, it lies 2^8 above: weights go up to 1.
+#include <type_traits>
+
 #include "attention.h"
 #include "kernel_common.h"
 
@@ -48,12 +50,15 @@ struct AttnArgs {
   int count_at, q_heads, kv_heads, group, page_shift, window, n_req, n_pages;
 };
 
+// The two 16-bit types as these kernels need them: the wide matrix product, the rounding of two values to one register, the sum of
+// two rounded ones, the bits of the exponent
 template <typename T>
 struct Wide;
 template <>
 struct Wide<_Float16> {
   static __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ float add2(uint32_t p, float l) { return __builtin_amdgcn_fdot2(as<f16x2>(p), f16x2{1, 1}, l, false); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return as<uint32_t>(__builtin_convertvector((f32x2{lo, hi}), f16x2)); }
   static constexpr uint32_t EXPONENT = 0x7c00;
   static constexpr float AHEAD = 0.0f;         // the reference above the maximum
 };
@@ -61,6 +66,7 @@ template <>
 struct Wide<__bf16> {
   static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ float add2(uint32_t p, float l) { return __builtin_amdgcn_fdot2_f32_bf16(as<bf16x2>(p), bf16x2{1, 1}, l, false); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return as<uint32_t>(__builtin_convertvector((f32x2{lo, hi}), bf16x2)); }
   static constexpr uint32_t EXPONENT = 0x7f80;
   static constexpr float AHEAD = GROWTH;
 };
@@ -208,9 +214,11 @@ struct Softmax {
 __device__ __forceinline__ float row_log(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
 
 // ---- V that is not finite -----------------------------------------------------------------------------------------------------
-// A token that a row does not see has weight 0, and 0 times an infinity is not 0.  Where a tile holds tokens that some row does not
-// see and values that are not finite, the product runs over the finite ones alone, and a second one counts for each row and
-// column the others it does see: +infinity as 1, -infinity as 128, not a number as 16384 (at most 64 tokens a sum).
+// A token that a row does not see has weight 0, and 0 times an infinity is not 0.  Tiles that hold tokens some row does not see are
+// therefore looked through, and where one holds a value that is not finite the tile's rows are done again the careful way
+// (a loop of its own, which costs the common one no registers): the product runs over the finite values alone, and a second one
+// counts for each row and column the others that the row does see: +infinity as 1, -infinity as 128, not a number as 16384
+// (at most 64 tokens a sum).
 // Bits 15 and 31 of `finite` stay set while the values are finite: 0x7fff added to what an exponent lacks of all ones carries
 template <typename T>
 __device__ __forceinline__ void check_finite(u32x4 v, uint32_t &finite) {
@@ -289,10 +297,12 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
 
   f32x4 o[DB];
 #pragma unroll
-  for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
+  for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};        // (a wave may have no tile)
   Softmax<T> sm;
 
-  auto compute = [&](int k) {
+  bool odd = false;                                             // a value that is not finite where some row does not see
+  auto compute = [&](auto careful, int k) {
+    constexpr bool CAREFUL = decltype(careful)::value;
     const int base = base_of(k);
     const uint32_t kt = mem + (k & 1) * F::BUFFER, vt = kt + F::TILE;
     f32x4 s[2];
@@ -302,14 +312,25 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
 #pragma unroll
       for (int i = 0; i < CH; ++i) s[tt] = Traits<T>::mfma(as<vec8>(lds16(L::k_at(kt, lrow, kg, i * 4) + tt * 16 * L::ROW)), q[i], s[tt]);
     }
-    const int32_t page = lds_word(slices + (k & 3) * 256 + (lane & 31) * 4);
-    const uint32_t bad = (uint32_t)__ballot(bad_page(c, page));
-    const bool masked = base < sure_from || base + FEW_TOKENS - 1 > sure_last || base + FEW_TOKENS > c.end || bad;
+    const int vtok = kg * 4 + (lrow >> 2);
+    auto values = [&](int db) {
+      const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane & 3) >> 1, 2 * db);
+      struct { s16x4 lo, hi; } v{lds_turned(at), lds_turned(at + 16 * L::ROW)};
+      return as<u32x4>(v);
+    };
+    const uint32_t bad = (uint32_t)__ballot(bad_page(c, lds_word(slices + (k & 3) * 256 + (lane & 31) * 4)));
     uint32_t seen = 0;                                          // bit tt * 16 + i: the lane's row sees token tt * 16 + kg * 4 + i
-    if (masked) {
+    if (CAREFUL || base < sure_from || base + FEW_TOKENS - 1 > sure_last || base + FEW_TOKENS > c.end || bad) {
       seen = (uint32_t)(run(from - base, min(last, c.end - 1) - base) & ~(uint64_t)bad) >> kg * 4;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = unless(s[i >> 2][i & 3], bit(seen, (i >> 2) * 16 + (i & 3)));
+      if constexpr (!CAREFUL) {
+        uint32_t finite = ~0u;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) check_finite<T>(values(db), finite);
+        odd = odd || !all_finite(finite);
+        requested();      // (the values are read again below: to keep them would take registers)
+      }
     }
     float hi = s[0][0];
 #pragma unroll
@@ -327,25 +348,11 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
       // (the sum is that of the rounded weights, which the product takes: a row that looks at one token gets exactly its v)
       const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
       const float ex = exp2_(fmaf(x, a.c, sm.minus)), ey = exp2_(fmaf(y, a.c, sm.minus));
-      p[i] = Traits<T>::pack2(ex, ey);
+      p[i] = Wide<T>::pack(ex, ey);
       sm.l = Wide<T>::add2(p[i], sm.l);
       if constexpr (SUMS) sm.sum += ex + ey;
     }
-    const int vtok = kg * 4 + (lrow >> 2);
-    auto values = [&](int db) {
-      const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane & 3) >> 1, 2 * db);
-      struct { s16x4 lo, hi; } v{lds_turned(at), lds_turned(at + 16 * L::ROW)};
-      return as<u32x4>(v);
-    };
-    bool plain = true;
-    if (masked) {
-      uint32_t finite = ~0u;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) check_finite<T>(values(db), finite);
-      plain = all_finite(finite);
-      one_by_one();     // (the values are read again: to keep them would take the registers of the whole tile)
-    }
-    if (plain) {
+    if constexpr (!CAREFUL) {
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = Traits<T>::mfma(as<vec8>(values(db)), as<vec8>(p), o[db]);
     } else {
@@ -364,9 +371,11 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
       }
     }
   };
-
-  if (mine > 0) {
+  auto sweep = [&](auto careful) {
     constexpr int GROUP = 2 * FEW_TOKENS * L::P / 64 + 1;      // loads of one tile: K, V, the page numbers of a later one
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
+    sm = Softmax<T>();
     load_pages(c, base_of(0), slices, lane & 31);
     load_pages(c, base_of(1), slices + 256, lane & 31);
     wait_vmcnt<0>();
@@ -382,9 +391,12 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
       } else {
         wait_vmcnt<0>();
       }
-      compute(k);
+      compute(careful, k);
     }
-  }
+    wait_lgkmcnt0();
+  };
+  if (mine > 0) sweep(std::false_type{});
+  if (odd) sweep(std::true_type{});
 
   // ---- the waves' sums
   sm.l += __shfl_xor(sm.l, 16);
@@ -425,7 +437,7 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
     if (slot >= 0) {
       *reinterpret_cast<f32x4 *>(a.part_o + (((int64_t)slot * a.kv_heads + head) * FEW_ROWS + r) * D + d) = x;
     } else {
-      uint2 y{Traits<T>::pack2(x[0], x[1]), Traits<T>::pack2(x[2], x[3])};
+      uint2 y{Wide<T>::pack(x[0], x[1]), Wide<T>::pack(x[2], x[3])};
       *reinterpret_cast<uint2 *>(a.out + (int64_t)(tok0 + t) * a.out_stride + h * D + d) = y;
     }
   }
@@ -450,6 +462,7 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
   constexpr int CH = D / 16, DB = D / 32, TOKENS = F::TOKENS, BL = TOKENS / 32;
   using vec8 = typename Traits<T>::vec8;
   __shared__ __align__(256) char lds[F::TOTAL];
+  __shared__ int again;                                         // the tile's rows are done again the careful way
   const int rec_i = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x - (unsigned)rec_i * a.kv_heads);
   if (rec_i >= a.plan[a.count_at]) return;
   const int32_t *rec = a.records + (int64_t)rec_i * AT_REC;
@@ -479,10 +492,12 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
 
   f32x16 o[DB];
 #pragma unroll
-  for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+  for (int i = 0; i < DB; ++i) o[i] = f32x16{};                 // (there may be no tile)
   Softmax<T> sm;
 
-  auto compute = [&](int k) {
+  bool odd = false;                                             // a value that is not finite where some row does not see
+  auto compute = [&](auto careful, int k, uint64_t bad) {
+    constexpr bool CAREFUL = decltype(careful)::value;
     const int base = base_of(k);
     const uint32_t kt = mem + (k & 1) * F::BUFFER, vt = kt + F::TILE;
     f32x16 s[BL];
@@ -492,16 +507,33 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
 #pragma unroll
       for (int i = 0; i < CH; ++i) s[b] = Wide<T>::mfma(as<vec8>(lds16(L::k_at(kt, lrow, half, i * 2) + b * 32 * L::ROW)), q[i], s[b]);
     }
-    const uint64_t bad = __ballot(bad_page(c, lds_word(slices + (k & 3) * 256 + lane * 4)));   // (lanes behind the tile: of later tokens)
-    const bool masked = base < sure_from || base + TOKENS - 1 > sure_last || base + TOKENS > c.end || bad;
+    // tokens 16 g + 4 half .. + 3 and 8 further, of the lane's column of 32 from 32 db on
+    const int vtok = half * 4 + ((lane & 15) >> 2);
+    auto values = [&](int g, int db) {
+      const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane >> 4 & 1) * 2 + ((lane & 3) >> 1), 4 * db) + g * 16 * L::ROW;
+      struct { s16x4 lo, hi; } v{lds_turned(at), lds_turned(at + 8 * L::ROW)};
+      return as<u32x4>(v);
+    };
     uint32_t seen[BL] = {};                                     // bit 8 x + i of b: the lane's row sees token 32 b + 8 x + 4 half + i
-    if (masked) {
+    // (one way for all tiles: two would keep the accumulators twice)
+    if (CAREFUL || base < sure_from || base + TOKENS - 1 > sure_last || base + TOKENS > c.end || bad) {
       const uint64_t sees = (run(from - base, min(last, c.end - 1) - base) & ~bad) >> half * 4;
 #pragma unroll
       for (int b = 0; b < BL; ++b) {
         seen[b] = (uint32_t)(sees >> 32 * b);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[b][i] = unless(s[b][i], bit(seen[b], (i >> 2) * 8 + (i & 3)));
+      }
+      if constexpr (!CAREFUL) {
+        uint32_t finite = ~0u;
+#pragma unroll
+        for (int g = 0; g < 2 * BL; ++g) {
+#pragma unroll
+          for (int db = 0; db < DB; ++db) check_finite<T>(values(g, db), finite);
+          here(finite);
+          one_by_one();   // (the values are read again below: to keep them would take the registers of the whole tile)
+        }
+        odd = odd || !all_finite(finite);
       }
     }
     float hi = s[0][0];
@@ -520,41 +552,24 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
       for (int i = 0; i < 4; ++i) {
         const float x = s[g >> 1][(g & 1) * 8 + 2 * i], y = s[g >> 1][(g & 1) * 8 + 2 * i + 1];
         const float ex = exp2_(fmaf(x, a.c, sm.minus)), ey = exp2_(fmaf(y, a.c, sm.minus));
-        p[g][i] = Traits<T>::pack2(ex, ey);
+        p[g][i] = Wide<T>::pack(ex, ey);
         sm.l = Wide<T>::add2(p[g][i], sm.l);
         if constexpr (SUMS) sm.sum += ex + ey;
       }
-    // tokens 16 g + 4 half .. + 3 and 8 further, of the lane's column of 32 from 32 db on
-    const int vtok = half * 4 + ((lane & 15) >> 2);
-    auto values = [&](int g, int db) {
-      const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane >> 4 & 1) * 2 + ((lane & 3) >> 1), 4 * db) + g * 16 * L::ROW;
-      struct { s16x4 lo, hi; } v{lds_turned(at), lds_turned(at + 8 * L::ROW)};
-      return as<u32x4>(v);
-    };
-    bool plain = true;
-    if (masked) {
-      uint32_t finite = ~0u;
+    if constexpr (!CAREFUL) {
 #pragma unroll
-      for (int g = 0; g < 2 * BL; ++g) {
+      for (int g = 0; g < 2 * BL; ++g)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) check_finite<T>(values(g, db), finite);
-        one_by_one();     // (the values are read again: to keep them would take the registers of the whole tile)
-      }
-      plain = all_finite(finite);
-    }
-    // (a branch for each 32 columns: over all of them at once the two ways would keep the accumulators twice)
+        for (int db = 0; db < DB; ++db) o[db] = Wide<T>::mfma(as<vec8>(values(g, db)), as<vec8>(p[g]), o[db]);
+    } else {
 #pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      if (plain) {
-#pragma unroll
-        for (int g = 0; g < 2 * BL; ++g) o[db] = Wide<T>::mfma(as<vec8>(values(g, db)), as<vec8>(p[g]), o[db]);
-      } else {
+      for (int db = 0; db < DB; ++db) {
         f32x16 n{};
 #pragma unroll
         for (int g = 0; g < 2 * BL; ++g) {
           u32x4 ones, v = values(g, db), code;
           uint32_t sees = seen[g >> 1];
-          here(sees);      // (the flags are made again for each 32 columns: kept, they would take registers from the common way)
+          here(sees);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int at = (g & 1) * 16 + (i >> 1) * 8 + (i & 1) * 2;
@@ -571,8 +586,10 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
       }
     }
   };
-
-  if (tiles > 0) {
+  auto sweep = [&](auto careful) {
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+    sm = Softmax<T>();
     load_pages(c, base_of(0), slices, lane);
     load_pages(c, base_of(1), slices + 256, lane);
     wait_vmcnt<0>();
@@ -590,8 +607,17 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
       }
       const int base = base_of(k);
       if (!works || base > any_last || base + TOKENS <= any_from) continue;
-      compute(k);
+      const uint64_t bad = __ballot(bad_page(c, lds_word(slices + (k & 3) * 256 + lane * 4)));   // (lanes behind the tile: of later tokens)
+      compute(careful, k, bad);
     }
+  };
+  if (tiles > 0) {
+    if (threadIdx.x == 0) again = 0;
+    sweep(std::false_type{});
+    if (odd && lane == 0) again = 1;
+    wait_lgkmcnt0();
+    __syncthreads();                                            // (also: the buffers have been read by everyone)
+    if (again) sweep(std::true_type{});
   }
 
   if (!works) return;
@@ -615,8 +641,8 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint2 y{Traits<T>::pack2(o[db][4 * i] * inv, o[db][4 * i + 1] * inv),
-                    Traits<T>::pack2(o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv)};
+      const uint2 y{Wide<T>::pack(o[db][4 * i] * inv, o[db][4 * i + 1] * inv),
+                    Wide<T>::pack(o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv)};
       *reinterpret_cast<uint2 *>(op + db * 32 + i * 8 + half * 4) = y;
     }
   if (SUMS && half == 0) a.lse[(int64_t)(tok0 + tok) * a.q_heads + hq] = row_log(sm.m, sm.sum);
@@ -671,7 +697,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(JoinArgs j) {
   for (int n = 0; n < N; ++n) {
     const int d = (n * JOIN_PER_ROW + part) * 4;
     if (d >= D) continue;
-    const uint2 y{Traits<T>::pack2(x[n][0] * inv, x[n][1] * inv), Traits<T>::pack2(x[n][2] * inv, x[n][3] * inv)};
+    const uint2 y{Wide<T>::pack(x[n][0] * inv, x[n][1] * inv), Wide<T>::pack(x[n][2] * inv, x[n][3] * inv)};
     *reinterpret_cast<uint2 *>(a.out + (int64_t)(tok0 + t) * a.out_stride + h * D + d) = y;
   }
   if (a.lse && part == 0) a.lse[(int64_t)(tok0 + t) * a.q_heads + h] = row_log(m, sum);
