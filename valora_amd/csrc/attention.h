@@ -9,16 +9,19 @@ namespace mlora {
 // r % group of the key head's `group`), so the heads of a group share what is read of the cache.  Requests of up to FEW_ROWS rows
 // (decoding ones) are one tile of the few-rows kernel, the others tiles of TALL_ROWS rows of the tall kernel.  A tile's span of
 // the cache is cut into pieces where there are too few tiles to fill the device; a piece leaves its rows' sums, not yet
-// divided, in a slot of the workspace, and the combining kernel joins them.
+// divided, in a slot of the workspace; the last piece of a tile of few rows joins them, a launch of its own those of tall tiles.
 constexpr int FEW_ROWS = 16, TALL_ROWS = 128;
 constexpr int AT_PIECE_STEP = 64;            // a piece's length is a multiple of this
 
 // plan buffer (int32 words): hdr[32] | few[max_few][8] | tall[max_tall][8] | joins[max_joins][8] | requests[n_req + 1][4]
+// | arrive[max_joins][kv_heads]
 // record: {request, first row, rows, begin, end, slot (-1: the tile's only piece), first new token in q, position of the
-// request's new token 0}; the piece covers cache indices [begin, end)
+// request's new token 0}; the piece covers cache indices [begin, end); rows of the few-rows list hold the index of the tile's
+// join in the upper half
 // join:   {first slot, pieces, rows, first row, first new token in q, 1 in the tall list, 0, 0}
 // request: {blocks of WEIGHT_TOKENS cached tokens of the requests before, first new token in q, new tokens, cached tokens};
 // the last one holds the count of all blocks only
+// arrive: pieces of a tile that have left their sums, zero between calls
 constexpr int AT_HDR = 32, AT_REC = 8, AT_REQ = 4;
 enum AttnHdr { AH_FEW = 0, AH_TALL = 1, AH_JOINS = 2, AH_BLOCKS = 3 };
 constexpr int WEIGHT_TOKENS = 256;
@@ -27,7 +30,7 @@ struct AttnLayout {
   int64_t group;
   int64_t max_few, max_tall, max_joins;      // records
   int64_t slots_few, slots_tall;
-  int64_t off_few, off_tall, off_joins, off_requests, words;
+  int64_t off_few, off_tall, off_joins, off_requests, off_arrive, words;
   int few_items, tall_items;                 // (piece, key head) pairs the lists are cut for
   int few_least, tall_least;                 // a piece is no shorter than this
 };

@@ -36,18 +36,19 @@ constexpr float GROWTH = 8.0f;         // in powers of two
 
 struct AttnArgs {
   const int32_t *plan;
-  const int32_t *records;              // of the launch's list
   uint16_t *out;
   const uint16_t *q, *k, *v;
   const int32_t *table;
-  float *part_o;                       // of the launch's list
-  float4 *part_ml;                     // {reference, sum of the rounded weights, sum of the weights, -}
+  float *few_o, *tall_o;               // sums of the pieces (csrc/attention.h)
+  float4 *few_ml, *tall_ml;            // {reference, sum of the rounded weights, sum of the weights, -}
   float *lse;                          // null: not wanted
   float *weights;
-  int64_t out_stride, q_stride, table_stride, weights_stride, n_rows;
+  int64_t out_stride, q_stride, table_stride, weights_stride;
+  int64_t off_few, off_tall, off_joins, off_arrive, off_requests;
   uint32_t k_stride, v_stride;         // bytes
   float c;                             // scale * log2(e)
-  int count_at, q_heads, kv_heads, group, page_shift, window, n_req, n_pages;
+  int tall_blocks;                     // workgroups of the tall list; those of the other follow
+  int q_heads, kv_heads, group, page_shift, window, n_req, n_pages;
 };
 
 // The two 16-bit types as these kernels need them: the wide matrix product, the rounding of two values to one register, the sum of
@@ -252,37 +253,69 @@ __device__ __forceinline__ float not_finite(float code) {
 }
 
 // ---- few rows: up to 16, every wave on tokens of its own ------------------------------------------------------------------------
-// Decoding: bound by the bytes of K and V.  Each wave streams tiles of 32 tokens through a double buffer of its own, without
-// barriers; at the end the waves' sums are joined through LDS.
-constexpr int FEW_TOKENS = 32;
+// Decoding: bound by the bytes of K and V.  Each wave streams tiles of 32 tokens through a K and a V buffer of its own, without
+// barriers: K of the next tile is asked for as soon as the scores are there, V as soon as the product is, so one of the two is
+// always on its way.  At the end the waves' sums are joined through LDS.
+constexpr int FEW_TOKENS = 32, THREADS = 256;
 template <int D>
 struct Few {
-  static constexpr int WAVES = D <= 128 ? 4 : 2;
-  static constexpr uint32_t TILE = FEW_TOKENS * D * 2, BUFFER = 2 * TILE, SLICES = 4, WAVE = 2 * BUFFER + SLICES * 256;
-  static constexpr int O_STRIDE = D + 4;     // floats of a row of a wave's sums
-  static_assert(WAVES * FEW_ROWS * (O_STRIDE + 4) * 4 <= WAVES * WAVE, "the sums fit where the tiles were");
+  static constexpr int WAVES = D <= 128 ? 4 : 2;              // that have tokens (the buffers of two fill the room at 256)
+  static constexpr uint32_t TILE = FEW_TOKENS * D * 2, SLICES = 4, WAVE = 2 * TILE + SLICES * 256, TOTAL = WAVES * WAVE;
+  static constexpr int O_STRIDE = D + 4;                      // floats of a row of a wave's sums
+  static_assert(WAVES * FEW_ROWS * (O_STRIDE + 4) * 4 <= TOTAL, "the sums fit where the tiles were");
 };
 
+// Sums of several pieces or waves: {reference, sum of the rounded weights, sum of the weights} and the lane's four columns
+struct Joined {
+  float m = -INFINITY, l = 0.0f, sum = 0.0f;
+  f32x4 x{0, 0, 0, 0};
+
+  __device__ __forceinline__ void add(float4 ml, f32x4 o) {
+    if (ml.x == -INFINITY) return;                            // (saw nothing)
+    const float to = fmaxf(m, ml.x), mine = m == -INFINITY ? 0.0f : exp2_(m - to), its = exp2_(ml.x - to);
+    m = to;
+    l = l * mine + ml.y * its;
+    sum = sum * mine + ml.z * its;
+    x = x * mine + o * its;
+  }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const AttnArgs &a, int tok, int head, int d, const Joined &j) {
+  const float inv = j.l == 0.0f ? 0.0f : 1.0f / j.l;
+  const uint2 y{Wide<T>::pack(j.x[0] * inv, j.x[1] * inv), Wide<T>::pack(j.x[2] * inv, j.x[3] * inv)};
+  *reinterpret_cast<uint2 *>(a.out + (int64_t)tok * a.out_stride + head * D + d) = y;
+  if (a.lse && d == 0) a.lse[(int64_t)tok * a.q_heads + head] = row_log(j.m, j.sum);
+}
+
+// Stores and loads that other XCDs see and that see what they stored: past the L2, which the XCDs do not share
+__device__ __forceinline__ void store_shared(void *p, f32x4 v) {
+  typedef __attribute__((address_space(1))) u32x4 *GP;
+  __builtin_amdgcn_global_store_b128((GP)(uintptr_t)p, as<u32x4>(v), "agent");
+}
+__device__ __forceinline__ f32x4 load_shared(const void *p) {
+  typedef __attribute__((address_space(1))) u32x4 *GP;
+  return as<f32x4>(__builtin_amdgcn_global_load_b128((GP)(uintptr_t)p, "agent"));
+}
+
 template <typename T, int D, bool SUMS>
-__global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs a) {
+__device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i, int head) {
   using F = Few<D>;
   using L = Tile<D>;
   constexpr int WAVES = F::WAVES, CH = D / 32, DB = D / 16;
   using vec8 = typename Traits<T>::vec8;
-  __shared__ __align__(256) char lds[WAVES * F::WAVE];
-  const int rec_i = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x - (unsigned)rec_i * a.kv_heads);
-  if (rec_i >= a.plan[a.count_at]) return;
-  const int32_t *rec = a.records + (int64_t)rec_i * AT_REC;
-  const int req = rec[0], row0 = rec[1], rows = rec[2], slot = rec[5], tok0 = rec[6], pos0 = rec[7];
+  if (rec_i >= a.plan[AH_FEW]) return;
+  const int32_t *rec = a.plan + a.off_few + (int64_t)rec_i * AT_REC;
+  const int req = rec[0], row0 = rec[1], rows = rec[2] & 0xffff, join = rec[2] >> 16, slot = rec[5], tok0 = rec[6], pos0 = rec[7];
   if (rows <= 0) return;
   const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
   const int lrow = lane & 15, kg = lane >> 4;
   Cache c{a.table + (int64_t)req * a.table_stride, reinterpret_cast<const char *>(a.k) + head * D * 2,
           reinterpret_cast<const char *>(a.v) + head * D * 2, a.k_stride, a.v_stride, rec[3], rec[4], a.page_shift, a.n_pages};
-  const uint32_t mem = lds_offset(lds) + wave * F::WAVE, slices = mem + 2 * F::BUFFER;
+  const uint32_t mem = lds_offset(lds) + wave * F::WAVE, kt = mem, vt = mem + F::TILE, slices = mem + 2 * F::TILE;
 
   const int tiles = (c.end - c.begin + FEW_TOKENS - 1) / FEW_TOKENS;
-  const int mine = tiles > wave ? (tiles - wave + WAVES - 1) / WAVES : 0;
+  const int mine = wave < WAVES && tiles > wave ? (tiles - wave + WAVES - 1) / WAVES : 0;
   auto base_of = [&](int k) { return c.begin + (wave + k * WAVES) * FEW_TOKENS; };
 
   // the lane's row: q, and what it sees
@@ -301,10 +334,30 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
   Softmax<T> sm;
 
   bool odd = false;                                             // a value that is not finite where some row does not see
-  auto compute = [&](auto careful, int k) {
+  constexpr int EACH = FEW_TOKENS * L::P / 64;                  // loads of a tile of K, as of V
+  uint32_t rows_of[EACH];                                       // pool rows of the tile whose K was asked for last
+  auto load_k = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int unit = i * 64 + lane, t = unit / L::P, place = unit - t * L::P;
+      rows_of[i] = row_of(c, base_of(k), t, slices + (k & 3) * 256);
+      to_lds16(c.k + (uint64_t)rows_of[i] * c.k_stride + L::piece(place, L::k_turn(t)) * 16, uniform(kt + i * 1024));
+    }
+    load_pages(c, base_of(k + 2), slices + ((k + 2) & 3) * 256, lane & 31);
+  };
+  auto load_v = [&] {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int unit = i * 64 + lane, t = unit / L::P, place = unit - t * L::P;
+      to_lds16(c.v + (uint64_t)rows_of[i] * c.v_stride + L::piece(place, L::v_turn(t)) * 16, uniform(vt + i * 1024));
+    }
+  };
+  auto step = [&](auto careful, int k) {
     constexpr bool CAREFUL = decltype(careful)::value;
+    const bool more = k + 1 < mine;
     const int base = base_of(k);
-    const uint32_t kt = mem + (k & 1) * F::BUFFER, vt = kt + F::TILE;
+    // K has come; V and the page numbers of a later tile are on their way
+    wait_vmcnt<EACH + 1>();
     f32x4 s[2];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
@@ -312,25 +365,15 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
 #pragma unroll
       for (int i = 0; i < CH; ++i) s[tt] = Traits<T>::mfma(as<vec8>(lds16(L::k_at(kt, lrow, kg, i * 4) + tt * 16 * L::ROW)), q[i], s[tt]);
     }
-    const int vtok = kg * 4 + (lrow >> 2);
-    auto values = [&](int db) {
-      const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane & 3) >> 1, 2 * db);
-      struct { s16x4 lo, hi; } v{lds_turned(at), lds_turned(at + 16 * L::ROW)};
-      return as<u32x4>(v);
-    };
     const uint32_t bad = (uint32_t)__ballot(bad_page(c, lds_word(slices + (k & 3) * 256 + (lane & 31) * 4)));
+    wait_lgkmcnt0();
+    if (more) load_k(k + 1);
     uint32_t seen = 0;                                          // bit tt * 16 + i: the lane's row sees token tt * 16 + kg * 4 + i
-    if (CAREFUL || base < sure_from || base + FEW_TOKENS - 1 > sure_last || base + FEW_TOKENS > c.end || bad) {
+    const bool masked = CAREFUL || base < sure_from || base + FEW_TOKENS - 1 > sure_last || base + FEW_TOKENS > c.end || bad;
+    if (masked) {
       seen = (uint32_t)(run(from - base, min(last, c.end - 1) - base) & ~(uint64_t)bad) >> kg * 4;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = unless(s[i >> 2][i & 3], bit(seen, (i >> 2) * 16 + (i & 3)));
-      if constexpr (!CAREFUL) {
-        uint32_t finite = ~0u;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) check_finite<T>(values(db), finite);
-        odd = odd || !all_finite(finite);
-        requested();      // (the values are read again below: to keep them would take registers)
-      }
     }
     float hi = s[0][0];
 #pragma unroll
@@ -352,7 +395,22 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
       sm.l = Wide<T>::add2(p[i], sm.l);
       if constexpr (SUMS) sm.sum += ex + ey;
     }
+    if (more) wait_vmcnt<EACH + 1>();
+    else wait_vmcnt<0>();
+    const int vtok = kg * 4 + (lrow >> 2);
+    auto values = [&](int db) {
+      const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane & 3) >> 1, 2 * db);
+      struct { s16x4 lo, hi; } v{lds_turned(at), lds_turned(at + 16 * L::ROW)};
+      return as<u32x4>(v);
+    };
     if constexpr (!CAREFUL) {
+      if (masked) {
+        uint32_t finite = ~0u;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) check_finite<T>(values(db), finite);
+        odd = odd || !all_finite(finite);
+        requested();      // (the values are read again below: to keep them would take registers)
+      }
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = Traits<T>::mfma(as<vec8>(values(db)), as<vec8>(p), o[db]);
     } else {
@@ -370,30 +428,19 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
         one_by_one();
       }
     }
+    wait_lgkmcnt0();
+    if (more) load_v();
   };
   auto sweep = [&](auto careful) {
-    constexpr int GROUP = 2 * FEW_TOKENS * L::P / 64 + 1;      // loads of one tile: K, V, the page numbers of a later one
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
     sm = Softmax<T>();
     load_pages(c, base_of(0), slices, lane & 31);
     load_pages(c, base_of(1), slices + 256, lane & 31);
     wait_vmcnt<0>();
-    load_tile<D, FEW_TOKENS, 1>(c, base_of(0), slices, mem, mem + F::TILE, 0, lane);
-    load_pages(c, base_of(2), slices + 2 * 256, lane & 31);
-    for (int k = 0; k < mine; ++k) {
-      wait_lgkmcnt0();                                          // the buffer of tile k - 1 has been read
-      if (k + 1 < mine) {
-        const uint32_t kt = mem + ((k + 1) & 1) * F::BUFFER;
-        load_tile<D, FEW_TOKENS, 1>(c, base_of(k + 1), slices + ((k + 1) & 3) * 256, kt, kt + F::TILE, 0, lane);
-        load_pages(c, base_of(k + 3), slices + ((k + 3) & 3) * 256, lane & 31);
-        wait_vmcnt<GROUP>();
-      } else {
-        wait_vmcnt<0>();
-      }
-      compute(careful, k);
-    }
-    wait_lgkmcnt0();
+    load_k(0);
+    load_v();
+    for (int k = 0; k < mine; ++k) step(careful, k);
   };
   if (mine > 0) sweep(std::false_type{});
   if (odd) sweep(std::true_type{});
@@ -408,42 +455,85 @@ __global__ __launch_bounds__(Few<D>::WAVES * 64) void attend_few_kernel(AttnArgs
   float *so = reinterpret_cast<float *>(lds);                   // [wave][row][O_STRIDE]
   float4 *ml = reinterpret_cast<float4 *>(so + WAVES * FEW_ROWS * F::O_STRIDE);
   __syncthreads();
+  if (wave < WAVES) {
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
-    *reinterpret_cast<f32x4 *>(so + (wave * FEW_ROWS + lrow) * F::O_STRIDE + db * 16 + kg * 4) = o[db];
-  if (kg == 0) ml[wave * FEW_ROWS + lrow] = float4{sm.m, sm.l, sm.sum, 0.0f};
+    for (int db = 0; db < DB; ++db)
+      *reinterpret_cast<f32x4 *>(so + (wave * FEW_ROWS + lrow) * F::O_STRIDE + db * 16 + kg * 4) = o[db];
+    if (kg == 0) ml[wave * FEW_ROWS + lrow] = float4{sm.m, sm.l, sm.sum, 0.0f};
+  }
   __syncthreads();
-  constexpr int PER_ROW = WAVES * 64 / FEW_ROWS;                // threads of a row, four columns at a time
-  const int r = threadIdx.x / PER_ROW, part = threadIdx.x % PER_ROW;
-  if (r >= rows) return;
-  float m = -INFINITY, l = 0.0f, sum = 0.0f, f[WAVES];
+  constexpr int COLS = D / 4, SLOTS = THREADS / COLS;           // threads of a row, rows at a time
+  const int ty = threadIdx.x / COLS, d = (threadIdx.x - ty * COLS) * 4;
+  const int64_t step_ml = (int64_t)a.kv_heads * FEW_ROWS;       // rows from a slot to the next
+  if (ty < SLOTS)
+    for (int r = ty; r < rows; r += SLOTS) {
+      Joined j;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, ml[w * FEW_ROWS + r].x);
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const float4 x = ml[w * FEW_ROWS + r];
-    f[w] = x.x == -INFINITY ? 0.0f : exp2_(x.x - m);
-    l += f[w] * x.y;
-    sum += f[w] * x.z;
-  }
-  const int t = (row0 + r) / a.group, h = head * a.group + row0 + r - t * a.group;
-  const float inv = slot >= 0 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-  for (int d = part * 4; d < D; d += PER_ROW * 4) {
-    f32x4 x{0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w)
-      if (ml[w * FEW_ROWS + r].x != -INFINITY) x += *reinterpret_cast<const f32x4 *>(so + (w * FEW_ROWS + r) * F::O_STRIDE + d) * f[w];
-    x *= inv;
-    if (slot >= 0) {
-      *reinterpret_cast<f32x4 *>(a.part_o + (((int64_t)slot * a.kv_heads + head) * FEW_ROWS + r) * D + d) = x;
-    } else {
-      uint2 y{Wide<T>::pack(x[0], x[1]), Wide<T>::pack(x[2], x[3])};
-      *reinterpret_cast<uint2 *>(a.out + (int64_t)(tok0 + t) * a.out_stride + h * D + d) = y;
+      for (int w = 0; w < WAVES; ++w)
+        j.add(ml[w * FEW_ROWS + r], *reinterpret_cast<const f32x4 *>(so + (w * FEW_ROWS + r) * F::O_STRIDE + d));
+      if (slot < 0) {
+        const int t = (row0 + r) / a.group;
+        write_row<T, D>(a, tok0 + t, head * a.group + row0 + r - t * a.group, d, j);
+      } else {
+        const int64_t at = slot * step_ml + head * FEW_ROWS + r;
+        store_shared(a.few_o + at * D + d, j.x);
+        if (d == 0) store_shared(a.few_ml + at, f32x4{j.m, j.l, j.sum, 0.0f});
+      }
     }
+  if (slot < 0) return;
+
+  // ---- the pieces' sums: whoever of a tile's pieces comes last joins them, in their order
+  const int32_t *jn = a.plan + a.off_joins + (int64_t)join * AT_REC;
+  const int slot0 = jn[0], pieces = jn[1];
+  uint32_t *arrive = reinterpret_cast<uint32_t *>(const_cast<int32_t *>(a.plan) + a.off_arrive) + (int64_t)join * a.kv_heads + head;
+  int *flag = reinterpret_cast<int *>(lds);
+  wait_vmcnt<0>();                                              // its sums are where the others see them
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t before = __hip_atomic_fetch_add(arrive, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (before + 1 == (uint32_t)pieces) __hip_atomic_store(arrive, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+    *flag = before + 1 == (uint32_t)pieces;
   }
-  if (part == 0) {
-    if (slot >= 0) a.part_ml[((int64_t)slot * a.kv_heads + head) * FEW_ROWS + r] = float4{m, l, sum, 0.0f};
-    else if (SUMS) a.lse[(int64_t)(tok0 + t) * a.q_heads + h] = row_log(m, sum);
+  __syncthreads();
+  if (!*flag) return;
+  __syncthreads();
+  // Rows times COLS threads go over the pieces; where there are threads for it, several groups take turns, joined through LDS
+  const int groups = rows < SLOTS ? SLOTS / rows : 1;
+  const int grp = rows < SLOTS ? ty / rows : 0;
+  const int64_t first = slot0 * step_ml + head * FEW_ROWS;
+  for (int r = rows < SLOTS ? ty - grp * rows : ty; r < rows; r += SLOTS) {
+    Joined j;
+    if (ty < SLOTS && grp < groups) {
+      constexpr int AHEAD = 4;
+      for (int i = grp; i < pieces; i += AHEAD * groups) {
+        f32x4 x[AHEAD], p[AHEAD];
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+          const int64_t at = first + min(i + n * groups, pieces - 1) * step_ml + r;
+          p[n] = load_shared(a.few_ml + at);
+          x[n] = load_shared(a.few_o + at * D + d);
+        }
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n)
+          if (i + n * groups < pieces) j.add(as<float4>(p[n]), x[n]);
+      }
+    }
+    if (groups > 1) {
+      if (ty < SLOTS && grp < groups) {
+        *reinterpret_cast<f32x4 *>(so + ty * F::O_STRIDE + d) = j.x;
+        if (d == 0) *reinterpret_cast<float4 *>(so + ty * F::O_STRIDE + D) = float4{j.m, j.l, j.sum, 0.0f};
+      }
+      __syncthreads();
+      if (ty >= rows) return;
+      for (int g = 1; g < groups; ++g) {
+        const float *other = so + (g * rows + r) * F::O_STRIDE;
+        j.add(*reinterpret_cast<const float4 *>(other + D), *reinterpret_cast<const f32x4 *>(other + d));
+      }
+    }
+    if (ty < SLOTS && grp == 0) {
+      const int t = (row0 + r) / a.group;
+      write_row<T, D>(a, tok0 + t, head * a.group + row0 + r - t * a.group, d, j);
+    }
   }
 }
 
@@ -456,16 +546,14 @@ struct Tall {
 };
 
 template <typename T, int D, bool SUMS>
-__global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall_kernel(AttnArgs a) {
+__device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_i, int head) {
   using F = Tall<D>;
   using L = Tile<D>;
   constexpr int CH = D / 16, DB = D / 32, TOKENS = F::TOKENS, BL = TOKENS / 32;
   using vec8 = typename Traits<T>::vec8;
-  __shared__ __align__(256) char lds[F::TOTAL];
-  __shared__ int again;                                         // the tile's rows are done again the careful way
-  const int rec_i = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x - (unsigned)rec_i * a.kv_heads);
-  if (rec_i >= a.plan[a.count_at]) return;
-  const int32_t *rec = a.records + (int64_t)rec_i * AT_REC;
+  if (rec_i >= a.plan[AH_TALL]) return;
+  int *again = reinterpret_cast<int *>(lds + F::TOTAL);         // the tile's rows are done again the careful way
+  const int32_t *rec = a.plan + a.off_tall + (int64_t)rec_i * AT_REC;
   const int req = rec[0], row0 = rec[1], rows = rec[2], slot = rec[5], tok0 = rec[6], pos0 = rec[7];
   if (rows <= 0) return;
   const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
@@ -612,12 +700,12 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
     }
   };
   if (tiles > 0) {
-    if (threadIdx.x == 0) again = 0;
+    if (threadIdx.x == 0) *again = 0;
     sweep(std::false_type{});
-    if (odd && lane == 0) again = 1;
+    if (odd && lane == 0) *again = 1;
     wait_lgkmcnt0();
     __syncthreads();                                            // (also: the buffers have been read by everyone)
-    if (again) sweep(std::true_type{});
+    if (*again) sweep(std::true_type{});
   }
 
   if (!works) return;
@@ -630,9 +718,9 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4 *>(a.part_o + at * D + db * 32 + i * 8 + half * 4) =
+        *reinterpret_cast<f32x4 *>(a.tall_o + at * D + db * 32 + i * 8 + half * 4) =
             f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
-    if (half == 0) a.part_ml[at] = float4{sm.m, sm.l, sm.sum, 0.0f};
+    if (half == 0) a.tall_ml[at] = float4{sm.m, sm.l, sm.sum, 0.0f};
     return;
   }
   const float inv = sm.l == 0.0f ? 0.0f : 1.0f / sm.l;
@@ -648,59 +736,67 @@ __global__ __launch_bounds__(TALL_WAVES * 64, D <= 128 ? 2 : 1) void attend_tall
   if (SUMS && half == 0) a.lse[(int64_t)(tok0 + tok) * a.q_heads + hq] = row_log(sm.m, sm.sum);
 }
 
-// ---- joining the pieces of a tile ---------------------------------------------------------------------------------------------------
-// One workgroup per tile, key head and 16 rows; always in the order of the pieces.
-struct JoinArgs {
-  AttnArgs a;
-  const int32_t *joins;
-  const float *few_o, *tall_o;
-  const float4 *few_ml, *tall_ml;
-};
-constexpr int JOIN_ROWS = 16, JOIN_THREADS = 256, JOIN_PER_ROW = JOIN_THREADS / JOIN_ROWS;
+// ---- the launch: tall tiles first, which take longest ---------------------------------------------------------------------------------
+enum { TALL_LIST = 1, FEW_LIST = 2 };
+
+template <typename T, int D, bool SUMS, int LISTS>
+__global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attend_kernel(AttnArgs a) {
+  constexpr uint32_t ROOM = Few<D>::TOTAL > Tall<D>::TOTAL + 16 ? Few<D>::TOTAL : Tall<D>::TOTAL + 16;
+  __shared__ __align__(256) char lds[ROOM];
+  const bool tall = LISTS == TALL_LIST || (LISTS != FEW_LIST && (int)blockIdx.x < a.tall_blocks);
+  const unsigned block = blockIdx.x - (tall ? 0 : a.tall_blocks);
+  // the key heads of a piece follow each other: they read the same pages, and what reads the same head's rows again is eight, or a
+  // multiple of it, further where kv_heads is: on the same XCD
+  const int rec = (int)(block / (unsigned)a.kv_heads), head = (int)(block - (unsigned)rec * a.kv_heads);
+  if (tall) tall_tile<T, D, SUMS>(a, lds, rec, head);
+  else few_tile<T, D, SUMS>(a, lds, rec, head);
+}
+
+template <typename T, int D, bool SUMS>
+int launch_lists(hipStream_t st, const AttnLayout &L, AttnArgs a) {
+  const int64_t few = L.max_few * a.kv_heads, tall = L.max_tall * a.kv_heads;
+  if (few + tall > 0x7fffffff) return fail(MLORA_ERR_NO_KERNEL, "paged_attention: too many tiles");
+  a.tall_blocks = (int)tall;
+  if constexpr (D <= 128) {
+    hipLaunchKernelGGL((attend_kernel<T, D, SUMS, TALL_LIST | FEW_LIST>), dim3((unsigned)(tall + few)), dim3(THREADS), 0, st, a);
+    return check_launch("attend_kernel");
+  } else {      // (both in one kernel do not fit the scalar registers)
+    if (tall > 0) {
+      hipLaunchKernelGGL((attend_kernel<T, D, SUMS, TALL_LIST>), dim3((unsigned)tall), dim3(THREADS), 0, st, a);
+      if (int rc = check_launch("attend_kernel")) return rc;
+    }
+    a.tall_blocks = 0;
+    hipLaunchKernelGGL((attend_kernel<T, D, SUMS, FEW_LIST>), dim3((unsigned)few), dim3(THREADS), 0, st, a);
+    return check_launch("attend_kernel");
+  }
+}
+
+// ---- joining the pieces of tall tiles ---------------------------------------------------------------------------------------------
+// One workgroup per tile, key head and 16 rows; always in the order of the pieces.  (A launch of its own: a tile's pieces are 64 KB
+// each, which one workgroup would be long about.)
+constexpr int JOIN_ROWS = 16;
 
 template <typename T, int D>
-__global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(JoinArgs j) {
-  const AttnArgs &a = j.a;
+__global__ __launch_bounds__(THREADS) void attend_join_kernel(AttnArgs a) {
+  constexpr int COLS = D / 4, SLOTS = THREADS / COLS;
   const int join_i = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x - (unsigned)join_i * a.kv_heads);
   if (join_i >= a.plan[AH_JOINS]) return;
-  const int32_t *join = j.joins + (int64_t)join_i * AT_REC;
+  const int32_t *join = a.plan + a.off_joins + (int64_t)join_i * AT_REC;
   const int slot0 = join[0], pieces = join[1], rows = join[2], row0 = join[3], tok0 = join[4];
-  const bool tall = join[5];
-  const int r = blockIdx.y * JOIN_ROWS + threadIdx.x / JOIN_PER_ROW, part = threadIdx.x % JOIN_PER_ROW;
-  if (pieces <= 0 || r >= rows) return;
-  const int height = tall ? TALL_ROWS : FEW_ROWS;
-  const int64_t step = (int64_t)a.kv_heads * height, at = ((int64_t)slot0 * a.kv_heads + head) * height + r;
-  const float4 *ml = (tall ? j.tall_ml : j.few_ml) + at;
-  const float *po = (tall ? j.tall_o : j.few_o) + at * D;
-  float m = -INFINITY;
-  for (int i = 0; i < pieces; ++i) m = fmaxf(m, ml[i * step].x);
-  constexpr int N = (D + 4 * JOIN_PER_ROW - 1) / (4 * JOIN_PER_ROW);
-  f32x4 x[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) x[n] = f32x4{0, 0, 0, 0};
-  float l = 0.0f, sum = 0.0f;
-#pragma unroll 2
-  for (int i = 0; i < pieces; ++i) {
-    const float4 p = ml[i * step];
-    const float f = p.x == -INFINITY ? 0.0f : exp2_(p.x - m);
-    l += f * p.y;
-    sum += f * p.z;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int d = (n * JOIN_PER_ROW + part) * 4;
-      if (d < D && p.x != -INFINITY) x[n] += *reinterpret_cast<const f32x4 *>(po + i * step * D + d) * f;
-    }
+  if (!join[5] || pieces <= 0) return;
+  const int ty = threadIdx.x / COLS, d = (threadIdx.x - ty * COLS) * 4;
+  if (ty >= SLOTS) return;
+  const int64_t step = (int64_t)a.kv_heads * TALL_ROWS;
+  const int end = min((int)(blockIdx.y + 1) * JOIN_ROWS, rows);
+  for (int r = blockIdx.y * JOIN_ROWS + ty; r < end; r += SLOTS) {
+    const int64_t at = slot0 * step + head * TALL_ROWS + r;
+    Joined j;
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i)
+      j.add(a.tall_ml[at + i * step], *reinterpret_cast<const f32x4 *>(a.tall_o + (at + i * step) * D + d));
+    const int t = (row0 + r) / a.group;
+    write_row<T, D>(a, tok0 + t, head * a.group + row0 + r - t * a.group, d, j);
   }
-  const int t = (row0 + r) / a.group, h = head * a.group + row0 + r - t * a.group;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int d = (n * JOIN_PER_ROW + part) * 4;
-    if (d >= D) continue;
-    const uint2 y{Wide<T>::pack(x[n][0] * inv, x[n][1] * inv), Wide<T>::pack(x[n][2] * inv, x[n][3] * inv)};
-    *reinterpret_cast<uint2 *>(a.out + (int64_t)(tok0 + t) * a.out_stride + h * D + d) = y;
-  }
-  if (a.lse && part == 0) a.lse[(int64_t)(tok0 + t) * a.q_heads + h] = row_log(m, sum);
 }
 
 // ---- weights: how much attention each cached token got ---------------------------------------------------------------------------
@@ -714,7 +810,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
   constexpr int CH = D / 32;
   using vec8 = typename Traits<T>::vec8;
   __shared__ int found;
-  const int32_t *requests = a.records;
+  const int32_t *requests = a.plan + a.off_requests;
   const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6), lrow = lane & 15, kg = lane >> 4;
   const int total = a.plan[AH_BLOCKS];
   for (int item = blockIdx.x; item < total; item += gridDim.x) {
@@ -788,36 +884,13 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
 }
 
 template <typename T, int D>
-int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, AttnArgs a, char *ws, const AttnWorkspace &w) {
-  const auto *few_o = reinterpret_cast<float *>(ws + w.few_o);
-  const auto *tall_o = reinterpret_cast<float *>(ws + w.tall_o);
-  const auto *few_ml = reinterpret_cast<float4 *>(ws + w.few_ml);
-  const auto *tall_ml = reinterpret_cast<float4 *>(ws + w.tall_ml);
-  const int32_t *plan = a.plan;
-  if (L.max_tall > 0) {
-    a.records = plan + L.off_tall;
-    a.count_at = AH_TALL;
-    a.part_o = const_cast<float *>(tall_o);
-    a.part_ml = const_cast<float4 *>(tall_ml);
-    hipLaunchKernelGGL((a.lse ? attend_tall_kernel<T, D, true> : attend_tall_kernel<T, D, false>), dim3((unsigned)(L.max_tall * a.kv_heads)), dim3(TALL_WAVES * 64), 0, st, a);
-    if (int rc = check_launch("attend_tall_kernel")) return rc;
-  }
-  if (L.max_few > 0) {
-    a.records = plan + L.off_few;
-    a.count_at = AH_FEW;
-    a.part_o = const_cast<float *>(few_o);
-    a.part_ml = const_cast<float4 *>(few_ml);
-    hipLaunchKernelGGL((a.lse ? attend_few_kernel<T, D, true> : attend_few_kernel<T, D, false>), dim3((unsigned)(L.max_few * a.kv_heads)), dim3(Few<D>::WAVES * 64), 0, st, a);
-    if (int rc = check_launch("attend_few_kernel")) return rc;
-  }
-  if (L.max_joins > 0) {
-    const JoinArgs j{a, plan + L.off_joins, few_o, tall_o, few_ml, tall_ml};
-    hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3((unsigned)(L.max_joins * a.kv_heads), L.slots_tall ? TALL_ROWS / JOIN_ROWS : 1),
-                       dim3(JOIN_THREADS), 0, st, j);
+int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, const AttnArgs &a) {
+  if (int rc = a.lse ? launch_lists<T, D, true>(st, L, a) : launch_lists<T, D, false>(st, L, a)) return rc;
+  if (L.slots_tall > 0) {
+    hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3((unsigned)(L.max_joins * a.kv_heads), TALL_ROWS / JOIN_ROWS), dim3(THREADS), 0, st, a);
     if (int rc = check_launch("attend_join_kernel")) return rc;
   }
   if (a.weights && p.max_kv_len > 0) {
-    a.records = plan + L.off_requests;
     // as many workgroups as the device holds at once: how many blocks there are it knows
     const int64_t most = p.n_req * ((p.max_kv_len + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS);
     hipLaunchKernelGGL((attend_weights_kernel<T, D>), dim3((unsigned)(most < 1024 ? most : 1024)), dim3(WEIGHT_WAVES * 64), 0, st, a);
@@ -827,13 +900,13 @@ int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, A
 }
 
 template <typename T>
-int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, const AttnArgs &a, char *ws, const AttnWorkspace &w) {
+int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, const AttnArgs &a) {
   switch (p.head_dim) {
-    case 32: return launch<T, 32>(st, p, L, a, ws, w);
-    case 64: return launch<T, 64>(st, p, L, a, ws, w);
-    case 96: return launch<T, 96>(st, p, L, a, ws, w);
-    case 128: return launch<T, 128>(st, p, L, a, ws, w);
-    default: return launch<T, 256>(st, p, L, a, ws, w);
+    case 32: return launch<T, 32>(st, p, L, a);
+    case 64: return launch<T, 64>(st, p, L, a);
+    case 96: return launch<T, 96>(st, p, L, a);
+    case 128: return launch<T, 128>(st, p, L, a);
+    default: return launch<T, 256>(st, p, L, a);
   }
 }
 
@@ -887,7 +960,17 @@ extern "C" int mlora_paged_attention(void *stream, const mlora_attention_plan *p
   a.k = static_cast<const uint16_t *>(key_buffer);
   a.v = static_cast<const uint16_t *>(value_buffer);
   a.table = table;
-  a.lse = weights ? reinterpret_cast<float *>(static_cast<char *>(workspace) + w.lse) : nullptr;
+  char *ws = static_cast<char *>(workspace);
+  a.few_o = reinterpret_cast<float *>(ws + w.few_o);
+  a.tall_o = reinterpret_cast<float *>(ws + w.tall_o);
+  a.few_ml = reinterpret_cast<float4 *>(ws + w.few_ml);
+  a.tall_ml = reinterpret_cast<float4 *>(ws + w.tall_ml);
+  a.lse = weights ? reinterpret_cast<float *>(ws + w.lse) : nullptr;
+  a.off_few = L.off_few;
+  a.off_tall = L.off_tall;
+  a.off_joins = L.off_joins;
+  a.off_arrive = L.off_arrive;
+  a.off_requests = L.off_requests;
   a.weights = weights;
   a.out_stride = out_stride;
   a.q_stride = q_stride;
@@ -903,7 +986,6 @@ extern "C" int mlora_paged_attention(void *stream, const mlora_attention_plan *p
   a.window = plan->window;
   a.n_req = (int)plan->n_req;
   a.n_pages = (int)n_pages;
-  char *ws = static_cast<char *>(workspace);
   hipStream_t st = (hipStream_t)stream;
-  return dtype == MLORA_F16 ? launch<_Float16>(st, *plan, L, a, ws, w) : launch<__bf16>(st, *plan, L, a, ws, w);
+  return dtype == MLORA_F16 ? launch<_Float16>(st, *plan, L, a) : launch<__bf16>(st, *plan, L, a);
 }

@@ -68,6 +68,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
   const int per = (a.n_req + AP_THREADS - 1) / AP_THREADS;
   const int lo = min(tid * per, a.n_req), hi = min(lo + per, a.n_req);
 
+  for (int64_t i = tid; i < a.L.max_joins * a.kv_heads; i += AP_THREADS) a.plan[a.L.off_arrive + i] = 0;
   int64_t few = 0, tall = 0;
   for (int b = lo; b < hi; ++b) {
     const Request r = request(a, b);
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
       const int p0 = begin + i * piece;
       rec[0] = b;
       rec[1] = row0;
-      rec[2] = fits ? rows : 0;
+      rec[2] = fits ? (is_tall || k == 1 ? rows : rows | at[JOINS] << 16) : 0;
       rec[3] = k > 1 ? p0 : begin;
       rec[4] = k > 1 ? min(p0 + piece, end) : end;
       rec[5] = k > 1 ? at[slots] + i : -1;
@@ -232,7 +233,8 @@ AttnLayout attention_layout(const mlora_attention_plan &p) {
   L.off_tall = L.off_few + L.max_few * AT_REC;
   L.off_joins = L.off_tall + L.max_tall * AT_REC;
   L.off_requests = L.off_joins + L.max_joins * AT_REC;
-  L.words = L.off_requests + (p.n_req + 1) * AT_REQ;
+  L.off_arrive = L.off_requests + (p.n_req + 1) * AT_REQ;
+  L.words = L.off_arrive + L.max_joins * p.kv_heads;
   return L;
 }
 
