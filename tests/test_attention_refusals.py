@@ -36,7 +36,7 @@ def test_the_lists_hold_any_batch_the_bounds_allow():
     and lengths within n_tokens, max_seq_len and max_kv_len."""
     import random
     L, rng = _lib.lib(), random.Random(1)
-    step, few_rows, tall_rows, few_items, tall_items, few_least, tall_least = 64, 16, 128, 1024, 512, 256, 512
+    step, few_rows, tall_rows, few_items, tall_items, few_least, tall_least = 64, 16, 128, 1024, 512, 128, 512
     up = lambda a, b: -(-a // b)  # noqa: E731
     for _ in range(300):
         hkv, group = rng.choice([1, 2, 8, 32]), rng.choice([1, 4, 7, 8])
@@ -61,7 +61,7 @@ def test_the_lists_hold_any_batch_the_bounds_allow():
             counts[name] = records, slots, joins
         p = plan(n_req=n_req, n_tokens=max(1, sum(new)), max_seq_len=max_seq, max_kv_len=max_kv, q_heads=hkv * group, kv_heads=hkv)
         words = L.mlora_attention_plan_bytes(p) // 4
-        need = 32 + 8 * (counts["few"][0] + counts["tall"][0] + counts["few"][2] + counts["tall"][2]) + 4 * (n_req + 1)
+        need = hkv * (counts["few"][2] + counts["tall"][2]) + 32 + 8 * (counts["few"][0] + counts["tall"][0] + counts["few"][2] + counts["tall"][2]) + 4 * (n_req + 1)
         assert need <= words, (counts, words)
         room = L.mlora_attention_workspace_bytes(p, 0)
         floats = hkv * (128 + 4) * 4

@@ -157,6 +157,17 @@ struct Cache {
   int begin, end, shift, n_pages;
 };
 
+// A record of the plan's lists, asked for at once and before it is known whether it is one (the lists have room for it either way)
+struct Record {
+  int w[AT_REC];
+  __device__ __forceinline__ Record(const int32_t *plan, int64_t list, int i) {
+    const int32_t *rec = plan + list + (int64_t)i * AT_REC;
+#pragma unroll
+    for (int n = 0; n < AT_REC; ++n) w[n] = rec[n];
+    requested();
+  }
+};
+
 // page numbers of tokens [base, base + 64), token base + l by lane l
 __device__ __forceinline__ void load_pages(const Cache &c, int base, uint32_t slice, int lane) {
   const int t = min(base + lane, c.end - 1);
@@ -304,14 +315,13 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
   using L = Tile<D>;
   constexpr int WAVES = F::WAVES, CH = D / 32, DB = D / 16;
   using vec8 = typename Traits<T>::vec8;
-  if (rec_i >= a.plan[AH_FEW]) return;
-  const int32_t *rec = a.plan + a.off_few + (int64_t)rec_i * AT_REC;
-  const int req = rec[0], row0 = rec[1], rows = rec[2] & 0xffff, join = rec[2] >> 16, slot = rec[5], tok0 = rec[6], pos0 = rec[7];
-  if (rows <= 0) return;
+  const Record rec(a.plan, a.off_few, rec_i);
+  const int req = rec.w[0], row0 = rec.w[1], rows = rec.w[2] & 0xffff, join = rec.w[2] >> 16, slot = rec.w[5], tok0 = rec.w[6], pos0 = rec.w[7];
+  if (rec_i >= a.plan[AH_FEW] || rows <= 0) return;
   const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
   const int lrow = lane & 15, kg = lane >> 4;
   Cache c{a.table + (int64_t)req * a.table_stride, reinterpret_cast<const char *>(a.k) + head * D * 2,
-          reinterpret_cast<const char *>(a.v) + head * D * 2, a.k_stride, a.v_stride, rec[3], rec[4], a.page_shift, a.n_pages};
+          reinterpret_cast<const char *>(a.v) + head * D * 2, a.k_stride, a.v_stride, rec.w[3], rec.w[4], a.page_shift, a.n_pages};
   const uint32_t mem = lds_offset(lds) + wave * F::WAVE, kt = mem, vt = mem + F::TILE, slices = mem + 2 * F::TILE;
 
   const int tiles = (c.end - c.begin + FEW_TOKENS - 1) / FEW_TOKENS;
@@ -551,15 +561,14 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
   using L = Tile<D>;
   constexpr int CH = D / 16, DB = D / 32, TOKENS = F::TOKENS, BL = TOKENS / 32;
   using vec8 = typename Traits<T>::vec8;
-  if (rec_i >= a.plan[AH_TALL]) return;
   int *again = reinterpret_cast<int *>(lds + F::TOTAL);         // the tile's rows are done again the careful way
-  const int32_t *rec = a.plan + a.off_tall + (int64_t)rec_i * AT_REC;
-  const int req = rec[0], row0 = rec[1], rows = rec[2], slot = rec[5], tok0 = rec[6], pos0 = rec[7];
-  if (rows <= 0) return;
+  const Record rec(a.plan, a.off_tall, rec_i);
+  const int req = rec.w[0], row0 = rec.w[1], rows = rec.w[2], slot = rec.w[5], tok0 = rec.w[6], pos0 = rec.w[7];
+  if (rec_i >= a.plan[AH_TALL] || rows <= 0) return;
   const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
   const int lrow = lane & 31, half = lane >> 5;
   Cache c{a.table + (int64_t)req * a.table_stride, reinterpret_cast<const char *>(a.k) + head * D * 2,
-          reinterpret_cast<const char *>(a.v) + head * D * 2, a.k_stride, a.v_stride, rec[3], rec[4], a.page_shift, a.n_pages};
+          reinterpret_cast<const char *>(a.v) + head * D * 2, a.k_stride, a.v_stride, rec.w[3], rec.w[4], a.page_shift, a.n_pages};
   const uint32_t mem = lds_offset(lds), slices = mem + 2 * F::BUFFER + wave * F::SLICES * 256;
   const int tiles = (c.end - c.begin + TOKENS - 1) / TOKENS;
   auto base_of = [&](int k) { return c.begin + k * TOKENS; };

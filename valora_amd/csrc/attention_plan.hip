@@ -215,7 +215,7 @@ AttnLayout attention_layout(const mlora_attention_plan &p) {
   L.group = p.q_heads / p.kv_heads;
   L.few_items = 1024;
   L.tall_items = 512;
-  L.few_least = 256;
+  L.few_least = 128;
   L.tall_least = 512;
   const int64_t T = p.n_tokens, n = p.n_req < T ? p.n_req : T;      // requests with new tokens
   const bool tall = p.max_seq_len * L.group > FEW_ROWS;
