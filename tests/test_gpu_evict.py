@@ -83,11 +83,15 @@ def test_values_that_are_not_finite(dev):
 
 
 def test_more_pages_than_stay_in_shared_memory(dev):
+    """Tables of 16384 and 32768 pages are the widest that registers and shared memory hold."""
     lens = [36864, 36865, 60000, 5]
     table, w = make(lens, extra=1, seed=3)
     check(dev, table, lens, w, 5000, 100, 4)
-    table, w = make([36864 - 7], extra=7, seed=4, kind="zeros")      # the last size that does
-    check(dev, table, [36864 - 7], w, 20000, 64, 4)
+    for width in (16384, 16385, 32768, 32769, 36864):
+        lens = [width - 7, width, 40, width // 2]
+        for kind in ("zeros", "heavy"):
+            table, w = make(lens, extra=0, seed=width, kind=kind)
+            check(dev, table, lens, w, width // 3, 64, 4)
 
 
 def test_what_is_behind_a_request_does_not_matter(dev):
