@@ -31,41 +31,78 @@ def test_plan_shapes():
         assert L.mlora_build_attention_plan(None, plan(**kw), None, None, None) < 0
 
 
+def cut_few(spans, hkv):
+    """Records, slots and joins of the few-rows list, as the plan kernel cuts it."""
+    up = lambda a, b: -(-a // b)  # noqa: E731
+    piece = max(128, up(up(sum(spans) * hkv, 1024), 64) * 64)
+    ks = [1 if s <= piece else up(s, up(up(s, up(s, piece)), 64) * 64) for s in spans]
+    return sum(ks), sum(k for k in ks if k > 1), sum(k > 1 for k in ks)
+
+
+def cut_tall(spans, shares):
+    """(records, slots, joins, pieces per tile, first record of each share) of the tall list, as the plan kernel cuts it."""
+    least, overhead = 512, 192
+    line = sum(s + overhead for s in spans)
+    n = min(-(-line // least), shares)
+    share = -(-line // n) if n else 1
+    n = -(-line // share)
+    at, pieces, first, records = 0, [], {}, 0
+    for s in spans:
+        ends, last, j = [], 0, -(-at // share)
+        marks = []
+        while j * share < at + s + overhead:
+            inside = j * share - at - overhead // 2
+            cut = int((inside + 32) / 64) * 64
+            if inside < least // 2 or s < least:
+                cut = 0 if inside * 2 < s else s
+            elif inside > s - least // 2:
+                cut = s
+            if last < cut < s:
+                ends.append(cut)
+                last = cut
+            marks.append((j, None if cut >= s and s > 0 else len(ends)))
+            j += 1
+        k = len(ends) + 1
+        for j, i in marks:
+            first[j] = records + (k if i is None else i)
+        pieces.append([b - a for a, b in zip([0] + ends, ends + [s])])
+        records += k
+        at += s + overhead
+    return records, sum(len(p) for p in pieces if len(p) > 1), sum(len(p) > 1 for p in pieces), pieces, [first[j] for j in range(n)]
+
+
 def test_the_lists_hold_any_batch_the_bounds_allow():
     """The records that the plan kernel would write, counted as it counts them, against the room the plan has: requests of all kinds
-    and lengths within n_tokens, max_seq_len and max_kv_len."""
+    and lengths within n_tokens, max_seq_len and max_kv_len; and the shares, which are even up to what is not cut."""
     import random
     L, rng = _lib.lib(), random.Random(1)
-    step, few_rows, tall_rows, few_items, tall_items, few_least, tall_least = 64, 16, 128, 1024, 512, 128, 512
-    up = lambda a, b: -(-a // b)  # noqa: E731
-    for _ in range(300):
-        hkv, group = rng.choice([1, 2, 8, 32]), rng.choice([1, 4, 7, 8])
-        n_req, max_seq, max_kv = rng.randint(1, 300), rng.choice([1, 2, 5, 40, 900]), rng.choice([1, 64, 256, 300, 5000, 70000])
+    for _ in range(400):
+        hkv, group = rng.choice([1, 2, 8, 32, 40]), rng.choice([1, 4, 7, 8])
+        n_req, max_seq, max_kv = rng.randint(1, 300), rng.choice([1, 2, 5, 40, 900]), rng.choice([1, 64, 256, 300, 511, 512, 5000, 70000])
         new = [rng.choice([0, 1, 1, rng.randint(1, max_seq)]) for _ in range(n_req)]
         kv = [rng.randint(0, max_kv) if rng.random() < 0.8 else max_kv for _ in range(n_req)]
-        spans = {"few": [], "tall": []}
+        few, tall = [], []
         for n, l in zip(new, kv):
             rows = n * group
-            tiles = [(0, rows)] if 0 < rows <= few_rows else [(r, min(tall_rows, rows - r)) for r in range(0, rows, tall_rows)]
-            for r0, r in tiles:
-                spans["few" if rows <= few_rows else "tall"].append(max(0, l - n + (r0 + r - 1) // group + 1))
-        counts = {}
-        for name, items, least in (("few", few_items, few_least), ("tall", tall_items, tall_least)):
-            piece = max(least, up(up(sum(spans[name]) * hkv, items), step) * step)
-            records = slots = joins = 0
-            for s in spans[name]:
-                k = 1
-                if s > piece:
-                    k = up(s, up(up(s, up(s, piece)), step) * step)
-                records, slots, joins = records + k, slots + (k if k > 1 else 0), joins + (k > 1)
-            counts[name] = records, slots, joins
+            if 0 < rows <= 16:
+                few.append(max(0, l))
+            else:
+                tall += [max(0, l - n + (min(r + 128, rows) - 1) // group + 1) for r in range(0, rows, 128)]
         p = plan(n_req=n_req, n_tokens=max(1, sum(new)), max_seq_len=max_seq, max_kv_len=max_kv, q_heads=hkv * group, kv_heads=hkv)
-        words = L.mlora_attention_plan_bytes(p) // 4
-        need = hkv * (counts["few"][2] + counts["tall"][2]) + 32 + 8 * (counts["few"][0] + counts["tall"][0] + counts["few"][2] + counts["tall"][2]) + 4 * (n_req + 1)
-        assert need <= words, (counts, words)
-        room = L.mlora_attention_workspace_bytes(p, 0)
-        floats = hkv * (128 + 4) * 4
-        assert (counts["few"][1] * few_rows + counts["tall"][1] * tall_rows) * floats <= room, (counts, room)
+        words, room = L.mlora_attention_plan_bytes(p) // 4, L.mlora_attention_workspace_bytes(p, 0)
+        shares = 512 // hkv
+        f, t = cut_few(few, hkv), cut_tall(tall, shares)
+        need = 32 + 8 * (f[0] + t[0] + f[2] + t[2] + n_req) + len(t[4]) + 1 + hkv * (f[2] + t[2])
+        assert need <= words, (f, t[:3], words)
+        assert (f[1] * 16 + t[1] * 128) * hkv * (128 + 4) * 4 <= room, (f, t[:3], room)
+        assert all(sum(p) == s and (len(p) == 1 or min(p) >= 192) for p, s in zip(t[3], tall))
+        if t[4]:
+            assert t[4][0] == 0 and t[4] == sorted(t[4]) and t[4][-1] <= t[0]
+            flat = [x + (192 if i == 0 else 0) for q in t[3] for i, x in enumerate(q)]
+            share = -(-sum(flat) // len(t[4]))
+            bounds = t[4] + [t[0]]
+            # a share is off by what its two ends are moved: half of what is not cut, and the start of a tile
+            assert all(sum(flat[a:b]) <= share + 512 + 192 + 128 for a, b in zip(bounds, bounds[1:]))
 
 
 def test_attention_arguments():

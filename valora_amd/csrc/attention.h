@@ -7,32 +7,39 @@ namespace mlora {
 
 // A call's work is cut into tiles of packed rows: row r of a request and key head is (new token r / group, query head
 // r % group of the key head's `group`), so the heads of a group share what is read of the cache.  Requests of up to FEW_ROWS rows
-// (decoding ones) are one tile of the few-rows kernel, the others tiles of TALL_ROWS rows of the tall kernel.  A tile's span of
-// the cache is cut into pieces where there are too few tiles to fill the device; a piece leaves its rows' sums, not yet
-// divided, in a slot of the workspace; the last piece of a tile of few rows joins them, a launch of its own those of tall tiles.
+// (decoding ones) are one tile of the few-rows list, the others tiles of TALL_ROWS rows of the tall list.  A tile's span of the
+// cache is cut into pieces where that evens out the work; a piece leaves its rows' sums, not yet divided, in a slot of the
+// workspace; the last piece of a tile of few rows joins them, a launch of its own those of tall tiles.
+//
+// Few rows: spans above an even share of the whole are cut into equal pieces, a workgroup each.  Tall: the tiles stand in a line, each
+// as long as its span and TALL_OVERHEAD tokens for its start and end; the line is cut into as many equal shares as the
+// device holds workgroups, and a workgroup goes over the tiles of its share.  (One workgroup a piece: 616 of them for 512 places
+// took a third longer.)
 constexpr int FEW_ROWS = 16, TALL_ROWS = 128;
 constexpr int AT_PIECE_STEP = 64;            // a piece's length is a multiple of this
+constexpr int TALL_OVERHEAD = 192;
 
-// plan buffer (int32 words): hdr[32] | few[max_few][8] | tall[max_tall][8] | joins[max_joins][8] | requests[n_req + 1][4]
-// | arrive[max_joins][kv_heads]
-// record: {request, first row, rows, begin, end, slot (-1: the tile's only piece), first new token in q, position of the
+// plan buffer (int32 words): hdr[32] | few[max_few][8] | tall[max_tall][8] | joins[max_joins][8] | requests[n_req][8]
+// | shares[max_shares + 1] | arrive[max_joins][kv_heads]
+// record:  {request, first row, rows, begin, end, slot (-1: the tile's only piece), first new token in q, position of the
 // request's new token 0}; the piece covers cache indices [begin, end); rows of the few-rows list hold the index of the tile's
 // join in the upper half
-// join:   {first slot, pieces, rows, first row, first new token in q, 1 in the tall list, 0, 0}
-// request: {blocks of WEIGHT_TOKENS cached tokens of the requests before, first new token in q, new tokens, cached tokens};
-// the last one holds the count of all blocks only
-// arrive: pieces of a tile that have left their sums, zero between calls
-constexpr int AT_HDR = 32, AT_REC = 8, AT_REQ = 4;
-enum AttnHdr { AH_FEW = 0, AH_TALL = 1, AH_JOINS = 2, AH_BLOCKS = 3 };
+// join:    {first slot, pieces, rows, first row, first new token in q, 1 in the tall list, 0, 0}
+// request: {blocks of WEIGHT_TOKENS cached tokens of the requests before, first new token in q, new tokens, cached tokens, tall tiles
+// of the requests before, 0, 0, 0}
+// share:   its first record of the tall list
+// arrive:  pieces of a tile that have left their sums, zero between calls
+constexpr int AT_HDR = 32, AT_REC = 8;
+enum AttnHdr { AH_FEW = 0, AH_TALL = 1, AH_JOINS = 2, AH_BLOCKS = 3, AH_SHARES = 4 };
 constexpr int WEIGHT_TOKENS = 256;
 
 struct AttnLayout {
   int64_t group;
-  int64_t max_few, max_tall, max_joins;      // records
+  int64_t max_few, max_tall, max_joins, max_shares;
   int64_t slots_few, slots_tall;
-  int64_t off_few, off_tall, off_joins, off_requests, off_arrive, words;
-  int few_items, tall_items;                 // (piece, key head) pairs the lists are cut for
-  int few_least, tall_least;                 // a piece is no shorter than this
+  int64_t off_few, off_tall, off_joins, off_requests, off_shares, off_arrive, words;
+  int few_items;                             // (piece, key head) pairs the list is cut for
+  int few_least, tall_least;                 // spans up to these are not cut
 };
 
 AttnLayout attention_layout(const mlora_attention_plan &p);

@@ -44,7 +44,7 @@ struct AttnArgs {
   float *lse;                          // null: not wanted
   float *weights;
   int64_t out_stride, q_stride, table_stride, weights_stride;
-  int64_t off_few, off_tall, off_joins, off_arrive, off_requests;
+  int64_t off_few, off_tall, off_joins, off_arrive, off_requests, off_shares;
   uint32_t k_stride, v_stride;         // bytes
   float c;                             // scale * log2(e)
   int tall_blocks;                     // workgroups of the tall list; those of the other follow
@@ -564,7 +564,7 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
   int *again = reinterpret_cast<int *>(lds + F::TOTAL);         // the tile's rows are done again the careful way
   const Record rec(a.plan, a.off_tall, rec_i);
   const int req = rec.w[0], row0 = rec.w[1], rows = rec.w[2], slot = rec.w[5], tok0 = rec.w[6], pos0 = rec.w[7];
-  if (rec_i >= a.plan[AH_TALL] || rows <= 0) return;
+  if (rows <= 0) return;
   const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
   const int lrow = lane & 31, half = lane >> 5;
   Cache c{a.table + (int64_t)req * a.table_stride, reinterpret_cast<const char *>(a.k) + head * D * 2,
@@ -626,9 +626,13 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
 #pragma unroll
         for (int g = 0; g < 2 * BL; ++g) {
 #pragma unroll
-          for (int db = 0; db < DB; ++db) check_finite<T>(values(g, db), finite);
-          here(finite);
-          one_by_one();   // (the values are read again below: to keep them would take the registers of the whole tile)
+          for (int db = 0; db < DB; ++db) {
+            check_finite<T>(values(g, db), finite);
+            if (db % 4 == 3 || db == DB - 1) {     // (the values are read again below: to keep them would take the registers of the whole tile)
+              here(finite);
+              one_by_one();
+            }
+          }
         }
         odd = odd || !all_finite(finite);
       }
@@ -756,14 +760,23 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attend_kernel(AttnA
   const unsigned block = blockIdx.x - (tall ? 0 : a.tall_blocks);
   // the key heads of a piece follow each other: they read the same pages, and what reads the same head's rows again is eight, or a
   // multiple of it, further where kv_heads is: on the same XCD
-  const int rec = (int)(block / (unsigned)a.kv_heads), head = (int)(block - (unsigned)rec * a.kv_heads);
-  if (tall) tall_tile<T, D, SUMS>(a, lds, rec, head);
-  else few_tile<T, D, SUMS>(a, lds, rec, head);
+  const int i = (int)(block / (unsigned)a.kv_heads), head = (int)(block - (unsigned)i * a.kv_heads);
+  if (!tall) {
+    few_tile<T, D, SUMS>(a, lds, i, head);
+    return;
+  }
+  const int32_t *shares = a.plan + a.off_shares;
+  if (i >= a.plan[AH_SHARES]) return;
+  const int last = min(shares[i + 1], a.plan[AH_TALL]);
+  for (int rec = shares[i]; rec < last; ++rec) {
+    tall_tile<T, D, SUMS>(a, lds, rec, head);
+    __syncthreads();                                            // (what the next one loads goes where this one's was)
+  }
 }
 
 template <typename T, int D, bool SUMS>
 int launch_lists(hipStream_t st, const AttnLayout &L, AttnArgs a) {
-  const int64_t few = L.max_few * a.kv_heads, tall = L.max_tall * a.kv_heads;
+  const int64_t few = L.max_few * a.kv_heads, tall = L.max_shares * a.kv_heads;
   if (few + tall > 0x7fffffff) return fail(MLORA_ERR_NO_KERNEL, "paged_attention: too many tiles");
   a.tall_blocks = (int)tall;
   if constexpr (D <= 128) {
@@ -826,10 +839,10 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
     // the request whose run of blocks holds the item
     __syncthreads();
     for (int b = threadIdx.x; b < a.n_req; b += WEIGHT_WAVES * 64)
-      if (requests[b * AT_REQ] <= item && item < requests[(b + 1) * AT_REQ]) found = b;
+      if (requests[(int64_t)b * AT_REC] <= item && (b + 1 == a.n_req || item < requests[(int64_t)(b + 1) * AT_REC])) found = b;
     __syncthreads();
     const int b = (int)uniform((uint32_t)found);
-    const int32_t *rq = requests + (int64_t)b * AT_REQ;
+    const int32_t *rq = requests + (int64_t)b * AT_REC;
     const int tok0 = rq[1], n = rq[2], kv = rq[3], pos0 = kv - n, rows = n * a.group;
     const int begin = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
     const int base = begin + (item - rq[0]) * WEIGHT_TOKENS + wave * 64;
@@ -980,6 +993,7 @@ extern "C" int mlora_paged_attention(void *stream, const mlora_attention_plan *p
   a.off_joins = L.off_joins;
   a.off_arrive = L.off_arrive;
   a.off_requests = L.off_requests;
+  a.off_shares = L.off_shares;
   a.weights = weights;
   a.out_stride = out_stride;
   a.q_stride = q_stride;

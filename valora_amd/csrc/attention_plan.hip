@@ -15,7 +15,7 @@ struct PlanArgs {
   int n_req, group, max_seq, max_kv, kv_heads, window;
 };
 
-constexpr int AP_THREADS = 1024, AP_WAVES = AP_THREADS / 64;
+constexpr int AP_THREADS = 512, AP_WAVES = AP_THREADS / 64;
 
 struct Request {
   int n, start, kv, rows;
@@ -45,6 +45,38 @@ __device__ __forceinline__ int64_t wave_sum(int64_t v) {
   return v;
 }
 
+// Sum over the workgroup, for everyone
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t (&part)[AP_WAVES]) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+  for (int i = 0; i < AP_WAVES; ++i) v += part[i];
+  return v;
+}
+
+// Sum over the threads before this one, and over all in `total`
+__device__ __forceinline__ int64_t block_before(int64_t mine, int64_t &total, int64_t (&part)[AP_WAVES]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t v = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t up = __shfl_up(v, d);
+    if (lane >= d) v += up;
+  }
+  __syncthreads();
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  int64_t before = v - mine;
+  total = 0;
+  for (int i = 0; i < AP_WAVES; ++i) {
+    before += i < wave ? part[i] : 0;
+    total += part[i];
+  }
+  return before;
+}
+
 // pieces of a span, none longer than `piece`; its length is evened out
 __device__ __forceinline__ int cut(int len, int &piece) {
   if (len <= piece) return 1;
@@ -53,156 +85,199 @@ __device__ __forceinline__ int cut(int len, int &piece) {
   return (len + piece - 1) / piece;
 }
 
-__device__ __forceinline__ int piece_length(int64_t total, int kv_heads, int items, int least) {
-  const int64_t c = (total * kv_heads + items - 1) / items;
-  const int64_t r = (c + AT_PIECE_STEP - 1) / AT_PIECE_STEP * AT_PIECE_STEP;
-  return (int)(r < least ? least : r > (1 << 30) ? (1 << 30) : r);
-}
+// counts of records, slots and joins travel through the sums as one number (each below 2^20: csrc/attention_plan.hip, layout)
+__device__ __forceinline__ int64_t pack(int64_t records, int64_t slots, int64_t joins) { return records | slots << 21 | joins << 42; }
+constexpr int64_t PACKED = (1 << 21) - 1;
 
-// One workgroup; a thread owns a run of requests, so places in the lists follow from one sum over the threads.
+// One workgroup, a thread per request and then per tall tile, in rounds where there are more.
 __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) {
-  enum { FEW, TALL, JOINS, SLOTS_F, SLOTS_T, BLOCKS, COUNTS };
-  __shared__ int64_t totals[2][AP_WAVES];
-  __shared__ int counts[COUNTS][AP_WAVES];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (a.n_req + AP_THREADS - 1) / AP_THREADS;
-  const int lo = min(tid * per, a.n_req), hi = min(lo + per, a.n_req);
-
+  __shared__ int64_t part[AP_WAVES];
+  const int tid = threadIdx.x;
+  int32_t *requests = a.plan + a.L.off_requests, *shares = a.plan + a.L.off_shares;
   for (int64_t i = tid; i < a.L.max_joins * a.kv_heads; i += AP_THREADS) a.plan[a.L.off_arrive + i] = 0;
-  int64_t few = 0, tall = 0;
-  for (int b = lo; b < hi; ++b) {
-    const Request r = request(a, b);
-    int begin, end;
-    if (r.rows > FEW_ROWS) {
-      for (int row = 0; row < r.rows; row += TALL_ROWS) {
-        span(a, r, row, min(TALL_ROWS, r.rows - row), begin, end);
-        tall += end - begin;
-      }
-    } else if (r.rows > 0) {
-      span(a, r, 0, r.rows, begin, end);
-      few += end - begin;
-    }
-  }
-  few = wave_sum(few);
-  tall = wave_sum(tall);
-  if (lane == 0) {
-    totals[0][wave] = few;
-    totals[1][wave] = tall;
-  }
-  __syncthreads();
-  few = tall = 0;
-  for (int i = 0; i < AP_WAVES; ++i) {
-    few += totals[0][i];
-    tall += totals[1][i];
-  }
-  const int few_piece = piece_length(few, a.kv_heads, a.L.few_items, a.L.few_least);
-  const int tall_piece = piece_length(tall, a.kv_heads, a.L.tall_items, a.L.tall_least);
 
-  int mine[COUNTS] = {0, 0, 0, 0, 0, 0};
-  auto count = [&](int list, int slots, int len, int piece) {
-    const int k = cut(len, piece);
-    mine[list] += k;
-    if (k > 1) {
-      ++mine[JOINS];
-      mine[slots] += k;
-    }
-  };
-  auto blocks = [&](const Request &r) {
-    if (r.rows == 0) return 0;
-    int begin, end;
-    span(a, r, 0, r.rows, begin, end);
-    return (end - begin + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS;
-  };
-  for (int b = lo; b < hi; ++b) {
-    const Request r = request(a, b);
-    int begin, end;
-    if (r.rows > FEW_ROWS) {
-      for (int row = 0; row < r.rows; row += TALL_ROWS) {
-        span(a, r, row, min(TALL_ROWS, r.rows - row), begin, end);
-        count(TALL, SLOTS_T, end - begin, tall_piece);
+  // ---- requests
+  int64_t few = 0, blocks_before = 0, tiles = 0;
+  for (int b0 = 0; b0 < a.n_req; b0 += AP_THREADS) {
+    const int b = b0 + tid;
+    Request r{};
+    int begin = 0, end = 0, n_blocks = 0, n_tiles = 0;
+    if (b < a.n_req) {
+      r = request(a, b);
+      if (r.rows > 0) {
+        span(a, r, 0, r.rows, begin, end);
+        n_blocks = (end - begin + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS;
+        n_tiles = r.rows > FEW_ROWS ? (r.rows + TALL_ROWS - 1) / TALL_ROWS : 0;
+        if (n_tiles == 0) few += end - begin;
       }
-    } else if (r.rows > 0) {
-      span(a, r, 0, r.rows, begin, end);
-      count(FEW, SLOTS_F, end - begin, few_piece);
     }
-    mine[BLOCKS] += blocks(r);
-  }
-  int at[COUNTS];
-#pragma unroll
-  for (int c = 0; c < COUNTS; ++c) {
-    int v = mine[c];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(v, d);
-      if (lane >= d) v += up;
+    int64_t all;
+    const int64_t before = block_before(n_blocks | (int64_t)n_tiles << 32, all, part);
+    if (b < a.n_req) {
+      int32_t *rq = requests + (int64_t)b * AT_REC;
+      rq[0] = (int32_t)(blocks_before + (before & 0xffffffff));
+      rq[1] = r.start;
+      rq[2] = r.n;
+      rq[3] = r.kv;
+      rq[4] = (int32_t)(tiles + (before >> 32));
     }
-    at[c] = v - mine[c];
-    if (lane == 63) counts[c][wave] = v;
+    blocks_before += all & 0xffffffff;
+    tiles += all >> 32;
   }
-  __syncthreads();
-#pragma unroll
-  for (int c = 0; c < COUNTS; ++c)
-    for (int i = 0; i < wave; ++i) at[c] += counts[c][i];
-  if (tid == AP_THREADS - 1) {
+  few = block_sum(few, part);
+  int64_t records = 0, slots = 0, joins = 0;
+
+  auto emit_join = [&](int64_t at, int64_t slot0, int pieces, int rows, int row0, int start, bool tall) {
+    if (at >= a.L.max_joins) return;
+    int32_t *j = a.plan + a.L.off_joins + at * AT_REC;
+    j[0] = (int32_t)slot0;
+    j[1] = pieces;
+    j[2] = rows;
+    j[3] = row0;
+    j[4] = start;
+    j[5] = tall;
+    j[6] = j[7] = 0;
+  };
+  auto emit = [&](int32_t *list, int64_t at, int64_t max, int b, int row0, int rows, int begin, int end, int64_t slot, const Request &r) {
+    if (at >= max) return;
+    int32_t *rec = list + at * AT_REC;
+    rec[0] = b;
+    rec[1] = row0;
+    rec[2] = rows;
+    rec[3] = begin;
+    rec[4] = end;
+    rec[5] = (int32_t)slot;
+    rec[6] = r.start;
+    rec[7] = r.kv - r.n;
+  };
+
+  // ---- few rows: a request's tile into equal pieces
+  const int64_t even = ((few * a.kv_heads + a.L.few_items - 1) / a.L.few_items + AT_PIECE_STEP - 1) / AT_PIECE_STEP * AT_PIECE_STEP;
+  const int few_piece = (int)(even < a.L.few_least ? a.L.few_least : even > (1 << 30) ? (1 << 30) : even);
+  for (int b0 = 0; b0 < a.n_req; b0 += AP_THREADS) {
+    const int b = b0 + tid;
+    Request r{};
+    int begin = 0, end = 0, k = 0, piece = few_piece;
+    if (b < a.n_req) {
+      r = request(a, b);
+      if (r.rows > 0 && r.rows <= FEW_ROWS) {
+        span(a, r, 0, r.rows, begin, end);
+        k = cut(end - begin, piece);
+      }
+    }
+    int64_t all;
+    const int64_t before = block_before(k > 0 ? pack(k, k > 1 ? k : 0, k > 1) : 0, all, part);
+    const int64_t rec = records + (before & PACKED), slot = slots + (before >> 21 & PACKED), join = joins + (before >> 42);
     // (requests that overlap in q could ask for more than the lists hold: what is beyond is left out)
-    a.plan[AH_FEW] = (int)min<int64_t>(at[FEW] + mine[FEW], a.L.max_few);
-    a.plan[AH_TALL] = (int)min<int64_t>(at[TALL] + mine[TALL], a.L.max_tall);
-    a.plan[AH_JOINS] = (int)min<int64_t>(at[JOINS] + mine[JOINS], a.L.max_joins);
-    a.plan[AH_BLOCKS] = at[BLOCKS] + mine[BLOCKS];
-    a.plan[a.L.off_requests + (int64_t)a.n_req * AT_REQ] = at[BLOCKS] + mine[BLOCKS];
+    const bool fits = rec + k <= a.L.max_few && (k < 2 || (slot + k <= a.L.slots_few && join < a.L.max_joins));
+    for (int i = 0; i < k; ++i)
+      emit(a.plan + a.L.off_few, rec + i, a.L.max_few, b, 0, !fits ? 0 : k > 1 ? r.rows | (int)join << 16 : r.rows, begin + (k > 1 ? i * piece : 0),
+           k > 1 ? min(begin + (i + 1) * piece, end) : end, k > 1 ? slot + i : -1, r);
+    if (k > 1) emit_join(join, slot, fits ? k : 0, r.rows, 0, r.start, false);
+    records += all & PACKED;
+    slots += all >> 21 & PACKED;
+    joins += all >> 42;
   }
+  if (tid == 0) a.plan[AH_FEW] = (int)min<int64_t>(records, a.L.max_few);
 
-  auto emit = [&](int b, const Request &r, int row0, int rows, int list, int slots, int piece) {
-    int begin, end;
-    span(a, r, row0, rows, begin, end);
-    const int k = cut(end - begin, piece);
-    const bool is_tall = list == TALL;
-    const int64_t max_records = is_tall ? a.L.max_tall : a.L.max_few, max_slots = is_tall ? a.L.slots_tall : a.L.slots_few;
-    int32_t *records = a.plan + (is_tall ? a.L.off_tall : a.L.off_few);
-    const bool fits = at[list] + k <= max_records && (k == 1 || (at[slots] + k <= max_slots && at[JOINS] < a.L.max_joins));
-    for (int i = 0; i < k; ++i) {
-      if (at[list] + i >= max_records) break;
-      int32_t *rec = records + (int64_t)(at[list] + i) * AT_REC;
-      const int p0 = begin + i * piece;
-      rec[0] = b;
-      rec[1] = row0;
-      rec[2] = fits ? (is_tall || k == 1 ? rows : rows | at[JOINS] << 16) : 0;
-      rec[3] = k > 1 ? p0 : begin;
-      rec[4] = k > 1 ? min(p0 + piece, end) : end;
-      rec[5] = k > 1 ? at[slots] + i : -1;
-      rec[6] = r.start;
-      rec[7] = r.kv - r.n;
-    }
-    if (k > 1) {
-      if (at[JOINS] < a.L.max_joins) {
-        int32_t *join = a.plan + a.L.off_joins + (int64_t)at[JOINS] * AT_REC;
-        join[0] = at[slots];
-        join[1] = fits ? k : 0;
-        join[2] = rows;
-        join[3] = row0;
-        join[4] = r.start;
-        join[5] = is_tall;
-        join[6] = join[7] = 0;
-      }
-      ++at[JOINS];
-      at[slots] += k;
-    }
-    at[list] += k;
+  // ---- tall tiles, in a line
+  struct Place {
+    Request r;
+    int b, row0, rows, begin, end;
   };
-  for (int b = lo; b < hi; ++b) {
-    const Request r = request(a, b);
-    int32_t *rq = a.plan + a.L.off_requests + (int64_t)b * AT_REQ;
-    rq[0] = at[BLOCKS];
-    rq[1] = r.start;
-    rq[2] = r.n;
-    rq[3] = r.kv;
-    at[BLOCKS] += blocks(r);
-    if (r.rows > FEW_ROWS) {      // the last rows see most: first
-      for (int row = (r.rows - 1) / TALL_ROWS * TALL_ROWS; row >= 0; row -= TALL_ROWS)
-        emit(b, r, row, min(TALL_ROWS, r.rows - row), TALL, SLOTS_T, tall_piece);
-    } else if (r.rows > 0) {
-      emit(b, r, 0, r.rows, FEW, SLOTS_F, few_piece);
+  auto tile = [&](int64_t t) {
+    // the last request whose tiles begin at or before t
+    int lo = 0, hi = a.n_req;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (requests[(int64_t)mid * AT_REC + 4] <= t) lo = mid;
+      else hi = mid;
     }
+    const int32_t *rq = requests + (int64_t)lo * AT_REC;
+    Place p;
+    p.r = Request{rq[2], rq[1], rq[3], rq[2] * a.group};
+    p.b = lo;
+    p.row0 = (int)((t - rq[4]) * TALL_ROWS);
+    p.rows = min(TALL_ROWS, p.r.rows - p.row0);
+    span(a, p.r, p.row0, p.rows, p.begin, p.end);
+    return p;
+  };
+  __syncthreads();                       // (the requests are written)
+  int64_t line = 0;
+  for (int64_t t = tid; t < tiles; t += AP_THREADS) {
+    const Place p = tile(t);
+    line += p.end - p.begin + TALL_OVERHEAD;
+  }
+  line = block_sum(line, part);
+  int64_t n_shares = (line + a.L.tall_least - 1) / a.L.tall_least;
+  n_shares = n_shares < a.L.max_shares ? n_shares : a.L.max_shares;
+  const int64_t share = n_shares > 0 ? (line + n_shares - 1) / n_shares : 1;
+  n_shares = (line + share - 1) / share;      // (one that begins behind the line is none)
+  records = slots = 0;
+  int64_t at = 0;                        // where on the line the round's first tile begins
+  for (int64_t t0 = 0; t0 < tiles; t0 += AP_THREADS) {
+    const int64_t t = t0 + tid;
+    Place p{};
+    int64_t length = 0;
+    if (t < tiles) {
+      p = tile(t);
+      length = p.end - p.begin + TALL_OVERHEAD;
+    }
+    int64_t all;
+    const int64_t from = at + block_before(length, all, part);
+    at += all;
+    // f(index of the share that begins here, cut) for the shares that begin within the tile; a cut near an end is none
+    auto cuts = [&](auto f) {
+      const int len = p.end - p.begin;
+      for (int64_t j = (from + share - 1) / share; j * share < from + length; ++j) {
+        const int64_t inside = j * share - from - TALL_OVERHEAD / 2;
+        int cut = (int)((inside + AT_PIECE_STEP / 2) / AT_PIECE_STEP * AT_PIECE_STEP);
+        if (inside < a.L.tall_least / 2 || len < a.L.tall_least) cut = inside * 2 < len ? 0 : len;
+        else if (inside > len - a.L.tall_least / 2) cut = len;
+        f(j, cut);
+      }
+    };
+    int k = 0;
+    if (t < tiles) {
+      int last = 0;
+      const int len = p.end - p.begin;
+      cuts([&](int64_t, int cut) {
+        if (cut > last && cut < len) {
+          ++k;
+          last = cut;
+        }
+      });
+      ++k;
+    }
+    const int64_t before = block_before(k > 0 ? pack(k, k > 1 ? k : 0, k > 1) : 0, all, part);
+    const int64_t rec = records + (before & PACKED), slot = slots + (before >> 21 & PACKED), join = joins + (before >> 42);
+    if (t < tiles) {
+      const bool fits = rec + k <= a.L.max_tall && (k < 2 || (slot + k <= a.L.slots_tall && join < a.L.max_joins));
+      const int len = p.end - p.begin;
+      int last = 0, i = 0;
+      cuts([&](int64_t j, int cut) {
+        if (cut > last && cut < len) {
+          emit(a.plan + a.L.off_tall, rec + i, a.L.max_tall, p.b, p.row0, fits ? p.rows : 0, p.begin + last, p.begin + cut, slot + i, p.r);
+          ++i;
+          last = cut;
+        }
+        // (the tile's last piece begins a share that is cut at the tile's start or within it; one cut at its end begins with the next tile)
+        if (j < n_shares) shares[j] = (int32_t)(rec + (cut >= len && len > 0 ? k : i));
+      });
+      emit(a.plan + a.L.off_tall, rec + i, a.L.max_tall, p.b, p.row0, fits ? p.rows : 0, p.begin + last, p.end, k > 1 ? slot + i : -1, p.r);
+      if (k > 1) emit_join(join, slot, fits ? k : 0, p.rows, p.row0, p.r.start, true);
+    }
+    records += all & PACKED;
+    slots += all >> 21 & PACKED;
+    joins += all >> 42;
+  }
+  if (tid == 0) {
+    const int32_t tall = (int32_t)min<int64_t>(records, a.L.max_tall);
+    a.plan[AH_TALL] = tall;
+    a.plan[AH_JOINS] = (int)min<int64_t>(joins, a.L.max_joins);
+    a.plan[AH_BLOCKS] = (int32_t)blocks_before;
+    a.plan[AH_SHARES] = (int32_t)n_shares;
+    shares[n_shares] = tall;
   }
 }
 
@@ -214,26 +289,28 @@ AttnLayout attention_layout(const mlora_attention_plan &p) {
   AttnLayout L{};
   L.group = p.q_heads / p.kv_heads;
   L.few_items = 1024;
-  L.tall_items = 512;
   L.few_least = 128;
   L.tall_least = 512;
+  constexpr int64_t TALL_PLACES = 512;       // two workgroups on each of 256 CUs
   const int64_t T = p.n_tokens, n = p.n_req < T ? p.n_req : T;      // requests with new tokens
   const bool tall = p.max_seq_len * L.group > FEW_ROWS;
-  // sum of ceil(span / piece) <= tiles + sum of spans / piece, and a tile of k > 1 pieces has a span above (k - 1) pieces
-  const int64_t few_more = ceil_div(L.few_items, p.kv_heads), tall_more = ceil_div(L.tall_items, p.kv_heads);
-  const int64_t few_cut = ceil_div(p.max_kv_len, L.few_least), tall_cut = ceil_div(p.max_kv_len, L.tall_least);
   const auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  // few rows: sum of ceil(span / piece) <= tiles + sum of spans / piece, and a tile of k > 1 pieces has a span above (k - 1) pieces
+  const int64_t few_more = ceil_div(L.few_items, p.kv_heads), few_cut = ceil_div(p.max_kv_len, L.few_least);
   L.max_few = least(n + few_more, n * (few_cut > 1 ? few_cut : 1));
   L.slots_few = few_cut > 1 ? least(2 * few_more, n * few_cut) : 0;
+  // tall: a share's beginning cuts one tile at most; k pieces of a tile are k - 1 cuts, and a cut tile has two pieces at least
   const int64_t tiles = tall ? T * L.group / TALL_ROWS + n : 0;
-  L.max_tall = tall ? least(tiles + tall_more, tiles * (tall_cut > 1 ? tall_cut : 1)) : 0;
-  L.slots_tall = tall && tall_cut > 1 ? least(2 * tall_more, tiles * tall_cut) : 0;
+  L.max_shares = least(TALL_PLACES / p.kv_heads > 0 ? TALL_PLACES / p.kv_heads : 1, tiles * ceil_div(p.max_kv_len + TALL_OVERHEAD, L.tall_least));
+  L.max_tall = tiles > 0 ? tiles + (p.max_kv_len >= L.tall_least ? L.max_shares : 0) : 0;
+  L.slots_tall = tiles > 0 && p.max_kv_len >= L.tall_least ? 2 * L.max_shares : 0;
   L.max_joins = L.slots_few / 2 + L.slots_tall / 2;
   L.off_few = AT_HDR;
   L.off_tall = L.off_few + L.max_few * AT_REC;
   L.off_joins = L.off_tall + L.max_tall * AT_REC;
   L.off_requests = L.off_joins + L.max_joins * AT_REC;
-  L.off_arrive = L.off_requests + (p.n_req + 1) * AT_REQ;
+  L.off_shares = L.off_requests + p.n_req * AT_REC;
+  L.off_arrive = L.off_shares + L.max_shares + 1;
   L.words = L.off_arrive + L.max_joins * p.kv_heads;
   return L;
 }
