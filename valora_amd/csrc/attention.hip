@@ -44,11 +44,11 @@ struct AttnArgs {
   float *lse;                          // null: not wanted
   float *weights;
   int64_t out_stride, q_stride, table_stride, weights_stride;
-  int64_t off_few, off_tall, off_joins, off_arrive, off_requests, off_shares;
   uint32_t k_stride, v_stride;         // bytes
   float c;                             // scale * log2(e)
   int tall_blocks;                     // workgroups of the tall list; those of the other follow
   int q_heads, kv_heads, group, page_shift, window, n_req, n_pages;
+  int off_few, off_tall, off_joins, off_arrive, off_requests, off_shares;      // of the plan, words
 };
 
 // The two 16-bit types as these kernels need them: the wide matrix product, the rounding of two values to one register, the sum of
@@ -105,6 +105,17 @@ __device__ __forceinline__ void to_lds16(const void *p, uint32_t base) {
 }
 __device__ __forceinline__ void to_lds4(const void *p, uint32_t base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(p) : "memory");
+}
+// The loads have arrived.  (Left to itself the compiler waits for them where they are first used, which is in the loop: every time round
+// it would wait for what the loop has just asked for.)
+template <typename V, int N>
+__device__ __forceinline__ void arrived(V (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    u32x4 v = as<u32x4>(x[i]);
+    asm volatile("" : "+v"(v));
+    x[i] = as<V>(v);
+  }
 }
 __device__ __forceinline__ uint32_t lds_offset(const void *p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
@@ -337,6 +348,7 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
   vec8 q[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 32 + kg * 8));
+  arrived(q);
 
   f32x4 o[DB];
 #pragma unroll
@@ -586,6 +598,7 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
   vec8 q[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 16 + half * 8));
+  arrived(q);
 
   f32x16 o[DB];
 #pragma unroll
@@ -718,35 +731,51 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
     if (odd && lane == 0) *again = 1;
     wait_lgkmcnt0();
     __syncthreads();                                            // (also: the buffers have been read by everyone)
-    if (*again) sweep(std::true_type{});
+    if (*again) {
+      sweep(std::true_type{});
+      __syncthreads();
+    }
   }
 
   if (!works) return;
   sm.l += __shfl_xor(sm.l, 32);
   if constexpr (SUMS) sm.sum += __shfl_xor(sm.sum, 32);
-  if (lrow >= wrows) return;
+  const int first = (int)uniform((uint32_t)(row0 + wrow));
   if (slot >= 0) {
-    const int64_t at = ((int64_t)slot * a.kv_heads + head) * TALL_ROWS + wrow + lrow;
+    if (lrow < wrows) {
+      const int64_t at = ((int64_t)slot * a.kv_heads + head) * TALL_ROWS + wrow + lrow;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4 *>(a.tall_o + at * D + db * 32 + i * 8 + half * 4) =
+              f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+      if (half == 0) a.tall_ml[at] = float4{sm.m, sm.l, sm.sum, 0.0f};
+    }
+  } else {
+    // A lane holds 16 bytes of columns here and there of one row: through LDS, which the wave has a part of to itself now, the
+    // rows go out whole.
+    const float inv = sm.l == 0.0f ? 0.0f : 1.0f / sm.l;
+    constexpr int STRIDE = L::ROW + 16;
+    static_assert(TALL_WAVES * 32 * STRIDE <= (int)F::TOTAL, "a part for each wave");
+    char *mine = lds + wave * 32 * STRIDE;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4 *>(a.tall_o + at * D + db * 32 + i * 8 + half * 4) =
-            f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
-    if (half == 0) a.tall_ml[at] = float4{sm.m, sm.l, sm.sum, 0.0f};
-    return;
-  }
-  const float inv = sm.l == 0.0f ? 0.0f : 1.0f / sm.l;
-  uint16_t *op = a.out + (int64_t)(tok0 + tok) * a.out_stride + hq * D;
+        *reinterpret_cast<uint2 *>(mine + lrow * STRIDE + (db * 32 + i * 8 + half * 4) * 2) =
+            uint2{Wide<T>::pack(o[db][4 * i] * inv, o[db][4 * i + 1] * inv), Wide<T>::pack(o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv)};
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint2 y{Wide<T>::pack(o[db][4 * i] * inv, o[db][4 * i + 1] * inv),
-                    Wide<T>::pack(o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv)};
-      *reinterpret_cast<uint2 *>(op + db * 32 + i * 8 + half * 4) = y;
+    for (int i = 0; i < L::P / 2; ++i) {
+      const int unit = i * 64 + lane, r = unit / L::P, piece = unit - r * L::P;
+      const int t = (first + r) / a.group, h = head * a.group + first + r - t * a.group;
+      if (r < wrows) store16(a.out + (int64_t)(tok0 + t) * a.out_stride + h * D + piece * 8, *reinterpret_cast<const u32x4 *>(mine + r * STRIDE + piece * 16));
     }
-  if (SUMS && half == 0) a.lse[(int64_t)(tok0 + tok) * a.q_heads + hq] = row_log(sm.m, sm.sum);
+    if (SUMS && half == 0 && lrow < wrows) {
+      const int t = (first + lrow) / a.group, h = head * a.group + first + lrow - t * a.group;
+      a.lse[(int64_t)(tok0 + t) * a.q_heads + h] = row_log(sm.m, sm.sum);
+    }
+  }
 }
 
 // ---- the launch: tall tiles first, which take longest ---------------------------------------------------------------------------------
@@ -988,12 +1017,12 @@ extern "C" int mlora_paged_attention(void *stream, const mlora_attention_plan *p
   a.few_ml = reinterpret_cast<float4 *>(ws + w.few_ml);
   a.tall_ml = reinterpret_cast<float4 *>(ws + w.tall_ml);
   a.lse = weights ? reinterpret_cast<float *>(ws + w.lse) : nullptr;
-  a.off_few = L.off_few;
-  a.off_tall = L.off_tall;
-  a.off_joins = L.off_joins;
-  a.off_arrive = L.off_arrive;
-  a.off_requests = L.off_requests;
-  a.off_shares = L.off_shares;
+  a.off_few = (int)L.off_few;
+  a.off_tall = (int)L.off_tall;
+  a.off_joins = (int)L.off_joins;
+  a.off_arrive = (int)L.off_arrive;
+  a.off_requests = (int)L.off_requests;
+  a.off_shares = (int)L.off_shares;
   a.weights = weights;
   a.out_stride = out_stride;
   a.q_stride = q_stride;
