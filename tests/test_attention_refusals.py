@@ -21,7 +21,8 @@ def test_plan_shapes():
     assert L.mlora_attention_plan_bytes(plan()) > 0 and L.mlora_attention_workspace_bytes(plan(), 0) > 0
     # a cache that no request can fill beyond one piece needs no room for pieces, with weights a logarithm a row
     assert L.mlora_attention_workspace_bytes(plan(max_kv_len=128), 0) == 0
-    assert L.mlora_attention_workspace_bytes(plan(max_kv_len=128), 1) == 8 * 8 * 4
+    assert L.mlora_attention_workspace_bytes(plan(max_kv_len=128), 1) == 8 * 8 * 4 + 3 * 16 * 2 * 128 * 4      # and scores
+    assert L.mlora_attention_workspace_bytes(plan(n_req=4096, n_tokens=4096, max_kv_len=100000), 1) <= (256 << 20) + (64 << 20)
     for kw, message in ((dict(q_heads=7), b"multiple of kv_heads"), (dict(kv_heads=0), b"kv_heads=0"), (dict(head_dim=100), b"head_dim=100"),
                         (dict(head_dim=512), b"head_dim=512"), (dict(page_size=12), b"page_size=12"), (dict(page_size=512), b"page_size=512"),
                         (dict(page_size=0), b"page_size=0"), (dict(n_req=-1), b"negative"), (dict(window=-1), b"negative"),

@@ -231,6 +231,32 @@ def test_weights(dev, dtype, hq, hkv, d, page, window):
     assert torch.allclose(alone.sum(1).cpu().double(), rows, rtol=1e-4, atol=1e-4)
 
 
+def test_weights_where_the_scores_have_no_room(dev):
+    """16 new tokens on 64 heads over 66000 cached ones: more scores than are kept, so K is read again."""
+    n, length, h, d = 16, 66000, 64, 32
+    g = torch.Generator(device=dev).manual_seed(21)
+    q = (torch.randn(n, h, d, device=dev, generator=g) * 2).to(BF16)
+    kb, vb = (torch.randn(length, h, d, device=dev, generator=g).to(BF16) for _ in range(2))
+    table = torch.randperm(length, device=dev, generator=g).to(torch.int32)[None]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    plan = AttentionPlan(i32([0]), i32([n]), i32([length]), n_tokens=n, max_seq_len=n, max_kv_len=length, q_heads=h, kv_heads=h, head_dim=d)
+    assert n * h * length > 1 << 26
+    out, w = torch.empty_like(q), torch.zeros(1, length, device=dev)
+    plan.attend(out, q, kb, vb, table, weights=w)
+    rows, j = table[0].long(), torch.arange(length, device=dev)
+    hidden = j[None] > torch.arange(length - n, length, device=dev)[:, None]
+    want, size = torch.zeros(length, dtype=torch.float64, device=dev), torch.zeros(length, dtype=torch.float64, device=dev)
+    for head in range(h):
+        K, Q = kb[rows, head].double(), q[:, head].double()
+        p = torch.softmax((Q @ K.T.contiguous() * d ** -0.5).masked_fill(hidden, -math.inf), -1)
+        rel = (2 * d + 8) * 2.0 ** -24 * float((Q.abs() @ K.abs().T.contiguous()).max()) * d ** -0.5 + 2.0 ** -20
+        want += p.sum(0)
+        size += p.sum(0) * (2 * rel + (length + 64) * 2.0 ** -24)
+        o = p @ vb[rows, head].double()
+        assert float((out[:, head].double() - o).abs().max()) <= 2.0 ** -8 * 2.5 * float((p @ vb[rows, head].double().abs()).max())
+    assert bool(((w[0].double() - want).abs() <= size + 2.0 ** -60).all())
+
+
 def test_the_same_call_gives_the_same_bits(dev):
     c = make(dev, BF16, 8, 2, 128, 1, MIXED + [(1, 6000)], seed=15)
     w = [torch.zeros(len(c["lens"]), c["table"].shape[1], device=dev) for _ in range(3)]

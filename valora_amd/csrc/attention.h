@@ -26,17 +26,19 @@ constexpr int TALL_OVERHEAD = 192;
 // join in the upper half
 // join:    {first slot, pieces, rows, first row, first new token in q, 1 in the tall list, 0, 0}
 // request: {blocks of WEIGHT_TOKENS cached tokens of the requests before, first new token in q, new tokens, cached tokens, tall tiles
-// of the requests before, 0, 0, 0}
+// of the requests before, where its scores begin (two words), its row length of them}
 // share:   its first record of the tall list
 // arrive:  pieces of a tile that have left their sums, zero between calls
 constexpr int AT_HDR = 32, AT_REC = 8;
-enum AttnHdr { AH_FEW = 0, AH_TALL = 1, AH_JOINS = 2, AH_BLOCKS = 3, AH_SHARES = 4 };
+enum AttnHdr { AH_FEW = 0, AH_TALL = 1, AH_JOINS = 2, AH_BLOCKS = 3, AH_SHARES = 4, AH_SCORES = 5 };
 constexpr int WEIGHT_TOKENS = 256;
+constexpr int64_t MAX_SCORES = 1 << 26;      // floats
 
 struct AttnLayout {
   int64_t group;
   int64_t max_few, max_tall, max_joins, max_shares;
   int64_t slots_few, slots_tall;
+  int64_t scores;                            // room for scores of requests of few rows, floats
   int64_t off_few, off_tall, off_joins, off_requests, off_shares, off_arrive, words;
   int few_items;                             // (piece, key head) pairs the list is cut for
   int few_least, tall_least;                 // spans up to these are not cut
@@ -46,9 +48,10 @@ AttnLayout attention_layout(const mlora_attention_plan &p);
 int check_attention_plan(const mlora_attention_plan *p, const char *who);
 
 // workspace: sums of the slots [slot][key head][rows][head_dim] floats, their references and
-// sums [slot][key head][rows][4], and with weights the logarithm of each row's sum [token][query head]
+// sums [slot][key head][rows][4]; with weights the logarithm of each row's sum [token][query head], and where all of them fit
+// (AH_SCORES) the scores of the requests of few rows [request][key head][row][token, from the first that any row sees on]
 struct AttnWorkspace {
-  int64_t few_o, tall_o, few_ml, tall_ml, lse, bytes;
+  int64_t few_o, tall_o, few_ml, tall_ml, lse, scores, bytes;
 };
 AttnWorkspace attention_workspace(const mlora_attention_plan &p, const AttnLayout &L, bool weights);
 

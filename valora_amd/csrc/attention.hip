@@ -42,6 +42,7 @@ struct AttnArgs {
   float *few_o, *tall_o;               // sums of the pieces (csrc/attention.h)
   float4 *few_ml, *tall_ml;            // {reference, sum of the rounded weights, sum of the weights, -}
   float *lse;                          // null: not wanted
+  float *scores;
   float *weights;
   int64_t out_stride, q_stride, table_stride, weights_stride;
   uint32_t k_stride, v_stride;         // bytes
@@ -343,6 +344,14 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
   const int row = row0 + min(lrow, rows - 1);
   const int tok = row / a.group, hq = head * a.group + row - tok * a.group;
   const int last = pos0 + tok, from = a.window > 0 ? last - a.window + 1 : 0;
+  // with weights: where the lane's scores go, token 0 of the cache at 0 (null: nowhere)
+  float *scores = nullptr;
+  if constexpr (SUMS) {
+    const int32_t *rq = a.plan + a.off_requests + (int64_t)req * AT_REC;
+    const int64_t its = (int64_t)((uint64_t)(uint32_t)rq[5] | (uint64_t)(uint32_t)rq[6] << 32);
+    const int first = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
+    if (a.plan[AH_SCORES] && lrow < rows) scores = a.scores + its + ((int64_t)head * rows + lrow) * rq[7] - first;
+  }
   const int sure_from = a.window > 0 ? pos0 + (row0 + rows - 1) / a.group - a.window + 1 : 0, sure_last = pos0 + row0 / a.group;
   const uint16_t *qp = a.q + (int64_t)(tok0 + tok) * a.q_stride + hq * D;
   vec8 q[CH];
@@ -417,8 +426,16 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
       sm.l = Wide<T>::add2(p[i], sm.l);
       if constexpr (SUMS) sm.sum += ex + ey;
     }
+    // (what is stored below is counted too, and only makes the waits stricter)
     if (more) wait_vmcnt<EACH + 1>();
     else wait_vmcnt<0>();
+    if constexpr (SUMS && !CAREFUL) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const int j = base + tt * 16 + kg * 4;
+        if (scores && j < c.end) *reinterpret_cast<f32x4 *>(scores + j) = s[tt];
+      }
+    }
     const int vtok = kg * 4 + (lrow >> 2);
     auto values = [&](int db) {
       const uint32_t at = L::v_at(vt + (lane & 1) * 8, vtok, (lane & 3) >> 1, 2 * db);
@@ -852,8 +869,10 @@ __global__ __launch_bounds__(THREADS) void attend_join_kernel(AttnArgs a) {
 
 // ---- weights: how much attention each cached token got ---------------------------------------------------------------------------
 //     weights[b][j] += sum over the call's rows of exp(scale q.k_j - log sum)
-// A wave owns 64 cached tokens and goes over all key heads and rows, so a weight is one thread's sum in a fixed order.  K is
-// read a second time (the sum of a row is not known before its last token).
+// The sum of a row is not known before its last token.  Decoding tiles therefore leave their scores, 4 bytes for the 512 of a token's
+// K and V that each query head of a group shares, and a thread sums those of a token.  (K read a second time: 64 requests of
+// 1000 to 4100 tokens, 8 key heads, 68 us of 194.)  For tall tiles, and where the scores have no room, a wave owns 64 cached
+// tokens and goes over all key heads and rows again.  A weight is one sum in a fixed order either way.
 constexpr int WEIGHT_WAVES = WEIGHT_TOKENS / 64;
 
 template <typename T, int D>
@@ -874,6 +893,23 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
     const int32_t *rq = requests + (int64_t)b * AT_REC;
     const int tok0 = rq[1], n = rq[2], kv = rq[3], pos0 = kv - n, rows = n * a.group;
     const int begin = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
+    if (rows <= FEW_ROWS && a.plan[AH_SCORES]) {
+      // the scores are there: a thread a token
+      const int j = begin + (item - rq[0]) * WEIGHT_TOKENS + (int)threadIdx.x;
+      if (j >= kv) continue;
+      const float *sc = a.scores + (int64_t)((uint64_t)(uint32_t)rq[5] | (uint64_t)(uint32_t)rq[6] << 32) + (j - begin);
+      const int stride = rq[7], n_rows = rows * a.kv_heads;
+      float x = 0.0f;
+#pragma unroll 8
+      for (int r = 0; r < n_rows; ++r) {
+        const int head = r / rows, row = r - head * rows, tok = row / a.group;
+        const float lse = a.lse[(int64_t)(tok0 + tok) * a.q_heads + head * a.group + row - tok * a.group];
+        const float e = exp2_(fmaf(sc[(int64_t)r * stride], a.c, -lse));
+        x += lse == -INFINITY ? 0.0f : e;
+      }
+      a.weights[(int64_t)b * a.weights_stride + j] += x;
+      continue;
+    }
     const int base = begin + (item - rq[0]) * WEIGHT_TOKENS + wave * 64;
     if (base >= kv) continue;
     // rows that see any of the tokens
@@ -1017,6 +1053,7 @@ extern "C" int mlora_paged_attention(void *stream, const mlora_attention_plan *p
   a.few_ml = reinterpret_cast<float4 *>(ws + w.few_ml);
   a.tall_ml = reinterpret_cast<float4 *>(ws + w.tall_ml);
   a.lse = weights ? reinterpret_cast<float *>(ws + w.lse) : nullptr;
+  a.scores = reinterpret_cast<float *>(ws + w.scores);
   a.off_few = (int)L.off_few;
   a.off_tall = (int)L.off_tall;
   a.off_joins = (int)L.off_joins;

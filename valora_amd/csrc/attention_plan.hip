@@ -97,22 +97,28 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
   for (int64_t i = tid; i < a.L.max_joins * a.kv_heads; i += AP_THREADS) a.plan[a.L.off_arrive + i] = 0;
 
   // ---- requests
-  int64_t few = 0, blocks_before = 0, tiles = 0;
+  int64_t few = 0, blocks_before = 0, tiles = 0, scores = 0;
   for (int b0 = 0; b0 < a.n_req; b0 += AP_THREADS) {
     const int b = b0 + tid;
     Request r{};
-    int begin = 0, end = 0, n_blocks = 0, n_tiles = 0;
+    int begin = 0, end = 0, n_blocks = 0, n_tiles = 0, row_scores = 0;
+    int64_t n_scores = 0;
     if (b < a.n_req) {
       r = request(a, b);
       if (r.rows > 0) {
         span(a, r, 0, r.rows, begin, end);
         n_blocks = (end - begin + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS;
         n_tiles = r.rows > FEW_ROWS ? (r.rows + TALL_ROWS - 1) / TALL_ROWS : 0;
-        if (n_tiles == 0) few += end - begin;
+        if (n_tiles == 0) {
+          few += end - begin;
+          row_scores = (end - begin + 63) / 64 * 64;
+          n_scores = (int64_t)r.rows * a.kv_heads * row_scores;
+        }
       }
     }
-    int64_t all;
+    int64_t all, all_scores;
     const int64_t before = block_before(n_blocks | (int64_t)n_tiles << 32, all, part);
+    const int64_t its_scores = scores + block_before(n_scores, all_scores, part);
     if (b < a.n_req) {
       int32_t *rq = requests + (int64_t)b * AT_REC;
       rq[0] = (int32_t)(blocks_before + (before & 0xffffffff));
@@ -120,9 +126,13 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
       rq[2] = r.n;
       rq[3] = r.kv;
       rq[4] = (int32_t)(tiles + (before >> 32));
+      rq[5] = (int32_t)its_scores;
+      rq[6] = (int32_t)(its_scores >> 32);
+      rq[7] = row_scores;
     }
     blocks_before += all & 0xffffffff;
     tiles += all >> 32;
+    scores += all_scores;
   }
   few = block_sum(few, part);
   int64_t records = 0, slots = 0, joins = 0;
@@ -277,6 +287,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
     a.plan[AH_JOINS] = (int)min<int64_t>(joins, a.L.max_joins);
     a.plan[AH_BLOCKS] = (int32_t)blocks_before;
     a.plan[AH_SHARES] = (int32_t)n_shares;
+    a.plan[AH_SCORES] = scores <= a.L.scores;
     shares[n_shares] = tall;
   }
 }
@@ -305,6 +316,8 @@ AttnLayout attention_layout(const mlora_attention_plan &p) {
   L.max_tall = tiles > 0 ? tiles + (p.max_kv_len >= L.tall_least ? L.max_shares : 0) : 0;
   L.slots_tall = tiles > 0 && p.max_kv_len >= L.tall_least ? 2 * L.max_shares : 0;
   L.max_joins = L.slots_few / 2 + L.slots_tall / 2;
+  const int64_t rows = least(FEW_ROWS, p.max_seq_len * L.group);
+  L.scores = least(MAX_SCORES, n * least(MAX_SCORES, rows * p.kv_heads * ceil_div(p.max_kv_len, 64) * 64));
   L.off_few = AT_HDR;
   L.off_tall = L.off_few + L.max_few * AT_REC;
   L.off_joins = L.off_tall + L.max_tall * AT_REC;
@@ -328,6 +341,7 @@ AttnWorkspace attention_workspace(const mlora_attention_plan &p, const AttnLayou
   w.few_ml = take(L.slots_few * p.kv_heads * FEW_ROWS * 16);
   w.tall_ml = take(L.slots_tall * p.kv_heads * TALL_ROWS * 16);
   w.lse = take(weights ? p.n_tokens * p.q_heads * 4 : 0);
+  w.scores = take(weights ? L.scores * 4 : 0);
   w.bytes = at;
   return w;
 }

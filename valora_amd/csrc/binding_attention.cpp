@@ -144,7 +144,7 @@ struct NativeRotary {
 // ---- attention -------------------------------------------------------------------------------------------------------------
 struct NativeAttentionPlan {
   mlora_attention_plan plan{};
-  at::Tensor start, seq, kv, buf, workspace;
+  at::Tensor start, seq, kv, buf, workspace, weights_workspace;
 
   NativeAttentionPlan(const at::Tensor &b_start_loc, const at::Tensor &b_seq_len, const at::Tensor &b_kv_len, int64_t n_tokens,
                       int64_t max_seq_len, int64_t max_kv_len, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
@@ -170,9 +170,9 @@ struct NativeAttentionPlan {
     plan.window = (int32_t)window;
     const size_t bytes = mlora_attention_plan_bytes(&plan);
     if (bytes == 0) check_rc(MLORA_ERR_INVALID);
-    // both stay where they are for as long as the plan lives: a graph captured from it keeps pointing at live memory
+    // they stay where they are for as long as the plan lives: a graph captured from it keeps pointing at live memory
     buf = at::empty({(int64_t)bytes}, start.options().dtype(at::kByte));
-    workspace = at::empty({(int64_t)mlora_attention_workspace_bytes(&plan, 1)}, start.options().dtype(at::kByte));
+    workspace = at::empty({(int64_t)mlora_attention_workspace_bytes(&plan, 0)}, start.options().dtype(at::kByte));
     plan.dev = buf.data_ptr();
     plan.bytes = bytes;
     rebuild();
@@ -222,11 +222,14 @@ struct NativeAttentionPlan {
       w_stride = plan.n_req > 1 ? weights->stride(0) : weights->size(1);
       if (w_stride < plan.max_kv_len) raise("weights: rows overlap");
     }
+    if (w && !weights_workspace.defined())      // (up to 256 MB, for those who ask for weights)
+      weights_workspace = at::empty({(int64_t)mlora_attention_workspace_bytes(&plan, 1)}, start.options().dtype(at::kByte));
+    const at::Tensor room = w ? weights_workspace : workspace;
     const float s = scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)plan.head_dim);
     const c10::DeviceGuard on(dev);
     const hipStream_t st = stream_of(dev);
     check_unlocked([&] {
-      return mlora_paged_attention(st, &plan, workspace.data_ptr(), (size_t)workspace.numel(), ho.data, ho.row_stride, hq.data, hq.row_stride,
+      return mlora_paged_attention(st, &plan, room.data_ptr(), (size_t)room.numel(), ho.data, ho.row_stride, hq.data, hq.row_stride,
                                    hk.data, hk.row_stride, hv.data, hv.row_stride, hk.rows, static_cast<const int32_t *>(table.data_ptr()),
                                    plan.n_req > 1 ? table.stride(0) : table.size(1), table.size(1), s, w, w_stride, code);
     });
