@@ -424,7 +424,7 @@ int mlora_rotary(void *stream, const mlora_rotary_part *parts, int32_t n_parts, 
  * of q and out, and the last b_seq_len[b] of its b_kv_len[b] cached tokens: token i sees the cache indices up to its own,
  * b_kv_len[b] - b_seq_len[b] + i, and of those the last `window` only where window > 0.  Requests without new tokens, and
  * those whose rows lie outside [0, n_tokens) or are more than max_seq_len, are left out; a b_kv_len above max_kv_len counts
- * as max_kv_len, one below 0 as 0.  The caller fills everything but the buffer's contents.       */
+ * as max_kv_len, one below 0 as 0.  Requests' rows must not overlap.  The caller fills everything but the buffer's contents. */
 typedef struct {
   void *dev;                /* mlora_attention_plan_bytes() bytes, 16-byte aligned                     */
   size_t bytes;
@@ -438,7 +438,8 @@ typedef struct {
   int32_t window;           /* 0: no bound                                                             */
 } mlora_attention_plan;
 size_t mlora_attention_plan_bytes(const mlora_attention_plan *plan);
-/* Bytes of workspace a call needs, 256-byte aligned; calls that share it must not overlap in time.   */
+/* Bytes of workspace a call needs, 256-byte aligned; with weights up to 256 MB more.  Calls that share a workspace or a plan
+ * must not overlap in time.                                                                      */
 size_t mlora_attention_workspace_bytes(const mlora_attention_plan *plan, int32_t weights);
 /* Cuts the batch's work on the device, in one launch (b_start_loc, b_seq_len, b_kv_len: device int32 [n_req]).  Once for
  * the layers of a forward pass; again, in place, when the lengths have changed.                  */

@@ -26,7 +26,8 @@ def test_plan_shapes():
     for kw, message in ((dict(q_heads=7), b"multiple of kv_heads"), (dict(kv_heads=0), b"kv_heads=0"), (dict(head_dim=100), b"head_dim=100"),
                         (dict(head_dim=512), b"head_dim=512"), (dict(page_size=12), b"page_size=12"), (dict(page_size=512), b"page_size=512"),
                         (dict(page_size=0), b"page_size=0"), (dict(n_req=-1), b"negative"), (dict(window=-1), b"negative"),
-                        (dict(max_kv_len=1 << 31), b"too large"), (dict(n_tokens=1 << 40), b"too large")):
+                        (dict(max_kv_len=1 << 31), b"too large"), (dict(n_tokens=1 << 40), b"too large"),
+                        (dict(n_req=1 << 20, max_kv_len=1 << 30), b"too large")):
         assert L.mlora_attention_plan_bytes(plan(**kw)) == 0 and message in L.mlora_last_error(), kw
         assert L.mlora_attention_workspace_bytes(plan(**kw), 1) == 0
         assert L.mlora_build_attention_plan(None, plan(**kw), None, None, None) < 0

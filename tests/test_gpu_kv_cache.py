@@ -108,6 +108,8 @@ def test_prompts_decoding_eviction_and_release(dev, dtype, hq, hkv, d):
     cache.release(1)
     dense.pop(1), seen.pop(1)
     step([3, 1], [20, 5])                                # rows and slot are used again
+    empty = cache.step([], [])                           # a pass without tokens
+    assert empty.attention(0)(*(torch.empty(0, h * d, dtype=dtype, device=dev) for h in (hq, hkv, hkv))).shape == (0, hq * d)
     cache.release(0), cache.release(1), cache.release(2), cache.release(3)
     assert mem.can_use_mem_size == free and int(mem.mem_state.sum()) == free and not cache.weights.any()
 

@@ -114,6 +114,23 @@ def test_store(dev, dtype, hq, hkv, d, rotary_dim, interleaved, T):
     assert torch.equal(qd, out) and torch.equal(fd[:, hq * d:].cpu(), fused[:, hq * d:])
 
 
+def test_slices_that_begin_anywhere(dev):
+    """Rows and heads that are not multiples of 16 bytes apart, or begin in between."""
+    g = torch.Generator().manual_seed(9)
+    wide = torch.randn(50, 3, 131, generator=g).to(F16)
+    positions = torch.randint(0, 3000, (50,), generator=g)
+    rot = Rotary(64, device=dev)
+    for at in (0, 1, 2, 8, 67):
+        wd = wide.to(dev)
+        x = wd[:, :, at:at + 64]
+        rot.apply(positions.to(dev), x)
+        torch.cuda.synchronize()
+        check(x, *turned(wide[:, :, at:at + 64], positions, *frequencies(64), 64, False))
+        rest = torch.ones(131, dtype=torch.bool)
+        rest[at:at + 64] = False
+        assert torch.equal(wd.cpu()[:, :, rest], wide[:, :, rest])
+
+
 def test_values_that_are_not_finite_stay_in_their_pair(dev):
     q = torch.ones(4, 1, 64, dtype=F16)
     q[0, 0, 3], q[1, 0, 40], q[2, 0, 60] = math.nan, math.inf, -math.inf

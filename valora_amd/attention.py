@@ -22,12 +22,13 @@ class AttentionPlan:
     so a fixed set of slots can serve a changing batch).  New token i sees the cached tokens up to itself, and with
     ``window > 0`` the last ``window`` of those only.  ``max_seq_len`` and ``max_kv_len`` bound the lengths on the host:
     grids, table and workspace go by them, the work itself by the lengths on the device.  A request with more new tokens than
-    ``max_seq_len`` is left out; cached tokens beyond ``max_kv_len`` do not count.
+    ``max_seq_len`` is left out; cached tokens beyond ``max_kv_len`` do not count.  Requests' rows must not overlap.
 
     Query head h reads key head ``h // (q_heads // kv_heads)``.  ``head_dim`` is 32, 64, 96, 128 or 256; ``page_size`` a power of two
     up to 256 (1: the table names pool rows, as ``MemoryAllocator.alloc`` hands them out).
 
-    Calls that share a plan must not overlap in time (they share its workspace): one plan per stream.
+    Calls that share a plan must not overlap in time (they share its workspace): one plan per stream.  The first call with
+    ``weights`` takes a workspace of its own, up to 256 MB larger.
     """
 
     def __init__(self, b_start_loc: torch.Tensor, b_seq_len: torch.Tensor, b_kv_len: torch.Tensor, n_tokens: int, max_seq_len: int,

@@ -362,6 +362,8 @@ int check_attention_plan(const mlora_attention_plan *p, const char *who) {
       p->max_seq_len > (1 << 30))
     return fail(MLORA_ERR_NO_KERNEL, "%s: n_req=%lld n_tokens=%lld max_kv_len=%lld too large", who, (long long)p->n_req,
                 (long long)p->n_tokens, (long long)p->max_kv_len);
+  if (p->n_req * ((p->max_kv_len + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS) > 0x7fffffff)
+    return fail(MLORA_ERR_NO_KERNEL, "%s: n_req=%lld times max_kv_len=%lld too large", who, (long long)p->n_req, (long long)p->max_kv_len);
   if (attention_layout(*p).words > 0x7fffffff) return fail(MLORA_ERR_NO_KERNEL, "%s: the plan would have more than 2^31 - 1 words", who);
   return MLORA_OK;
 }
