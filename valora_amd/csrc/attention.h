@@ -19,24 +19,26 @@ constexpr int FEW_ROWS = 16, TALL_ROWS = 128;
 constexpr int AT_PIECE_STEP = 64;            // a piece's length is a multiple of this
 constexpr int TALL_OVERHEAD = 192;
 
-// plan buffer (int32 words): hdr[32] | few[max_few][8] | tall[max_tall][8] | joins[max_joins][8] | requests[n_req][8]
-// | shares[max_shares + 1] | arrive[max_joins][kv_heads]
+// plan buffer (int32 words): hdr[32] | few[max_few][8] | tall[max_tall][8] | joins[few_joins + tall_joins][8] | requests[n_req][8]
+// | shares[max_shares + 1] | arrive[few_joins][kv_heads]
 // record:  {request, first row, rows, begin, end, slot (-1: the tile's only piece), first new token in q, position of the
 // request's new token 0}; the piece covers cache indices [begin, end); rows of the few-rows list hold the index of the tile's
 // join in the upper half
-// join:    {first slot, pieces, rows, first row, first new token in q, 1 in the tall list, 0, 0}
+// join:    {first slot, pieces, rows, first row, first new token in q, 0, 0, 0}; those of the few-rows list first, those of the tall
+// list from few_joins on
 // request: {blocks of WEIGHT_TOKENS cached tokens of the requests before, first new token in q, new tokens, cached tokens, tall tiles
 // of the requests before, where its scores begin (two words), its row length of them}
 // share:   its first record of the tall list
 // arrive:  pieces of a tile that have left their sums, zero between calls
 constexpr int AT_HDR = 32, AT_REC = 8;
-enum AttnHdr { AH_FEW = 0, AH_TALL = 1, AH_JOINS = 2, AH_BLOCKS = 3, AH_SHARES = 4, AH_SCORES = 5 };
+enum AttnHdr { AH_FEW = 0, AH_TALL = 1, AH_TALL_JOINS = 2, AH_BLOCKS = 3, AH_SHARES = 4, AH_SCORES = 5 };
 constexpr int WEIGHT_TOKENS = 256;
 constexpr int64_t MAX_SCORES = 1 << 26;      // floats
 
 struct AttnLayout {
   int64_t group;
-  int64_t max_few, max_tall, max_joins, max_shares;
+  int64_t max_few, max_tall, max_shares;
+  int64_t few_joins, tall_joins;             // room for joins of either list
   int64_t slots_few, slots_tall;
   int64_t scores;                            // room for scores of requests of few rows, floats
   int64_t off_few, off_tall, off_joins, off_requests, off_shares, off_arrive, words;

@@ -49,7 +49,7 @@ struct AttnArgs {
   float c;                             // scale * log2(e)
   int tall_blocks;                     // workgroups of the tall list; those of the other follow
   int q_heads, kv_heads, group, page_shift, window, n_req, n_pages;
-  int off_few, off_tall, off_joins, off_arrive, off_requests, off_shares;      // of the plan, words
+  int off_few, off_tall, off_joins, off_tall_joins, off_arrive, off_requests, off_shares;      // of the plan, words
 };
 
 // The two 16-bit types as these kernels need them: the wide matrix product, the rounding of two values to one register, the sum of
@@ -848,10 +848,10 @@ template <typename T, int D>
 __global__ __launch_bounds__(THREADS) void attend_join_kernel(AttnArgs a) {
   constexpr int COLS = D / 4, SLOTS = THREADS / COLS;
   const int join_i = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x - (unsigned)join_i * a.kv_heads);
-  if (join_i >= a.plan[AH_JOINS]) return;
-  const int32_t *join = a.plan + a.off_joins + (int64_t)join_i * AT_REC;
+  if (join_i >= a.plan[AH_TALL_JOINS]) return;
+  const int32_t *join = a.plan + a.off_tall_joins + (int64_t)join_i * AT_REC;
   const int slot0 = join[0], pieces = join[1], rows = join[2], row0 = join[3], tok0 = join[4];
-  if (!join[5] || pieces <= 0) return;
+  if (pieces <= 0) return;
   const int ty = threadIdx.x / COLS, d = (threadIdx.x - ty * COLS) * 4;
   if (ty >= SLOTS) return;
   const int64_t step = (int64_t)a.kv_heads * TALL_ROWS;
@@ -973,8 +973,8 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
 template <typename T, int D>
 int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, const AttnArgs &a) {
   if (int rc = a.lse ? launch_lists<T, D, true>(st, L, a) : launch_lists<T, D, false>(st, L, a)) return rc;
-  if (L.slots_tall > 0) {
-    hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3((unsigned)(L.max_joins * a.kv_heads), TALL_ROWS / JOIN_ROWS), dim3(THREADS), 0, st, a);
+  if (L.tall_joins > 0) {
+    hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3((unsigned)(L.tall_joins * a.kv_heads), TALL_ROWS / JOIN_ROWS), dim3(THREADS), 0, st, a);
     if (int rc = check_launch("attend_join_kernel")) return rc;
   }
   if (a.weights && p.max_kv_len > 0) {
@@ -1057,6 +1057,7 @@ extern "C" int mlora_paged_attention(void *stream, const mlora_attention_plan *p
   a.off_few = (int)L.off_few;
   a.off_tall = (int)L.off_tall;
   a.off_joins = (int)L.off_joins;
+  a.off_tall_joins = (int)(L.off_joins + L.few_joins * AT_REC);
   a.off_arrive = (int)L.off_arrive;
   a.off_requests = (int)L.off_requests;
   a.off_shares = (int)L.off_shares;

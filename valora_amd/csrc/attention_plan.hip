@@ -94,7 +94,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
   __shared__ int64_t part[AP_WAVES];
   const int tid = threadIdx.x;
   int32_t *requests = a.plan + a.L.off_requests, *shares = a.plan + a.L.off_shares;
-  for (int64_t i = tid; i < a.L.max_joins * a.kv_heads; i += AP_THREADS) a.plan[a.L.off_arrive + i] = 0;
+  for (int64_t i = tid; i < a.L.few_joins * a.kv_heads; i += AP_THREADS) a.plan[a.L.off_arrive + i] = 0;
 
   // ---- requests
   int64_t few = 0, blocks_before = 0, tiles = 0, scores = 0;
@@ -137,16 +137,15 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
   few = block_sum(few, part);
   int64_t records = 0, slots = 0, joins = 0;
 
-  auto emit_join = [&](int64_t at, int64_t slot0, int pieces, int rows, int row0, int start, bool tall) {
-    if (at >= a.L.max_joins) return;
-    int32_t *j = a.plan + a.L.off_joins + at * AT_REC;
+  auto emit_join = [&](int64_t at, int64_t first, int64_t max, int64_t slot0, int pieces, int rows, int row0, int start) {
+    if (at >= max) return;
+    int32_t *j = a.plan + a.L.off_joins + (first + at) * AT_REC;
     j[0] = (int32_t)slot0;
     j[1] = pieces;
     j[2] = rows;
     j[3] = row0;
     j[4] = start;
-    j[5] = tall;
-    j[6] = j[7] = 0;
+    j[5] = j[6] = j[7] = 0;
   };
   auto emit = [&](int32_t *list, int64_t at, int64_t max, int b, int row0, int rows, int begin, int end, int64_t slot, const Request &r) {
     if (at >= max) return;
@@ -179,11 +178,11 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
     const int64_t before = block_before(k > 0 ? pack(k, k > 1 ? k : 0, k > 1) : 0, all, part);
     const int64_t rec = records + (before & PACKED), slot = slots + (before >> 21 & PACKED), join = joins + (before >> 42);
     // (requests that overlap in q could ask for more than the lists hold: what is beyond is left out)
-    const bool fits = rec + k <= a.L.max_few && (k < 2 || (slot + k <= a.L.slots_few && join < a.L.max_joins));
+    const bool fits = rec + k <= a.L.max_few && (k < 2 || (slot + k <= a.L.slots_few && join < a.L.few_joins));
     for (int i = 0; i < k; ++i)
       emit(a.plan + a.L.off_few, rec + i, a.L.max_few, b, 0, !fits ? 0 : k > 1 ? r.rows | (int)join << 16 : r.rows, begin + (k > 1 ? i * piece : 0),
            k > 1 ? min(begin + (i + 1) * piece, end) : end, k > 1 ? slot + i : -1, r);
-    if (k > 1) emit_join(join, slot, fits ? k : 0, r.rows, 0, r.start, false);
+    if (k > 1) emit_join(join, 0, a.L.few_joins, slot, fits ? k : 0, r.rows, 0, r.start);
     records += all & PACKED;
     slots += all >> 21 & PACKED;
     joins += all >> 42;
@@ -223,7 +222,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
   n_shares = n_shares < a.L.max_shares ? n_shares : a.L.max_shares;
   const int64_t share = n_shares > 0 ? (line + n_shares - 1) / n_shares : 1;
   n_shares = (line + share - 1) / share;      // (one that begins behind the line is none)
-  records = slots = 0;
+  records = slots = joins = 0;
   int64_t at = 0;                        // where on the line the round's first tile begins
   for (int64_t t0 = 0; t0 < tiles; t0 += AP_THREADS) {
     const int64_t t = t0 + tid;
@@ -262,7 +261,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
     const int64_t before = block_before(k > 0 ? pack(k, k > 1 ? k : 0, k > 1) : 0, all, part);
     const int64_t rec = records + (before & PACKED), slot = slots + (before >> 21 & PACKED), join = joins + (before >> 42);
     if (t < tiles) {
-      const bool fits = rec + k <= a.L.max_tall && (k < 2 || (slot + k <= a.L.slots_tall && join < a.L.max_joins));
+      const bool fits = rec + k <= a.L.max_tall && (k < 2 || (slot + k <= a.L.slots_tall && join < a.L.tall_joins));
       const int len = p.end - p.begin;
       int last = 0, i = 0;
       cuts([&](int64_t j, int cut) {
@@ -275,7 +274,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
         if (j < n_shares) shares[j] = (int32_t)(rec + (cut >= len && len > 0 ? k : i));
       });
       emit(a.plan + a.L.off_tall, rec + i, a.L.max_tall, p.b, p.row0, fits ? p.rows : 0, p.begin + last, p.end, k > 1 ? slot + i : -1, p.r);
-      if (k > 1) emit_join(join, slot, fits ? k : 0, p.rows, p.row0, p.r.start, true);
+      if (k > 1) emit_join(join, a.L.few_joins, a.L.tall_joins, slot, fits ? k : 0, p.rows, p.row0, p.r.start);
     }
     records += all & PACKED;
     slots += all >> 21 & PACKED;
@@ -284,7 +283,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
   if (tid == 0) {
     const int32_t tall = (int32_t)min<int64_t>(records, a.L.max_tall);
     a.plan[AH_TALL] = tall;
-    a.plan[AH_JOINS] = (int)min<int64_t>(joins, a.L.max_joins);
+    a.plan[AH_TALL_JOINS] = (int)min<int64_t>(joins, a.L.tall_joins);
     a.plan[AH_BLOCKS] = (int32_t)blocks_before;
     a.plan[AH_SHARES] = (int32_t)n_shares;
     a.plan[AH_SCORES] = scores <= a.L.scores;
@@ -315,16 +314,17 @@ AttnLayout attention_layout(const mlora_attention_plan &p) {
   L.max_shares = least(TALL_PLACES / p.kv_heads > 0 ? TALL_PLACES / p.kv_heads : 1, tiles * ceil_div(p.max_kv_len + TALL_OVERHEAD, L.tall_least));
   L.max_tall = tiles > 0 ? tiles + (p.max_kv_len >= L.tall_least ? L.max_shares : 0) : 0;
   L.slots_tall = tiles > 0 && p.max_kv_len >= L.tall_least ? 2 * L.max_shares : 0;
-  L.max_joins = L.slots_few / 2 + L.slots_tall / 2;
+  L.few_joins = L.slots_few / 2;
+  L.tall_joins = L.slots_tall / 2;
   const int64_t rows = least(FEW_ROWS, p.max_seq_len * L.group);
   L.scores = least(MAX_SCORES, n * least(MAX_SCORES, rows * p.kv_heads * ceil_div(p.max_kv_len, 64) * 64));
   L.off_few = AT_HDR;
   L.off_tall = L.off_few + L.max_few * AT_REC;
   L.off_joins = L.off_tall + L.max_tall * AT_REC;
-  L.off_requests = L.off_joins + L.max_joins * AT_REC;
+  L.off_requests = L.off_joins + (L.few_joins + L.tall_joins) * AT_REC;
   L.off_shares = L.off_requests + p.n_req * AT_REC;
   L.off_arrive = L.off_shares + L.max_shares + 1;
-  L.words = L.off_arrive + L.max_joins * p.kv_heads;
+  L.words = L.off_arrive + L.few_joins * p.kv_heads;
   return L;
 }
 
