@@ -130,7 +130,7 @@ __device__ __forceinline__ s16x4 lds_turned(uint32_t at) {
 }
 
 // ---- a tile in LDS: rows of D elements, 16-byte pieces of a row exchanged so that what is read together lies in different banks --
-// K is read 16 bytes of 16 or 32 rows at a time, V 32 bytes of 8 rows.
+// K is read 16 bytes of 16 or 32 rows at a time, V 64 bytes of 4 rows (tall tiles) or 32 bytes of 8.
 template <int D>
 struct Tile {
   static constexpr int P = D / 8, ROW = D * 2;
@@ -138,7 +138,7 @@ struct Tile {
     return D >= 128 ? t & 15 : D == 64 ? (t >> 1) & 7 : D == 32 ? (t >> 2) & 3 : (t >> 2) & 3;
   }
   static __device__ __forceinline__ int v_turn(int t) {
-    return D >= 128 ? (t & 7) << 1 : D == 64 ? ((t >> 1) & 3) << 1 : ((t >> 2) & 1) << 1;
+    return D >= 128 ? (t & 3) << 2 | (t & 4) >> 1 : D == 64 ? (t & 2) << 1 | (t & 4) >> 1 : (t & 4) >> 1;
   }
   // 12 pieces (D = 96) are no power of two: they are rotated, where the others are exchanged
   static __device__ __forceinline__ int place(int piece, int turn) {
@@ -238,19 +238,20 @@ struct Softmax {
 __device__ __forceinline__ float row_log(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
 
 // ---- V that is not finite -----------------------------------------------------------------------------------------------------
-// A token that a row does not see has weight 0, and 0 times an infinity is not 0.  Tiles that hold tokens some row does not see are
-// therefore looked through, and where one holds a value that is not finite the tile's rows are done again the careful way
-// (a loop of its own, which costs the common one no registers): the product runs over the finite values alone, and a second one
-// counts for each row and column the others that the row does see: +infinity as 1, -infinity as 128, not a number as 16384
+// A token that a row does not see has weight 0, and 0 times an infinity is not 0 but no number, which then stays in the row's sums
+// whatever they are scaled by.  Rows whose sums are not finite at the end of a piece are therefore done again the careful way (a loop of
+// its own, which costs the common one no registers and no look at V): the product runs over the finite values alone, and a second
+// one counts for each row and column the others that the row does see: +infinity as 1, -infinity as 128, not a number as 16384
 // (at most 64 tokens a sum).
-// Bits 15 and 31 of `finite` stay set while the values are finite: 0x7fff added to what an exponent lacks of all ones carries
-template <typename T>
-__device__ __forceinline__ void check_finite(u32x4 v, uint32_t &finite) {
-  constexpr uint32_t E = Wide<T>::EXPONENT, E2 = E << 16 | E;
+template <typename V, int N, int W = sizeof(V) / 4>
+__device__ __forceinline__ bool any_not_finite(const V (&x)[N]) {
+  float zero = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) finite &= (~v[i] & E2) + 0x7fff7fffu;
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) zero = fmaf(x[i][j], 0.0f, zero);
+  return __any(zero != 0.0f);
 }
-__device__ __forceinline__ bool all_finite(uint32_t finite) { return !__any((finite & 0x80008000u) != 0x80008000u); }
 template <typename T>
 __device__ __forceinline__ void split_not_finite(u32x4 &v, u32x4 &code) {
   constexpr uint32_t E = Wide<T>::EXPONENT;
@@ -364,7 +365,6 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
   for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};        // (a wave may have no tile)
   Softmax<T> sm;
 
-  bool odd = false;                                             // a value that is not finite where some row does not see
   constexpr int EACH = FEW_TOKENS * L::P / 64;                  // loads of a tile of K, as of V
   uint32_t rows_of[EACH];                                       // pool rows of the tile whose K was asked for last
   auto load_k = [&](int k) {
@@ -443,13 +443,6 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
       return as<u32x4>(v);
     };
     if constexpr (!CAREFUL) {
-      if (masked) {
-        uint32_t finite = ~0u;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) check_finite<T>(values(db), finite);
-        odd = odd || !all_finite(finite);
-        requested();      // (the values are read again below: to keep them would take registers)
-      }
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = Traits<T>::mfma(as<vec8>(values(db)), as<vec8>(p), o[db]);
     } else {
@@ -481,8 +474,10 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     load_v();
     for (int k = 0; k < mine; ++k) step(careful, k);
   };
-  if (mine > 0) sweep(std::false_type{});
-  if (odd) sweep(std::true_type{});
+  if (mine > 0) {
+    sweep(std::false_type{});
+    if (any_not_finite(o)) sweep(std::true_type{});
+  }
 
   // ---- the waves' sums
   sm.l += __shfl_xor(sm.l, 16);
@@ -588,7 +583,7 @@ template <typename T, int D, bool SUMS>
 __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_i, int head) {
   using F = Tall<D>;
   using L = Tile<D>;
-  constexpr int CH = D / 16, DB = D / 32, TOKENS = F::TOKENS, BL = TOKENS / 32;
+  constexpr int CH = D / 16, DB = D / 32, TOKENS = F::TOKENS, BL = TOKENS / 32, AHEAD = 4;
   using vec8 = typename Traits<T>::vec8;
   int *again = reinterpret_cast<int *>(lds + F::TOTAL);         // the tile's rows are done again the careful way
   const Record rec(a.plan, a.off_tall, rec_i);
@@ -622,17 +617,24 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
   for (int i = 0; i < DB; ++i) o[i] = f32x16{};                 // (there may be no tile)
   Softmax<T> sm;
 
-  bool odd = false;                                             // a value that is not finite where some row does not see
   auto compute = [&](auto careful, int k, uint64_t bad) {
     constexpr bool CAREFUL = decltype(careful)::value;
     const int base = base_of(k);
     const uint32_t kt = mem + (k & 1) * F::BUFFER, vt = kt + F::TILE;
+    // Both products read LDS AHEAD steps before the matrix instruction that takes it, in an order of their own: left to itself the
+    // compiler reads right before it, and waits.
+    vec8 ks[AHEAD];
+    auto key = [&](int n) { return as<vec8>(lds16(L::k_at(kt, lrow, half, n / BL * 2) + n % BL * 32 * L::ROW)); };
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) ks[n] = key(n);
     f32x16 s[BL];
 #pragma unroll
-    for (int b = 0; b < BL; ++b) {
-      s[b] = f32x16{};
+    for (int b = 0; b < BL; ++b) s[b] = f32x16{};
 #pragma unroll
-      for (int i = 0; i < CH; ++i) s[b] = Wide<T>::mfma(as<vec8>(lds16(L::k_at(kt, lrow, half, i * 2) + b * 32 * L::ROW)), q[i], s[b]);
+    for (int n = 0; n < BL * CH; ++n) {
+      s[n % BL] = Wide<T>::mfma(ks[n % AHEAD], q[n / BL], s[n % BL]);
+      if (n + AHEAD < BL * CH) ks[n % AHEAD] = key(n + AHEAD);
+      one_by_one();
     }
     // tokens 16 g + 4 half .. + 3 and 8 further, of the lane's column of 32 from 32 db on
     const int vtok = half * 4 + ((lane & 15) >> 2);
@@ -651,21 +653,6 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[b][i] = unless(s[b][i], bit(seen[b], (i >> 2) * 8 + (i & 3)));
       }
-      if constexpr (!CAREFUL) {
-        uint32_t finite = ~0u;
-#pragma unroll
-        for (int g = 0; g < 2 * BL; ++g) {
-#pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            check_finite<T>(values(g, db), finite);
-            if (db % 4 == 3 || db == DB - 1) {     // (the values are read again below: to keep them would take the registers of the whole tile)
-              here(finite);
-              one_by_one();
-            }
-          }
-        }
-        odd = odd || !all_finite(finite);
-      }
     }
     float hi = s[0][0];
 #pragma unroll
@@ -677,22 +664,36 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
       for (int i = 0; i < DB; ++i) o[i] *= alpha;
     }
     u32x4 p[2 * BL];
-#pragma unroll
-    for (int g = 0; g < 2 * BL; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = s[g >> 1][(g & 1) * 8 + 2 * i], y = s[g >> 1][(g & 1) * 8 + 2 * i + 1];
-        const float ex = exp2_(fmaf(x, a.c, sm.minus)), ey = exp2_(fmaf(y, a.c, sm.minus));
-        p[g][i] = Wide<T>::pack(ex, ey);
-        sm.l = Wide<T>::add2(p[g][i], sm.l);
-        if constexpr (SUMS) sm.sum += ex + ey;
-      }
+    auto weigh = [&](int g, int i) {
+      const float x = s[g >> 1][(g & 1) * 8 + 2 * i], y = s[g >> 1][(g & 1) * 8 + 2 * i + 1];
+      const float ex = exp2_(fmaf(x, a.c, sm.minus)), ey = exp2_(fmaf(y, a.c, sm.minus));
+      p[g][i] = Wide<T>::pack(ex, ey);
+      sm.l = Wide<T>::add2(p[g][i], sm.l);
+      if constexpr (SUMS) sm.sum += ex + ey;
+    };
     if constexpr (!CAREFUL) {
+      // between the matrix instructions of a group of 16 tokens the weights of the next
+      u32x4 vs[AHEAD];
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) vs[n] = values(n / DB, n % DB);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) weigh(0, i);
+      one_by_one();
+#pragma unroll
+      for (int n = 0; n < 2 * BL * DB; ++n) {
+        const int g = n / DB, db = n % DB;
+        o[db] = Wide<T>::mfma(as<vec8>(vs[n % AHEAD]), as<vec8>(p[g]), o[db]);
+        if (n + AHEAD < 2 * BL * DB) vs[n % AHEAD] = values((n + AHEAD) / DB, (n + AHEAD) % DB);
+        if (g + 1 < 2 * BL)
+#pragma unroll
+          for (int i = db * 4 / DB; i < (db + 1) * 4 / DB; ++i) weigh(g + 1, i);
+        one_by_one();
+      }
+    } else {
 #pragma unroll
       for (int g = 0; g < 2 * BL; ++g)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = Wide<T>::mfma(as<vec8>(values(g, db)), as<vec8>(p[g]), o[db]);
-    } else {
+        for (int i = 0; i < 4; ++i) weigh(g, i);
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
         f32x16 n{};
@@ -745,7 +746,7 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
   if (tiles > 0) {
     if (threadIdx.x == 0) *again = 0;
     sweep(std::false_type{});
-    if (odd && lane == 0) *again = 1;
+    if (any_not_finite(o) && lane == 0) *again = 1;
     wait_lgkmcnt0();
     __syncthreads();                                            // (also: the buffers have been read by everyone)
     if (*again) {
