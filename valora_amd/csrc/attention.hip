@@ -188,10 +188,9 @@ __device__ __forceinline__ void load_pages(const Cache &c, int base, uint32_t sl
 
 __device__ __forceinline__ bool bad_page(const Cache &c, int32_t page) { return (uint32_t)page >= (uint32_t)c.n_pages; }
 
-// Pool row of token base + t, whose page number is in the slice; row 0 where the page is none of the pool
-__device__ __forceinline__ uint32_t row_of(const Cache &c, int base, int t, uint32_t slice) {
-  const int32_t page = lds_word(slice + t * 4);
-  const int tok = min(base + t, c.end - 1);
+// Pool row of token `at`, whose page number is given; row 0 where the page is none of the pool
+__device__ __forceinline__ uint32_t row_of(const Cache &c, int at, int32_t page) {
+  const int tok = min(at, c.end - 1);
   return bad_page(c, page) ? 0 : ((uint32_t)page << c.shift) + (tok & ((1 << c.shift) - 1));
 }
 
@@ -201,11 +200,14 @@ __device__ __forceinline__ void load_tile(const Cache &c, int base, uint32_t sli
   using L = Tile<D>;
   constexpr int EACH = N * L::P / 64 / WAVES;
   static_assert(EACH * 64 * WAVES == N * L::P, "whole loads");
+  int32_t pages[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) pages[i] = lds_word(slice + ((i * WAVES + wave) * 64 + lane) / L::P * 4);
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int first = (i * WAVES + wave) * 64, unit = first + lane;
     const int t = unit / L::P, place = unit - t * L::P;
-    const uint64_t row = row_of(c, base, t, slice);
+    const uint64_t row = row_of(c, base + t, pages[i]);
     to_lds16(c.k + row * c.k_stride + L::piece(place, L::k_turn(t)) * 16, uniform(kt + first * 16));
     to_lds16(c.v + row * c.v_stride + L::piece(place, L::v_turn(t)) * 16, uniform(vt + first * 16));
   }
@@ -368,10 +370,13 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
   constexpr int EACH = FEW_TOKENS * L::P / 64;                  // loads of a tile of K, as of V
   uint32_t rows_of[EACH];                                       // pool rows of the tile whose K was asked for last
   auto load_k = [&](int k) {
+    int32_t pages[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) pages[i] = lds_word(slices + (k & 3) * 256 + (i * 64 + lane) / L::P * 4);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int unit = i * 64 + lane, t = unit / L::P, place = unit - t * L::P;
-      rows_of[i] = row_of(c, base_of(k), t, slices + (k & 3) * 256);
+      rows_of[i] = row_of(c, base_of(k) + t, pages[i]);
       to_lds16(c.k + (uint64_t)rows_of[i] * c.k_stride + L::piece(place, L::k_turn(t)) * 16, uniform(kt + i * 1024));
     }
     load_pages(c, base_of(k + 2), slices + ((k + 2) & 3) * 256, lane & 31);
@@ -672,7 +677,9 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
       if constexpr (SUMS) sm.sum += ex + ey;
     };
     if constexpr (!CAREFUL) {
-      // between the matrix instructions of a group of 16 tokens the weights of the next
+      // between the matrix instructions of a group of 16 tokens the weights of the next; ahead of the SIMD's other wave, so that the
+      // two come to differ in what they do (563 us instead of 598 for 1000 tokens over 31000, D = 128, group 4)
+      __builtin_amdgcn_s_setprio(1);
       u32x4 vs[AHEAD];
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) vs[n] = values(n / DB, n % DB);
@@ -689,6 +696,7 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
           for (int i = db * 4 / DB; i < (db + 1) * 4 / DB; ++i) weigh(g + 1, i);
         one_by_one();
       }
+      __builtin_amdgcn_s_setprio(0);
     } else {
 #pragma unroll
       for (int g = 0; g < 2 * BL; ++g)
