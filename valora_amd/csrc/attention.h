@@ -43,6 +43,7 @@ struct AttnLayout {
   int64_t scores;                            // room for scores of requests of few rows, floats
   int64_t off_few, off_tall, off_joins, off_requests, off_shares, off_arrive, words;
   int few_items;                             // (piece, key head) pairs the list is cut for
+  bool tall_each;                            // a share a tall tile: none is long enough to be cut
   int few_least, tall_least;                 // spans up to these are not cut
 };
 

@@ -219,9 +219,10 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
   }
   line = block_sum(line, part);
   int64_t n_shares = (line + a.L.tall_least - 1) / a.L.tall_least;
+  if (a.L.tall_each) n_shares = tiles;
   n_shares = n_shares < a.L.max_shares ? n_shares : a.L.max_shares;
   const int64_t share = n_shares > 0 ? (line + n_shares - 1) / n_shares : 1;
-  n_shares = (line + share - 1) / share;      // (one that begins behind the line is none)
+  if (!a.L.tall_each) n_shares = (line + share - 1) / share;      // (one that begins behind the line is none)
   records = slots = joins = 0;
   int64_t at = 0;                        // where on the line the round's first tile begins
   for (int64_t t0 = 0; t0 < tiles; t0 += AP_THREADS) {
@@ -237,6 +238,10 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
     at += all;
     // f(index of the share that begins here, cut) for the shares that begin within the tile; a cut near an end is none
     auto cuts = [&](auto f) {
+      if (a.L.tall_each) {
+        f(t, 0);
+        return;
+      }
       const int len = p.end - p.begin;
       for (int64_t j = (from + share - 1) / share; j * share < from + length; ++j) {
         const int64_t inside = j * share - from - TALL_OVERHEAD / 2;
@@ -311,7 +316,9 @@ AttnLayout attention_layout(const mlora_attention_plan &p) {
   L.slots_few = few_cut > 1 ? least(2 * few_more, n * few_cut) : 0;
   // tall: a share's beginning cuts one tile at most; k pieces of a tile are k - 1 cuts, and a cut tile has two pieces at least
   const int64_t tiles = tall ? T * L.group / TALL_ROWS + n : 0;
+  L.tall_each = p.max_kv_len < L.tall_least;
   L.max_shares = least(TALL_PLACES / p.kv_heads > 0 ? TALL_PLACES / p.kv_heads : 1, tiles * ceil_div(p.max_kv_len + TALL_OVERHEAD, L.tall_least));
+  if (L.tall_each) L.max_shares = tiles;
   L.max_tall = tiles > 0 ? tiles + (p.max_kv_len >= L.tall_least ? L.max_shares : 0) : 0;
   L.slots_tall = tiles > 0 && p.max_kv_len >= L.tall_least ? 2 * L.max_shares : 0;
   L.few_joins = L.slots_few / 2;
