@@ -26,7 +26,8 @@ def test_plan_shapes():
     for kw, message in ((dict(q_heads=7), b"multiple of kv_heads"), (dict(kv_heads=0), b"kv_heads=0"), (dict(head_dim=100), b"head_dim=100"),
                         (dict(head_dim=512), b"head_dim=512"), (dict(page_size=12), b"page_size=12"), (dict(page_size=512), b"page_size=512"),
                         (dict(page_size=0), b"page_size=0"), (dict(n_req=-1), b"negative"), (dict(window=-1), b"negative"),
-                        (dict(max_kv_len=1 << 31), b"too large"), (dict(n_tokens=1 << 40), b"too large"),
+                        (dict(max_kv_len=1 << 31), b"too large"),
+                        (dict(n_tokens=1 << 40), b"too large"), (dict(n_tokens=1 << 62), b"too large"),
                         (dict(n_req=1 << 20, max_kv_len=1 << 30), b"too large")):
         assert L.mlora_attention_plan_bytes(plan(**kw)) == 0 and message in L.mlora_last_error(), kw
         assert L.mlora_attention_workspace_bytes(plan(**kw), 1) == 0
@@ -44,6 +45,8 @@ def cut_few(spans, hkv):
 def cut_tall(spans, shares):
     """(records, slots, joins, pieces per tile, first record of each share) of the tall list, as the plan kernel cuts it."""
     least, overhead = 512, 192
+    if shares is None:        # none can be cut: a share a tile
+        return len(spans), 0, 0, [[s] for s in spans], list(range(len(spans)))
     line = sum(s + overhead for s in spans)
     n = min(-(-line // least), shares)
     share = -(-line // n) if n else 1
@@ -92,13 +95,13 @@ def test_the_lists_hold_any_batch_the_bounds_allow():
                 tall += [max(0, l - n + (min(r + 128, rows) - 1) // group + 1) for r in range(0, rows, 128)]
         p = plan(n_req=n_req, n_tokens=max(1, sum(new)), max_seq_len=max_seq, max_kv_len=max_kv, q_heads=hkv * group, kv_heads=hkv)
         words, room = L.mlora_attention_plan_bytes(p) // 4, L.mlora_attention_workspace_bytes(p, 0)
-        shares = 512 // hkv
+        shares = 512 // hkv if max_kv >= 512 else None
         f, t = cut_few(few, hkv), cut_tall(tall, shares)
-        need = 32 + 8 * (f[0] + t[0] + f[2] + t[2] + n_req) + len(t[4]) + 1 + hkv * (f[2] + t[2])
+        need = 32 + 8 * (f[0] + t[0] + f[2] + t[2] + n_req) + len(t[4]) + 1 + hkv * f[2]
         assert need <= words, (f, t[:3], words)
         assert (f[1] * 16 + t[1] * 128) * hkv * (128 + 4) * 4 <= room, (f, t[:3], room)
         assert all(sum(p) == s and (len(p) == 1 or min(p) >= 192) for p, s in zip(t[3], tall))
-        if t[4]:
+        if t[4] and shares is not None:
             assert t[4][0] == 0 and t[4] == sorted(t[4]) and t[4][-1] <= t[0]
             flat = [x + (192 if i == 0 else 0) for q in t[3] for i, x in enumerate(q)]
             share = -(-sum(flat) // len(t[4]))

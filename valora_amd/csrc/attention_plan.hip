@@ -1,5 +1,8 @@
 // The plan of the attention calls of a batch: which rows of which request each workgroup takes, and which part of the
 // request's cache.  Cut on the device from the lengths that are there, once per forward pass, for all its layers.
+//
+// One workgroup: requests, then tall tiles, a thread each, with a running sum over the threads for where each one's records go.
+// Bound by the latency of its passes (8 us for 256 decoding requests, 15 for 130 mixed ones).
 #include "attention.h"
 #include "kernel_common.h"
 
@@ -90,11 +93,13 @@ __device__ __forceinline__ int64_t pack(int64_t records, int64_t slots, int64_t 
 constexpr int64_t PACKED = (1 << 21) - 1;
 
 // One workgroup, a thread per request and then per tall tile, in rounds where there are more.
+// EACH: the layout's tall_each
+template <bool EACH>
 __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) {
   __shared__ int64_t part[AP_WAVES];
   const int tid = threadIdx.x;
   int32_t *requests = a.plan + a.L.off_requests, *shares = a.plan + a.L.off_shares;
-  for (int64_t i = tid; i < a.L.few_joins * a.kv_heads; i += AP_THREADS) a.plan[a.L.off_arrive + i] = 0;
+  for (int64_t i = tid; i < (int64_t)a.L.few_joins * a.kv_heads; i += AP_THREADS) a.plan[a.L.off_arrive + i] = 0;
 
   // ---- requests
   int64_t few = 0, blocks_before = 0, tiles = 0, scores = 0;
@@ -133,6 +138,10 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
     blocks_before += all & 0xffffffff;
     tiles += all >> 32;
     scores += all_scores;
+  }
+  if (tid == 0) {
+    a.plan[AH_BLOCKS] = (int32_t)blocks_before;
+    a.plan[AH_SCORES] = scores <= a.L.scores;
   }
   few = block_sum(few, part);
   int64_t records = 0, slots = 0, joins = 0;
@@ -189,6 +198,15 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
   }
   if (tid == 0) a.plan[AH_FEW] = (int)min<int64_t>(records, a.L.max_few);
 
+  auto finish = [&](int64_t tall, int64_t tall_joins, int64_t n_shares) {
+    if (tid != 0) return;
+    tall = min<int64_t>(tall, a.L.max_tall);
+    a.plan[AH_TALL] = (int32_t)tall;
+    a.plan[AH_TALL_JOINS] = (int32_t)min<int64_t>(tall_joins, a.L.tall_joins);
+    a.plan[AH_SHARES] = (int32_t)n_shares;
+    shares[n_shares] = (int32_t)tall;
+  };
+
   // ---- tall tiles, in a line
   struct Place {
     Request r;
@@ -212,17 +230,25 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
     return p;
   };
   __syncthreads();                       // (the requests are written)
+  if constexpr (EACH) {
+    const int64_t n = min(min(tiles, a.L.max_tall), a.L.max_shares);
+    for (int64_t t = tid; t < n; t += AP_THREADS) {
+      const Place p = tile(t);
+      emit(a.plan + a.L.off_tall, t, a.L.max_tall, p.b, p.row0, p.rows, p.begin, p.end, -1, p.r);
+      shares[t] = (int32_t)t;
+    }
+    finish(n, 0, n);
+    return;
+  }
   int64_t line = 0;
   for (int64_t t = tid; t < tiles; t += AP_THREADS) {
     const Place p = tile(t);
     line += p.end - p.begin + TALL_OVERHEAD;
   }
   line = block_sum(line, part);
-  int64_t n_shares = (line + a.L.tall_least - 1) / a.L.tall_least;
-  if (a.L.tall_each) n_shares = tiles;
-  n_shares = n_shares < a.L.max_shares ? n_shares : a.L.max_shares;
+  int n_shares = (int)min<int64_t>((line + a.L.tall_least - 1) / a.L.tall_least, a.L.max_shares);
   const int64_t share = n_shares > 0 ? (line + n_shares - 1) / n_shares : 1;
-  if (!a.L.tall_each) n_shares = (line + share - 1) / share;      // (one that begins behind the line is none)
+  n_shares = (int)((line + share - 1) / share);      // (one that begins behind the line is none)
   records = slots = joins = 0;
   int64_t at = 0;                        // where on the line the round's first tile begins
   for (int64_t t0 = 0; t0 < tiles; t0 += AP_THREADS) {
@@ -238,13 +264,11 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
     at += all;
     // f(index of the share that begins here, cut) for the shares that begin within the tile; a cut near an end is none
     auto cuts = [&](auto f) {
-      if (a.L.tall_each) {
-        f(t, 0);
-        return;
-      }
       const int len = p.end - p.begin;
-      for (int64_t j = (from + share - 1) / share; j * share < from + length; ++j) {
-        const int64_t inside = j * share - from - TALL_OVERHEAD / 2;
+      int64_t step = share;
+      asm volatile("" : "+v"(step));     // (as a vector: the scalars of the division would be spilled)
+      for (int64_t j = (from + step - 1) / step; j * step < from + length; ++j) {
+        const int64_t inside = j * step - from - TALL_OVERHEAD / 2;
         int cut = (int)((inside + AT_PIECE_STEP / 2) / AT_PIECE_STEP * AT_PIECE_STEP);
         if (inside < a.L.tall_least / 2 || len < a.L.tall_least) cut = inside * 2 < len ? 0 : len;
         else if (inside > len - a.L.tall_least / 2) cut = len;
@@ -285,15 +309,7 @@ __global__ __launch_bounds__(AP_THREADS) void attention_plan_kernel(PlanArgs a) 
     slots += all >> 21 & PACKED;
     joins += all >> 42;
   }
-  if (tid == 0) {
-    const int32_t tall = (int32_t)min<int64_t>(records, a.L.max_tall);
-    a.plan[AH_TALL] = tall;
-    a.plan[AH_TALL_JOINS] = (int)min<int64_t>(joins, a.L.tall_joins);
-    a.plan[AH_BLOCKS] = (int32_t)blocks_before;
-    a.plan[AH_SHARES] = (int32_t)n_shares;
-    a.plan[AH_SCORES] = scores <= a.L.scores;
-    shares[n_shares] = tall;
-  }
+  finish(records, joins, n_shares);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -321,17 +337,23 @@ AttnLayout attention_layout(const mlora_attention_plan &p) {
   if (L.tall_each) L.max_shares = tiles;
   L.max_tall = tiles > 0 ? tiles + (p.max_kv_len >= L.tall_least ? L.max_shares : 0) : 0;
   L.slots_tall = tiles > 0 && p.max_kv_len >= L.tall_least ? 2 * L.max_shares : 0;
-  L.few_joins = L.slots_few / 2;
-  L.tall_joins = L.slots_tall / 2;
+  L.few_joins = (int)(L.slots_few / 2);
+  L.tall_joins = (int)(L.slots_tall / 2);
   const int64_t rows = least(FEW_ROWS, p.max_seq_len * L.group);
   L.scores = least(MAX_SCORES, n * least(MAX_SCORES, rows * p.kv_heads * ceil_div(p.max_kv_len, 64) * 64));
-  L.off_few = AT_HDR;
-  L.off_tall = L.off_few + L.max_few * AT_REC;
-  L.off_joins = L.off_tall + L.max_tall * AT_REC;
-  L.off_requests = L.off_joins + (L.few_joins + L.tall_joins) * AT_REC;
-  L.off_shares = L.off_requests + p.n_req * AT_REC;
-  L.off_arrive = L.off_shares + L.max_shares + 1;
-  L.words = L.off_arrive + L.few_joins * p.kv_heads;
+  int64_t at = AT_HDR;
+  auto take = [&](int64_t words) {
+    const int64_t here = at;
+    at += words;
+    return (int)here;
+  };
+  L.off_few = take(L.max_few * AT_REC);
+  L.off_tall = take(L.max_tall * AT_REC);
+  L.off_joins = take(((int64_t)L.few_joins + L.tall_joins) * AT_REC);
+  L.off_requests = take(p.n_req * AT_REC);
+  L.off_shares = take(L.max_shares + 1);
+  L.off_arrive = take((int64_t)L.few_joins * p.kv_heads);
+  L.words = at;
   return L;
 }
 
@@ -365,7 +387,7 @@ int check_attention_plan(const mlora_attention_plan *p, const char *who) {
   if (p->page_size < 1 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
     return fail(MLORA_ERR_NO_KERNEL, "No suitable kernel. %s: page_size=%d (a power of two up to 256)", who, p->page_size);
   // rows, cache indices and positions are kept in 32 bits
-  if (p->n_req > (1 << 20) || p->q_heads > 1024 || p->n_tokens * p->q_heads > (1ll << 30) || p->max_kv_len > (1 << 30) ||
+  if (p->n_req > (1 << 20) || p->q_heads > 1024 || p->n_tokens > (1 << 30) || p->n_tokens * p->q_heads > (1 << 30) || p->max_kv_len > (1 << 30) ||
       p->max_seq_len > (1 << 30))
     return fail(MLORA_ERR_NO_KERNEL, "%s: n_req=%lld n_tokens=%lld max_kv_len=%lld too large", who, (long long)p->n_req,
                 (long long)p->n_tokens, (long long)p->max_kv_len);
@@ -401,7 +423,7 @@ int mlora_build_attention_plan(void *stream, const mlora_attention_plan *plan, c
     return fail(MLORA_ERR_INVALID, "build_attention_plan: null pointer");
   PlanArgs a{static_cast<int32_t *>(plan->dev), b_start_loc, b_seq_len, b_kv_len, L, plan->n_tokens, (int)plan->n_req,
              (int)L.group, (int)plan->max_seq_len, (int)plan->max_kv_len, plan->kv_heads, plan->window};
-  hipLaunchKernelGGL(attention_plan_kernel, dim3(1), dim3(AP_THREADS), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(L.tall_each ? attention_plan_kernel<true> : attention_plan_kernel<false>, dim3(1), dim3(AP_THREADS), 0, (hipStream_t)stream, a);
   return check_launch("attention_plan_kernel");
 }
 

@@ -9,8 +9,9 @@
 // 10^6 in 32 bits would be off by 0.03 radians), the fraction is rounded to 32 bits (2^-25 turns) and sine and cosine are
 // taken in 32 bits.  Each product is rounded to 16 bits once.
 //
-// Bound by bytes.  One workgroup per token (and, for few tokens, per piece of the token's heads): its first wave works out the
-// token's sines and cosines while the other operands are in flight, and every head uses them from LDS.
+// Bound by bytes (8191 tokens, 32 query and 8 key heads of 128, bf16: 201 MB in 40 us, as a copy; one token: 3.1 us, a launch).  One
+// workgroup per token (and, for few tokens, per piece of the token's heads): it works out the token's sines and cosines while
+// the other operands are in flight, and every head uses them from LDS.
 #include "kernel_common.h"
 
 namespace mlora {
