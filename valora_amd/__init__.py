@@ -9,6 +9,8 @@ Modules mirror the reference's import points:
                                               <- ``valora.models.peft.triton_kernel.lora.lora_prefill``
 * ``valora_amd.segments``                     <- ``set_sgmm_args`` / ``count_consecutive_requests``
 * ``valora_amd.plan.LoraPlan``                once-per-batch plan + shrink/expand in one call
+* ``valora_amd.kv_cache.KVCache``             the served requests' cache in rows of the same pool, over ``valora_amd.rotary``
+                                              (positions), ``valora_amd.attention`` (paged attention) and ``evict``
 """
 __version__ = "0.1.0"
 
