@@ -147,6 +147,16 @@ def test_what_a_row_does_not_see_does_not_show(dev, dtype, n, length, value):
             assert bool(torch.isfinite(got[window:n - 3].float()).all())
 
 
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("reqs", [[(1, 200), (2, 70)], [(100, 300)], [(100, 1300)]])
+def test_an_infinity_that_every_row_sees(dev, value, reqs):
+    """In tiles that no mask touches, in a request of one piece and of several: it shows in its column and nowhere else."""
+    c = make(dev, F16, 2, 2, 64, 1, reqs, seed=22)
+    for b in range(len(reqs)):
+        c["vb"][int(c["table"][b, 5]), 0, 3] = value
+    check(dev, c, 1)
+
+
 def test_infinities_of_both_signs_and_scores_of_minus_infinity(dev):
     c = make(dev, BF16, 2, 2, 64, 1, [(20, 20), (40, 70)], seed=8)
     rows = c["table"][0].long()
@@ -160,6 +170,21 @@ def test_infinities_of_both_signs_and_scores_of_minus_infinity(dev):
         c["vb"][c["table"][b].long()[:1], 0, :] = 3.0
     got = run(dev, c, 1)
     assert bool(torch.isfinite(got.float()).all()) and not got[0].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("reqs", [[(1, 100), (5, 300), (3, 9)], [(40, 90), (150, 400)], [(1, 30), (140, 600), (2, 40)]])
+def test_a_row_of_nan_stands_alone(dev, dtype, reqs):
+    """q of one row a request is not a number: that row is none either, the others do not notice."""
+    c = make(dev, dtype, 4, 2, 64, 1, reqs, seed=21)
+    want, _, bound, _ = reference(c["q"], c["kb"], c["vb"], c["table"], c["starts"], c["news"], c["lens"], 1, 0, 64 ** -0.5)
+    for at, n in zip(c["starts"], c["news"]):
+        c["q"][at + n // 2, 1, 7] = math.nan
+        bound[at + n // 2, 1] = math.nan
+    got = run(dev, c, 1)
+    check_out(got, want, bound)
+    for at, n in zip(c["starts"], c["news"]):
+        assert bool(torch.isnan(got[at + n // 2, 1].float()).all())
 
 
 @pytest.mark.parametrize("scale", [1e-6, 0.05, 30.0])

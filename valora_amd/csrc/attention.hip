@@ -300,7 +300,7 @@ struct Joined {
   f32x4 x{0, 0, 0, 0};
 
   __device__ __forceinline__ void add(float4 ml, f32x4 o) {
-    if (ml.x == -INFINITY) return;                            // (saw nothing)
+    if (ml.x == -INFINITY && ml.y == 0.0f) return;            // saw nothing (scores that are no numbers leave no reference, but a sum)
     const float to = fmaxf(m, ml.x), mine = m == -INFINITY ? 0.0f : exp2_(m - to), its = exp2_(ml.x - to);
     m = to;
     l = l * mine + ml.y * its;
