@@ -146,12 +146,16 @@ def test_rotary_and_evict_arguments():
                               (dict(r=66), -2, b"rotary_dim=66"), (dict(r=0), -2, b"rotary_dim=0"), (dict(pos=None), -1, b"null"), (dict(f=None), -1, b"null")):
         assert rot(part(), **kw) == code and message in L.mlora_last_error(), kw
     assert rot(part(flags=3)) == -1 and b"loc" in L.mlora_last_error()
+    for kw in (dict(dst_token_stride=0), dict(dst_head_stride=0), dict(dst_head_stride=63)):
+        assert rot(part(**kw)) == -1 and b"overlap" in L.mlora_last_error(), kw
+    assert rot(part(flags=3, dst_token_stride=0), loc=64, rows=5) == -1 and b"overlap" in L.mlora_last_error()
     assert rot(part(src=None)) == -1 and rot(part(heads=-1)) == -1 and rot(part(heads=0)) == 0 and rot(part(), T=0) == 0
     ev = lambda n=2, width=10, page=1, budget=4, recent=1, sinks=0, ts=10, ws=None, t=64, out=64: L.mlora_cache_evict(  # noqa: E731
         None, t, ts, 64, 64, width * page if ws is None else ws, n, width, page, budget, recent, sinks, out, 64, 64, 64)
     for kw, code, message in ((dict(n=-1), -1, b"negative"), (dict(page=3), -2, b"page_size=3"), (dict(page=512), -2, b"page_size=512"), (dict(recent=0), -1, b"recent=0"),
                               (dict(budget=0), -1, b"budget=0"), (dict(sinks=-1), -1, b"sinks=-1"), (dict(sinks=4), -1, b"budget=4"), (dict(ts=9), -1, b"shorter"),
-                              (dict(ws=9), -1, b"shorter"), (dict(t=None), -1, b"null"), (dict(out=None), -1, b"null"), (dict(width=1 << 30, page=256, ts=1 << 30), -2, b"2^31")):
+                              (dict(ws=9), -1, b"shorter"), (dict(t=None), -1, b"null"), (dict(out=None), -1, b"null"), (dict(width=1 << 30, page=256, ts=1 << 30), -2, b"2^31"),
+                              (dict(width=1 << 55, page=256, ts=1 << 55, ws=1 << 55), -2, b"2^31")):
         assert ev(**kw) == code and message in L.mlora_last_error(), kw
     assert ev(n=0) == 0
 
@@ -188,6 +192,8 @@ def test_rotary_frequencies():
     for kw in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, base=0.0), dict(rotary_dim=8, scaling=dict(type="other", factor=2.0)),
                dict(rotary_dim=8, scaling=dict(type="linear")), dict(rotary_dim=8, scaling=dict(type="linear", factor=-1.0)), dict(rotary_dim=2, scaling=dict(type="ntk", factor=2.0)),
                dict(rotary_dim=8, scaling=dict(type="bands", factor=2.0)), dict(rotary_dim=8, scaling=dict(type="linear", factor=2.0, extra=1)),
-               dict(rotary_dim=8, scaling=dict(type="bands", factor=2.0, low=4.0, high=1.0, original_max_position=10))):
+               dict(rotary_dim=8, scaling=dict(type="bands", factor=2.0, low=4.0, high=1.0, original_max_position=10)),
+               dict(rotary_dim=8, scaling=dict(type="bands", factor=2.0, original_max_position=0)), dict(rotary_dim=8, base=1.0, scaling=dict(type="yarn", factor=2.0, original_max_position=10)),
+               dict(rotary_dim=8, scaling=dict(type="yarn", factor=2.0, original_max_position=10, beta_slow=0.0))):
         with pytest.raises(RuntimeError):
             frequencies(**kw)

@@ -240,7 +240,7 @@ extern "C" int mlora_cache_evict(void *stream, const int32_t *table, int64_t tab
   while (shift < 8 && (1 << shift) < page_size) ++shift;
   if (page_size < 1 || (1 << shift) != page_size)
     return fail(MLORA_ERR_NO_KERNEL, "No suitable kernel. cache_evict: page_size=%d (a power of two up to 256)", page_size);
-  if (width << shift > 0x7fffffff) return fail(MLORA_ERR_NO_KERNEL, "cache_evict: more than 2^31 - 1 tokens a request");
+  if (width > 0x7fffffff || width << shift > 0x7fffffff) return fail(MLORA_ERR_NO_KERNEL, "cache_evict: more than 2^31 - 1 tokens a request");
   if (recent < 1 || sinks < 0 || recent > 0x3fffffff || sinks > 0x3fffffff || budget > 0x7fffffff || budget < recent + sinks)
     return fail(MLORA_ERR_INVALID, "cache_evict: budget=%lld must hold recent=%lld (at least 1) and sinks=%lld pages",
                 (long long)budget, (long long)recent, (long long)sinks);

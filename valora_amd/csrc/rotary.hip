@@ -183,6 +183,9 @@ extern "C" int mlora_rotary(void *stream, const mlora_rotary_part *parts, int32_
     if (T > 0 && p.heads > 0 && (!p.src || !p.dst)) return fail(MLORA_ERR_INVALID, "rotary: null pointer");
     if ((p.flags & MLORA_ROTARY_TO_ROWS) && T > 0 && p.heads > 0 && !loc)
       return fail(MLORA_ERR_INVALID, "rotary: loc is null");
+    const int64_t dst_rows = p.flags & MLORA_ROTARY_TO_ROWS ? n_rows : T;
+    if ((dst_rows > 1 && p.dst_token_stride < head_dim) || (p.heads > 1 && p.dst_head_stride < head_dim))
+      return fail(MLORA_ERR_INVALID, "rotary: heads of a destination overlap");
     vec = vec && ((p.src_token_stride | p.src_head_stride | p.dst_token_stride | p.dst_head_stride) & 7) == 0 &&
           ((reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.dst)) & 15) == 0;
   }

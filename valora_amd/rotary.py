@@ -59,6 +59,8 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[Dict] 
             context = float(s.pop("original_max_position"))
         except KeyError:
             raise RuntimeError(f"{kind} scaling needs original_max_position") from None
+        if not context > 0:
+            raise RuntimeError(f"{kind} scaling needs a positive original_max_position, got {context}")
         if kind == "bands":
             low, high = float(s.pop("low", 1.0)), float(s.pop("high", 4.0))
             if not high > low:
@@ -66,6 +68,8 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[Dict] 
             share = [min(1.0, max(0.0, (context * f / (2 * math.pi) - low) / (high - low))) for f in plain]   # kept
         else:
             fast, slow, given = float(s.pop("beta_fast", 32.0)), float(s.pop("beta_slow", 1.0)), s.pop("attention_factor", None)
+            if not (base > 1 and fast >= slow > 0):
+                raise RuntimeError("yarn scaling needs base > 1 and beta_fast >= beta_slow > 0")
 
             def dimension(turns):
                 return rotary_dim * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(base))
