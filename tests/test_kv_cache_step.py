@@ -1,0 +1,75 @@
+"""The cache's bookkeeping without a GPU, over a pool of host memory: a call that raises leaves the cache and the pool as they were."""
+import pytest
+import torch
+
+from valora_amd import kv_cache
+from valora_amd.kv_cache import KVCache
+
+
+class Pool:
+    """What the cache uses of ``MemoryAllocator``."""
+
+    def __init__(self, rows=100, head_num=2, head_dim=64, dtype=torch.float16):
+        self.head_num, self.head_dim, self.dtype, self.device, self.tot_size = head_num, head_dim, dtype, torch.device("cpu"), rows
+        self.mem_state, self.can_use_mem_size = torch.ones(rows, dtype=torch.bool), rows
+        self.key_buffer = torch.empty(1, rows, head_num, head_dim, dtype=dtype)
+
+    def alloc(self, n):
+        if n > self.can_use_mem_size:
+            raise Exception("no enough pool space")
+        rows = torch.nonzero(self.mem_state).flatten()[:n]
+        self.mem_state[rows] = False
+        self.can_use_mem_size -= n
+        return rows
+
+    def free(self, rows):
+        self.mem_state[rows] = True
+        self.can_use_mem_size += rows.numel()
+
+
+class Turn:
+    """And of ``Rotary``."""
+
+    def __init__(self, head_dim=64):
+        self.head_dim, self.freqs = head_dim, torch.zeros(head_dim // 2, dtype=torch.float64)
+
+
+class Plan:
+    def __init__(self, *a, **kw):
+        pass
+
+
+def state(cache):
+    return (list(cache.lens), list(cache.seen), cache._changes, cache.mem.can_use_mem_size, cache.mem.mem_state.tolist(), cache.table.tolist())
+
+
+class Full(torch.Tensor):
+    """Rows that cannot be turned into page numbers, as where memory runs out."""
+
+    def to(self, *a, **kw):
+        raise torch.OutOfMemoryError("no memory")
+
+
+@pytest.mark.parametrize("where", ["plan", "rows", "pool"])
+def test_a_step_that_raises_changes_nothing(monkeypatch, where):
+    monkeypatch.setattr(kv_cache, "AttentionPlan", Plan)
+    cache = KVCache(Pool(), max_requests=3, max_len=90, q_heads=4, rotary=Turn())
+    before_it = cache.step([0, 2], [5, 7])
+    before = state(cache)
+    with monkeypatch.context() as m:
+        if where == "plan":
+            def broken(*a, **kw):
+                raise torch.OutOfMemoryError("no memory")
+            m.setattr(kv_cache, "AttentionPlan", broken)
+        elif where == "rows":
+            alloc = cache.mem.alloc
+            m.setattr(cache.mem, "alloc", lambda n: alloc(n).as_subclass(Full))
+            m.setattr(cache.mem, "free", lambda rows: Pool.free(cache.mem, rows.as_subclass(torch.Tensor)))
+        with pytest.raises(Exception, match="pool space" if where == "pool" else "no memory"):
+            cache.step([2, 1], [1, 88 if where == "pool" else 3])
+    assert state(cache) == before and before_it._changes == cache._changes
+    # and the same pass again is as if it had not been tried
+    step = cache.step([2, 1], [1, 3])
+    assert step.positions.tolist() == [7, 0, 1, 2] and step.loc.tolist() == [12, 13, 14, 15]
+    assert cache.lens == [5, 3, 8] and cache.mem.can_use_mem_size == 100 - 16
+    assert cache.table[1, :4].tolist() == [13, 14, 15, -1] and cache.table[2, 7].item() == 12

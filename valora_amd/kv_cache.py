@@ -83,7 +83,8 @@ class KVCache:
 
     def step(self, slots: Sequence[int], seq_lens: Sequence[int]) -> CacheStep:
         """Rows for ``seq_lens[i]`` new tokens of slot ``slots[i]``, whose tokens follow each other in the pass's rows in this
-        order.  Raises as ``MemoryAllocator.alloc`` does when the pool is full; nothing has changed then."""
+        order.  Raises as ``MemoryAllocator.alloc`` does when the pool is full.  Whatever it raises, nothing has changed then:
+        neither the pool nor the cache, and the step before is still good."""
         slots, seq_lens = [int(s) for s in slots], [int(n) for n in seq_lens]
         if len(slots) != len(seq_lens) or len(set(slots)) != len(slots):
             raise RuntimeError("step takes distinct slots with one length each")
@@ -93,24 +94,30 @@ class KVCache:
             if n < 1 or self.lens[s] + n > self.max_len:
                 raise RuntimeError(f"slot {s}: {n} new tokens behind {self.lens[s]}, max_len={self.max_len}")
         total = sum(seq_lens)
-        loc = self.mem.alloc(total)
-        start, new = [0] * len(self.lens), [0] * len(self.lens)
+        lens, seen = list(self.lens), list(self.seen)
+        start, new = [0] * len(lens), [0] * len(lens)
         rows, columns, positions, at = [], [], [], 0
         for s, n in zip(slots, seq_lens):
             start[s], new[s] = at, n
             rows += [s] * n
-            columns += range(self.lens[s], self.lens[s] + n)
-            positions += range(self.seen[s], self.seen[s] + n)
+            columns += range(lens[s], lens[s] + n)
+            positions += range(seen[s], seen[s] + n)
             at += n
-            self.lens[s] += n
-            self.seen[s] += n
+            lens[s] += n
+            seen[s] += n
         dev = self.mem.device
         index = torch.tensor([rows, columns, positions], dtype=torch.long).to(dev)
-        lengths = torch.tensor([start, new, self.lens], dtype=torch.int32).to(dev)
-        self.table[index[0], index[1]] = loc.to(torch.int32)
+        lengths = torch.tensor([start, new, lens], dtype=torch.int32).to(dev)
         plan = AttentionPlan(lengths[0], lengths[1], lengths[2], n_tokens=total, max_seq_len=max(seq_lens, default=0),
-                             max_kv_len=max((self.lens[s] for s in slots), default=0), q_heads=self.q_heads,
+                             max_kv_len=max((lens[s] for s in slots), default=0), q_heads=self.q_heads,
                              kv_heads=self.mem.head_num, head_dim=self.mem.head_dim, window=self.window)
+        loc = self.mem.alloc(total)
+        try:
+            self.table[index[0], index[1]] = loc.to(torch.int32)
+        except BaseException:
+            self.mem.free(loc)
+            raise
+        self.lens, self.seen = lens, seen
         self._changes += 1
         return CacheStep(self, index[2], loc, plan)
 
