@@ -73,3 +73,17 @@ def test_a_step_that_raises_changes_nothing(monkeypatch, where):
     assert step.positions.tolist() == [7, 0, 1, 2] and step.loc.tolist() == [12, 13, 14, 15]
     assert cache.lens == [5, 3, 8] and cache.mem.can_use_mem_size == 100 - 16
     assert cache.table[1, :4].tolist() == [13, 14, 15, -1] and cache.table[2, 7].item() == 12
+
+
+def test_heads_that_attention_does_not_take_are_refused_when_the_cache_is_made():
+    for pool, kw, message in ((dict(head_dim=80), {}, "head_dim=80"), (dict(head_dim=112), {}, "head_dim=112"), (dict(head_num=3), {}, "multiple of kv_heads=3"),
+                              (dict(head_num=8), {}, "multiple of kv_heads=8"), ({}, dict(q_heads=0), "q_heads=0"), ({}, dict(window=-1), "negative"),
+                              ({}, dict(max_requests=(1 << 20) + 1), "too large"), (dict(dtype=torch.float32), {}, "dtype=torch.float32")):
+        mem = Pool(**pool)
+        with pytest.raises(RuntimeError, match=message):
+            KVCache(mem, **dict(dict(max_requests=2, max_len=16, q_heads=4, rotary=Turn(mem.head_dim)), **kw))
+    far = Turn()
+    far.freqs = far.freqs.to("meta")
+    with pytest.raises(RuntimeError, match="the rotary is on meta"):
+        KVCache(Pool(), 2, 16, 4, far)
+    KVCache(Pool(), 0, 0, 4, Turn())

@@ -67,12 +67,21 @@ class CacheStep:
 class KVCache:
     """``max_requests`` slots of up to ``max_len`` cached tokens each, over the rows of ``mem`` (``head_num`` and ``head_dim`` of
     which are the key heads').  With ``track`` the attention that cached tokens get is added up over layers and passes, which
-    ``evict`` goes by.  All calls go to the current stream; one cache serves one stream."""
+    ``evict`` goes by.  Heads, types and sizes that attention does not take are refused when the cache is made.  All calls go to
+    the current stream; one cache serves one stream."""
 
     def __init__(self, mem: MemoryAllocator, max_requests: int, max_len: int, q_heads: int, rotary: Rotary, window: int = 0,
                  track: bool = False):
         if rotary.head_dim != mem.head_dim:
             raise RuntimeError(f"the rotary's head_dim={rotary.head_dim} is not the pool's {mem.head_dim}")
+        if rotary.freqs.device != mem.key_buffer.device:
+            raise RuntimeError(f"the rotary is on {rotary.freqs.device}, the pool on {mem.key_buffer.device}")
+        if _lib.dtype_code(mem.dtype) < 0:
+            raise RuntimeError(f"No suitable kernel. kv_cache: dtype={mem.dtype}")
+        # heads and sizes that attention has no kernel for are refused here, not by the first step
+        if not _lib.lib().mlora_attention_plan_bytes(_lib.AttentionPlan(None, 0, max_requests, 0, 0, max_len, q_heads, mem.head_num,
+                                                                        mem.head_dim, 1, window)):
+            raise RuntimeError(_lib.lib().mlora_last_error().decode("utf-8", "replace"))
         self.mem, self.max_len, self.q_heads, self.rotary, self.window = mem, max_len, q_heads, rotary, window
         dev = mem.device
         self.table = torch.full((max_requests, max_len), -1, dtype=torch.int32, device=dev)
