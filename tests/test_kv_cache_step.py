@@ -87,3 +87,15 @@ def test_heads_that_attention_does_not_take_are_refused_when_the_cache_is_made()
     with pytest.raises(RuntimeError, match="the rotary is on meta"):
         KVCache(Pool(), 2, 16, 4, far)
     KVCache(Pool(), 0, 0, 4, Turn())
+
+
+def test_a_slot_that_is_none_is_not_released(monkeypatch):
+    """-1 is not the last slot."""
+    monkeypatch.setattr(kv_cache, "AttentionPlan", Plan)
+    cache = KVCache(Pool(), max_requests=3, max_len=90, q_heads=4, rotary=Turn())
+    step = cache.step([0, 2], [5, 7])
+    before = state(cache)
+    for slot in (-1, -3, 3):
+        with pytest.raises(RuntimeError, match=rf"slot {slot} is outside \[0, 3\)"):
+            cache.release(slot)
+    assert state(cache) == before and step._changes == cache._changes

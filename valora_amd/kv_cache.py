@@ -149,6 +149,8 @@ class KVCache:
 
     def release(self, slot: int) -> None:
         """The slot's rows go back to the pool; the slot is empty."""
+        if not 0 <= slot < len(self.lens):
+            raise RuntimeError(f"slot {slot} is outside [0, {len(self.lens)})")
         n = self.lens[slot]
         self._changes += 1
         if n:
