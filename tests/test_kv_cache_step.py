@@ -99,3 +99,19 @@ def test_a_slot_that_is_none_is_not_released(monkeypatch):
         with pytest.raises(RuntimeError, match=rf"slot {slot} is outside \[0, 3\)"):
             cache.release(slot)
     assert state(cache) == before and step._changes == cache._changes
+
+
+def test_an_eviction_or_release_that_raises_changes_nothing(monkeypatch):
+    monkeypatch.setattr(kv_cache, "AttentionPlan", Plan)
+    cache = KVCache(Pool(), max_requests=2, max_len=20, q_heads=4, rotary=Turn(), track=True)
+    step = cache.step([0, 1], [5, 7])
+    cache.weights += 1
+    before, table, weights = state(cache), cache.table, cache.weights
+    monkeypatch.setattr(kv_cache, "evict", lambda t, l, w, *a: (t.clone().fill_(-1), l, torch.zeros_like(w), t.new_full(t.shape, -1).as_subclass(Full)))
+    for call in (lambda: cache.evict(4, 2), lambda: cache.release(1)):
+        with monkeypatch.context() as m:
+            m.setattr(KVCache, "_free", lambda self, rows, count: rows.as_subclass(Full).to(torch.long))
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+        assert state(cache) == before and step._changes == cache._changes
+        assert cache.table is table and cache.weights is weights and bool((weights == 1).all())

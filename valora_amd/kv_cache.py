@@ -132,7 +132,8 @@ class KVCache:
 
     def evict(self, budget: int, recent: int, sinks: int = 0) -> int:
         """Every slot with more than ``budget`` cached tokens gives up those that got the least attention (see the function
-        ``evict``); their rows go back to the pool.  Returns how many.  Positions go on from where they were."""
+        ``evict``); their rows go back to the pool.  Returns how many.  Positions go on from where they were.  Nothing has changed
+        where it raises."""
         if self.weights is None:
             raise RuntimeError("evict needs a cache that was made with track=True")
         if self.window > 0:
@@ -140,11 +141,11 @@ class KVCache:
         lens = torch.tensor(self.lens, dtype=torch.int32).to(self.mem.device)
         table, _, weights, freed = evict(self.table, lens, self.weights, budget, recent, sinks)
         count = sum(max(0, n - budget) for n in self.lens)
+        if count:
+            self._free(freed.view(-1), count)
         self.table, self.weights = table, weights
         self.lens = [min(n, budget) for n in self.lens]
         self._changes += 1
-        if count:
-            self._free(freed.view(-1), count)
         return count
 
     def release(self, slot: int) -> None:
@@ -152,13 +153,13 @@ class KVCache:
         if not 0 <= slot < len(self.lens):
             raise RuntimeError(f"slot {slot} is outside [0, {len(self.lens)})")
         n = self.lens[slot]
-        self._changes += 1
         if n:
             self._free(self.table[slot, :n], n)
             self.table[slot] = -1
             if self.weights is not None:
                 self.weights[slot] = 0
         self.lens[slot] = self.seen[slot] = 0
+        self._changes += 1
 
     def _free(self, rows: torch.Tensor, count: int) -> None:
         """``count`` rows among ``rows`` (others are -1, which the pool leaves out)."""
