@@ -435,7 +435,7 @@ typedef struct {
                                h / (q_heads / kv_heads)                                                */
   int32_t head_dim;         /* 32, 64, 96, 128 or 256                                                  */
   int32_t page_size;        /* a power of two up to 256                                                */
-  int32_t window;           /* 0: no bound                                                             */
+  int32_t window;           /* 0, or max_kv_len and more: no bound                                     */
 } mlora_attention_plan;
 size_t mlora_attention_plan_bytes(const mlora_attention_plan *plan);
 /* Bytes of workspace a call needs, 256-byte aligned; with weights up to 256 MB more.  Calls that share a workspace or a plan

@@ -49,6 +49,10 @@ struct AttnLayout {
   int few_least, tall_least;                 // spans up to these are not cut
 };
 
+// A window as long as the longest cache bounds nothing; those that do, and the positions that a row's first token follows from, then
+// stay within 2^30 either side of 0 (check_attention_plan), and their sums within 32 bits.
+inline int window_of(const mlora_attention_plan &p) { return p.window >= p.max_kv_len ? 0 : p.window; }
+
 AttnLayout attention_layout(const mlora_attention_plan &p);
 int check_attention_plan(const mlora_attention_plan *p, const char *who);
 

@@ -1092,7 +1092,7 @@ extern "C" int mlora_paged_attention(void *stream, const mlora_attention_plan *p
   a.kv_heads = plan->kv_heads;
   a.group = (int)L.group;
   a.page_shift = shift;
-  a.window = plan->window;
+  a.window = window_of(*plan);
   a.n_req = (int)plan->n_req;
   a.n_pages = (int)n_pages;
   hipStream_t st = (hipStream_t)stream;

@@ -422,7 +422,7 @@ int mlora_build_attention_plan(void *stream, const mlora_attention_plan *plan, c
   if (plan->n_req > 0 && (!b_start_loc || !b_seq_len || !b_kv_len))
     return fail(MLORA_ERR_INVALID, "build_attention_plan: null pointer");
   PlanArgs a{static_cast<int32_t *>(plan->dev), b_start_loc, b_seq_len, b_kv_len, L, plan->n_tokens, (int)plan->n_req,
-             (int)L.group, (int)plan->max_seq_len, (int)plan->max_kv_len, plan->kv_heads, plan->window};
+             (int)L.group, (int)plan->max_seq_len, (int)plan->max_kv_len, plan->kv_heads, window_of(*plan)};
   hipLaunchKernelGGL(L.tall_each ? attention_plan_kernel<true> : attention_plan_kernel<false>, dim3(1), dim3(AP_THREADS), 0, (hipStream_t)stream, a);
   return check_launch("attention_plan_kernel");
 }
