@@ -20,3 +20,50 @@ def test_windows_beyond_any_cache(dev, window, reqs):
         got, want, w_bound = check(dev, c, 1, window, weights=w)
         check_out(w, want, w_bound + 2.0 ** -60)
         assert torch.equal(run(dev, c, 1, 0), got)
+
+
+def probabilities(c, b, page, window=0):
+    """``(weights [new, heads, cached] of request b's rows, what each sees [new, cached])`` in 64 bits; nan where the row's q is."""
+    n, length, at = c["news"][b], c["lens"][b], c["starts"][b]
+    j = torch.arange(length)
+    pages = c["table"][b].long()[j // page]
+    ok = (pages >= 0) & (pages < c["kb"].shape[0] // page)
+    rows = torch.where(ok, pages, torch.zeros_like(pages)) * page + j % page
+    p = torch.arange(length - n, length)[:, None]
+    sees = (j[None] <= p) & ok[None]
+    if window:
+        sees = sees & (j[None] > p - window)
+    hq, hkv, d = c["q"].shape[1], c["kb"].shape[1], c["q"].shape[2]
+    out = torch.zeros(n, hq, length, dtype=torch.float64)
+    for h in range(hq):
+        s = c["q"][at:at + n, h].double() @ c["kb"][rows, h // (hq // hkv)].double().T * d ** -0.5
+        s = torch.where(sees, s, torch.full_like(s, -math.inf))
+        # (a row that sees nothing, or whose scores are all -infinity, gives no weight)
+        out[:, h] = torch.where((s == -math.inf).all(-1, keepdim=True), torch.zeros_like(s), torch.softmax(s, -1))
+    return out, sees
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("n,length,window", [(3, 40, 0), (4, 300, 7), (2, 700, 0), (1, 90, 0), (20, 60, 0), (60, 700, 9)])
+def test_weights_of_a_row_that_is_no_number(dev, n, length, window, value):
+    """It makes the weights of what it sees no numbers, and leaves those of later tokens, of tokens behind its window and of tokens whose
+    page is not there as the other rows make them; few rows and tall tiles alike."""
+    page, hq, hkv = 4, 4, 2
+    c = make(dev, BF16, hq, hkv, 64, page, [(n, length), (1, 30)], seed=32)
+    c["q"][0, 1, 5] = value                              # the first row of the first request
+    c["table"][0, 2], c["table"][0, (length - n) // page - 1] = -1, 2**30
+    w = torch.zeros(2, c["table"].shape[1] * page, device=dev)
+    run(dev, c, page, window, weights=w)
+    p, sees = probabilities(c, 0, page, window)
+    bad = ~torch.isfinite(p).all(-1)                     # [new, heads]
+    # (infinity times the three keys that the row of the window of 7 sees: -infinity each)
+    assert int(bad.sum()) == (0 if value == math.inf and window == 7 else 1)
+    poisoned = sees[0] & bad.any()
+    want = torch.where(bad[:, :, None], torch.zeros_like(p), p).sum((0, 1))
+    got = w[0, :length].cpu().double()
+    assert bool(torch.isnan(got[poisoned]).all())
+    assert int((~poisoned).sum()) >= 8 and not got[8:12].any()
+    # scores in 32 bits, of 64 products whose sizes add up to less than 16: off by 2 * 64 * 2^-24 * 16, as is a row's logarithm
+    assert torch.allclose(got[~poisoned], want[~poisoned], rtol=2.0 ** -11, atol=2.0 ** -30)
+    p1, _ = probabilities(c, 1, page, window)
+    assert torch.allclose(w[1, :30].cpu().double(), p1.sum((0, 1)), rtol=2.0 ** -11, atol=2.0 ** -30)
