@@ -6,6 +6,7 @@ import torch
 
 from tests._attention import attend as reference, check_out
 from tests.test_gpu_attention import BF16, F16, check, make, run
+from valora_amd.attention import AttentionPlan
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,32 @@ def test_weights_of_a_row_that_is_no_number(dev, n, length, window, value):
     assert torch.allclose(got[~poisoned], want[~poisoned], rtol=2.0 ** -11, atol=2.0 ** -30)
     p1, _ = probabilities(c, 1, page, window)
     assert torch.allclose(w[1, :30].cpu().double(), p1.sum((0, 1)), rtol=2.0 ** -11, atol=2.0 ** -30)
+
+
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("gap", [7.0, 12.0, 16.0, 18.0, 20.0])
+@pytest.mark.parametrize("n,n_req", [(1, 64), (20, 32)])
+def test_one_token_far_above_a_long_tail_in_fp16(dev, n, n_req, gap, first):
+    """One token's score lies `gap` above those of tens of thousands, whose weights together count all the same, in requests enough that a
+    wave has thousands of them beside it.  Weights keep their eleven bits down to 2^-21 of the largest and are off by at most 2^-32 of
+    it below: 2^7 of the 2^15 that fp16 goes to are used when the reference is set."""
+    length, heads, d = 60000, 16, 32
+    g = torch.Generator().manual_seed(33)
+    q = torch.zeros(n * n_req, heads, d, dtype=F16)
+    q[:, :, 0] = 8.0
+    kb = torch.zeros(length, heads, d, dtype=F16)
+    vb = (0.5 + torch.rand(length, heads, d, generator=g)).to(F16)
+    top = 0 if first else length - n
+    kb[top, :, 0] = gap                                  # 8 * gap / 8
+    vb[top] = 0
+    table = torch.arange(length, dtype=torch.int32).expand(n_req, length).contiguous()       # (all look at the same cache)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    plan = AttentionPlan(i32(list(range(0, n * n_req, n))), i32([n] * n_req), i32([length] * n_req), n_tokens=n * n_req, max_seq_len=n,
+                         max_kv_len=length, q_heads=heads, kv_heads=heads, head_dim=d)
+    got = plan.attend(torch.full_like(q, 7.0, device=dev), q.to(dev), kb.to(dev), vb.to(dev), table.to(dev), scale=0.125)
+    want, _, bound, _ = reference(q[:n], kb, vb, table, [0], [n], [length], 1, 0, 0.125)
+    # (the general bound allows 2^-25 of the largest weight a token: it knows of no reference below the maximum)
+    bound = bound - 2 * length * (2.0 ** -25 - 2.0 ** -32) * float(vb.abs().max())
+    assert bool((bound > 0).all())
+    for b in range(n_req):
+        check_out(got[b * n:(b + 1) * n], want, bound, f"request {b}")

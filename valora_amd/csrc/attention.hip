@@ -16,9 +16,12 @@
 // written in it.
 //
 // The maximum is followed lazily: a row's scores are taken relative to a reference that stays as long as no score of the wave
-// has grown 2^8 times above the maximum it was set by, and neither sums nor accumulators are scaled meanwhile.  In fp16 the
-// reference is that maximum: weights go up to 2^8, and the small ones keep what bits fp16 has for them.  In bf16, whose values may
-// be as large as the accumulators hold, it lies 2^8 above: weights go up to 1.
+// has grown 2^8 times above the maximum it was set by, and neither sums nor accumulators are scaled meanwhile.  The second product
+// takes the weights in the tensors' 16-bit type, as its matrix instructions do (half a step off each, and so is what divides: their sum, in 32
+// bits; a remainder in a product of its own would double that product).  In fp16 the reference lies 2^7 below the maximum: weights go up to
+// 2^15 of the 65504 that fp16 holds, keep their eleven bits down to 2^-21 of the largest and are 0 below 2^-32 of it.  (With the
+// maximum for a reference, tokens 18 below the highest score, in natural units, were lost: 60000 of them are 0.1 % of a row.)  In bf16,
+// whose values may be as large as the accumulators hold, it lies 2^8 above: weights go up to 1.
 #include <type_traits>
 
 #include "attention.h"
@@ -62,7 +65,7 @@ struct Wide<_Float16> {
   static __device__ __forceinline__ float add2(uint32_t p, float l) { return __builtin_amdgcn_fdot2(as<f16x2>(p), f16x2{1, 1}, l, false); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return as<uint32_t>(__builtin_convertvector((f32x2{lo, hi}), f16x2)); }
   static constexpr uint32_t EXPONENT = 0x7c00;
-  static constexpr float AHEAD = 0.0f;         // the reference above the maximum
+  static constexpr float AHEAD = -7.0f;        // the reference above the maximum
 };
 template <>
 struct Wide<__bf16> {
