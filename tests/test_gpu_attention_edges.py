@@ -97,3 +97,17 @@ def test_one_token_far_above_a_long_tail_in_fp16(dev, n, n_req, gap, first):
     assert bool((bound > 0).all())
     for b in range(n_req):
         check_out(got[b * n:(b + 1) * n], want, bound, f"request {b}")
+
+
+@pytest.mark.parametrize("n,length", [(1, 3000), (1, 100), (40, 700), (130, 4000)])
+def test_bf16_values_as_large_as_the_type_holds(dev, n, length):
+    """Their mean over many tokens is no larger than they are."""
+    big = torch.finfo(BF16).max
+    c = make(dev, BF16, 2, 1, 64, 1, [(n, length)], seed=35)
+    c["q"][:, 0] = 0                                     # a head that looks at all alike, and one that does not
+    c["vb"][:, :, :32], c["vb"][:, :, 32:] = big, -big
+    got = run(dev, c, 1).cpu().double()
+    want = torch.full_like(got, big)
+    want[:, :, 32:] = -big
+    # a rounding to bf16, sums in 32 bits
+    assert bool(((got - want).abs() <= (2.0 ** -8 + (length + 64) * 2.0 ** -24) * big).all()), float((got - want).abs().max() / big)

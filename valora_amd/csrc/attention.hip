@@ -21,7 +21,8 @@
 // bits; a remainder in a product of its own would double that product).  In fp16 the reference lies 2^7 below the maximum: weights go up to
 // 2^15 of the 65504 that fp16 holds, keep their eleven bits down to 2^-21 of the largest and are 0 below 2^-32 of it.  (With the
 // maximum for a reference, tokens 18 below the highest score, in natural units, were lost: 60000 of them are 0.1 % of a row.)  In bf16,
-// whose values may be as large as the accumulators hold, it lies 2^8 above: weights go up to 1.
+// whose values may be as large as the accumulators hold, it lies 2^8 above: weights go up to 1.  Rows whose sums come near what those
+// hold are done again with it 2^38 above: weights go up to 2^-30, and no sum over 2^30 tokens is larger than the values are.
 #include <type_traits>
 
 #include "attention.h"
@@ -65,7 +66,7 @@ struct Wide<_Float16> {
   static __device__ __forceinline__ float add2(uint32_t p, float l) { return __builtin_amdgcn_fdot2(as<f16x2>(p), f16x2{1, 1}, l, false); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return as<uint32_t>(__builtin_convertvector((f32x2{lo, hi}), f16x2)); }
   static constexpr uint32_t EXPONENT = 0x7c00;
-  static constexpr float AHEAD = -7.0f;        // the reference above the maximum
+  static constexpr float AHEAD = -7.0f, FAR = AHEAD;           // the reference above the maximum, and where values are large
 };
 template <>
 struct Wide<__bf16> {
@@ -73,7 +74,7 @@ struct Wide<__bf16> {
   static __device__ __forceinline__ float add2(uint32_t p, float l) { return __builtin_amdgcn_fdot2_f32_bf16(as<bf16x2>(p), bf16x2{1, 1}, l, false); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return as<uint32_t>(__builtin_convertvector((f32x2{lo, hi}), bf16x2)); }
   static constexpr uint32_t EXPONENT = 0x7f80;
-  static constexpr float AHEAD = GROWTH;
+  static constexpr float AHEAD = GROWTH, FAR = GROWTH + 30.0f;
 };
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -226,13 +227,15 @@ struct Softmax {
   float sum = 0.0f;          // and of the weights before they are rounded (where the row's logarithm is wanted)
 
   // the reference goes by the highest score seen; returns what accumulators are scaled by
+  template <bool CAREFUL>
   __device__ __forceinline__ float move(float highest) {
-    const float to = fmaxf(m, highest + Wide<T>::AHEAD);
+    constexpr float AHEAD = CAREFUL ? Wide<T>::FAR : Wide<T>::AHEAD;
+    const float to = fmaxf(m, highest + AHEAD);
     const float alpha = m == -INFINITY ? 0.0f : exp2_(m - to);
     const bool none = to == -INFINITY;
     m = to;
     minus = none ? 0.0f : -to;
-    limit = none ? -INFINITY : GROWTH - Wide<T>::AHEAD;
+    limit = none ? -INFINITY : GROWTH - AHEAD;
     l *= alpha;
     sum *= alpha;
     return alpha;
@@ -242,20 +245,20 @@ struct Softmax {
 // Logarithm of a row's sum, in powers of two; -infinity: the row sees nothing
 __device__ __forceinline__ float row_log(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
 
-// ---- V that is not finite -----------------------------------------------------------------------------------------------------
+// ---- V that is not finite, or as large as its type holds ----------------------------------------------------------------------
 // A token that a row does not see has weight 0, and 0 times an infinity is not 0 but no number, which then stays in the row's sums
-// whatever they are scaled by.  Rows whose sums are not finite at the end of a piece are therefore done again the careful way (a loop of
-// its own, which costs the common one no registers and no look at V): the product runs over the finite values alone, and a second
-// one counts for each row and column the others that the row does see: +infinity as 1, -infinity as 128, not a number as 16384
-// (at most 64 tokens a sum).
+// whatever they are scaled by.  Rows whose sums are not finite at the end of a piece, or so large (2^61 and more) that those of several pieces
+// might not be, are therefore done again the careful way (a loop of its own, which costs the common one no registers and no look at V):
+// the product runs over the finite values alone, and a second one counts for each row and column the others that the row does see:
+// +infinity as 1, -infinity as 128, not a number as 16384 (at most 64 tokens a sum).
 template <typename V, int N, int W = sizeof(V) / 4>
-__device__ __forceinline__ bool any_not_finite(const V (&x)[N]) {
-  float zero = 0.0f;
+__device__ __forceinline__ bool any_too_large(const V (&x)[N]) {
+  float squares = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int j = 0; j < W; ++j) zero = fmaf(x[i][j], 0.0f, zero);
-  return __any(zero != 0.0f);
+    for (int j = 0; j < W; ++j) squares = fmaf(x[i][j], x[i][j], squares);
+  return __any(!(squares < INFINITY));
 }
 template <typename T>
 __device__ __forceinline__ void split_not_finite(u32x4 &v, u32x4 &code) {
@@ -423,7 +426,7 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     if (__any(fmaf(hi, a.c, sm.minus) > sm.limit)) {
       hi = fmaxf(hi, __shfl_xor(hi, 16));
       hi = fmaxf(hi, __shfl_xor(hi, 32));
-      const float alpha = sm.move(hi * a.c);
+      const float alpha = sm.template move<CAREFUL>(hi * a.c);
 #pragma unroll
       for (int i = 0; i < DB; ++i) o[i] *= alpha;
     }
@@ -487,7 +490,7 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
   };
   if (mine > 0) {
     sweep(std::false_type{});
-    if (any_not_finite(o)) sweep(std::true_type{});
+    if (any_too_large(o)) sweep(std::true_type{});
   }
 
   // ---- the waves' sums
@@ -676,7 +679,7 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
     for (int i = 1; i < 16 * BL; ++i) hi = fmaxf(hi, s[i >> 4][i & 15]);
     if (__any(fmaf(hi, a.c, sm.minus) > sm.limit)) {
       hi = fmaxf(hi, __shfl_xor(hi, 32));
-      const float alpha = sm.move(hi * a.c);
+      const float alpha = sm.template move<CAREFUL>(hi * a.c);
 #pragma unroll
       for (int i = 0; i < DB; ++i) o[i] *= alpha;
     }
@@ -766,7 +769,7 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
   if (tiles > 0) {
     if (threadIdx.x == 0) *again = 0;
     sweep(std::false_type{});
-    if (any_not_finite(o) && lane == 0) *again = 1;
+    if (any_too_large(o) && lane == 0) *again = 1;
     wait_lgkmcnt0();
     __syncthreads();                                            // (also: the buffers have been read by everyone)
     if (*again) {
