@@ -450,7 +450,8 @@ int mlora_build_attention_plan(void *stream, const mlora_attention_plan *plan, c
  * [kv_heads][head_dim] of the layer; table: device int32 [n_req][table_width] page numbers.  A cached token whose page is not
  * in the pool is not seen by anyone.  Rows that see nothing become zeros; rows of out that belong to no request keep their
  * contents.  weights (float [n_req][>= max_kv_len], or null): weights[b][j] += what request b's rows give to cached token j,
- * over all heads.  out must not overlap an input.                                                */
+ * over all heads (no number where a row is none that sees j; nothing from a row whose scores, times log2 e, lie beyond 2^22).
+ * out must not overlap an input.                                                                 */
 int mlora_paged_attention(void *stream, const mlora_attention_plan *plan, void *workspace, size_t workspace_bytes,
                           void *out, int64_t out_stride, const void *q, int64_t q_stride, const void *key_buffer,
                           int64_t key_stride, const void *value_buffer, int64_t value_stride, int64_t n_rows,

@@ -111,3 +111,33 @@ def test_bf16_values_as_large_as_the_type_holds(dev, n, length):
     want[:, :, 32:] = -big
     # a rounding to bf16, sums in 32 bits
     assert bool(((got - want).abs() <= (2.0 ** -8 + (length + 64) * 2.0 ** -24) * big).all()), float((got - want).abs().max() / big)
+
+
+@pytest.mark.parametrize("dtype,size", [(F16, 8000.0), (F16, 65504.0), (BF16, 1e6), (BF16, 1e15)])
+@pytest.mark.parametrize("n,length", [(1, 90), (1, 3000), (40, 700), (130, 4000)])
+def test_scores_far_beyond_what_32_bits_resolve(dev, dtype, size, n, length):
+    """Equal ones give the mean; of unequal ones the highest takes all; and no weight is more than a row has."""
+    d = 128
+    c = make(dev, dtype, 2, 1, d, 1, [(n, length)], seed=36)
+    c["q"][:], c["kb"][:] = size, size
+    u = torch.finfo(dtype).eps / 2
+    rows = c["table"][0].long()[:length]
+    w = torch.zeros(1, c["table"].shape[1], device=dev)
+    got = run(dev, c, 1, weights=w).cpu().double()
+    V = c["vb"][rows, 0].double()
+    mean = V.cumsum(0) / torch.arange(1, length + 1)[:, None]
+    # all scores are the same number, so all weights are: what is left is the sums' rounding and the result's
+    err = (got - mean[length - n:, None]).abs()
+    assert bool((err <= u * mean[length - n:, None].abs() + 2 * (length + 64) * 2.0 ** -24 * float(V.abs().max())).all()), float(err.max())
+    assert bool(torch.isfinite(w).all()) and float(w.max()) <= 2 * n * (1 + 2.0 ** -10)
+    # each token's key a step of the type above or below the last one's: the highest is the row's last, or its first
+    step = torch.arange(length) % 64 * (4 * u)
+    for sign in (1.0, -1.0):
+        c["kb"][rows, 0] = (size / 2 * (1 + sign * step))[:, None].to(dtype).expand(length, d)
+        got = run(dev, c, 1, weights=w).cpu().double()
+        k = c["kb"][rows, 0, 0].double()
+        for i in range(n):
+            best = k[:length - n + i + 1] == k[:length - n + i + 1].max()
+            want = V[:length - n + i + 1][best].mean(0)
+            assert bool(((got[i] - want).abs() <= u * want.abs() + 2 * (length + 64) * 2.0 ** -24 * float(V.abs().max())).all()), (sign, i)
+        assert bool(torch.isfinite(w).all()) and float(w.max()) <= 6 * n * (1 + 2.0 ** -10)

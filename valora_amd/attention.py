@@ -59,6 +59,8 @@ class AttentionPlan:
         belong to no request keep their contents.  What no row sees does not show in ``out``, whatever it holds.
 
         ``weights`` (float32 ``[requests, >= max_kv_len]``): ``weights[b, j]`` grows by the attention that request b's rows
-        give to its cached token j, summed over the heads -- what ``valora_amd.kv_cache.evict`` goes by."""
+        give to its cached token j, summed over the heads -- what ``valora_amd.kv_cache.evict`` goes by.  A row that comes out as no
+        number makes the weights of what it sees none; one whose scores lie beyond 2^22, where 32 bits do not hold the logarithm of its
+        sum, adds none."""
         self._native.attend(out, q, key_buffer, value_buffer, table, scale, weights)
         return out

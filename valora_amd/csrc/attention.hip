@@ -218,20 +218,30 @@ __device__ __forceinline__ void load_tile(const Cache &c, int base, uint32_t sli
 }
 
 // ---- running maximum and sum of a lane's row ---------------------------------------------------------------------------------
+// A weight is 2^(c x - m) of a score x.  Where scores are so large that c times the highest is off by more than 1 when it is rounded
+// (2^25 and more), m does not fit it and weights could be infinite or 0: the row's sums are made no numbers, and the careful sweep does it
+// again relative to the highest score itself, 2^(c (x - highest) - AHEAD), two instructions instead of one.
 template <typename T>
 struct Softmax {
-  float m = -INFINITY;       // reference, in powers of two; -infinity: nothing seen yet
+  float m = -INFINITY;       // reference, in powers of two (in a careful sweep the highest score); -infinity: nothing seen yet
   float minus = 0.0f;        // -m, or 0
   float limit = -INFINITY;   // a score this much above m moves it
   float l = 0.0f;            // sum of the weights as the product takes them
   float sum = 0.0f;          // and of the weights before they are rounded (where the row's logarithm is wanted)
 
+  // how far a score lies above the reference, in powers of two
+  template <bool CAREFUL>
+  __device__ __forceinline__ float above(float x, float c) const {
+    return CAREFUL ? fmaf(x + minus, c, -Wide<T>::FAR) : fmaf(x, c, minus);
+  }
   // the reference goes by the highest score seen; returns what accumulators are scaled by
   template <bool CAREFUL>
-  __device__ __forceinline__ float move(float highest) {
+  __device__ __forceinline__ float move(float highest, float c) {
     constexpr float AHEAD = CAREFUL ? Wide<T>::FAR : Wide<T>::AHEAD;
-    const float to = fmaxf(m, highest + AHEAD);
-    const float alpha = m == -INFINITY ? 0.0f : exp2_(m - to);
+    const float top = highest * c;
+    const float to = fmaxf(m, CAREFUL ? highest : top + AHEAD);
+    float alpha = m == -INFINITY ? 0.0f : exp2_(CAREFUL ? (m - to) * c : m - to);
+    if (!CAREFUL && fabsf(fmaf(highest, c, -top)) > 1.0f) alpha = NAN;
     const bool none = to == -INFINITY;
     m = to;
     minus = none ? 0.0f : -to;
@@ -242,8 +252,12 @@ struct Softmax {
   }
 };
 
-// Logarithm of a row's sum, in powers of two; -infinity: the row sees nothing
-__device__ __forceinline__ float row_log(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
+// Logarithm of a row's sum, in powers of two; -infinity: the row gives no weights, as it sees nothing, or as the logarithm is so large
+// (2^22) that half of the sum and more is lost in its last bit
+__device__ __forceinline__ float row_log(float m, float sum) {
+  const float x = m + log2f(sum);
+  return sum == 0.0f || fabsf(x) >= 0x1p22f ? -INFINITY : x;
+}
 
 // ---- V that is not finite, or as large as its type holds ----------------------------------------------------------------------
 // A token that a row does not see has weight 0, and 0 times an infinity is not 0 but no number, which then stays in the row's sums
@@ -423,10 +437,10 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     float hi = s[0][0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) hi = fmaxf(hi, s[i >> 2][i & 3]);
-    if (__any(fmaf(hi, a.c, sm.minus) > sm.limit)) {
+    if (__any(sm.template above<CAREFUL>(hi, a.c) > sm.limit)) {
       hi = fmaxf(hi, __shfl_xor(hi, 16));
       hi = fmaxf(hi, __shfl_xor(hi, 32));
-      const float alpha = sm.template move<CAREFUL>(hi * a.c);
+      const float alpha = sm.template move<CAREFUL>(hi, a.c);
 #pragma unroll
       for (int i = 0; i < DB; ++i) o[i] *= alpha;
     }
@@ -435,7 +449,7 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     for (int i = 0; i < 4; ++i) {
       // (the sum is that of the rounded weights, which the product takes: a row that looks at one token gets exactly its v)
       const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
-      const float ex = exp2_(fmaf(x, a.c, sm.minus)), ey = exp2_(fmaf(y, a.c, sm.minus));
+      const float ex = exp2_(sm.template above<CAREFUL>(x, a.c)), ey = exp2_(sm.template above<CAREFUL>(y, a.c));
       p[i] = Wide<T>::pack(ex, ey);
       sm.l = Wide<T>::add2(p[i], sm.l);
       if constexpr (SUMS) sm.sum += ex + ey;
@@ -487,6 +501,7 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     load_k(0);
     load_v();
     for (int k = 0; k < mine; ++k) step(careful, k);
+    if (decltype(careful)::value) sm.m = fmaf(sm.m, a.c, Wide<T>::FAR);
   };
   if (mine > 0) {
     sweep(std::false_type{});
@@ -677,16 +692,16 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
     float hi = s[0][0];
 #pragma unroll
     for (int i = 1; i < 16 * BL; ++i) hi = fmaxf(hi, s[i >> 4][i & 15]);
-    if (__any(fmaf(hi, a.c, sm.minus) > sm.limit)) {
+    if (__any(sm.template above<CAREFUL>(hi, a.c) > sm.limit)) {
       hi = fmaxf(hi, __shfl_xor(hi, 32));
-      const float alpha = sm.template move<CAREFUL>(hi * a.c);
+      const float alpha = sm.template move<CAREFUL>(hi, a.c);
 #pragma unroll
       for (int i = 0; i < DB; ++i) o[i] *= alpha;
     }
     u32x4 p[2 * BL];
     auto weigh = [&](int g, int i) {
       const float x = s[g >> 1][(g & 1) * 8 + 2 * i], y = s[g >> 1][(g & 1) * 8 + 2 * i + 1];
-      const float ex = exp2_(fmaf(x, a.c, sm.minus)), ey = exp2_(fmaf(y, a.c, sm.minus));
+      const float ex = exp2_(sm.template above<CAREFUL>(x, a.c)), ey = exp2_(sm.template above<CAREFUL>(y, a.c));
       p[g][i] = Wide<T>::pack(ex, ey);
       sm.l = Wide<T>::add2(p[g][i], sm.l);
       if constexpr (SUMS) sm.sum += ex + ey;
@@ -765,6 +780,7 @@ __device__ __forceinline__ void tall_tile(const AttnArgs &a, char *lds, int rec_
       const uint64_t bad = __ballot(bad_page(c, lds_word(slices + (k & 3) * 256 + lane * 4)));   // (lanes behind the tile: of later tokens)
       compute(careful, k, bad);
     }
+    if (decltype(careful)::value) sm.m = fmaf(sm.m, a.c, Wide<T>::FAR);
   };
   if (tiles > 0) {
     if (threadIdx.x == 0) *again = 0;
