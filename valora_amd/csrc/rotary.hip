@@ -150,6 +150,16 @@ __global__ __launch_bounds__(RO_THREADS) void rotary_kernel(RotaryArgs a) {
   }
 }
 
+// Whether heads of `dim` elements at row * row_stride + head * head_stride can share some.  Either the heads of a row lie within the room between
+// two rows or the other way round; strides that interleave the two count as sharing.
+bool share_elements(int64_t rows, int64_t row_stride, int64_t heads, int64_t head_stride, int64_t dim) {
+  if ((rows > 1 && row_stride < dim) || (heads > 1 && head_stride < dim)) return true;
+  if (rows <= 1 || heads <= 1) return false;
+  const bool by_row = row_stride >= head_stride;
+  const int64_t inner = by_row ? head_stride : row_stride, outer = by_row ? row_stride : head_stride, n = by_row ? heads : rows;
+  return (outer - dim) / inner < n - 1;
+}
+
 template <typename T>
 void launch(hipStream_t st, dim3 grid, const RotaryArgs &a, bool interleaved, bool vec) {
   auto *k = interleaved ? (vec ? rotary_kernel<T, true, true> : rotary_kernel<T, true, false>)
@@ -184,7 +194,7 @@ extern "C" int mlora_rotary(void *stream, const mlora_rotary_part *parts, int32_
     if ((p.flags & MLORA_ROTARY_TO_ROWS) && T > 0 && p.heads > 0 && !loc)
       return fail(MLORA_ERR_INVALID, "rotary: loc is null");
     const int64_t dst_rows = p.flags & MLORA_ROTARY_TO_ROWS ? n_rows : T;
-    if ((dst_rows > 1 && p.dst_token_stride < head_dim) || (p.heads > 1 && p.dst_head_stride < head_dim))
+    if (share_elements(dst_rows, p.dst_token_stride, p.heads, p.dst_head_stride, head_dim))
       return fail(MLORA_ERR_INVALID, "rotary: heads of a destination overlap");
     vec = vec && ((p.src_token_stride | p.src_head_stride | p.dst_token_stride | p.dst_head_stride) & 7) == 0 &&
           ((reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.dst)) & 15) == 0;
