@@ -1,7 +1,10 @@
-"""Destinations of the rotary call whose heads would share elements, refused without a GPU."""
+"""Destinations of the rotary call whose heads would share elements, refused without a GPU; the gain of a context made shorter."""
+import math
+
 import pytest
 
 from valora_amd import _lib
+from valora_amd.rotary import frequencies
 
 
 def rotary(T, rows, **kw):
@@ -32,3 +35,11 @@ def test_one_head_or_one_token_alone():
                             (1, 0, dict(dst_head_stride=63), False), (1, 1, dict(dst_token_stride=0), True)):
         assert rotary(T, rows, **kw) == -1
         assert (b"null pointer" if ok else b"overlap") in _lib.lib().mlora_last_error(), kw
+
+
+def test_yarn_gain_of_a_shorter_context():
+    """Only a longer context sharpens the scores."""
+    for factor in (1e-6, 0.25, 0.999, 1.0):
+        assert frequencies(64, scaling=dict(type="yarn", factor=factor, original_max_position=4096))[1] == 1.0
+        assert frequencies(64, scaling=dict(type="yarn", factor=factor, original_max_position=4096, attention_factor=0.5))[1] == 0.5
+    assert frequencies(64, scaling=dict(type="yarn", factor=4.0, original_max_position=4096))[1] == 0.1 * math.log(4.0) + 1.0

@@ -31,7 +31,8 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[Dict] 
       by their turns
     * ``{"type": "yarn", "factor", "original_max_position", "beta_fast" = 32, "beta_slow" = 1, "attention_factor" = None}``:
       kept below the dimension that turns ``beta_fast`` times, divided from the one that turns ``beta_slow`` times on,
-      interpolated by dimension between; gain ``0.1 ln(factor) + 1`` unless ``attention_factor`` gives it
+      interpolated by dimension between; gain ``0.1 ln(factor) + 1``, 1 for factors below 1, unless
+      ``attention_factor`` gives it
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise RuntimeError(f"rotary_dim={rotary_dim} must be even and positive")
@@ -76,7 +77,7 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[Dict] 
 
             lo, hi = max(math.floor(dimension(fast)), 0), min(math.ceil(dimension(slow)), rotary_dim - 1)
             share = [1.0 - min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(rotary_dim // 2)]
-            gain = 0.1 * math.log(factor) + 1.0 if given is None else float(given)
+            gain = 0.1 * math.log(max(factor, 1.0)) + 1.0 if given is None else float(given)
         out = [f * t + f / factor * (1.0 - t) for f, t in zip(plain, share)]
     if s:
         raise RuntimeError(f"rotary scaling {kind}: unknown entries {sorted(s)}")
