@@ -940,25 +940,28 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
       if (j >= kv) continue;
       const float *sc = a.scores + (int64_t)((uint64_t)(uint32_t)rq[5] | (uint64_t)(uint32_t)rq[6] << 32) + (j - begin);
       const int stride = rq[7], n_rows = rows * a.kv_heads;
-      // the sum over the rows of tokens [lo, hi) of the request's new ones
-      auto sum = [&](auto some, int lo, int hi) {
-        float x = 0.0f;
-#pragma unroll 8
-        for (int r = 0; r < n_rows; ++r) {
-          const int head = r / rows, row = r - head * rows, tok = row / a.group;
-          const float lse = a.lse[(int64_t)(tok0 + tok) * a.q_heads + head * a.group + row - tok * a.group];
-          const float e = exp2_(fmaf(sc[(int64_t)r * stride], a.c, -lse));
-          x += lse == -INFINITY || (decltype(some)::value && (tok < lo || tok >= hi)) ? 0.0f : e;
-        }
-        return x;
+      auto share = [&](int r, int &tok) {
+        const int head = r / rows, row = r - head * rows;
+        tok = row / a.group;
+        const float lse = a.lse[(int64_t)(tok0 + tok) * a.q_heads + head * a.group + row - tok * a.group];
+        const float e = exp2_(fmaf(sc[(int64_t)r * stride], a.c, -lse));
+        return lse == -INFINITY ? 0.0f : e;
       };
-      float x = sum(std::false_type{}, 0, n);
+      float x = 0.0f;
+      int tok;
+#pragma unroll 8
+      for (int r = 0; r < n_rows; ++r) x += share(r, tok);
       if (x != x) {
         // A row whose own sum is no number makes that of all tokens, where one that does not see this token (its score is -infinity)
-        // would have added 0: once more, over the rows that see it.
+        // would have added 0: once more, over the rows of the tokens [j - pos0, behind), which see it.
         const int32_t page = a.table[(int64_t)b * a.table_stride + (j >> a.page_shift)];
-        const int behind = a.window > 0 ? j - pos0 + a.window : n;
-        x = sum(std::true_type{}, j - pos0, (uint32_t)page < (uint32_t)a.n_pages ? behind : 0);
+        const int behind = (uint32_t)page >= (uint32_t)a.n_pages ? 0 : a.window > 0 ? j - pos0 + a.window : n;
+        x = 0.0f;
+#pragma unroll 1
+        for (int r = 0; r < n_rows; ++r) {
+          const float e = share(r, tok);
+          x += tok >= j - pos0 && tok < behind ? e : 0.0f;
+        }
       }
       a.weights[(int64_t)b * a.weights_stride + j] += x;
       continue;
