@@ -602,11 +602,13 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
 
 // ---- tall tiles: 32 rows a wave, K and V shared by the workgroup ------------------------------------------------------------------
 // Prompts.  K and V of 64 tokens (two buffers, 64 KB) come in while the 64 before are worked on; a wave keeps its q and its
-// accumulators in registers, two waves a SIMD.  1000 tokens over 31000, 32 query and 8 key heads, D = 128, fp16: 553 to 587 us by
-// the card, 880 to 930 TFLOP/s; a large fp16 product of the library reaches 1180.  The matrix units are busy for 49 % of the cycles (two
-// products of 1024 cycles a SIMD against some 900 of exponentials and sums and 512 of loads into LDS, which overlap in part), at
-// 1.8 GHz of the 2.4 that short launches run at.  16 prompts of 272 to 384 tokens, 32 key heads, bf16: 51 to 54 us; 220 MB are read for 128
-// (a tile reads its request's K and V again), 41 written.
+// accumulators in registers, two waves a SIMD.  1000 tokens over 31000, 32 query and 8 key heads, D = 128, fp16, the whole call in a run of
+// passes: 547 to 588 us by the card, 880 to 945 TFLOP/s; a large fp16 product of the library reaches 1180.  (The first passes after the
+// device was idle are slower, up to 770 us, while its clock settles; the forty of a trace have a median of 598.)  The matrix units are busy
+// for 48 % of the cycles (two products of 1024 cycles a SIMD against some 900 of exponentials and sums and 512 of loads into LDS, which
+// overlap in part), at 1.8 GHz of the 2.4 that short launches run at.  16 prompts of 272 to 384 tokens, 32 key heads, bf16: 51 to 53 us for
+// the 123 MB read and 41 written that it takes, 3.2 TB/s, the matrix units busy for 14 %: neither bounds it, but that a workgroup is
+// short beside its start and end (record, page numbers, first tile, one after the other).
 constexpr int TALL_WAVES = TALL_ROWS / 32;
 template <int D>
 struct Tall {
