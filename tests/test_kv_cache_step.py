@@ -1,4 +1,6 @@
 """The cache's bookkeeping without a GPU, over a pool of host memory: a call that raises leaves the cache and the pool as they were."""
+import contextlib
+
 import pytest
 import torch
 
@@ -115,3 +117,32 @@ def test_an_eviction_or_release_that_raises_changes_nothing(monkeypatch):
                 call()
         assert state(cache) == before and step._changes == cache._changes
         assert cache.table is table and cache.weights is weights and bool((weights == 1).all())
+
+
+def test_the_pool_is_called_with_its_own_device_current(monkeypatch):
+    """Another device may be current where the cache is used."""
+    monkeypatch.setattr(kv_cache, "AttentionPlan", Plan)
+    current, calls = [], []
+
+    @contextlib.contextmanager
+    def on(device):
+        current.append(device)
+        yield
+        current.pop()
+
+    class Library:
+        def mlora_pool_free(self, *a):
+            calls.append(("free", list(current)))
+            return 0
+
+    cache = KVCache(Pool(), max_requests=2, max_len=20, q_heads=4, rotary=Turn(), track=True)
+    alloc = cache.mem.alloc
+    monkeypatch.setattr(cache.mem, "alloc", lambda n: (calls.append(("alloc", list(current))), alloc(n))[1])
+    monkeypatch.setattr(kv_cache, "_on", on)
+    monkeypatch.setattr(kv_cache._lib, "lib", Library)
+    monkeypatch.setattr(kv_cache._lib, "current_stream", lambda device: None)
+    monkeypatch.setattr(kv_cache, "evict", lambda t, l, w, *a: (t, l, w, t))
+    cache.step([0, 1], [5, 7])
+    cache.evict(4, 2)
+    cache.release(1)
+    assert calls == [(name, [torch.device("cpu")]) for name in ("alloc", "free", "free")]

@@ -17,7 +17,8 @@ how much attention each cached token has got -- and makes per forward pass the `
 """
 from __future__ import annotations
 
-from typing import Callable, Optional, Sequence, Tuple
+import contextlib
+from typing import Callable, ContextManager, Optional, Sequence, Tuple
 
 import torch
 
@@ -38,6 +39,11 @@ def evict(table: torch.Tensor, b_kv_len: torch.Tensor, weights: torch.Tensor, bu
     Returns new tensors ``(table, b_kv_len, weights, freed)``: the pages that stay, -1 behind them; the tokens left; their
     weights, 0 behind them; the pages given up, -1 behind them."""
     return _b.cache_evict(table, b_kv_len, weights, budget, recent, sinks, page_size)
+
+
+def _on(device: torch.device) -> ContextManager:
+    """The pool's launches go to the current device; here it is the pool's own."""
+    return torch.cuda.device(device) if device.type == "cuda" else contextlib.nullcontext()
 
 
 class CacheStep:
@@ -68,7 +74,7 @@ class KVCache:
     """``max_requests`` slots of up to ``max_len`` cached tokens each, over the rows of ``mem`` (``head_num`` and ``head_dim`` of
     which are the key heads').  With ``track`` the attention that cached tokens get is added up over layers and passes, which
     ``evict`` goes by.  Heads, types and sizes that attention does not take are refused when the cache is made.  All calls go to
-    the current stream; one cache serves one stream."""
+    the pool's device, whichever is current, and the current stream on it; one cache serves one stream."""
 
     def __init__(self, mem: MemoryAllocator, max_requests: int, max_len: int, q_heads: int, rotary: Rotary, window: int = 0,
                  track: bool = False):
@@ -120,12 +126,13 @@ class KVCache:
         plan = AttentionPlan(lengths[0], lengths[1], lengths[2], n_tokens=total, max_seq_len=max(seq_lens, default=0),
                              max_kv_len=max((lens[s] for s in slots), default=0), q_heads=self.q_heads,
                              kv_heads=self.mem.head_num, head_dim=self.mem.head_dim, window=self.window)
-        loc = self.mem.alloc(total)
-        try:
-            self.table[index[0], index[1]] = loc.to(torch.int32)
-        except BaseException:
-            self.mem.free(loc)
-            raise
+        with _on(dev):
+            loc = self.mem.alloc(total)
+            try:
+                self.table[index[0], index[1]] = loc.to(torch.int32)
+            except BaseException:
+                self.mem.free(loc)
+                raise
         self.lens, self.seen = lens, seen
         self._changes += 1
         return CacheStep(self, index[2], loc, plan)
@@ -164,6 +171,7 @@ class KVCache:
     def _free(self, rows: torch.Tensor, count: int) -> None:
         """``count`` rows among ``rows`` (others are -1, which the pool leaves out)."""
         mem, rows = self.mem, rows.to(torch.long)
-        _lib.check(_lib.lib().mlora_pool_free(_lib.current_stream(mem.device), _lib.ptr(mem.mem_state), mem.tot_size, _lib.ptr(rows),
-                                              rows.numel()))
+        with _on(mem.device):
+            _lib.check(_lib.lib().mlora_pool_free(_lib.current_stream(mem.device), _lib.ptr(mem.mem_state), mem.tot_size, _lib.ptr(rows),
+                                                  rows.numel()))
         mem.can_use_mem_size += count
