@@ -468,6 +468,65 @@ int mlora_cache_evict(void *stream, const int32_t *table, int64_t table_stride, 
                       int64_t budget, int64_t recent, int64_t sinks, int32_t *new_table, int32_t *new_kv_len,
                       float *new_weights, int32_t *freed);
 
+/* ---------------------------------------------------------------------------------------------
+ * The same cache in 8 bits.  A token's k or v of a key head is head_dim e4m3 codes times one power of two (e8m0: a byte,
+ * e + 127): the least e with which the head's largest finite element is at most 448, within [-15, 7] for fp16 and [-117, 119] for
+ * bf16, so that every code times its power is a value of the type.  A code is the nearest of x * 2^-e, the even one of two,
+ * +-448 beyond (infinities too); what is no number stays none.  A pool row of 16-bit elements holds two tokens
+ * (page_size 2, codes in place of the row), four bytes of powers a key head beside it.
+ * Slot s is token s % page_size of page s / page_size.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  void *key_codes, *value_codes;                    /* e4m3 [n_pages][kv_heads][page_size][head_dim], 16-byte aligned  */
+  void *powers;                                     /* e8m0 [n_pages][kv_heads][page_size][2]: k's, v's                */
+  int64_t n_pages;
+  int64_t key_stride, value_stride, powers_stride;  /* bytes from a page to the next (codes: multiples of 16)          */
+  int32_t kv_heads, head_dim, page_size;            /* head_dim 32, 64, 96, 128 or 256; page_size a power of two to 256 */
+} mlora_cache8;
+/* mlora_rotary into that cache: q (may be null) is rotated from q->src to q->dst, the rotated k and the v of token t become codes
+ * in slot loc[t] (device int64 [T], each at most once; those outside the cache are not stored).  k, v: [T][kv_heads][head_dim],
+ * elements of a head contiguous, strides in elements.  k is rotated, and the nearest code found, in 64 bits.             */
+int mlora_rotary_store_codes(void *stream, const mlora_rotary_part *q, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void *v, int64_t v_token_stride, int64_t v_head_stride, const mlora_cache8 *cache,
+                        const int64_t *positions, const int64_t *loc, int64_t T, int32_t rotary_dim, int32_t interleaved,
+                        const double *freqs, float gain, mlora_dtype dtype);
+/* k[i], v[i] = what slot loc[i] holds ([n][kv_heads][head_dim] of dtype, strides in elements between tokens, rows of 16-byte
+ * multiples); zeros where it is outside the cache.  k and v must not overlap each other or the cache.                */
+int mlora_cache_read_codes(void *stream, const mlora_cache8 *cache, const int64_t *loc, int64_t n, void *k, int64_t k_stride, void *v,
+                      int64_t v_stride, mlora_dtype dtype);
+/* mlora_paged_attention over that cache, with a plan of its kv_heads, head_dim and page_size; table: its pages.          */
+int mlora_paged_attention_codes(void *stream, const mlora_attention_plan *plan, void *workspace, size_t workspace_bytes,
+                           void *out, int64_t out_stride, const void *q, int64_t q_stride, const mlora_cache8 *cache,
+                           const int32_t *table, int64_t table_stride, int64_t table_width, float scale, float *weights,
+                           int64_t weights_stride, mlora_dtype dtype);
+
+/* ---------------------------------------------------------------------------------------------
+ * The norms around a layer's blocks, with the sum they stand at:
+ *
+ *     r = residual_scale * x + block_scale * gate * N(block; block_weight, block_bias),    out = N(r; weight, bias)
+ *     N(z; w, b) = z / sqrt(mean(z^2) + eps) * (offset + w) + b,  of z - mean(z) where `layer` is set
+ *
+ * in 32 bits, r and out each rounded once (out goes by the unrounded r).  Without block r is x; without block_weight the block joins as
+ * it is, without weight there is no out.  A null gate is 1, null biases are 0.
+ * ------------------------------------------------------------------------------------------- */
+enum {                          /* which of the vectors are float; the others are of dtype */
+  MLORA_NORM_F32_WEIGHT = 1, MLORA_NORM_F32_BIAS = 2, MLORA_NORM_F32_BLOCK_WEIGHT = 4, MLORA_NORM_F32_BLOCK_BIAS = 8,
+  MLORA_NORM_F32_GATE = 16
+};
+typedef struct {
+  const void *x, *block;                            /* [T][H], strides in elements between rows              */
+  int64_t x_stride, block_stride;
+  const void *weight, *bias, *block_weight, *block_bias;   /* [H]                                           */
+  const void *gate;                                 /* [T][H] by its strides, in elements                    */
+  int64_t gate_row_stride, gate_column_stride;      /* columns: 1, or 0 for one gate a row                   */
+  void *residual_out, *out;                         /* each may be x or block (with its stride): a row is read before it is written */
+  int64_t residual_stride, out_stride;
+  int64_t T, H;                                     /* H up to 32768 (16384 if rows are no 16-byte multiples, aligned) */
+  float residual_scale, block_scale, eps, offset;
+  int32_t layer, f32;
+} mlora_norm;
+int mlora_block_norm(void *stream, const mlora_norm *norm, mlora_dtype dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,11 +17,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ["api.hip", "tiles.hip", "plan.hip", "shrink.hip", "expand.hip", "decode.hip", "pool.hip", "merge.hip",
-           "rotary.hip", "attention_plan.hip", "attention.hip", "evict.hip"]
+           "rotary.hip", "attention_plan.hip", "attention.hip", "evict.hip", "cache8.hip", "attention8.hip", "norm.hip"]
 TABLE_JSON = os.path.join(HERE, "tile_table.json")
 TABLE_INC = os.path.join(CSRC, "tile_table_gen.inc")
 LIB_PATH = os.path.join(HERE, "libmlora.so")
-BINDING_SRCS = [os.path.join(CSRC, s) for s in ("binding.cpp", "binding_attention.cpp")]
+BINDING_SRCS = [os.path.join(CSRC, s) for s in ("binding.cpp", "binding_attention.cpp", "binding_norm.cpp")]
 BINDING_PATH = os.path.join(HERE, "_binding.so")
 
 HIPCC_FLAGS = [

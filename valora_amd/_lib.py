@@ -31,6 +31,7 @@ SYMBOLS = [
     "mlora_build_compensation_plan", "mlora_lora_compensate", "mlora_runs_in_one_launch",
     "mlora_targets_together", "mlora_rotary", "mlora_cache_evict", "mlora_attention_plan_bytes",
     "mlora_attention_workspace_bytes", "mlora_build_attention_plan", "mlora_paged_attention",
+    "mlora_rotary_store_codes", "mlora_cache_read_codes", "mlora_paged_attention_codes", "mlora_block_norm",
 ]
 
 
@@ -61,6 +62,19 @@ class AttentionPlan(ctypes.Structure):
     _fields_ = [("dev", c_void_p), ("bytes", c_size_t), ("n_req", c_int64), ("n_tokens", c_int64), ("max_seq_len", c_int64),
                 ("max_kv_len", c_int64), ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
                 ("page_size", c_int32), ("window", c_int32)]
+
+
+class Cache8(ctypes.Structure):
+    _fields_ = [("key_codes", c_void_p), ("value_codes", c_void_p), ("powers", c_void_p), ("n_pages", c_int64), ("key_stride", c_int64),
+                ("value_stride", c_int64), ("powers_stride", c_int64), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32)]
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("block", c_void_p), ("x_stride", c_int64), ("block_stride", c_int64), ("weight", c_void_p), ("bias", c_void_p),
+                ("block_weight", c_void_p), ("block_bias", c_void_p), ("gate", c_void_p), ("gate_row_stride", c_int64),
+                ("gate_column_stride", c_int64), ("residual_out", c_void_p), ("out", c_void_p), ("residual_stride", c_int64),
+                ("out_stride", c_int64), ("T", c_int64), ("H", c_int64), ("residual_scale", ctypes.c_float), ("block_scale", ctypes.c_float),
+                ("eps", ctypes.c_float), ("offset", ctypes.c_float), ("layer", c_int32), ("f32", c_int32)]
 
 
 ROTARY_PARTS, ROTARY_TURN, ROTARY_TO_ROWS = 3, 1, 2
@@ -147,6 +161,12 @@ def lib():
     L.mlora_paged_attention.argtypes = [c_void_p, POINTER(AttentionPlan), c_void_p, c_size_t, c_void_p, c_int64, c_void_p, c_int64,
                                         c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                         ctypes.c_float, c_void_p, c_int64, c_int]
+    L.mlora_rotary_store_codes.argtypes = [c_void_p, POINTER(RotaryPart), c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, POINTER(Cache8),
+                                      c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p, ctypes.c_float, c_int]
+    L.mlora_cache_read_codes.argtypes = [c_void_p, POINTER(Cache8), c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int]
+    L.mlora_paged_attention_codes.argtypes = [c_void_p, POINTER(AttentionPlan), c_void_p, c_size_t, c_void_p, c_int64, c_void_p, c_int64,
+                                         POINTER(Cache8), c_void_p, c_int64, c_int64, ctypes.c_float, c_void_p, c_int64, c_int]
+    L.mlora_block_norm.argtypes = [c_void_p, POINTER(Norm), c_int]
     for n in SYMBOLS[6:]:  # everything after the size queries returns a status (or a truth value)
         getattr(L, n).restype = c_int
     for n in ("mlora_attention_plan_bytes", "mlora_attention_workspace_bytes"):

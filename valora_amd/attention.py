@@ -64,3 +64,10 @@ class AttentionPlan:
         sum, adds none."""
         self._native.attend(out, q, key_buffer, value_buffer, table, scale, weights)
         return out
+
+    def attend8(self, out: torch.Tensor, q: torch.Tensor, key_codes: torch.Tensor, value_codes: torch.Tensor, powers: torch.Tensor,
+                table: torch.Tensor, scale: Optional[float] = None, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``attend`` over the cache of 8-bit codes (``valora_amd.cache8``): of the values they stand for, which are exact in q's type, everything
+        holds that ``attend`` says.  The codes' page size is the plan's; ``table`` holds their pages."""
+        self._native.attend8(out, q, key_codes, value_codes, powers, table, scale, weights)
+        return out

@@ -721,6 +721,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_readonly("scratch", &NativePlan::scratch)
       .def_readonly("scratch_per_target", &NativePlan::scratch_per_target);
   bind_attention(m);
+  bind_norm(m);
   m.def("tile_lookup", &tile_lookup);
   m.def("one_call_tile", &mlora::one_call_tile);
   m.def("cache_lookup", &cache_lookup);

@@ -55,6 +55,68 @@ Heads dense_heads(const at::Tensor &t, int64_t head_dim, int64_t heads, const ch
 
 void no_kernel(const char *what, const at::Tensor &t) { raise(std::string("No suitable kernel. ") + what + " dtype=" + dtype_name(t)); }
 
+// ---- the 8-bit cache: codes [pages, kv_heads, page_size, head_dim], powers [pages, kv_heads, page_size, 2]; a page is dense --------------
+mlora_cache8 cache8_of(const at::Tensor &key_codes, const at::Tensor &value_codes, const at::Tensor &powers, const c10::Device &dev) {
+  mlora_cache8 c{};
+  const auto page = [&](const at::Tensor &t, at::ScalarType type, const char *name) {
+    check_on(t, dev, name);
+    check_type(t, type, name);
+    if (t.dim() != 4) raise(std::string(name) + " must be [pages, kv_heads, page_size, " + (type == at::kFloat8_e8m0fnu ? "2]" : "head_dim]"));
+    int64_t dense = 1;
+    for (int i = 3; i >= 1; --i) {
+      if (t.size(i) > 1 && t.stride(i) != dense && t.numel() > 0) raise(std::string(name) + ": a page must be contiguous");
+      dense *= t.size(i);
+    }
+    if (t.size(0) > 1 && t.stride(0) < dense) raise(std::string(name) + ": pages overlap");
+    return t.size(0) > 1 ? t.stride(0) : dense;
+  };
+  c.key_stride = page(key_codes, at::kFloat8_e4m3fn, "key_codes");
+  c.value_stride = page(value_codes, at::kFloat8_e4m3fn, "value_codes");
+  c.powers_stride = page(powers, at::kFloat8_e8m0fnu, "powers");
+  if (key_codes.sizes() != value_codes.sizes()) raise("key_codes and value_codes must have the same shape");
+  if (powers.size(0) != key_codes.size(0) || powers.size(1) != key_codes.size(1) || powers.size(2) != key_codes.size(2) || powers.size(3) != 2)
+    raise("powers must be [pages, kv_heads, page_size, 2] of the codes");
+  for (const int i : {1, 2, 3})
+    if (key_codes.size(i) > 4096) raise("No suitable kernel. codes of " + std::to_string(key_codes.size(i)) + " heads, tokens or elements");
+  c.key_codes = key_codes.data_ptr();
+  c.value_codes = value_codes.data_ptr();
+  c.powers = powers.data_ptr();
+  c.n_pages = key_codes.size(0);
+  c.kv_heads = (int32_t)key_codes.size(1);
+  c.page_size = (int32_t)key_codes.size(2);
+  c.head_dim = (int32_t)key_codes.size(3);
+  return c;
+}
+
+py::tuple cache8_read(const at::Tensor &key_codes, const at::Tensor &value_codes, const at::Tensor &powers, const at::Tensor &loc,
+                      at::ScalarType type, const c10::optional<at::Tensor> &k_out, const c10::optional<at::Tensor> &v_out) {
+  if (!key_codes.is_cuda()) raise("key_codes must be a CUDA tensor");
+  const c10::Device dev = key_codes.device();
+  const mlora_cache8 c = cache8_of(key_codes, value_codes, powers, dev);
+  check_on(loc, dev, "loc");
+  check_type(loc, at::kLong, "loc");
+  if (loc.dim() != 1 || !loc.is_contiguous()) raise("loc must be a contiguous 1D tensor");
+  const int64_t n = loc.numel();
+  if (type != at::kHalf && type != at::kBFloat16) raise(std::string("No suitable kernel. cache8_read dtype=torch.") + c10::toString(type));
+  const auto result = [&](const c10::optional<at::Tensor> &given, const char *name) {
+    if (!given.has_value()) return at::empty({n, c.kv_heads, c.head_dim}, key_codes.options().dtype(type));
+    check_on(*given, dev, name);
+    check_type(*given, type, name);
+    return *given;
+  };
+  const at::Tensor k = result(k_out, "k_out"), v = result(v_out, "v_out");
+  const Heads hk = dense_heads(k, c.head_dim, c.kv_heads, "k_out"), hv = dense_heads(v, c.head_dim, c.kv_heads, "v_out");
+  if (hk.rows != n || hv.rows != n) raise("k_out and v_out must have a row per slot");
+  if (n > 0 && hk.data == hv.data) raise("k_out must not be v_out");
+  const c10::DeviceGuard on(dev);
+  const hipStream_t st = stream_of(dev);
+  const mlora_dtype code = dtype_code(k);
+  check_unlocked([&] {
+    return mlora_cache_read_codes(st, &c, static_cast<const int64_t *>(loc.data_ptr()), n, hk.data, hk.row_stride, hv.data, hv.row_stride, code);
+  });
+  return py::make_tuple(k, v);
+}
+
 // ---- rotary ----------------------------------------------------------------------------------------------------------------
 // freqs: float64 [rotary_dim / 2] in turns per position
 struct NativeRotary {
@@ -139,6 +201,34 @@ struct NativeRotary {
     if (key_buffer.size(0) != value_buffer.size(0)) raise("key_buffer and value_buffer must have the same rows");
     call(parts, 3, positions, static_cast<const int64_t *>(loc.data_ptr()), key_buffer.size(0), q);
   }
+
+  void store8(const at::Tensor &positions, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &key_codes,
+              const at::Tensor &value_codes, const at::Tensor &powers, const at::Tensor &loc, const c10::optional<at::Tensor> &q_out) const {
+    const int64_t T = tokens(positions);
+    const c10::Device dev = freqs.device();
+    const mlora_dtype code = dtype_code(q);
+    if ((int)code < 0) no_kernel("rotary", q);
+    if (k.scalar_type() != q.scalar_type()) no_kernel("k", k);
+    if (v.scalar_type() != q.scalar_type()) no_kernel("v", v);
+    const mlora_rotary_part part_q = part(q, q_out.has_value() ? *q_out : q, T, true, false, "q");
+    const mlora_cache8 c = cache8_of(key_codes, value_codes, powers, dev);
+    if (c.head_dim != head_dim) raise("the codes' head_dim=" + std::to_string(c.head_dim) + " is not the rotary's " + std::to_string(head_dim));
+    check_on(k, dev, "k");
+    check_on(v, dev, "v");
+    const Heads hk = heads_of(k, head_dim, "k"), hv = heads_of(v, head_dim, "v");
+    if (hk.rows != T || hv.rows != T) raise("k and v must have a row per position");
+    if (hk.heads != c.kv_heads || hv.heads != c.kv_heads) raise("k and v must have the codes' " + std::to_string(c.kv_heads) + " heads");
+    check_on(loc, dev, "loc");
+    check_type(loc, at::kLong, "loc");
+    if (loc.dim() != 1 || loc.numel() != T || !loc.is_contiguous()) raise("loc must be a contiguous 1D tensor with a slot per token");
+    const c10::DeviceGuard on(dev);
+    const hipStream_t st = stream_of(dev);
+    check_unlocked([&] {
+      return mlora_rotary_store_codes(st, &part_q, hk.data, hk.row_stride, hk.head_stride, hv.data, hv.row_stride, hv.head_stride, &c,
+                                 static_cast<const int64_t *>(positions.data_ptr()), static_cast<const int64_t *>(loc.data_ptr()), T,
+                                 (int32_t)rotary_dim, interleaved, static_cast<const double *>(freqs.data_ptr()), (float)gain, code);
+    });
+  }
 };
 
 // ---- attention -------------------------------------------------------------------------------------------------------------
@@ -187,25 +277,15 @@ struct NativeAttentionPlan {
     });
   }
 
-  void attend(const at::Tensor &out, const at::Tensor &q, const at::Tensor &key_buffer, const at::Tensor &value_buffer,
-              const at::Tensor &table, const c10::optional<double> &scale, const c10::optional<at::Tensor> &weights) {
+  // What attend and attend8 take beside the cache; `call` makes the call of the C ABI
+  template <typename F>
+  void attend_over(const at::Tensor &out, const at::Tensor &q, const at::Tensor &table, const c10::optional<double> &scale,
+                   const c10::optional<at::Tensor> &weights, F call) {
     const c10::Device dev = start.device();
-    check_on(out, dev, "out");
-    check_on(q, dev, "q");
-    check_on(key_buffer, dev, "key_buffer");
-    check_on(value_buffer, dev, "value_buffer");
-    check_on(table, dev, "table");
     const mlora_dtype code = dtype_code(q);
-    if ((int)code < 0) no_kernel("q", q);
-    if (out.scalar_type() != q.scalar_type()) no_kernel("out", out);
-    if (key_buffer.scalar_type() != q.scalar_type()) no_kernel("key_buffer", key_buffer);
-    if (value_buffer.scalar_type() != q.scalar_type()) no_kernel("value_buffer", value_buffer);
-    const Heads ho = dense_heads(out, plan.head_dim, plan.q_heads, "out"), hq = dense_heads(q, plan.head_dim, plan.q_heads, "q"),
-                hk = dense_heads(key_buffer, plan.head_dim, plan.kv_heads, "key_buffer"),
-                hv = dense_heads(value_buffer, plan.head_dim, plan.kv_heads, "value_buffer");
+    const Heads ho = dense_heads(out, plan.head_dim, plan.q_heads, "out"), hq = dense_heads(q, plan.head_dim, plan.q_heads, "q");
     if (ho.rows != plan.n_tokens || hq.rows != plan.n_tokens)
       raise("q and out must have the plan's " + std::to_string(plan.n_tokens) + " tokens");
-    if (hk.rows != hv.rows) raise("key_buffer and value_buffer must have the same rows");
     if (ho.data == hq.data && plan.n_tokens > 0) raise("out must not be q");
     check_type(table, at::kInt, "table");
     if (table.dim() != 2 || table.size(0) != plan.n_req || (table.numel() > 0 && table.stride(1) != 1))
@@ -229,10 +309,49 @@ struct NativeAttentionPlan {
     const c10::DeviceGuard on(dev);
     const hipStream_t st = stream_of(dev);
     check_unlocked([&] {
-      return mlora_paged_attention(st, &plan, room.data_ptr(), (size_t)room.numel(), ho.data, ho.row_stride, hq.data, hq.row_stride,
-                                   hk.data, hk.row_stride, hv.data, hv.row_stride, hk.rows, static_cast<const int32_t *>(table.data_ptr()),
-                                   plan.n_req > 1 ? table.stride(0) : table.size(1), table.size(1), s, w, w_stride, code);
+      return call(st, room.data_ptr(), (size_t)room.numel(), ho, hq, static_cast<const int32_t *>(table.data_ptr()),
+                  plan.n_req > 1 ? table.stride(0) : table.size(1), table.size(1), s, w, w_stride, code);
     });
+  }
+
+  void attend(const at::Tensor &out, const at::Tensor &q, const at::Tensor &key_buffer, const at::Tensor &value_buffer,
+              const at::Tensor &table, const c10::optional<double> &scale, const c10::optional<at::Tensor> &weights) {
+    const c10::Device dev = start.device();
+    check_on(out, dev, "out");
+    check_on(q, dev, "q");
+    check_on(key_buffer, dev, "key_buffer");
+    check_on(value_buffer, dev, "value_buffer");
+    check_on(table, dev, "table");
+    if ((int)dtype_code(q) < 0) no_kernel("q", q);
+    if (out.scalar_type() != q.scalar_type()) no_kernel("out", out);
+    if (key_buffer.scalar_type() != q.scalar_type()) no_kernel("key_buffer", key_buffer);
+    if (value_buffer.scalar_type() != q.scalar_type()) no_kernel("value_buffer", value_buffer);
+    const Heads hk = dense_heads(key_buffer, plan.head_dim, plan.kv_heads, "key_buffer"),
+                hv = dense_heads(value_buffer, plan.head_dim, plan.kv_heads, "value_buffer");
+    if (hk.rows != hv.rows) raise("key_buffer and value_buffer must have the same rows");
+    attend_over(out, q, table, scale, weights,
+                [&](hipStream_t st, void *room, size_t bytes, const Heads &ho, const Heads &hq, const int32_t *pages, int64_t stride, int64_t width,
+                    float by, float *w, int64_t w_stride, mlora_dtype code) {
+                  return mlora_paged_attention(st, &plan, room, bytes, ho.data, ho.row_stride, hq.data, hq.row_stride, hk.data, hk.row_stride,
+                                               hv.data, hv.row_stride, hk.rows, pages, stride, width, by, w, w_stride, code);
+                });
+  }
+
+  void attend8(const at::Tensor &out, const at::Tensor &q, const at::Tensor &key_codes, const at::Tensor &value_codes, const at::Tensor &powers,
+               const at::Tensor &table, const c10::optional<double> &scale, const c10::optional<at::Tensor> &weights) {
+    const c10::Device dev = start.device();
+    check_on(out, dev, "out");
+    check_on(q, dev, "q");
+    check_on(table, dev, "table");
+    if ((int)dtype_code(q) < 0) no_kernel("q", q);
+    if (out.scalar_type() != q.scalar_type()) no_kernel("out", out);
+    const mlora_cache8 c = cache8_of(key_codes, value_codes, powers, dev);
+    attend_over(out, q, table, scale, weights,
+                [&](hipStream_t st, void *room, size_t bytes, const Heads &ho, const Heads &hq, const int32_t *pages, int64_t stride, int64_t width,
+                    float by, float *w, int64_t w_stride, mlora_dtype code) {
+                  return mlora_paged_attention_codes(st, &plan, room, bytes, ho.data, ho.row_stride, hq.data, hq.row_stride, &c, pages, stride, width,
+                                                by, w, w_stride, code);
+                });
   }
 };
 
@@ -272,13 +391,16 @@ void bind_attention(py::module_ &m) {
   py::class_<NativeRotary>(m, "NativeRotary")
       .def(py::init<const at::Tensor &, int64_t, bool, double>())
       .def("apply", &NativeRotary::apply)
-      .def("store", &NativeRotary::store);
+      .def("store", &NativeRotary::store)
+      .def("store8", &NativeRotary::store8);
   py::class_<NativeAttentionPlan>(m, "NativeAttentionPlan")
       .def(py::init<const at::Tensor &, const at::Tensor &, const at::Tensor &, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
                     int64_t, int64_t>())
       .def("rebuild", &NativeAttentionPlan::rebuild)
       .def("attend", &NativeAttentionPlan::attend)
+      .def("attend8", &NativeAttentionPlan::attend8)
       .def_readonly("buf", &NativeAttentionPlan::buf)
       .def_readonly("workspace", &NativeAttentionPlan::workspace);
   m.def("cache_evict", &cache_evict);
+  m.def("cache8_read", &cache8_read);
 }

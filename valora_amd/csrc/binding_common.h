@@ -39,3 +39,4 @@ void check_unlocked(F call) {
 }
 
 void bind_attention(py::module_ &m);   // binding_attention.cpp
+void bind_norm(py::module_ &m);        // binding_norm.cpp

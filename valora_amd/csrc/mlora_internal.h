@@ -83,6 +83,8 @@ static inline int64_t partial_stride_lines(int64_t max_rank) { return align_up(m
 // ---- error reporting (api.hip) ---------------------------------------------------------------
 int fail(int code, const char *fmt, ...);
 int check_launch(const char *what);
+bool share_elements(int64_t rows, int64_t row_stride, int64_t heads, int64_t head_stride, int64_t dim);   // rotary.hip
+int check_cache8(const mlora_cache8 *c, int kv_heads, int head_dim, int page_size, const char *who);       // cache8.hip
 
 // ---- tile table (tiles.hip) --------------------------------------------------------------------
 mlora_tile_config tile_lookup(int64_t T, int64_t max_rank, int64_t hidden, int64_t A);

@@ -150,6 +150,15 @@ __global__ __launch_bounds__(RO_THREADS) void rotary_kernel(RotaryArgs a) {
   }
 }
 
+template <typename T>
+void launch(hipStream_t st, dim3 grid, const RotaryArgs &a, bool interleaved, bool vec) {
+  auto *k = interleaved ? (vec ? rotary_kernel<T, true, true> : rotary_kernel<T, true, false>)
+                        : (vec ? rotary_kernel<T, false, true> : rotary_kernel<T, false, false>);
+  hipLaunchKernelGGL(k, grid, dim3(RO_THREADS), 0, st, a);
+}
+
+}  // namespace
+
 // Whether heads of `dim` elements at row * row_stride + head * head_stride can share some.  Either the heads of a row lie within the room between
 // two rows or the other way round; strides that interleave the two count as sharing.
 bool share_elements(int64_t rows, int64_t row_stride, int64_t heads, int64_t head_stride, int64_t dim) {
@@ -159,15 +168,6 @@ bool share_elements(int64_t rows, int64_t row_stride, int64_t heads, int64_t hea
   const int64_t inner = by_row ? head_stride : row_stride, outer = by_row ? row_stride : head_stride, n = by_row ? heads : rows;
   return (outer - dim) / inner < n - 1;
 }
-
-template <typename T>
-void launch(hipStream_t st, dim3 grid, const RotaryArgs &a, bool interleaved, bool vec) {
-  auto *k = interleaved ? (vec ? rotary_kernel<T, true, true> : rotary_kernel<T, true, false>)
-                        : (vec ? rotary_kernel<T, false, true> : rotary_kernel<T, false, false>);
-  hipLaunchKernelGGL(k, grid, dim3(RO_THREADS), 0, st, a);
-}
-
-}  // namespace
 
 }  // namespace mlora
 

@@ -14,6 +14,9 @@ how much attention each cached token has got -- and makes per forward pass the `
     cache.release(3)
 
 ``evict`` alone works on any paged cache whose table and weights the caller keeps.
+
+With ``codes=True`` the cache is in 8 bits (``valora_amd.cache8``): a row holds two tokens, so the same pool holds twice as many, and passes over
+it read half the bytes.
 """
 from __future__ import annotations
 
@@ -22,7 +25,7 @@ from typing import Callable, ContextManager, Optional, Sequence, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, cache8
 from ._ext import binding as _b
 from .attention import AttentionPlan
 from .infer_adapter import MemoryAllocator
@@ -58,12 +61,15 @@ class CacheStep:
         """``attend(q, k, v)`` of a layer, on the projections' outputs ``[T, heads * head_dim]`` before any rotation: rotates q and
         k, stores k and v, attends over the cache."""
         c = self.cache
-        key_buffer, value_buffer = c.mem.key_buffer[layer], c.mem.value_buffer[layer]
+        key_buffer, value_buffer, powers = c.layer(layer)
 
         def attend(q, k, v):
             if self._changes != c._changes:
                 raise RuntimeError("the cache has changed since this step was made")
             turned, out = torch.empty_like(q), torch.empty_like(q)
+            if powers is not None:
+                c.rotary.store8(self.positions, q, k, v, key_buffer, value_buffer, powers, self.loc, q_out=turned)
+                return self.plan.attend8(out, turned, key_buffer, value_buffer, powers, c.table, weights=c.weights)
             c.rotary.store(self.positions, q, k, v, key_buffer, value_buffer, self.loc, q_out=turned)
             return self.plan.attend(out, turned, key_buffer, value_buffer, c.table, weights=c.weights)
 
@@ -73,11 +79,12 @@ class CacheStep:
 class KVCache:
     """``max_requests`` slots of up to ``max_len`` cached tokens each, over the rows of ``mem`` (``head_num`` and ``head_dim`` of
     which are the key heads').  With ``track`` the attention that cached tokens get is added up over layers and passes, which
-    ``evict`` goes by.  Heads, types and sizes that attention does not take are refused when the cache is made.  All calls go to
+    ``evict`` goes by.  With ``codes`` tokens are kept in 8 bits, two a row, with four bytes a row and key head of every layer
+    beside the pool.  Heads, types and sizes that attention does not take are refused when the cache is made.  All calls go to
     the pool's device, whichever is current, and the current stream on it; one cache serves one stream."""
 
     def __init__(self, mem: MemoryAllocator, max_requests: int, max_len: int, q_heads: int, rotary: Rotary, window: int = 0,
-                 track: bool = False):
+                 track: bool = False, codes: bool = False):
         if rotary.head_dim != mem.head_dim:
             raise RuntimeError(f"the rotary's head_dim={rotary.head_dim} is not the pool's {mem.head_dim}")
         if rotary.freqs.device != mem.key_buffer.device:
@@ -85,16 +92,47 @@ class KVCache:
         if _lib.dtype_code(mem.dtype) < 0:
             raise RuntimeError(f"No suitable kernel. kv_cache: dtype={mem.dtype}")
         # heads and sizes that attention has no kernel for are refused here, not by the first step
+        self.page = cache8.ROW_TOKENS if codes else 1      # tokens a row
         if not _lib.lib().mlora_attention_plan_bytes(_lib.AttentionPlan(None, 0, max_requests, 0, 0, max_len, q_heads, mem.head_num,
-                                                                        mem.head_dim, 1, window)):
+                                                                        mem.head_dim, self.page, window)):
             raise RuntimeError(_lib.lib().mlora_last_error().decode("utf-8", "replace"))
         self.mem, self.max_len, self.q_heads, self.rotary, self.window = mem, max_len, q_heads, rotary, window
         dev = mem.device
-        self.table = torch.full((max_requests, max_len), -1, dtype=torch.int32, device=dev)
-        self.weights: Optional[torch.Tensor] = torch.zeros(max_requests, max_len, device=dev) if track else None
+        pages = self._rows(max_len)
+        self.table = torch.full((max_requests, pages), -1, dtype=torch.int32, device=dev)
+        self.weights: Optional[torch.Tensor] = torch.zeros(max_requests, pages * self.page, device=dev) if track else None
+        self.powers: Optional[torch.Tensor] = None
+        if codes:
+            layers, rows, heads, _ = mem.key_buffer.shape
+            self.powers = cache8.new_powers((layers, rows, heads, self.page), dev)
         self.lens = [0] * max_requests           # cached tokens, and
         self.seen = [0] * max_requests           # tokens so far, evicted ones too: the next token's position
         self._changes = 0
+
+    def _rows(self, tokens: int) -> int:
+        return -(-tokens // self.page)
+
+    def layer(self, layer: int) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+        """A layer's keys and values as the attention calls take them, and with ``codes`` their powers."""
+        key_buffer, value_buffer = self.mem.key_buffer[layer], self.mem.value_buffer[layer]
+        if self.powers is None:
+            return key_buffer, value_buffer, None
+        return cache8.codes_of_rows(key_buffer), cache8.codes_of_rows(value_buffer), self.powers[layer]
+
+    def read(self, slot: int, layer: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``(k, v)``, ``[tokens, kv_heads, head_dim]`` of the pool's type: what the slot's cached tokens hold in a layer, new tensors."""
+        self._check_slot(slot)
+        key_buffer, value_buffer, powers = self.layer(layer)
+        n = self.lens[slot]
+        rows = self.table[slot, :self._rows(n)].to(torch.long)
+        if powers is None:
+            return key_buffer[rows], value_buffer[rows]
+        loc = (rows[:, None] * self.page + torch.arange(self.page, device=rows.device)).flatten()[:n].contiguous()
+        return cache8.read(key_buffer, value_buffer, powers, loc, self.mem.dtype)
+
+    def _check_slot(self, slot: int) -> None:
+        if not 0 <= slot < len(self.lens):
+            raise RuntimeError(f"slot {slot} is outside [0, {len(self.lens)})")
 
     def step(self, slots: Sequence[int], seq_lens: Sequence[int]) -> CacheStep:
         """Rows for ``seq_lens[i]`` new tokens of slot ``slots[i]``, whose tokens follow each other in the pass's rows in this
@@ -104,16 +142,28 @@ class KVCache:
         if len(slots) != len(seq_lens) or len(set(slots)) != len(slots):
             raise RuntimeError("step takes distinct slots with one length each")
         for s, n in zip(slots, seq_lens):
-            if not 0 <= s < len(self.lens):
-                raise RuntimeError(f"slot {s} is outside [0, {len(self.lens)})")
+            self._check_slot(s)
             if n < 1 or self.lens[s] + n > self.max_len:
                 raise RuntimeError(f"slot {s}: {n} new tokens behind {self.lens[s]}, max_len={self.max_len}")
         total = sum(seq_lens)
         lens, seen = list(self.lens), list(self.seen)
         start, new = [0] * len(lens), [0] * len(lens)
         rows, columns, positions, at = [], [], [], 0
+        new_rows, new_columns = [], []                      # where in the table the pool's rows go
+        old_rows, old_columns = [], []                      # rows that have room for a token
+        source = []                                         # of each token's row: among the new ones, or behind them among the old
         for s, n in zip(slots, seq_lens):
             start[s], new[s] = at, n
+            if self.page > 1:
+                full = self._rows(lens[s])
+                source += [len(new_rows) + c // self.page - full if c // self.page >= full else -1 - len(old_rows)
+                           for c in range(lens[s], lens[s] + n)]
+                if lens[s] % self.page:
+                    old_rows.append(s)
+                    old_columns.append(full - 1)
+            fresh = range(self._rows(lens[s]), self._rows(lens[s] + n))
+            new_rows += [s] * len(fresh)
+            new_columns += fresh
             rows += [s] * n
             columns += range(lens[s], lens[s] + n)
             positions += range(seen[s], seen[s] + n)
@@ -122,16 +172,25 @@ class KVCache:
             seen[s] += n
         dev = self.mem.device
         index = torch.tensor([rows, columns, positions], dtype=torch.long).to(dev)
+        fresh = index
+        if self.page > 1:
+            fresh = torch.tensor([new_rows, new_columns], dtype=torch.long).to(dev)
+            old = torch.tensor([old_rows, old_columns], dtype=torch.long).to(dev)
+            source = torch.tensor([i if i >= 0 else len(new_rows) - 1 - i for i in source], dtype=torch.long).to(dev)
         lengths = torch.tensor([start, new, lens], dtype=torch.int32).to(dev)
         plan = AttentionPlan(lengths[0], lengths[1], lengths[2], n_tokens=total, max_seq_len=max(seq_lens, default=0),
                              max_kv_len=max((lens[s] for s in slots), default=0), q_heads=self.q_heads,
-                             kv_heads=self.mem.head_num, head_dim=self.mem.head_dim, window=self.window)
+                             kv_heads=self.mem.head_num, head_dim=self.mem.head_dim, page_size=self.page, window=self.window)
         with _on(dev):
-            loc = self.mem.alloc(total)
+            got = self.mem.alloc(len(new_rows))
             try:
-                self.table[index[0], index[1]] = loc.to(torch.int32)
+                loc = got
+                if self.page > 1:
+                    its = torch.cat([got, self.table[old[0], old[1]].to(torch.long)])
+                    loc = its[source] * self.page + index[1] % self.page
+                self.table[fresh[0], fresh[1]] = got.to(torch.int32)
             except BaseException:
-                self.mem.free(loc)
+                self.mem.free(got)
                 raise
         self.lens, self.seen = lens, seen
         self._changes += 1
@@ -139,27 +198,30 @@ class KVCache:
 
     def evict(self, budget: int, recent: int, sinks: int = 0) -> int:
         """Every slot with more than ``budget`` cached tokens gives up those that got the least attention (see the function
-        ``evict``); their rows go back to the pool.  Returns how many.  Positions go on from where they were.  Nothing has changed
-        where it raises."""
+        ``evict``); their rows go back to the pool.  Returns how many rows.  With ``codes`` it goes by rows of two tokens: the budget is rounded
+        down to them, ``recent`` and ``sinks`` up.  Positions go on from where they were.  Nothing has changed where it raises."""
         if self.weights is None:
             raise RuntimeError("evict needs a cache that was made with track=True")
         if self.window > 0:
             raise RuntimeError("evict and window exclude each other: a window counts cached tokens")
         lens = torch.tensor(self.lens, dtype=torch.int32).to(self.mem.device)
-        table, _, weights, freed = evict(self.table, lens, self.weights, budget, recent, sinks)
-        count = sum(max(0, n - budget) for n in self.lens)
+        if self.page > 1:
+            budget //= self.page
+            recent, sinks = (self._rows(n) if n > 0 else n for n in (recent, sinks))      # (negative ones are refused below)
+        table, _, weights, freed = evict(self.table, lens, self.weights, budget, recent, sinks, self.page)
+        over = [max(0, self._rows(n) - budget) for n in self.lens]
+        count = sum(over)
         if count:
             self._free(freed.view(-1), count)
         self.table, self.weights = table, weights
-        self.lens = [min(n, budget) for n in self.lens]
+        self.lens = [n - k * self.page for n, k in zip(self.lens, over)]
         self._changes += 1
         return count
 
     def release(self, slot: int) -> None:
         """The slot's rows go back to the pool; the slot is empty."""
-        if not 0 <= slot < len(self.lens):
-            raise RuntimeError(f"slot {slot} is outside [0, {len(self.lens)})")
-        n = self.lens[slot]
+        self._check_slot(slot)
+        n = self._rows(self.lens[slot])
         if n:
             self._free(self.table[slot, :n], n)
             self.table[slot] = -1

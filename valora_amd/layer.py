@@ -14,7 +14,8 @@ extends the reference's: three (key, value) buffer pairs that share one row numb
 -- so an adapter still owns ``4 * r`` pool rows and every index tensor of the reference keeps its
 meaning.  The base projections, normalisation, rotary embedding and attention are stock PyTorch
 (`torch.mm`, `scaled_dot_product_attention`), unless the caller's attention is that of the paged cache
-(``valora_amd.kv_cache``), which has its own kernels for rotation, storing and attention; the LoRA
+(``valora_amd.kv_cache``), which has its own kernels for rotation, storing and attention, or the layer is asked for with
+``fused``, where each norm and the sum before it are one launch (``valora_amd.norm``); the LoRA
 deltas go through ``LoraPlan``: q, k, v in one multi-target call, gate and up in another, o and
 down in single calls -- four LoRA calls (8 to 12 launches) per layer for seven projections, where the
 reference issues 8 calls (16 launches, each followed by a synchronize) for its four
@@ -28,6 +29,7 @@ from typing import Callable, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from .norm import block_norm
 from .plan import LoraPlan
 
 
@@ -55,6 +57,19 @@ class LayerWeights:
     w_down: torch.Tensor
     ln1: torch.Tensor
     ln2: torch.Tensor
+    # of models that have them, for the fused norms: norms after attention and after the MLP, learned gates of either (a channel each), and what
+    # the residual stream and each block's output are multiplied by where they are added
+    post1: Optional[torch.Tensor] = None
+    post2: Optional[torch.Tensor] = None
+    gate1: Optional[torch.Tensor] = None
+    gate2: Optional[torch.Tensor] = None
+    residual_scale: float = 1.0
+    block_scale: float = 1.0
+
+    def around_blocks(self) -> bool:
+        """Whether there is more than a norm before each block."""
+        return (any(t is not None for t in (self.post1, self.post2, self.gate1, self.gate2)) or
+                self.residual_scale != 1.0 or self.block_scale != 1.0)
 
 
 class LayerPlans:
@@ -83,14 +98,23 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int) -> t
 
 def layer_forward(x: torch.Tensor, w: LayerWeights, pools: Optional[LayerPools], plans: Optional[LayerPlans],
                   attention: Callable[[torch.Tensor, torch.Tensor, torch.Tensor], torch.Tensor], heads: int,
-                  cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, fused: bool = False) -> torch.Tensor:
     """``x [T, H]`` -> ``[T, H]``.  ``pools`` / ``plans`` None runs the base model only.  ``attention(q, k, v)``
     takes and returns ``[T, H]`` matrices (it owns the KV cache and the request boundaries): ``segment_attention`` for whole
     prompts without a cache, ``valora_amd.kv_cache.KVCache.step(...).attention(layer)`` for new tokens over the paged cache, which
-    rotates q and k itself (``cos`` / ``sin`` None)."""
+    rotates q and k itself (``cos`` / ``sin`` None).
+
+    ``fused``: norms and residual sums by ``valora_amd.norm.block_norm``, in 32 bits to each result's one rounding (results differ from the
+    others' in the last bit); the weights' ``post1`` ... ``block_scale`` need it."""
+    if w.around_blocks() and not fused:
+        raise RuntimeError("norms after blocks, gates and scales need layer_forward(..., fused=True)")
+
+    def join(x, block, post, gate, ln):
+        return block_norm(x, ln, block=block, block_weight=post, gate=gate, residual_scale=w.residual_scale, block_scale=w.block_scale)
+
     lora = pools is not None and plans is not None
     idx = (pools.a_start, pools.a_len, pools.a_loc) if lora else None
-    h = rmsnorm(x, w.ln1)
+    h = block_norm(x, w.ln1)[1] if fused else rmsnorm(x, w.ln1)
     q, k, v = torch.mm(h, w.wq), torch.mm(h, w.wk), torch.mm(h, w.wv)
     if lora:
         plans.h.apply_multi([q, k, v], h, pools.attn[0], pools.attn[1], *idx, [0, 1, 2], pools.a_scaling)
@@ -100,8 +124,11 @@ def layer_forward(x: torch.Tensor, w: LayerWeights, pools: Optional[LayerPools],
     o = torch.mm(a, w.wo)
     if lora:
         plans.h.apply(o, a, pools.attn[0], pools.attn[1], *idx, 3, pools.a_scaling)
-    x = x + o
-    h2 = rmsnorm(x, w.ln2)
+    if fused:
+        x, h2 = join(x, o, w.post1, w.gate1, w.ln2)
+    else:
+        x = x + o
+        h2 = rmsnorm(x, w.ln2)
     g, u = torch.mm(h2, w.w_gate), torch.mm(h2, w.w_up)
     if lora:
         plans.h.apply_multi([g, u], h2, pools.up[0], pools.up[1], *idx, [0, 1], pools.a_scaling)
@@ -109,7 +136,7 @@ def layer_forward(x: torch.Tensor, w: LayerWeights, pools: Optional[LayerPools],
     d = torch.mm(m, w.w_down)
     if lora:
         plans.m.apply(d, m, pools.down[0], pools.down[1], *idx, 0, pools.a_scaling)
-    return x + d
+    return join(x, d, w.post2, w.gate2, None)[0] if fused else x + d
 
 
 def segment_attention(seq_lens, heads: int) -> Callable[[torch.Tensor, torch.Tensor, torch.Tensor], torch.Tensor]:

@@ -111,3 +111,10 @@ class Rotary:
         (int64, as ``MemoryAllocator.alloc`` returns it) names each row at most once; a token whose row is outside the
         buffers is not stored."""
         self._native.store(positions, q, k, v, key_buffer, value_buffer, loc, q_out)
+
+    def store8(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_codes: torch.Tensor,
+               value_codes: torch.Tensor, powers: torch.Tensor, loc: torch.Tensor, q_out: Optional[torch.Tensor] = None) -> None:
+        """``store`` into the cache of 8-bit codes (``valora_amd.cache8``): token t's rotated k and its v go to slot ``loc[t]`` (int64, page
+        times page size plus the place in the page; each at most once, those outside the cache are not stored).  ``head_dim`` is one that
+        attention takes.  k is rotated in 64 bits and rounded once, to the nearest code; q as ``store`` does, up to the last bit."""
+        self._native.store8(positions, q, k, v, key_codes, value_codes, powers, loc, q_out)
