@@ -57,6 +57,8 @@ struct AttnArgs {
   uint32_t e_stride;
   float c;                             // scale * log2(e)
   int tall_blocks;                     // workgroups of the tall list; those of the other follow
+  int max_few;                         // records that the other has room for
+  int heads_together;                  // codes: a piece's key heads go to one XCD
   int q_heads, kv_heads, group, page_shift, window, n_req, n_pages;
   int off_few, off_tall, off_joins, off_tall_joins, off_arrive, off_requests, off_shares;      // of the plan, words
 };
@@ -304,64 +306,66 @@ struct TileCodes {
 };
 
 // A wave's tile of 32 tokens.  K goes into the first product as it comes: lane (row, kg) holds, of tokens `row` and 16 + row, the 16 elements
-// from 16 kg on of each 64, and the 8 from 8 kg on of 32 that are left; q is read in that order too.
+// from 16 kg on of each 64, and the 8 from 8 kg on of 32 that are left; q is read in that order too.  Powers are loaded once a token,
+// by lane token and token + 32, and go round by ds_bpermute: loaded by each lane that needs one, they were 40 % of the look-ups
+// in the L1 (256 requests of 200 to 2000 tokens, 32 heads, 344 us; now 326).  What is left of their cost is lines: 13 us of the 326 for those
+// that hold the powers of a page of 2 tokens, which every XCD reads.  The loads of this loop without its work take 319, of 1.70 GB; with
+// codes of two tiles on their way (at 234 registers) it is no faster.
 template <int D>
 struct WaveCodes {
   static constexpr int B = D / 64, REST = D % 64 / 32, P = D / 16, EACH = D / 32;
   u32x4 k[2][B + 1], v[EACH];
   u32x2 rest[2];
-  uint32_t e[2], ve[EACH];
+  uint32_t e;
 
   // first element of the lane's eight of chunk i
   static __device__ __forceinline__ int element(int i, int kg) { return i < 2 * B ? i / 2 * 64 + kg * 16 + i % 2 * 8 : B * 64 + kg * 8; }
   __device__ __forceinline__ void load(const Cache &c, int base, uint32_t slice, int lane) {
     const int lrow = lane & 15, kg = lane >> 4;
     int32_t pages[2], vpages[EACH];
+    const int32_t its = lds_word(slice + (lane & 31) * 4);
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) pages[tt] = lds_word(slice + (tt * 16 + lrow) * 4);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) vpages[i] = lds_word(slice + (i * 64 + lane) / P * 4);
+    e = Slot<D>(c, base + (lane & 31), its).powers(c);
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      const Slot<D> s(c, base + tt * 16 + lrow, pages[tt]);
-      const char *p = s.k(c);
+      const char *p = Slot<D>(c, base + tt * 16 + lrow, pages[tt]).k(c);
 #pragma unroll
       for (int b = 0; b < B; ++b) k[tt][b] = *reinterpret_cast<const u32x4 *>(p + b * 64 + kg * 16);
       if constexpr (REST) rest[tt] = *reinterpret_cast<const u32x2 *>(p + B * 64 + kg * 8);
-      e[tt] = s.powers(c);
     }
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int unit = i * 64 + lane, t = unit / P, piece = unit - t * P;
-      const Slot<D> s(c, base + t, vpages[i]);
-      v[i] = *reinterpret_cast<const u32x4 *>(s.v(c) + piece * 16);
-      ve[i] = s.powers(c);
+      v[i] = *reinterpret_cast<const u32x4 *>(Slot<D>(c, base + t, vpages[i]).v(c) + piece * 16);
     }
     requested();
   }
+  __device__ __forceinline__ uint32_t powers(int token) const { return (uint32_t)__builtin_amdgcn_ds_bpermute(token * 4, (int)e); }
   __device__ __forceinline__ void keys_arrived() {
+    arrived(e);
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
       for (int b = 0; b < B; ++b) arrived(k[tt][b]);
       if constexpr (REST) arrived(rest[tt]);
-      arrived(e[tt]);
     }
   }
   template <typename T>
-  __device__ __forceinline__ typename Traits<T>::vec8 key(int tt, int i) const {
+  __device__ __forceinline__ typename Traits<T>::vec8 key(int tt, int i, float power) const {
     const u32x2 w = i < 2 * B ? u32x2{k[tt][i / 2][i % 2 * 2], k[tt][i / 2][i % 2 * 2 + 1]} : rest[tt];
-    return values_of<T>(w, k_power(e[tt]));
+    return values_of<T>(w, power);
   }
   template <typename T>
   __device__ __forceinline__ void write_values(uint32_t vt, int lane) {
+    uint32_t ve[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) ve[i] = powers((i * 64 + lane) / P);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       arrived(v[i]);
-      arrived(ve[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
       const int unit = i * 64 + lane, t = unit / P, piece = unit - t * P;
       write_codes<T, D>(vt, t, Tile<D>::v_turn(t), piece, v[i], v_power(ve[i]));
     }
@@ -576,12 +580,15 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     if constexpr (CODES) codes.keys_arrived();
     else wait_vmcnt<EACH + 1>();
     f32x4 s[2];
+    [[maybe_unused]] uint32_t powers[2];
+    if constexpr (CODES)
+      for (int tt = 0; tt < 2; ++tt) powers[tt] = codes.powers(tt * 16 + lrow);
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
       s[tt] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        if constexpr (CODES) s[tt] = Traits<T>::mfma(codes.template key<T>(tt, i), q[i], s[tt]);
+        if constexpr (CODES) s[tt] = Traits<T>::mfma(codes.template key<T>(tt, i, k_power(powers[tt])), q[i], s[tt]);
         else s[tt] = Traits<T>::mfma(as<vec8>(lds16(L::k_at(kt, lrow, kg, i * 4) + tt * 16 * L::ROW)), q[i], s[tt]);
       }
     }
@@ -1034,6 +1041,13 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attend_kernel(AttnA
   __shared__ __align__(256) char lds[ROOM];
   const bool tall = LISTS == TALL_LIST || (LISTS != FEW_LIST && (int)blockIdx.x < a.tall_blocks);
   const unsigned block = blockIdx.x - (tall ? 0 : a.tall_blocks);
+  if (CODES && !tall && a.heads_together) {
+    // Eight pieces at a time, all of whose heads follow each other on an XCD
+    const unsigned each = 8 * (unsigned)a.kv_heads, eight = block / each, rest = block - eight * each;
+    const int rec = (int)(eight * 8 + (rest & 7));
+    if (rec < a.max_few) few_tile<T, D, SUMS, CODES>(a, lds, rec, (int)(rest >> 3));
+    return;
+  }
   // the key heads of a piece follow each other: they read the same pages, and what reads the same head's rows again is eight, or a
   // multiple of it, further where kv_heads is: on the same XCD
   const int i = (int)(block / (unsigned)a.kv_heads), head = (int)(block - (unsigned)i * a.kv_heads);
@@ -1052,9 +1066,14 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attend_kernel(AttnA
 
 template <typename T, int D, bool SUMS, bool CODES>
 int launch_lists(hipStream_t st, const AttnLayout &L, AttnArgs a) {
-  const int64_t few = L.max_few * a.kv_heads, tall = L.max_shares * a.kv_heads;
+  // A head's codes of a page that are no whole lines share one with the next head's: those heads' workgroups go to one XCD, whose L2
+  // then has the line.  (64 requests of 2000 tokens, 8 key heads, pages of 2, us apart / together: heads of 32 30.4 / 20.6, of 96 58.7 / 55.2;
+  // whole lines: 32 heads of 128, 256 requests 343 / 358, as a page is then read by one XCD alone.)
+  a.heads_together = CODES && ((D << a.page_shift) & 127) != 0;
+  const int64_t few = (a.heads_together ? align_up(L.max_few, 8) : L.max_few) * a.kv_heads, tall = L.max_shares * a.kv_heads;
   if (few + tall > 0x7fffffff) return fail(MLORA_ERR_NO_KERNEL, "paged_attention: too many tiles");
   a.tall_blocks = (int)tall;
+  a.max_few = (int)L.max_few;
   // both lists in one kernel do not fit the scalar registers at 256; decoding over codes has a kernel without the room that tall tiles take
   const bool together = D <= 128 && (!CODES || tall > 0);
   if constexpr (D <= 128) {
