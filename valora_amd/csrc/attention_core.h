@@ -1041,17 +1041,17 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attend_kernel(AttnA
   __shared__ __align__(256) char lds[ROOM];
   const bool tall = LISTS == TALL_LIST || (LISTS != FEW_LIST && (int)blockIdx.x < a.tall_blocks);
   const unsigned block = blockIdx.x - (tall ? 0 : a.tall_blocks);
-  if (CODES && !tall && a.heads_together) {
-    // Eight pieces at a time, all of whose heads follow each other on an XCD
-    const unsigned each = 8 * (unsigned)a.kv_heads, eight = block / each, rest = block - eight * each;
-    const int rec = (int)(eight * 8 + (rest & 7));
-    if (rec < a.max_few) few_tile<T, D, SUMS, CODES>(a, lds, rec, (int)(rest >> 3));
-    return;
-  }
   // the key heads of a piece follow each other: they read the same pages, and what reads the same head's rows again is eight, or a
   // multiple of it, further where kv_heads is: on the same XCD
-  const int i = (int)(block / (unsigned)a.kv_heads), head = (int)(block - (unsigned)i * a.kv_heads);
+  int i = (int)(block / (unsigned)a.kv_heads), head = (int)(block - (unsigned)i * a.kv_heads);
   if (!tall) {
+    if (CODES && a.heads_together) {
+      // eight pieces at a time, all of whose heads follow each other on an XCD
+      const int in8 = (i & 7) * a.kv_heads + head;
+      i = (i & ~7) + (in8 & 7);
+      head = in8 >> 3;
+      if (i >= a.max_few) return;
+    }
     few_tile<T, D, SUMS, CODES>(a, lds, i, head);
     return;
   }
