@@ -1,9 +1,13 @@
 // The 8-bit cache (csrc/codes8.h) written and read back.
 //
-// Writing: as csrc/rotary.hip, but k and v become codes on their way to their slots.  A lane owns eight elements of a head, so a head is up to
-// 32 lanes of a wave, which find its largest element among themselves; a rotated element's partner is loaded a second time (it is in
-// the L1).  k is rotated in 64 bits, sines and all, and rounded once, to its code: in 32 bits one code in some hundred thousand would be a
-// neighbour of the nearest, a sixteenth off, and the vector units do 64 bits at the rate of 32.
+// Writing: as csrc/rotary.hip, but k and v become codes on their way to their slots.  A lane owns eight pairs of a head (both halves of it, so
+// nothing is loaded twice) or eight elements that pass through; a head's lanes are neighbours in a wave and find its largest element among
+// themselves.  k is rotated in 64 bits, sines and all, and rounded once, to its code: in 32 bits one code in some hundred thousand would be a
+// neighbour of the nearest, a sixteenth off, and the vector units do 64 bits at half the rate of 32.
+//
+// Bound by bytes (8191 tokens, 32 query and 8 key heads of 128, bf16: 185 MB in 40 us, 4.6 TB/s; a copy of as much takes 36).  Four tokens a
+// workgroup share one wait for positions, frequencies and sines (a token a workgroup: 49 us; two and eight: 41), and a lane that owned eight
+// elements and loaded their partners a second time took 55: half of it were the vector units.
 #include "codes8.h"
 
 namespace mlora {
@@ -17,118 +21,228 @@ struct StoreArgs {
   mlora_cache8 c;
   const int64_t *positions, *loc;
   const double *freqs;
-  int64_t n_slots;
+  int64_t n_slots, T;
   float gain;
-  int rotary_dim, page_shift;
+  int rotary_dim, page_shift, lane_shift;
   int heads, per_piece;                 // k's, v's and q's; of a workgroup
 };
 
 constexpr int ST_THREADS = 256;
+constexpr int MANY = 512;               // tokens: from here on a workgroup has four, below it a round of heads of one
 
-// pairs of the lane's elements: element at + i is turned with `other` of a pair's sine and cosine
-template <typename T, typename F, int D, bool INTERLEAVED, bool VEC, typename Table>
-__device__ __forceinline__ void turn(const StoreArgs &a, const uint16_t *head, int at, const Table *cs, F (&out)[8], bool rotate) {
-  const int R = rotate ? a.rotary_dim : 0;
-  uint16_t x[8], y[8];
-  if constexpr (VEC) {
-    const bool turned = at < R;
-    const u32x4 mine = load16(head + at), its = !INTERLEAVED && turned ? load16(head + (at < R / 2 ? at + R / 2 : at - R / 2)) : mine;
+// A lane's part of a head: n elements from a0 on and, where they are the first halves of pairs, as many from a1 on
+struct Part {
+  int a0, a1, n;
+  __device__ __forceinline__ Part(int lane, int D, int R, bool interleaved) {
+    const int turned = interleaved ? (R + 7) / 8 : (R / 2 + 7) / 8;         // parts that are rotated
+    if (lane < turned) {
+      a0 = lane * 8;
+      a1 = interleaved ? -1 : a0 + R / 2;
+      n = min(8, (interleaved ? R : R / 2) - a0);
+    } else {
+      a0 = R + (lane - turned) * 8;
+      a1 = -1;
+      n = min(8, D - a0);                                                    // (none, or less: a lane behind the head)
+    }
+  }
+};
+
+// (how many there are, as if it had just been found: comparisons kept from one use to the next would fill the scalar registers)
+__device__ __forceinline__ int anew(int n) {
+  asm volatile("" : "+v"(n));
+  return n;
+}
+template <bool VEC>
+__device__ __forceinline__ u32x4 load_eight(const uint16_t *p, int n) {
+  if constexpr (VEC) return load16(p);
+  u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = (uint16_t)(mine[i / 2] >> i % 2 * 16);
-      const int j = INTERLEAVED ? i ^ 1 : i;
-      y[i] = (uint16_t)(its[j / 2] >> j % 2 * 16);
+  for (int i = 0; i < 4; ++i) r[i] = (uint32_t)p[min(2 * i, n - 1)] | (uint32_t)p[min(2 * i + 1, n - 1)] << 16;
+  return r;
+}
+template <bool VEC>
+__device__ __forceinline__ void store_eight(uint16_t *p, int n, u32x4 x) {
+  if constexpr (VEC) {
+    store16(p, x);
+  } else {
+    n = anew(n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = (uint16_t)(x[i / 2] >> i % 2 * 16);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store_codes(char *p, int n, u32x2 x) {
+  if constexpr (VEC) {
+    *reinterpret_cast<u32x2 *>(p) = x;
+  } else {
+    n = anew(n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = (char)(x[i / 4] >> i % 4 * 8);
+  }
+}
+
+struct Loaded {
+  u32x4 a, b;
+};
+
+// Where the sine and cosine of a pair stand in LDS: those of eight lanes' pairs i, i + 1 side by side (lanes that read 8 of them in a row would
+// meet in the banks)
+template <int PAIRS>
+__device__ __forceinline__ int place_of(int pair) { return (((pair & 7) >> 1) * (PAIRS / 8) + (pair >> 3)) * 2 + (pair & 1); }
+
+// Rotates a lane's pairs: a (and b) in, out of them; in F, with sines of F
+template <typename T, typename F, bool INTERLEAVED, typename Sines>
+__device__ __forceinline__ void turn(const Loaded &p, Sines sines, F (&a)[8], F (&b)[8]) {
+  float f[8], g[8];
+  unpack8<T>(p.a, f);
+  if constexpr (INTERLEAVED) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto t = sines(i);
+      a[2 * i] = (F)f[2 * i] * t.x - (F)f[2 * i + 1] * t.y;
+      a[2 * i + 1] = (F)f[2 * i] * t.y + (F)f[2 * i + 1] * t.x;
     }
   } else {
+    unpack8<T>(p.b, g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int e = at + i, o = e >= R ? e : INTERLEAVED ? e ^ 1 : e < R / 2 ? e + R / 2 : e - R / 2;
-      x[i] = head[e];
-      y[i] = head[o];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int e = at + i;
-    const F f = (F)Traits<T>::to_float(x[i]), g = (F)Traits<T>::to_float(y[i]);
-    if (e < R) {
-      const bool second = INTERLEAVED ? e & 1 : e >= R / 2;
-      const Table t = cs[INTERLEAVED ? e / 2 : second ? e - R / 2 : e];
-      out[i] = second ? g * (F)t.y + f * (F)t.x : f * (F)t.x - g * (F)t.y;
-    } else {
-      out[i] = f;
+      const auto t = sines(i);
+      a[i] = (F)f[i] * t.x - (F)g[i] * t.y;
+      b[i] = (F)f[i] * t.y + (F)g[i] * t.x;
     }
   }
 }
 
-template <typename T, int D, typename F>
-__device__ __forceinline__ void keep(const StoreArgs &a, const F (&x)[8], bool mine, int64_t slot, int head, int at, int which) {
-  constexpr int LANES = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32;
-  float largest = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const F size = x[i] < 0 ? -x[i] : x[i];
-    if (mine && size < (F)INFINITY) largest = fmaxf(largest, not_below(size));
-  }
-#pragma unroll
-  for (int d = 1; d < LANES; d <<= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
-  if (!mine || slot < 0) return;
-  const uint32_t byte = power_byte<T>(largest);
-  const int64_t page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
-  char *codes = static_cast<char *>(which ? a.c.value_codes : a.c.key_codes) + page * (which ? a.c.value_stride : a.c.key_stride);
-  *reinterpret_cast<u32x2 *>(codes + (((int64_t)head << a.page_shift) + off) * D + at) = codes_of(x, byte);
-  if (at == 0) (static_cast<uint8_t *>(a.c.powers) + page * a.c.powers_stride)[(((int64_t)head << a.page_shift) + off) * 2 + which] = (uint8_t)byte;
-}
-
-template <typename T, int D, bool INTERLEAVED, bool VEC>
+// TOKENS of a workgroup: their sines are worked out together, a thread a pair, and their heads follow each other
+template <typename T, int D, bool INTERLEAVED, bool VEC, int TOKENS>
 __global__ __launch_bounds__(ST_THREADS) void store8_kernel(StoreArgs a) {
-  constexpr int LANES = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32, HEADS = ST_THREADS / LANES;
-  __shared__ double2 cs[D / 2];
-  const int64_t token = blockIdx.x;
-  int64_t slot = a.loc[token];
-  if (slot >= a.n_slots) slot = -1;
-  const int64_t pos = a.positions[token];
-  for (int i = threadIdx.x; i < a.rotary_dim / 2; i += ST_THREADS) {
-    const double turns = (double)pos * a.freqs[i];
+  constexpr int PAIRS = D / 2;
+  __shared__ __align__(16) double2 cs[TOKENS * PAIRS];
+  __shared__ __align__(16) float2 cs32[TOKENS * PAIRS];
+  __shared__ int64_t slots[TOKENS];
+  const int64_t first = (int64_t)blockIdx.x * TOKENS;
+  const int tokens = (int)min<int64_t>(TOKENS, a.T - first);
+  const int kv = a.c.kv_heads, R = a.rotary_dim, heads = ST_THREADS >> a.lane_shift, lanes = 1 << a.lane_shift;
+  const Part part((int)threadIdx.x & (lanes - 1), D, R, INTERLEAVED);
+  const bool rotates = part.a0 < R && part.n > 0, both = part.a1 >= 0;
+  const int lo = blockIdx.y * a.per_piece, hi = min(lo + a.per_piece, a.heads);
+  // heads in the order k's, v's, q's; a round's are asked for while those before are worked on, the first ones before the sines
+  struct Item {
+    int t, h;
+  };
+  auto load = [&](const Item &n) {
+    Loaded p{};
+    if (part.n > 0 && n.t < tokens) {
+      const int64_t token = first + n.t;
+      const uint16_t *src = n.h < kv ? a.k + token * a.k_token + n.h * a.k_head
+                            : n.h < 2 * kv ? a.v + token * a.v_token + (n.h - kv) * a.v_head
+                                           : static_cast<const uint16_t *>(a.q.src) + token * a.q.src_token_stride + (n.h - 2 * kv) * a.q.src_head_stride;
+      p.a = load_eight<VEC>(src + part.a0, part.n);
+      if (both) p.b = load_eight<VEC>(src + part.a1, part.n);
+    }
+    return p;
+  };
+  auto settle = [&](Item &n) {                                   // a head behind the last is one of the next token
+    while (n.h >= hi && n.t < tokens) {
+      n.h -= hi - lo;
+      ++n.t;
+    }
+  };
+  Item item{0, lo + ((int)threadIdx.x >> a.lane_shift)};
+  settle(item);
+  Loaded next = load(item);
+  requested();
+  for (int i = threadIdx.x; i < TOKENS * PAIRS; i += ST_THREADS) {
+    const int t = i / PAIRS, pair = i - t * PAIRS;
+    if (pair >= R / 2 || t >= tokens) continue;
+    const double turns = (double)a.positions[first + t] * a.freqs[pair];
     double s, c;
     sincospi(2.0 * (turns - rint(turns)), &s, &c);
-    cs[i] = double2{c * (double)a.gain, s * (double)a.gain};
+    const double2 v{c * (double)a.gain, s * (double)a.gain};
+    const int at = t * PAIRS + place_of<PAIRS>(pair);
+    cs[at] = v;
+    cs32[at] = float2{(float)v.x, (float)v.y};
+  }
+  if (threadIdx.x < TOKENS && (int)threadIdx.x < tokens) {
+    const int64_t slot = a.loc[first + threadIdx.x];
+    slots[threadIdx.x] = slot < a.n_slots ? slot : -1;
   }
   __syncthreads();
-  const int lane = threadIdx.x & (LANES - 1), at = lane * 8, kv = a.c.kv_heads;
-  const bool mine = at < D;                                      // (heads of 96 have twelve lanes of sixteen)
-  const int lo = blockIdx.y * a.per_piece, hi = min(lo + a.per_piece, a.heads);
-  for (int h0 = lo; h0 < hi; h0 += HEADS) {                      // (every lane goes round as often: they look at each other's)
-    const int h = h0 + (int)threadIdx.x / LANES;
-    const bool has = mine && h < hi;
-    if (h < kv) {
-      double x[8] = {};
-      if (has) turn<T, double, D, INTERLEAVED, VEC>(a, a.k + token * a.k_token + h * a.k_head, at, cs, x, true);
-      keep<T, D>(a, x, has, slot, h, at, 0);
-    } else if (h < 2 * kv) {
-      float x[8] = {};
-      if (has) turn<T, float, D, INTERLEAVED, VEC>(a, a.v + token * a.v_token + (h - kv) * a.v_head, at, cs, x, false);
-      keep<T, D>(a, x, has, slot, h - kv, at, 1);
-    } else if (has) {
-      const int64_t head = h - 2 * kv;
-      float x[8];
-      turn<T, float, D, INTERLEAVED, VEC>(a, static_cast<const uint16_t *>(a.q.src) + token * a.q.src_token_stride + head * a.q.src_head_stride, at, cs, x, true);
-      uint16_t *dst = static_cast<uint16_t *>(a.q.dst) + token * a.q.dst_token_stride + head * a.q.dst_head_stride + at;
-      if constexpr (VEC) {
-        store16(dst, pack8<T>(x));
-      } else {
+  const int pair0 = rotates ? (INTERLEAVED ? part.a0 / 2 : part.a0) : 0;
+  const int rounds = (tokens * (hi - lo) + heads - 1) / heads;
+  for (int r = 0; r < rounds; ++r) {                             // (every lane goes round as often: they look at each other's)
+    const Loaded p = next;
+    const Item n = item;
+    item.h += heads;
+    settle(item);
+    next = load(item);
+    requested();
+    const bool has = part.n > 0 && n.t < tokens;
+    const int t = min(n.t, tokens - 1), h = n.h;
+    float x[8], y[8];
+    if (h >= 2 * kv) {
+      if (!has) continue;                                        // (q's lanes look at no other's)
+      u32x4 first8 = p.a, second8 = p.b;
+      if (rotates) {
+        turn<T, float, INTERLEAVED>(p, [&](int i) { return cs32[t * PAIRS + place_of<PAIRS>(pair0 + i)]; }, x, y);
+        first8 = pack8<T>(x);
+        if constexpr (!INTERLEAVED) second8 = pack8<T>(y);
+      }
+      uint16_t *dst = static_cast<uint16_t *>(a.q.dst) + (first + t) * a.q.dst_token_stride + (h - 2 * kv) * a.q.dst_head_stride;
+      store_eight<VEC>(dst + part.a0, part.n, first8);
+      if (both) store_eight<VEC>(dst + part.a1, part.n, second8);
+      continue;
+    }
+    float largest = 0.0f;
+    if (h < kv && rotates) {
+      double u[8], w[8];
+      const int some = VEC ? 8 : anew(part.n);
+      turn<T, double, INTERLEAVED>(p, [&](int i) { return cs[t * PAIRS + place_of<PAIRS>(pair0 + i)]; }, u, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dst[i] = Traits<T>::from_float(x[i]);
+      for (int i = 0; i < 8; ++i) {
+        x[i] = sticky(u[i]);
+        if (i < some && fabs(u[i]) < (double)INFINITY) largest = fmaxf(largest, fabsf(x[i]));      // (one beyond 32 bits counts, as the largest)
+        if constexpr (!INTERLEAVED) {
+          y[i] = sticky(w[i]);
+          if (i < some && fabs(w[i]) < (double)INFINITY) largest = fmaxf(largest, fabsf(y[i]));
+        }
+      }
+    } else {
+      unpack8<T>(p.a, x);
+      unpack8<T>(p.b, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (fabsf(x[i]) < INFINITY) largest = fmaxf(largest, fabsf(x[i]));
+        if (fabsf(y[i]) < INFINITY) largest = fmaxf(largest, fabsf(y[i]));
       }
     }
+    for (int d = 1; d < lanes; d <<= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
+    const int64_t slot = slots[t];
+    if (!has || slot < 0) continue;
+    const uint32_t byte = power_byte<T>(largest);
+    const int which = h >= kv;
+    const int64_t page = slot >> a.page_shift, row = ((int64_t)(h - which * kv) << a.page_shift) + (slot & ((1 << a.page_shift) - 1));
+    char *codes = static_cast<char *>(which ? a.c.value_codes : a.c.key_codes) + page * (which ? a.c.value_stride : a.c.key_stride) + row * D;
+    store_codes<VEC>(codes + part.a0, part.n, codes_of(x, byte));
+    if (both) store_codes<VEC>(codes + part.a1, part.n, codes_of(y, byte));
+    if (part.a0 == 0) (static_cast<uint8_t *>(a.c.powers) + page * a.c.powers_stride)[row * 2 + which] = (uint8_t)byte;
   }
+}
+
+template <typename T, int D, int TOKENS>
+void launch_store(hipStream_t st, dim3 grid, const StoreArgs &a, bool interleaved, bool vec) {
+  auto *k = interleaved ? (vec ? store8_kernel<T, D, true, true, TOKENS> : store8_kernel<T, D, true, false, 1>)
+                        : (vec ? store8_kernel<T, D, false, true, TOKENS> : store8_kernel<T, D, false, false, 1>);
+  if (vec) grid.x = (grid.x + TOKENS - 1) / TOKENS;
+  hipLaunchKernelGGL(k, grid, dim3(ST_THREADS), 0, st, a);
 }
 
 template <typename T, int D>
 void launch_store(hipStream_t st, dim3 grid, const StoreArgs &a, bool interleaved, bool vec) {
-  auto *k = interleaved ? (vec ? store8_kernel<T, D, true, true> : store8_kernel<T, D, true, false>)
-                        : (vec ? store8_kernel<T, D, false, true> : store8_kernel<T, D, false, false>);
-  hipLaunchKernelGGL(k, grid, dim3(ST_THREADS), 0, st, a);
+  if (a.T >= MANY) launch_store<T, D, 4>(st, grid, a, interleaved, vec);
+  else launch_store<T, D, 1>(st, grid, a, interleaved, vec);
 }
 
 template <typename T>
@@ -261,13 +375,16 @@ extern "C" int mlora_rotary_store_codes(void *stream, const mlora_rotary_part *q
   a.loc = loc;
   a.freqs = freqs;
   a.n_slots = cache->n_pages * cache->page_size;
+  a.T = T;
   a.gain = gain;
   a.rotary_dim = rotary_dim;
   a.page_shift = log2_of(cache->page_size);
   a.heads = 2 * cache->kv_heads + q_heads;
+  // lanes of a head: a power of two, so that they find each other by exchanging bits
+  a.lane_shift = log2_of((interleaved ? (rotary_dim + 7) / 8 : (rotary_dim / 2 + 7) / 8) + (d - rotary_dim + 7) / 8);
   // Few tokens: a workgroup a round of heads, as in csrc/rotary.hip
-  const int per_round = ST_THREADS / (d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32);
-  const int rounds = (a.heads + per_round - 1) / per_round, pieces = T >= 512 ? 1 : rounds;
+  const int per_round = ST_THREADS >> a.lane_shift;
+  const int rounds = (a.heads + per_round - 1) / per_round, pieces = T >= MANY ? 1 : rounds;
   a.per_piece = (rounds + pieces - 1) / pieces * per_round;
   const dim3 grid((unsigned)T, (unsigned)((a.heads + a.per_piece - 1) / a.per_piece));
   if (dtype == MLORA_F16) launch_store<_Float16>((hipStream_t)stream, grid, a, interleaved != 0, vec);

@@ -48,35 +48,21 @@ __device__ __forceinline__ uint32_t power_byte(float largest) {
   const int e = (int)((as<uint32_t>(largest) + 0x1fffffu) >> 23) - 8;
   return (uint32_t)min(max(e, Powers<T>::LOWEST + 127), Powers<T>::HIGHEST + 127);
 }
-// The least float that is not below x >= 0
-__device__ __forceinline__ float not_below(double x) {
-  const float f = (float)x;
-  return (double)f < x ? as<float>(as<uint32_t>(f) + 1) : f;
-}
-__device__ __forceinline__ float not_below(float x) { return x; }
-// x in 32 bits for a conversion that is still to come: cut off, with the last bit set where something was, so that what is next to the border of
-// two codes stays on its side of it
+// x in 32 bits for a conversion that is still to come: its first 20 bits behind the point, with the last of them set where more followed, so that
+// what is next to the border of two codes, or above a power's largest value, stays on its side of it
 __device__ __forceinline__ float sticky(double x) {
-  float f = (float)x;
-  if ((double)f != x) {
-    const uint32_t b = as<uint32_t>(f) - (fabs((double)f) > fabs(x) ? 1u : 0u);
-    f = as<float>(b | 1u);
-  }
-  return f;
+  const uint64_t b = as<uint64_t>(x);
+  const uint32_t hi = (uint32_t)(b >> 32) | ((uint32_t)b ? 1u : 0u);
+  return (float)as<double>((uint64_t)hi << 32);
 }
-__device__ __forceinline__ float sticky(float x) { return x; }
 // Eight elements as codes of the power 2^(byte - 127)
-template <typename F>
-__device__ __forceinline__ u32x2 codes_of(const F (&x)[8], uint32_t byte) {
-  F down;                                          // 2^(127 - byte)
-  if constexpr (sizeof(F) == 8) down = as<double>((uint64_t)(1023 + 127 - byte) << 52);
-  else down = as<float>((254u - byte) << 23);
+__device__ __forceinline__ u32x2 codes_of(const float (&x)[8], uint32_t byte) {
+  const float down = as<float>((254u - byte) << 23);
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const F z = x[i] * down;
-    const float f = sticky(z > (F)448 ? (F)448 : z < (F)-448 ? (F)-448 : z);
-    y[i] = z != z ? NAN : f;
+    const float z = x[i] * down;
+    y[i] = z != z ? z : __builtin_amdgcn_fmed3f(z, -448.0f, 448.0f);
   }
   u32x2 r;
 #pragma unroll
