@@ -3,6 +3,10 @@
 //
 // A row is held in the registers of one workgroup (or one wave) between its load and its stores; sums go over lanes, then waves, in a
 // fixed order and 32 bits.  Variances are of differences from the mean, after it: no sum of squares loses them.
+//
+// Bound by bytes where rows are many: 8191 of 4096 with a gate, 268 MB in 46.9 us, 5.7 TB/s (part of it from the memory-side cache; a copy runs at
+// 5.1).  Few rows are one row's chain: its loads, a sum for each norm, its stores: 256 of 5120 with two norms 4.7 us, one of 4096 2.9 of
+// GPU time, which a launch takes too.
 #include <type_traits>
 #include <utility>
 
@@ -12,22 +16,50 @@ namespace mlora {
 
 namespace {
 
+// Runs of eight: a thread has one of up to NORM_ONE, which keeps its registers few and loads all it needs at once; rows of more would be workgroups
+// of many waves that wait for each other (8191 of 5120, one / two runs a thread: 63.4 / 62.5 us, 2048 of 7168 32.9 / 29.2), unless they are few
+// and the chain counts (256 of 5120 4.7 / 5.3 us).
+constexpr int NORM_ONE = 512, NORM_FEW_ROWS = 512;
 constexpr int NORM_MAX = 32768, NORM_MAX_PLAIN = 16384;      // (wider rows element by element do not fit the registers)
 
-template <int WAVES>
-__device__ __forceinline__ float row_sum(float x, float *part) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  if constexpr (WAVES > 1) {
-    __syncthreads();                     // (what was summed before has been read)
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = 0.0f;
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) x += part[i];
-  }
-  return x;
+// What lane l holds, and what the lane holds whose number differs in one way each: by quads, halves and rows of sixteen, rows, halves.  (No exchange
+// goes through LDS, where a butterfly's six would wait one after the other.)
+template <int CTRL>
+__device__ __forceinline__ float plus_dpp(float x) {
+  return x + as<float>((uint32_t)__builtin_amdgcn_mov_dpp((int)as<uint32_t>(x), CTRL, 0xf, 0xf, true));
 }
+__device__ __forceinline__ float wave_sum(float x) {
+  x = plus_dpp<0xb1>(x);                 // quad_perm 1 0 3 2
+  x = plus_dpp<0x4e>(x);                 // quad_perm 2 3 0 1
+  x = plus_dpp<0x141>(x);                // row_half_mirror
+  x = plus_dpp<0x140>(x);                // row_mirror
+  typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+  const u32x2 rows = __builtin_amdgcn_permlane16_swap(as<uint32_t>(x), as<uint32_t>(x), false, false);
+  x = as<float>(rows[0]) + as<float>(rows[1]);
+  const u32x2 halves = __builtin_amdgcn_permlane32_swap(as<uint32_t>(x), as<uint32_t>(x), false, false);
+  return as<float>(halves[0]) + as<float>(halves[1]);
+}
+
+// Over a row's lanes: a wave's, or with MANY those of all the workgroup's waves, 16 at most.  Every sum of a row has sixteen places of its own (0
+// for waves that are not there), so one barrier each is enough.
+constexpr int SUMS = 4, PLACES = 16;
+template <bool MANY>
+struct RowSum {
+  float *part;
+  __device__ __forceinline__ float operator()(float x) {
+    x = wave_sum(x);
+    if constexpr (MANY) {
+      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+      __syncthreads();
+      f32x4 s = *reinterpret_cast<const f32x4 *>(part);
+#pragma unroll
+      for (int i = 4; i < PLACES; i += 4) s += *reinterpret_cast<const f32x4 *>(part + i);
+      x = (s[0] + s[1]) + (s[2] + s[3]);
+      part += PLACES;
+    }
+    return x;
+  }
+};
 
 // Eight elements from `at` on; those behind the row are 0
 template <typename T, bool VEC>
@@ -54,21 +86,42 @@ __device__ __forceinline__ void store_row(void *p, int64_t at, int left, const f
       if (i < left) d[i] = Traits<T>::from_float(x[i]);
   }
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_vector(const void *p, bool f32, int at, int left, float (&x)[8]) {
-  if (!f32) return load_row<T, VEC>(p, at, left, x);
-  const float *s = static_cast<const float *>(p) + at;
+// A vector of the call, a thread's V runs of it.  EARLY: asked for with the row (behind a sum it would be a round trip more: 8191 rows of 4096
+// with a gate 53.8 -> 47.1 us); where none is float and a thread has one run, as the registers of more would cost waves (two runs: 59.8 -> 76).
+// Otherwise loaded where it is used.
+template <typename T, bool VEC, int V, bool EARLY>
+struct Vector {
+  const void *p;
+  bool f32;
+  u32x4 x[EARLY ? V : 1];
+  __device__ __forceinline__ Vector(const void *p_, bool f32_, int tid, int step, int H) : p(p_), f32(f32_) {
+    if constexpr (EARLY)
+      if (p)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float f = s[min(i, left - 1)];
-    x[i] = i < left ? f : 0.0f;
+        for (int v = 0; v < V; ++v) {
+          const int at = tid * 8 + v * step;
+          x[v] = at < H ? load16(static_cast<const uint16_t *>(p) + at) : u32x4{0, 0, 0, 0};
+        }
   }
-}
+  __device__ __forceinline__ void get(int v, int at, int left, float (&f)[8]) const {
+    if constexpr (EARLY) {
+      unpack8<T>(x[v], f);
+    } else if (!f32) {
+      load_row<T, VEC>(p, at, left, f);
+    } else {
+      const float *s = static_cast<const float *>(p) + at;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float one = s[min(i, left - 1)];
+        f[i] = i < left ? one : 0.0f;
+      }
+    }
+  }
+};
 
 // x (of H elements, V runs of eight a thread) becomes its norm
-template <typename T, bool VEC, int WAVES, int V>
-__device__ __forceinline__ void normalise(float (&x)[V][8], const mlora_norm &n, const void *w, bool w32, const void *b, bool b32, int tid, float *part) {
-  constexpr int STEP = WAVES * 64 * 8;
+template <bool MANY, int V, typename Vec>
+__device__ __forceinline__ void normalise(float (&x)[V][8], const mlora_norm &n, const Vec &w, const Vec &b, int tid, int step, RowSum<MANY> &row_sum) {
   const int H = (int)n.H;
   const float inv = 1.0f / (float)H;
   float mean = 0.0f;
@@ -78,104 +131,103 @@ __device__ __forceinline__ void normalise(float (&x)[V][8], const mlora_norm &n,
     for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += x[v][i];
-    mean = row_sum<WAVES>(s, part) * inv;
+    mean = row_sum(s) * inv;
   }
   float s = 0.0f;
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      x[v][i] -= tid * 8 + v * STEP + i < H ? mean : 0.0f;
+      x[v][i] -= tid * 8 + v * step + i < H ? mean : 0.0f;
       s = fmaf(x[v][i], x[v][i], s);
     }
-  const float r = 1.0f / sqrtf(row_sum<WAVES>(s, part) * inv + n.eps);
+  const float r = 1.0f / sqrtf(row_sum(s) * inv + n.eps);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int at = tid * 8 + v * STEP;
-    float wv[8], bv[8];
-    load_vector<T, VEC>(w, w32, at, H - at, wv);
+    const int at = tid * 8 + v * step;
+    float f[8];
+    w.get(v, at, H - at, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[v][i] *= r * (n.offset + wv[i]);
-    if (b) {
-      load_vector<T, VEC>(b, b32, at, H - at, bv);
+    for (int i = 0; i < 8; ++i) x[v][i] *= r * (n.offset + f[i]);
+    if (b.p) {
+      b.get(v, at, H - at, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[v][i] += bv[i];
+      for (int i = 0; i < 8; ++i) x[v][i] += f[i];
     }
   }
 }
 
-// WAVES a row; where it is one, four rows a workgroup
-template <typename T, bool VEC, int WAVES, int V>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void block_norm_kernel(mlora_norm n) {
-  __shared__ float part[WAVES];
-  constexpr int ROWS = WAVES == 1 ? 4 : 1, STEP = WAVES * 64 * 8;
+// A workgroup a row, or a wave (four rows a workgroup)
+template <typename T, bool VEC, bool MANY, int V, bool EARLY>
+__global__ __launch_bounds__(MANY ? 1024 : 256) void block_norm_kernel(mlora_norm n) {
+  __shared__ __align__(16) float part[SUMS * PLACES];
+  RowSum<MANY> row_sum{part};
+  constexpr int ROWS = MANY ? 1 : 4;
+  const int step = MANY ? blockDim.x * 8 : 512;
+  using Vec = Vector<T, VEC, V, EARLY>;
   const int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x >> 6 : 0);
   if (row >= n.T) return;
   const int tid = ROWS > 1 ? threadIdx.x & 63 : threadIdx.x, H = (int)n.H;
-  float x[V][8];
+  if (MANY && tid < SUMS * PLACES && (tid & (PLACES - 1)) >= (int)blockDim.x >> 6) part[tid] = 0.0f;
+  float x[V][8], o[V][8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int at = tid * 8 + v * STEP;
+    const int at = tid * 8 + v * step;
+    if (n.block) load_row<T, VEC>(n.block, row * n.block_stride + at, H - at, o[v]);
     load_row<T, VEC>(n.x, row * n.x_stride + at, H - at, x[v]);
   }
+  const Vec bw(n.block_weight, n.f32 & MLORA_NORM_F32_BLOCK_WEIGHT, tid, step, H), bb(n.block_bias, n.f32 & MLORA_NORM_F32_BLOCK_BIAS, tid, step, H);
+  const Vec gate(n.gate && n.gate_column_stride ? static_cast<const char *>(n.gate) + row * n.gate_row_stride * (n.f32 & MLORA_NORM_F32_GATE ? 4 : 2) : nullptr,
+                 n.f32 & MLORA_NORM_F32_GATE, tid, step, H);
+  float row_gate = 1.0f;
+  if (n.gate && !n.gate_column_stride) {
+    const int64_t at = row * n.gate_row_stride;
+    row_gate = n.f32 & MLORA_NORM_F32_GATE ? static_cast<const float *>(n.gate)[at] : Traits<T>::to_float(static_cast<const uint16_t *>(n.gate)[at]);
+  }
+  const Vec w(n.weight, n.f32 & MLORA_NORM_F32_WEIGHT, tid, step, H), b(n.bias, n.f32 & MLORA_NORM_F32_BIAS, tid, step, H);
+  if (EARLY) requested();
   if (n.block) {
-    float o[V][8];
+    if (n.block_weight) normalise<MANY, V>(o, n, bw, bb, tid, step, row_sum);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int at = tid * 8 + v * STEP;
-      load_row<T, VEC>(n.block, row * n.block_stride + at, H - at, o[v]);
-    }
-    if (n.block_weight)
-      normalise<T, VEC, WAVES, V>(o, n, n.block_weight, n.f32 & MLORA_NORM_F32_BLOCK_WEIGHT, n.block_bias, n.f32 & MLORA_NORM_F32_BLOCK_BIAS, tid, part);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int at = tid * 8 + v * STEP;
-      if (n.gate) {
+      const int at = tid * 8 + v * step;
+      if (gate.p) {
         float g[8];
-        const bool f32 = n.f32 & MLORA_NORM_F32_GATE;
-        if (n.gate_column_stride) {
-          const char *p = static_cast<const char *>(n.gate) + row * n.gate_row_stride * (f32 ? 4 : 2);
-          load_vector<T, VEC>(p, f32, at, H - at, g);
-        } else {
-          const int64_t to = row * n.gate_row_stride;
-          const float one = f32 ? static_cast<const float *>(n.gate)[to] : Traits<T>::to_float(static_cast<const uint16_t *>(n.gate)[to]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = one;
-        }
+        gate.get(v, at, H - at, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[v][i] *= g[i];
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[v][i] = fmaf(n.block_scale, o[v][i], n.residual_scale * x[v][i]);
+      for (int i = 0; i < 8; ++i) x[v][i] = fmaf(n.block_scale, o[v][i] * row_gate, n.residual_scale * x[v][i]);
       if (n.residual_out) store_row<T, VEC>(n.residual_out, row * n.residual_stride + at, H - at, x[v]);
     }
   }
   if (!n.weight) return;
-  normalise<T, VEC, WAVES, V>(x, n, n.weight, n.f32 & MLORA_NORM_F32_WEIGHT, n.bias, n.f32 & MLORA_NORM_F32_BIAS, tid, part);
+  normalise<MANY, V>(x, n, w, b, tid, step, row_sum);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int at = tid * 8 + v * STEP;
+    const int at = tid * 8 + v * step;
     store_row<T, VEC>(n.out, row * n.out_stride + at, H - at, x[v]);
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool EARLY>
 int launch(hipStream_t st, const mlora_norm &n) {
   const int units = (int)((n.H + 7) / 8);
-  const auto go = [&](auto waves, auto v) {
-    constexpr int W = decltype(waves)::value, V = decltype(v)::value;
-    const int64_t blocks = W == 1 ? (n.T + 3) / 4 : n.T;
-    hipLaunchKernelGGL((block_norm_kernel<T, VEC, W, V>), dim3((unsigned)blocks), dim3(W == 1 ? 256 : W * 64), 0, st, n);
+  const auto go = [&](auto many, auto v) {
+    constexpr bool MANY = decltype(many)::value;
+    constexpr int V = decltype(v)::value;
+    const int64_t blocks = MANY ? n.T : (n.T + 3) / 4;
+    const int threads = MANY ? ((units + V - 1) / V + 63) / 64 * 64 : 256;
+    hipLaunchKernelGGL((block_norm_kernel<T, VEC, MANY, V, EARLY && V == 1>), dim3((unsigned)blocks), dim3((unsigned)threads), 0, st, n);
     return check_launch("block_norm_kernel");
   };
   using std::integral_constant;
-  if (units <= 64) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-  if (units <= 128) return go(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-  if (units <= 256) return go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  if (units <= 512) return go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-  if (units <= 1024) return go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
-  if (units <= 2048) return go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
-  if constexpr (VEC) return go(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  using one = integral_constant<int, 1>;
+  if (units <= 64) return go(std::false_type{}, one{});
+  if (units <= NORM_ONE || (units <= 1024 && n.T <= NORM_FEW_ROWS)) return go(std::true_type{}, one{});
+  if (units <= 2048) return go(std::true_type{}, integral_constant<int, 2>{});
+  if constexpr (VEC) return go(std::true_type{}, integral_constant<int, 4>{});
   return fail(MLORA_ERR_NO_KERNEL, "No suitable kernel. block_norm: H=%lld above %d needs rows of 16-byte multiples, 16-byte aligned", (long long)n.H, NORM_MAX_PLAIN);
 }
 
@@ -239,6 +291,7 @@ extern "C" int mlora_block_norm(void *stream, const mlora_norm *norm, mlora_dtyp
   mlora_norm m = n;
   if (!m.block) m.residual_scale = 1.0f;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == MLORA_F16) return vec ? launch<_Float16, true>(st, m) : launch<_Float16, false>(st, m);
-  return vec ? launch<__bf16, true>(st, m) : launch<__bf16, false>(st, m);
+  const bool early = vec && m.f32 == 0;
+  if (dtype == MLORA_F16) return early ? launch<_Float16, true, true>(st, m) : vec ? launch<_Float16, true, false>(st, m) : launch<_Float16, false, false>(st, m);
+  return early ? launch<__bf16, true, true>(st, m) : vec ? launch<__bf16, true, false>(st, m) : launch<__bf16, false, false>(st, m);
 }
