@@ -256,38 +256,37 @@ void launch_store(hipStream_t st, dim3 grid, const StoreArgs &a, bool interleave
   }
 }
 
-// ---- reading back: a thread sixteen codes of k and of v --------------------------------------------------------------------------------
+// ---- reading back: a thread eight codes of k and of v ----------------------------------------------------------------------------------
 struct ReadArgs {
   mlora_cache8 c;
   const int64_t *loc;
   uint16_t *k, *v;
   int64_t n, k_stride, v_stride;
-  int page_shift, pieces;               // of sixteen codes, of a token
+  int page_shift, pieces, tokens;       // of eight codes, of a token; of a workgroup
+  float inv_pieces, inv_each;
 };
+constexpr int READ_THREADS = 256;
 
 template <typename T>
-__global__ __launch_bounds__(256) void read8_kernel(ReadArgs a) {
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, token = unit / a.pieces;
-  if (token >= a.n) return;
-  const int part = (int)(unit - token * a.pieces), each = a.c.head_dim / 16;
-  const int head = part / each, at = (part - head * each) * 16;
+__global__ __launch_bounds__(READ_THREADS) void read8_kernel(ReadArgs a) {
+  uint32_t t, part, head, at;
+  divmod24(threadIdx.x, (uint32_t)a.pieces, a.inv_pieces, t, part);      // (t is 0 where a token has more pieces than a workgroup threads)
+  part += blockIdx.y * READ_THREADS;
+  const int64_t token = (int64_t)blockIdx.x * a.tokens + t;
+  if ((int)t >= a.tokens || token >= a.n || (int)part >= a.pieces) return;
+  divmod24(part, (uint32_t)a.c.head_dim / 8, a.inv_each, head, at);
+  at *= 8;
   const int64_t slot = a.loc[token], page = slot >> a.page_shift, row = ((int64_t)head << a.page_shift) + (slot & ((1 << a.page_shift) - 1));
-  u32x4 k[2] = {}, v[2] = {};
+  u32x4 k{}, v{};
   if (slot >= 0 && page < a.c.n_pages) {
-    const u32x4 kc = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(a.c.key_codes) + page * a.c.key_stride + row * a.c.head_dim + at);
-    const u32x4 vc = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(a.c.value_codes) + page * a.c.value_stride + row * a.c.head_dim + at);
+    const u32x2 kc = *reinterpret_cast<const u32x2 *>(static_cast<const char *>(a.c.key_codes) + page * a.c.key_stride + row * a.c.head_dim + at);
+    const u32x2 vc = *reinterpret_cast<const u32x2 *>(static_cast<const char *>(a.c.value_codes) + page * a.c.value_stride + row * a.c.head_dim + at);
     const uint32_t e = *reinterpret_cast<const uint16_t *>(static_cast<const char *>(a.c.powers) + page * a.c.powers_stride + row * 2);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      k[i] = as<u32x4>(values_of<T>(u32x2{kc[2 * i], kc[2 * i + 1]}, k_power(e)));
-      v[i] = as<u32x4>(values_of<T>(u32x2{vc[2 * i], vc[2 * i + 1]}, v_power(e)));
-    }
+    k = as<u32x4>(values_of<T>(kc, k_power(e)));
+    v = as<u32x4>(values_of<T>(vc, v_power(e)));
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    store16(a.k + token * a.k_stride + part * 16 + i * 8, k[i]);
-    store16(a.v + token * a.v_stride + part * 16 + i * 8, v[i]);
-  }
+  store16(a.k + token * a.k_stride + part * 8, k);
+  store16(a.v + token * a.v_stride + part * 8, v);
 }
 
 int log2_of(int n) {
@@ -403,13 +402,15 @@ extern "C" int mlora_cache_read_codes(void *stream, const mlora_cache8 *cache, c
   if (n > 1 && (k_stride < w || v_stride < w)) return fail(MLORA_ERR_INVALID, "%s: rows of k or v overlap", who);
   if ((k_stride | v_stride) & 7 || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15))
     return fail(MLORA_ERR_INVALID, "%s: rows of k and v must be multiples of 16 bytes and 16-byte aligned", who);
-  if (n > 0x7fffffffll * 256 / (w / 16)) return fail(MLORA_ERR_NO_KERNEL, "%s: n=%lld too large", who, (long long)n);
+  const int pieces = (int)(w / 8), tokens = pieces >= READ_THREADS ? 1 : READ_THREADS / pieces;
+  if (n > 0x7fffffffll * tokens) return fail(MLORA_ERR_NO_KERNEL, "%s: n=%lld too large", who, (long long)n);
   if (n == 0) return MLORA_OK;
   if (!loc || !k || !v) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
   if (cache->n_pages > 0 && (!cache->key_codes || !cache->value_codes || !cache->powers)) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
-  ReadArgs a{*cache, loc, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v), n, k_stride, v_stride, log2_of(cache->page_size), (int)(w / 16)};
-  const dim3 grid((unsigned)((n * a.pieces + 255) / 256));
-  if (dtype == MLORA_F16) hipLaunchKernelGGL((read8_kernel<_Float16>), grid, dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL((read8_kernel<__bf16>), grid, dim3(256), 0, (hipStream_t)stream, a);
+  ReadArgs a{*cache, loc, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v), n, k_stride, v_stride, log2_of(cache->page_size), pieces, tokens,
+             1.0f / (float)pieces, 8.0f / (float)cache->head_dim};
+  const dim3 grid((unsigned)((n + tokens - 1) / tokens), (unsigned)((pieces + READ_THREADS - 1) / READ_THREADS));
+  if (dtype == MLORA_F16) hipLaunchKernelGGL((read8_kernel<_Float16>), grid, dim3(READ_THREADS), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL((read8_kernel<__bf16>), grid, dim3(READ_THREADS), 0, (hipStream_t)stream, a);
   return check_launch("read8_kernel");
 }
