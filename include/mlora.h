@@ -521,7 +521,7 @@ typedef struct {
   int64_t gate_row_stride, gate_column_stride;      /* columns: 1, or 0 for one gate a row                   */
   void *residual_out, *out;                         /* each may be x or block (with its stride): a row is read before it is written */
   int64_t residual_stride, out_stride;
-  int64_t T, H;                                     /* H up to 32768 (16384 if rows are no 16-byte multiples, aligned) */
+  int64_t T, H;                                     /* H up to 32768                                         */
   float residual_scale, block_scale, eps, offset;
   int32_t layer, f32;
 } mlora_norm;

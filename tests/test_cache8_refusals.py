@@ -125,9 +125,6 @@ def test_norm():
                             (dict(gate=A + (1 << 23), gate_row_stride=64), -1, b"gate"), (dict(gate=A + (1 << 22) + 10), -1, b"gate"),
                             (dict(bias=A + (1 << 23)), -1, b"vector"), (dict(weight=A + (1 << 22) + 4 * 128 - 2), -1, b"vector")):
         assert L.mlora_block_norm(None, norm(**kw), 0) == rc and message in L.mlora_last_error(), (kw, L.mlora_last_error())
-    wide = dict(x_stride=20001, block_stride=20001, residual_stride=20001, out_stride=20001, block=1 << 30, weight=1 << 31, residual_out=1 << 32, out=1 << 33)
-    for kw in (dict(H=20001), dict(H=20000, x_stride=20001), dict(H=20000, weight=(1 << 31) + 2)):
-        assert L.mlora_block_norm(None, norm(**dict(wide, **kw)), 0) == -2 and b"above 16384" in L.mlora_last_error(), kw
     assert L.mlora_block_norm(None, norm(), 3) == -2 and b"dtype=3" in L.mlora_last_error()
     assert L.mlora_block_norm(None, None, 0) == -1
     assert L.mlora_block_norm(None, norm(T=0), 0) == 0

@@ -178,3 +178,39 @@ def test_no_result_depends_on_the_split(dev):
     c = coded(dev, 2, F16, 8, 2, 128, [(1, 3000), (1, 40), (64, 900)], seed=12)
     a, b = run(dev, c, 2), run(dev, c, 2)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (8, 8), (10, 5), (24, 3), (16, 16)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_weights_of_prompts_by_heads(dev, hq, hkv, window):
+    """Heads fewer and more than the waves that share them out, rows that do not divide."""
+    reqs = [(37, 300), (130, 130), (1, 200), (3, 70), (66, 65)]
+    c = coded(dev, 2, BF16, hq, hkv, 64, reqs, seed=13)
+    w = torch.zeros(len(reqs), c["table"].shape[1] * 2, device=dev)
+    _, want, bound = check(dev, c, 2, window, weights=w)
+    err = (w.cpu().double() - want).abs()
+    assert bool((err <= bound + 2.0 ** -22).all()), float((err - bound).max())
+
+
+def test_weights_where_the_scores_have_no_room(dev):
+    """More scores than the workspace's bound: the keys are read a second time."""
+    n, length = 200, 20000
+    g = torch.Generator(device="cpu").manual_seed(14)
+    hq, hkv, d, page = 32, 4, 32, 64
+    pages = 400
+    kb, vb = torch.randn(pages * page, hkv, d, generator=g), torch.randn(pages * page, hkv, d, generator=g)
+    kc, vc, powers, k, v = cache_of(kb, vb, page, BF16)
+    table = torch.randint(0, pages, (n, -(-length // page)), generator=g).to(torch.int32)
+    q = torch.randn(n, hq, d, generator=g).to(BF16)
+    i32 = lambda t: torch.tensor(t, dtype=torch.int32, device=dev)  # noqa: E731
+    plan = AttentionPlan(i32(range(n)), i32([1] * n), i32([length] * n), n_tokens=n, max_seq_len=1, max_kv_len=length, q_heads=hq, kv_heads=hkv,
+                         head_dim=d, page_size=page)
+    w = torch.zeros(n, length, device=dev)
+    out = torch.empty(n, hq, d, dtype=BF16, device=dev)
+    plan.attend8(out, q.to(dev), kc.to(dev), vc.to(dev), powers.to(dev), table.to(dev), weights=w)
+    torch.cuda.synchronize()
+    for b in (0, 117, 199):
+        want, weights, bound, w_bound = reference(q[b:b + 1], k, v, table[b:b + 1], [0], [1], [length], page, 0, d ** -0.5)
+        check_out(out[b:b + 1], want, bound)
+        assert bool(((w[b].cpu().double() - weights[0, :length]).abs() <= w_bound[0, :length] + 2.0 ** -22).all())
+    assert float((w.sum(1) - hq).abs().max()) <= 1e-3 * hq

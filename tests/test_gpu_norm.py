@@ -86,7 +86,7 @@ def check(dev, c, a=1.0, s=1.0, eps=1e-6, kind="rms", offset=0.0, **kw):
     return r, h
 
 
-WIDTHS = [1, 2, 7, 8, 9, 64, 96, 511, 512, 513, 1000, 1024, 1032, 2048, 4096, 4104, 5120, 8192, 8200, 11008, 16384, 20000, 32768]
+WIDTHS = [1, 2, 7, 8, 9, 64, 96, 511, 512, 513, 1000, 1024, 1032, 2048, 4096, 4104, 5120, 8192, 8200, 11008, 16384, 20000, 20001, 32761, 32768]
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])

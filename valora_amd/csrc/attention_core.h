@@ -1133,7 +1133,7 @@ __global__ __launch_bounds__(THREADS) void attend_join_kernel(AttnArgs a) {
 // for leaving the scores, 15 for this launch, 152 in all.)
 constexpr int WEIGHT_WAVES = WEIGHT_TOKENS / 64;
 
-template <typename T, int D, bool CODES>
+template <typename T, int D>
 __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(AttnArgs a) {
   constexpr int CH = D / 32;
   using vec8 = typename Traits<T>::vec8;
@@ -1166,8 +1166,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
       };
       float x = 0.0f;
       int tok;
-      constexpr int ROUND = CODES ? 4 : 8;                      // (the scalar registers)
-#pragma unroll ROUND
+#pragma unroll 8
       for (int r = 0; r < n_rows; ++r) x += share(r, tok);
       if (x != x) {
         // A row whose own sum is no number makes that of all tokens, where one that does not see this token (its score is -infinity)
@@ -1193,41 +1192,23 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
 
     const int32_t *table = a.table + (int64_t)b * a.table_stride;
     int64_t at[4];                                              // this lane's token of each 16: pool row
-    [[maybe_unused]] const char *kc[4], *ke[4];                 // codes: where they and their powers are, of the head that is next
     uint64_t bad = 0;                                           // tokens whose page is none of the pool
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
       const int j = min(base + tt * 16 + lrow, kv - 1);
       const int32_t page = table[j >> a.page_shift];
       const bool none = (uint32_t)page >= (uint32_t)a.n_pages;
-      const int off = j & ((1 << a.page_shift) - 1);
-      if constexpr (CODES) {
-        kc[tt] = reinterpret_cast<const char *>(a.k) + (none ? 0 : (int64_t)page * a.k_stride) + off * D + kg * 8;
-        ke[tt] = reinterpret_cast<const char *>(a.e) + (none ? 0 : (int64_t)page * a.e_stride) + off * 2;
-      } else {
-        at[tt] = none ? 0 : ((int64_t)page << a.page_shift) + off;
-      }
+      at[tt] = none ? 0 : ((int64_t)page << a.page_shift) + (j & ((1 << a.page_shift) - 1));
       bad |= (uint64_t)(__ballot(none) & 0xffffu) << tt * 16;
     }
     float w[4][4] = {};
-    [[maybe_unused]] uint32_t next = 1u << a.page_shift;        // slots from a head of a page to the next (as a vector: the scalars would be spilled)
-    if constexpr (CODES) here(next);
     for (int head = 0; head < a.kv_heads; ++head) {
       const char *kp = reinterpret_cast<const char *>(a.k) + head * D * 2 + kg * 16;
       vec8 kf[4][CH];
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        if constexpr (CODES) {
-          const float power = k_power(*reinterpret_cast<const uint8_t *>(ke[tt]));
+      for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-          for (int i = 0; i < CH; ++i) kf[tt][i] = values_of<T>(*reinterpret_cast<const u32x2 *>(kc[tt] + i * 32), power);
-          kc[tt] += next * D;
-          ke[tt] += next * 2;
-        } else {
-#pragma unroll
-          for (int i = 0; i < CH; ++i) kf[tt][i] = as<vec8>(*reinterpret_cast<const u32x4 *>(kp + at[tt] * a.k_stride + i * 64));
-        }
-      }
+        for (int i = 0; i < CH; ++i) kf[tt][i] = as<vec8>(*reinterpret_cast<const u32x4 *>(kp + at[tt] * a.k_stride + i * 64));
       for (int r0 = row_lo; r0 < row_hi; r0 += 16) {
         const int row = r0 + lrow < rows ? r0 + lrow : rows - 1;
         const int tok = row / a.group, h = head * a.group + row - tok * a.group;
@@ -1262,6 +1243,150 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(At
   }
 }
 
+// Over codes the same sums are two kernels.  Where the scores are there, a thread sums a token's, as above; where they are not, 64 tokens are a
+// workgroup's, whose waves share out heads, and their rows where heads are few, and add up their parts in order.  (A wave alone with 64
+// tokens leaves most of the device idle where few are cached.  us in all, alone / shared: a prompt of 2048, 32 heads of 128, 3070 / 633;
+// 500 tokens over 11500 among 31 decoding requests, 8 key heads, 900 / 286.  64 decoding requests of 1000 to 4100: 99 either way.)
+
+// The request whose run of blocks of WEIGHT_TOKENS holds the block, for everyone
+__device__ __forceinline__ int request_of(const AttnArgs &a, int block, int *found) {
+  const int32_t *requests = a.plan + a.off_requests;
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.n_req; b += blockDim.x)
+    if (requests[(int64_t)b * AT_REC] <= block && (b + 1 == a.n_req || block < requests[(int64_t)(b + 1) * AT_REC])) *found = b;
+  __syncthreads();
+  return (int)uniform((uint32_t)*found);
+}
+__device__ __forceinline__ bool has_scores(const AttnArgs &a, const int32_t *rq) { return rq[2] * a.group <= FEW_ROWS && a.plan[AH_SCORES]; }
+
+template <bool CODES>
+__global__ __launch_bounds__(WEIGHT_TOKENS) void attend_scores_kernel(AttnArgs a) {
+  __shared__ int found;
+  const int total = a.plan[AH_BLOCKS];
+  for (int block = blockIdx.x; block < total; block += gridDim.x) {
+    const int b = request_of(a, block, &found);
+    const int32_t *rq = a.plan + a.off_requests + (int64_t)b * AT_REC;
+    if (!has_scores(a, rq)) continue;
+    const int tok0 = rq[1], n = rq[2], kv = rq[3], pos0 = kv - n, rows = n * a.group, stride = rq[7], n_rows = rows * a.kv_heads;
+    const int begin = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
+    const int j = begin + (block - rq[0]) * WEIGHT_TOKENS + (int)threadIdx.x;
+    if (j >= kv) continue;
+    const float *sc = a.scores + (int64_t)((uint64_t)(uint32_t)rq[5] | (uint64_t)(uint32_t)rq[6] << 32) + (j - begin);
+    auto share = [&](int r, int &tok) {
+      const int head = r / rows, row = r - head * rows;
+      tok = row / a.group;
+      const float lse = a.lse[(int64_t)(tok0 + tok) * a.q_heads + head * a.group + row - tok * a.group];
+      const float e = exp2_(fmaf(sc[(int64_t)r * stride], a.c, -lse));
+      return lse == -INFINITY ? 0.0f : e;
+    };
+    float x = 0.0f;
+    int tok;
+#pragma unroll 8
+    for (int r = 0; r < n_rows; ++r) x += share(r, tok);
+    if (x != x) {
+      // (as above: rows that are no numbers count where they see the token)
+      const int32_t page = a.table[(int64_t)b * a.table_stride + (j >> a.page_shift)];
+      const int behind = (uint32_t)page >= (uint32_t)a.n_pages ? 0 : a.window > 0 ? j - pos0 + a.window : n;
+      x = 0.0f;
+#pragma unroll 1
+      for (int r = 0; r < n_rows; ++r) {
+        const float e = share(r, tok);
+        x += tok >= j - pos0 && tok < behind ? e : 0.0f;
+      }
+    }
+    a.weights[(int64_t)b * a.weights_stride + j] += x;
+  }
+}
+
+constexpr int SHARED_WAVES = 8;
+template <typename T, int D>
+__global__ __launch_bounds__(SHARED_WAVES * 64) void attend_weights_codes_kernel(AttnArgs a) {
+  constexpr int CH = D / 32, PARTS = WEIGHT_TOKENS / 64;
+  using vec8 = typename Traits<T>::vec8;
+  __shared__ int found;
+  __shared__ float parts[SHARED_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6), lrow = lane & 15, kg = lane >> 4;
+  const int total = a.plan[AH_BLOCKS] * PARTS;
+  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    const int b = request_of(a, item / PARTS, &found);
+    const int32_t *rq = a.plan + a.off_requests + (int64_t)b * AT_REC;
+    if (has_scores(a, rq)) continue;
+    const int tok0 = rq[1], n = rq[2], kv = rq[3], pos0 = kv - n, rows = n * a.group;
+    const int begin = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
+    const int base = begin + (item - rq[0] * PARTS) * 64;
+    if (base >= kv) continue;
+    // rows that see any of the tokens
+    const int row_lo = base > pos0 ? (base - pos0) * a.group & ~15 : 0;
+    const int64_t hi = a.window > 0 ? ((int64_t)base + 63 - pos0 + a.window) * a.group : rows;
+    const int row_hi = hi < rows ? (int)hi : rows;
+    const int32_t *table = a.table + (int64_t)b * a.table_stride;
+    const char *kc[4], *ke[4];                                  // this lane's token of each 16: where its codes and powers are
+    uint64_t bad = 0;                                           // tokens whose page is none of the pool
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      const int j = min(base + tt * 16 + lrow, kv - 1);
+      const int32_t page = table[j >> a.page_shift];
+      const bool none = (uint32_t)page >= (uint32_t)a.n_pages;
+      const int64_t at = none ? 0 : page, off = j & ((1 << a.page_shift) - 1);
+      kc[tt] = reinterpret_cast<const char *>(a.k) + at * a.k_stride + off * D + kg * 8;
+      ke[tt] = reinterpret_cast<const char *>(a.e) + at * a.e_stride + off * 2;
+      bad |= (uint64_t)(__ballot(none) & 0xffffu) << tt * 16;
+    }
+    // heads, and where they are fewer than waves runs of their rows
+    const int runs = (SHARED_WAVES + a.kv_heads - 1) / a.kv_heads;
+    const int each = ((row_hi - row_lo + 15) / 16 + runs - 1) / runs * 16;
+    float w[4][4] = {};
+    for (int pair = wave; pair < a.kv_heads * runs; pair += SHARED_WAVES) {
+      const int head = pair / runs, first = row_lo + (pair - head * runs) * each, last_row = min(first + each, row_hi);
+      if (first >= last_row) continue;
+      vec8 kf[4][CH];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const int64_t slots = (int64_t)head << a.page_shift;
+        const float power = k_power(*reinterpret_cast<const uint8_t *>(ke[tt] + slots * 2));
+#pragma unroll
+        for (int i = 0; i < CH; ++i) kf[tt][i] = values_of<T>(*reinterpret_cast<const u32x2 *>(kc[tt] + slots * D + i * 32), power);
+      }
+      for (int r0 = first; r0 < last_row; r0 += 16) {
+        const int row = r0 + lrow < rows ? r0 + lrow : rows - 1;
+        const int tok = row / a.group, h = head * a.group + row - tok * a.group;
+        const float lse = r0 + lrow < rows ? a.lse[(int64_t)(tok0 + tok) * a.q_heads + h] : -INFINITY;
+        const uint16_t *qp = a.q + (int64_t)(tok0 + tok) * a.q_stride + h * D + kg * 8;
+        vec8 q[CH];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 32));
+        const int last = pos0 + tok, from = a.window > 0 ? last - a.window + 1 : 0;
+        const uint64_t sees = lse == -INFINITY ? 0 : (run(from - base, last - base) & ~bad) >> kg * 4;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          f32x4 s{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < CH; ++i) s = Traits<T>::mfma(kf[tt][i], q[i], s);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[tt][i] += as<float>(as<uint32_t>(exp2_(fmaf(s[i], a.c, -lse))) & bit((uint32_t)(sees >> (tt >> 1) * 32), (tt & 1) * 16 + i));
+        }
+      }
+    }
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = w[tt][i];
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
+        if (lrow == 0) parts[wave][tt * 16 + kg * 4 + i] = x;
+      }
+    __syncthreads();
+    if (threadIdx.x < 64 && base + lane < kv) {
+      float x = 0.0f;
+#pragma unroll
+      for (int i = 0; i < SHARED_WAVES; ++i) x += parts[i][lane];
+      a.weights[(int64_t)b * a.weights_stride + base + lane] += x;
+    }
+  }
+}
+
 template <typename T, int D, bool CODES>
 int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, const AttnArgs &a) {
   if (int rc = a.lse ? launch_lists<T, D, true, CODES>(st, L, a) : launch_lists<T, D, false, CODES>(st, L, a)) return rc;
@@ -1272,7 +1397,17 @@ int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, c
   if (a.weights && p.max_kv_len > 0) {
     // as many workgroups as the device holds at once: how many blocks there are it knows
     const int64_t most = p.n_req * ((p.max_kv_len + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS);
-    hipLaunchKernelGGL((attend_weights_kernel<T, D, CODES>), dim3((unsigned)(most < 1024 ? most : 1024)), dim3(WEIGHT_WAVES * 64), 0, st, a);
+    if constexpr (CODES) {
+      hipLaunchKernelGGL(attend_scores_kernel<CODES>, dim3((unsigned)(most < 1024 ? most : 1024)), dim3(WEIGHT_TOKENS), 0, st, a);
+      if (int rc = check_launch("attend_scores_kernel")) return rc;
+      // requests without scores: those of more rows, and all where their room is bounded and may not do
+      if (L.max_shares > 0 || L.scores >= MAX_SCORES) {
+        const int64_t items = most * (WEIGHT_TOKENS / 64);
+        hipLaunchKernelGGL((attend_weights_codes_kernel<T, D>), dim3((unsigned)(items < 1024 ? items : 1024)), dim3(SHARED_WAVES * 64), 0, st, a);
+      }
+    } else {
+      hipLaunchKernelGGL((attend_weights_kernel<T, D>), dim3((unsigned)(most < 1024 ? most : 1024)), dim3(WEIGHT_WAVES * 64), 0, st, a);
+    }
     if (int rc = check_launch("attend_weights_kernel")) return rc;
   }
   return MLORA_OK;

@@ -20,7 +20,7 @@ namespace {
 // of many waves that wait for each other (8191 of 5120, one / two runs a thread: 63.4 / 62.5 us, 2048 of 7168 32.9 / 29.2), unless they are few
 // and the chain counts (256 of 5120 4.7 / 5.3 us).
 constexpr int NORM_ONE = 512, NORM_FEW_ROWS = 512;
-constexpr int NORM_MAX = 32768, NORM_MAX_PLAIN = 16384;      // (wider rows element by element do not fit the registers)
+constexpr int NORM_MAX = 32768;
 
 // What lane l holds, and what the lane holds whose number differs in one way each: by quads, halves and rows of sixteen, rows, halves.  (No exchange
 // goes through LDS, where a butterfly's six would wait one after the other.)
@@ -61,31 +61,40 @@ struct RowSum {
   }
 };
 
-// Eight elements from `at` on; those behind the row are 0
+// Eight elements from `at` on; those behind the row are 0.  VEC: rows are whole runs of eight, at 16 bytes.  Otherwise a run is one access all the
+// same, at whatever address, and the row's last one goes by elements (all by elements: 8000 rows of 4097 with a gate an element 208 us, now 81).
+typedef u32x4 __attribute__((aligned(2))) u32x4_at2;
+typedef f32x4 __attribute__((aligned(4))) f32x4_at4;
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_row(const void *p, int64_t at, int left, float (&x)[8]) {
   const uint16_t *s = static_cast<const uint16_t *>(p) + at;
+  u32x4 r{0, 0, 0, 0};
   if constexpr (VEC) {
-    unpack8<T>(left > 0 ? load16(s) : u32x4{0, 0, 0, 0}, x);
+    if (left > 0) r = load16(s);
+  } else if (left >= 8) {
+    r = *reinterpret_cast<const u32x4_at2 *>(s);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float f = Traits<T>::to_float(s[min(i, left - 1)]);           // (behind the row: its last)
-      x[i] = i < left ? f : 0.0f;
-    }
+    for (int i = 0; i < 7; ++i)
+      if (i < left) r[i / 2] |= (uint32_t)s[i] << i % 2 * 16;
   }
+  unpack8<T>(r, x);
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store_row(void *p, int64_t at, int left, const float (&x)[8]) {
   uint16_t *d = static_cast<uint16_t *>(p) + at;
+  const u32x4 r = pack8<T>(x);
   if constexpr (VEC) {
-    if (left > 0) store16(d, pack8<T>(x));
+    if (left > 0) store16(d, r);
+  } else if (left >= 8) {
+    *reinterpret_cast<u32x4_at2 *>(d) = r;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) d[i] = Traits<T>::from_float(x[i]);
+    for (int i = 0; i < 7; ++i)
+      if (i < left) d[i] = (uint16_t)(r[i / 2] >> i % 2 * 16);
   }
 }
+
 // A vector of the call, a thread's V runs of it.  EARLY: asked for with the row (behind a sum it would be a round trip more: 8191 rows of 4096
 // with a gate 53.8 -> 47.1 us); where none is float and a thread has one run, as the registers of more would cost waves (two runs: 59.8 -> 76).
 // Otherwise loaded where it is used.
@@ -110,10 +119,22 @@ struct Vector {
       load_row<T, VEC>(p, at, left, f);
     } else {
       const float *s = static_cast<const float *>(p) + at;
+      f32x4 lo{0, 0, 0, 0}, hi = lo;
+      if (left >= 8) {
+        lo = *reinterpret_cast<const f32x4_at4 *>(s);
+        hi = *reinterpret_cast<const f32x4_at4 *>(s + 4);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float one = s[min(i, left - 1)];
-        f[i] = i < left ? one : 0.0f;
+        for (int i = 0; i < 7; ++i) {
+          const float one = i < left ? s[i] : 0.0f;
+          if (i < 4) lo[i] = one;
+          else hi[i - 4] = one;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = lo[i];
+        f[4 + i] = hi[i];
       }
     }
   }
@@ -227,8 +248,7 @@ int launch(hipStream_t st, const mlora_norm &n) {
   if (units <= 64) return go(std::false_type{}, one{});
   if (units <= NORM_ONE || (units <= 1024 && n.T <= NORM_FEW_ROWS)) return go(std::true_type{}, one{});
   if (units <= 2048) return go(std::true_type{}, integral_constant<int, 2>{});
-  if constexpr (VEC) return go(std::true_type{}, integral_constant<int, 4>{});
-  return fail(MLORA_ERR_NO_KERNEL, "No suitable kernel. block_norm: H=%lld above %d needs rows of 16-byte multiples, 16-byte aligned", (long long)n.H, NORM_MAX_PLAIN);
+  return go(std::true_type{}, integral_constant<int, 4>{});
 }
 
 }  // namespace
