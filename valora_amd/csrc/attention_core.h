@@ -308,7 +308,7 @@ struct TileCodes {
 // A wave's tile of 32 tokens.  K goes into the first product as it comes: lane (row, kg) holds, of tokens `row` and 16 + row, the 16 elements
 // from 16 kg on of each 64, and the 8 from 8 kg on of 32 that are left; q is read in that order too.  Powers are loaded once a token,
 // by lane token and token + 32, and go round by ds_bpermute: loaded by each lane that needs one, they were 40 % of the look-ups
-// in the L1 (256 requests of 200 to 2000 tokens, 32 heads, 344 us; now 326).  What is left of their cost is lines: 13 us of the 326 for those
+// in the L1 (256 requests of 200 to 2000 tokens, 32 heads, 344 us; then 326).  What is left of their cost is lines: 13 us of those 326 for the ones
 // that hold the powers of a page of 2 tokens, which every XCD reads.  The loads of this loop without its work take 319, of 1.70 GB; with
 // codes of two tiles on their way (at 234 registers) it is no faster.
 template <int D>
@@ -1051,6 +1051,10 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attend_kernel(AttnA
       i = (i & ~7) + (in8 & 7);
       head = in8 >> 3;
       if (i >= a.max_few) return;
+    } else if (CODES && (a.kv_heads & 7) == 0) {
+      // heads that are neighbours go to one XCD: they share the line of a page's powers (256 requests of 32 heads, pages of 2, 326 -> 321 us,
+      // 128 of 40 heads 213 -> 202; pages of 16 and of 1, and 16 heads, the same either way)
+      head = (head & 7) * (a.kv_heads >> 3) + (head >> 3);
     }
     few_tile<T, D, SUMS, CODES>(a, lds, i, head);
     return;
