@@ -217,3 +217,87 @@ def test_nothing_to_do(dev):
     rotary.store8(torch.empty(0, dtype=torch.long, device=dev), none, none, none, kc, vc, powers, torch.empty(0, dtype=torch.long, device=dev))
     k, v = cache8.read(kc, vc, powers, torch.empty(0, dtype=torch.long, device=dev), dtype=BF16)
     assert k.shape == v.shape == (0, 1, 64)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("T,hq,hk,d,R,interleaved", [(6001, 4, 4, 128, 128, False), (14002, 3, 1, 64, 32, False), (2103, 8, 8, 256, 256, True),
+                                                     (1301, 40, 8, 96, 96, False), (27001, 1, 2, 32, 32, True), (53002, 1, 2, 32, 32, False)])
+def test_many_tokens(dev, dtype, T, hq, hk, d, R, interleaved):
+    """Several tokens a workgroup, the last one's not all there; codes against those of the same tokens in small calls."""
+    g = torch.Generator().manual_seed(T)
+    q, k, v = (torch.randn(T, h, d, generator=g).to(dtype).to(dev) for h in (hq, hk, hk))
+    positions = torch.randint(0, 1 << 18, (T,), generator=g).to(dev)
+    page = 16
+    pages = T // page + 3
+    loc = torch.randperm(pages * page, generator=g)[:T].to(dev)
+    loc[T - 2] = -1
+    rotary = Rotary(d, rotary_dim=R, interleaved=interleaved, device=dev)
+    whole, parts = empty(dev, pages, hk, page, d), empty(dev, pages, hk, page, d)
+    out, out_parts = torch.empty_like(q), torch.empty_like(q)
+    rotary.store8(positions, q, k, v, *whole, loc, q_out=out)
+    step = 40 if T < 10000 else 400
+    for at in range(0, T, step):
+        some = slice(at, at + step)
+        rotary.store8(positions[some], q[some], k[some], v[some], *parts, loc[some], q_out=out_parts[some])
+    assert torch.equal(out, out_parts)
+    for a, b in zip(whole, parts):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    few = slice(T - 40, T)
+    k64 = rotated(k.cpu(), positions.cpu(), rotary.freqs.cpu(), R, interleaved)
+    kc, vc, powers = empty(dev, pages, hk, page, d)
+    rotary.store8(positions[few], q[few], k[few], v[few], kc, vc, powers, loc[few])
+    check_stored(kc, vc, powers, loc[few].cpu(), k64[few], v[few].cpu().double(), dtype, page)
+
+
+def test_without_q(dev):
+    """The C entry takes k and v alone."""
+    import ctypes
+    from valora_amd import _lib
+    g = torch.Generator().manual_seed(8)
+    T, hk, d, page = 13, 3, 64, 2
+    k, v = (torch.randn(T, hk, d, generator=g).to(F16).to(dev) for _ in range(2))
+    positions, loc = torch.arange(T, device=dev) * 11, torch.randperm(20, generator=g)[:T].to(dev)
+    rotary = Rotary(d, device=dev)
+    want, got = empty(dev, 10, hk, page, d), empty(dev, 10, hk, page, d)
+    rotary.store8(positions, torch.zeros(T, 1, d, dtype=F16, device=dev), k, v, *want, loc)
+    cache = _lib.Cache8(got[0].data_ptr(), got[1].data_ptr(), got[2].data_ptr(), 10, hk * page * d, hk * page * d, hk * page * 2, hk, d, page)
+    _lib.check(_lib.lib().mlora_rotary_store_codes(_lib.current_stream(dev), None, _lib.ptr(k), hk * d, d, _lib.ptr(v), hk * d, d, ctypes.byref(cache),
+                                                   _lib.ptr(positions), _lib.ptr(loc), T, d, 0, _lib.ptr(rotary.freqs), 1.0, 0))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_refusals(dev):
+    rotary = Rotary(64, device=dev)
+    kc, vc, powers = empty(dev, 4, 2, 2, 64)
+    x = torch.zeros(3, 2, 64, dtype=BF16, device=dev)
+    pos, loc = torch.zeros(3, dtype=torch.long, device=dev), torch.arange(3, device=dev)
+    good = dict(positions=pos, q=x.clone(), k=x, v=x, key_codes=kc, value_codes=vc, powers=powers, loc=loc)
+    rotary.store8(**good)
+    for kw, message in ((dict(key_codes=kc.view(torch.uint8)), "key_codes"), (dict(powers=powers.view(torch.uint8)), "powers"),
+                        (dict(powers=powers[:3]), "powers must be"), (dict(value_codes=vc[:3]), "same shape"), (dict(value_codes=kc), "overlap"),
+                        (dict(key_codes=kc.transpose(1, 2)), "contiguous"), (dict(key_codes=kc[0]), "must be"), (dict(loc=loc.int()), "loc"),
+                        (dict(loc=loc[:2]), "slot per token"), (dict(k=x[:, :1]), "heads"), (dict(k=x[:2]), "row per position"),
+                        (dict(v=x.half()), "No suitable kernel"), (dict(q=x.float()), "No suitable kernel"), (dict(positions=pos[:2]), "tokens"),
+                        (dict(k=x.cpu()), "CUDA tensor"), (dict(powers=powers.cpu()), "CUDA tensor"), (dict(loc=loc.cpu()), "CUDA tensor")):
+        with pytest.raises(RuntimeError, match=message):
+            rotary.store8(**dict(good, **kw))
+    with pytest.raises(RuntimeError, match="head_dim=32"):
+        rotary.store8(**dict(good, key_codes=kc[..., :32].contiguous(), value_codes=vc[..., :32].contiguous()))
+    for kw, message in ((dict(dtype=torch.float32), "No suitable kernel"), (dict(loc=loc.int()), "loc"), (dict(k_out=x[:2]), "row per slot"),
+                        (dict(k_out=x.half()), "k_out"), (dict(k_out=x[..., ::2]), "k_out"), (dict(k_out=x, v_out=x), "k_out must not be v_out")):
+        with pytest.raises(RuntimeError, match=message):
+            cache8.read(**dict(dict(key_codes=kc, value_codes=vc, powers=powers, loc=loc, dtype=BF16), **kw))
+    from valora_amd.attention import AttentionPlan
+    i32 = lambda t: torch.tensor(t, dtype=torch.int32, device=dev)  # noqa: E731
+    plan = AttentionPlan(i32([0]), i32([3]), i32([3]), n_tokens=3, max_seq_len=3, max_kv_len=3, q_heads=2, kv_heads=2, head_dim=64, page_size=2)
+    out, table = torch.empty_like(x), i32([[0, 1]])
+    good = dict(out=out, q=x, key_codes=kc, value_codes=vc, powers=powers, table=table)
+    plan.attend8(**good)
+    for kw, message in ((dict(q=x.float()), "No suitable kernel"), (dict(out=out.half()), "No suitable kernel"), (dict(out=x), "out must not be q"),
+                        (dict(key_codes=kc.view(torch.uint8)), "key_codes"), (dict(table=table.long()), "table"), (dict(table=table[:, :1]), "max_kv_len"),
+                        (dict(key_codes=kc[:, :1].contiguous(), value_codes=vc[:, :1].contiguous(), powers=powers[:, :1].contiguous()), "2 of 64 in pages of 2"),
+                        (dict(weights=torch.zeros(1, 2, device=dev)), "max_kv_len"), (dict(scale=-1.0), "positive")):
+        with pytest.raises(RuntimeError, match=message):
+            plan.attend8(**dict(good, **kw))

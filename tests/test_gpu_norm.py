@@ -212,3 +212,26 @@ def test_replays_of_a_captured_norm(dev):
         torch.cuda.synchronize()
         again = block_norm(x, w, **args)
         assert torch.equal(r, again[0]) and torch.equal(h, again[1])
+
+
+def test_refusals(dev):
+    x, w = torch.zeros(4, 64, dtype=F16, device=dev), torch.ones(64, dtype=F16, device=dev)
+    good = dict(x=x, weight=w, block=x.clone())
+    block_norm(**good)
+    for kw, message in ((dict(x=x.float()), "No suitable kernel"), (dict(x=x[0]), r"\[tokens, width\]"), (dict(weight=w.double()), "No suitable kernel"),
+                        (dict(weight=w[:63]), "x's width"), (dict(weight=w.cpu()), "CUDA tensor"), (dict(block=x[:3]), "x's shape"),
+                        (dict(block=x.bfloat16()), "No suitable kernel"), (dict(block=x.t().contiguous().t()), "contiguous"), (dict(gate=w[:3]), "gate must be"),
+                        (dict(gate=torch.zeros(3, 64, dtype=F16, device=dev)), "gate must be"), (dict(gate=w[::2].repeat(2)[::2]), "gate must be"),
+                        (dict(block=None, gate=w), "without block"), (dict(block=None, residual_scale=2.0), "without block"),
+                        (dict(block=None, weight=None), "neither"), (dict(bias=w, weight=None), "bias without weight"),
+                        (dict(block_bias=w), "without block_weight"), (dict(weight=None, out=x.clone()), "out without weight"),
+                        (dict(out=x[1:]), "x's shape"), (dict(eps=-1.0), "negative"), (dict(kind="none"), "unknown norm")):
+        with pytest.raises(RuntimeError, match=message):
+            block_norm(**dict(good, **kw))
+    wide = torch.zeros(5, 64, dtype=F16, device=dev)
+    with pytest.raises(RuntimeError, match="other rows"):
+        block_norm(wide[:4], w, out=wide[1:])
+    with pytest.raises(RuntimeError, match="results overlap"):
+        block_norm(x, w, block=x.clone(), residual_out=wide[:4], out=wide[:4])
+    with pytest.raises(RuntimeError, match="overlaps a vector"):
+        block_norm(x, wide[4], block=x.clone(), out=wide[1:])

@@ -10,7 +10,9 @@ Modules mirror the reference's import points:
 * ``valora_amd.segments``                     <- ``set_sgmm_args`` / ``count_consecutive_requests``
 * ``valora_amd.plan.LoraPlan``                once-per-batch plan + shrink/expand in one call
 * ``valora_amd.kv_cache.KVCache``             the served requests' cache in rows of the same pool, over ``valora_amd.rotary``
-                                              (positions), ``valora_amd.attention`` (paged attention) and ``evict``
+                                              (positions), ``valora_amd.attention`` (paged attention) and ``evict``; in 8 bits
+                                              over ``valora_amd.cache8``
+* ``valora_amd.norm.block_norm``              norms around a layer's blocks, with the residual sums they stand at
 """
 __version__ = "0.1.0"
 

@@ -5,7 +5,7 @@
 // themselves.  k is rotated in 64 bits, sines and all, and rounded once, to its code: in 32 bits one code in some hundred thousand would be a
 // neighbour of the nearest, a sixteenth off, and the vector units do 64 bits at half the rate of 32.
 //
-// Bound by bytes (8191 tokens, 32 query and 8 key heads of 128, bf16: 185 MB in 40 us, 4.6 TB/s; a copy of as much takes 36).  Four tokens a
+// Bound by bytes (8191 tokens, 32 query and 8 key heads of 128, bf16: 185 MB in 40 us, 4.6 TB/s; a copy of as much takes 36).  Where tokens are many, four a
 // workgroup share one wait for positions, frequencies and sines (a token a workgroup: 49 us; two and eight: 41), and a lane that owned eight
 // elements and loaded their partners a second time took 55: half of it were the vector units.
 #include "codes8.h"
@@ -25,10 +25,14 @@ struct StoreArgs {
   float gain;
   int rotary_dim, page_shift, lane_shift;
   int heads, per_piece;                 // k's, v's and q's; of a workgroup
+  bool many;
 };
 
 constexpr int ST_THREADS = 256;
-constexpr int MANY = 512;               // tokens: from here on a workgroup has four, below it a round of heads of one
+// A round is what a workgroup's threads take at once, some heads of a token.  From MANY on a workgroup has four tokens, whose heads are cut in pieces
+// while there are fewer than FULL tokens; below it a round of one token (us of either, 32 query heads of 128: 1024 and 2048 tokens of 8 key
+// heads, 1536 and 3072 rounds, 14.4 / 12.7 and 16.8 / 19.3; 512 and 1024 of 32 key heads 15.0 / 12.8 and 17.6 / 20.1).
+constexpr int MANY = 2048, FULL = 4096;
 
 // A lane's part of a head: n elements from a0 on and, where they are the first halves of pairs, as many from a1 on
 struct Part {
@@ -241,7 +245,7 @@ void launch_store(hipStream_t st, dim3 grid, const StoreArgs &a, bool interleave
 
 template <typename T, int D>
 void launch_store(hipStream_t st, dim3 grid, const StoreArgs &a, bool interleaved, bool vec) {
-  if (a.T >= MANY) launch_store<T, D, 4>(st, grid, a, interleaved, vec);
+  if (a.many) launch_store<T, D, 4>(st, grid, a, interleaved, vec);
   else launch_store<T, D, 1>(st, grid, a, interleaved, vec);
 }
 
@@ -381,10 +385,10 @@ extern "C" int mlora_rotary_store_codes(void *stream, const mlora_rotary_part *q
   a.heads = 2 * cache->kv_heads + q_heads;
   // lanes of a head: a power of two, so that they find each other by exchanging bits
   a.lane_shift = log2_of((interleaved ? (rotary_dim + 7) / 8 : (rotary_dim / 2 + 7) / 8) + (d - rotary_dim + 7) / 8);
-  // Few tokens: a workgroup a round of heads, as in csrc/rotary.hip
-  const int per_round = ST_THREADS >> a.lane_shift;
-  const int rounds = (a.heads + per_round - 1) / per_round, pieces = T >= MANY ? 1 : rounds;
-  a.per_piece = (rounds + pieces - 1) / pieces * per_round;
+  const int per_round = ST_THREADS >> a.lane_shift, rounds = (a.heads + per_round - 1) / per_round;
+  a.many = T * a.heads >= (int64_t)MANY * per_round;
+  const int64_t pieces = !a.many ? rounds : T >= FULL ? 1 : FULL / T < rounds ? FULL / T : rounds;
+  a.per_piece = (int)((rounds + pieces - 1) / pieces) * per_round;
   const dim3 grid((unsigned)T, (unsigned)((a.heads + a.per_piece - 1) / a.per_piece));
   if (dtype == MLORA_F16) launch_store<_Float16>((hipStream_t)stream, grid, a, interleaved != 0, vec);
   else launch_store<__bf16>((hipStream_t)stream, grid, a, interleaved != 0, vec);
