@@ -301,3 +301,19 @@ def test_refusals(dev):
                         (dict(weights=torch.zeros(1, 2, device=dev)), "max_kv_len"), (dict(scale=-1.0), "positive")):
         with pytest.raises(RuntimeError, match=message):
             plan.attend8(**dict(good, **kw))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_any_codes_and_powers(dev, dtype):
+    """Every code, with powers that the type does not hold all values of: rounded to the nearest, infinite beyond."""
+    g = torch.Generator().manual_seed(9)
+    n, d = 3000, 32
+    codes = torch.randint(0, 256, (n, 1, 1, d), generator=g, dtype=torch.int16).to(torch.uint8)
+    powers = torch.randint(127 - 40, 127 + 20, (n, 1, 1, 2), generator=g).to(torch.uint8)
+    powers[:20] = 255
+    on = lambda t, f: t.to(dev).view(f)  # noqa: E731
+    k, v = cache8.read(on(codes, torch.float8_e4m3fn), on(codes.flip(0), torch.float8_e4m3fn), on(powers, torch.float8_e8m0fnu), torch.arange(n, device=dev), dtype)
+    for got, c, which in ((k, codes, 0), (v, codes.flip(0), 1)):
+        want = decode(c[:, 0], powers[:, 0, :, which]).to(dtype)
+        got = got.cpu().view_as(want)
+        assert bool(((got == want) | (torch.isnan(got) & torch.isnan(want))).all())

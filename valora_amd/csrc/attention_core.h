@@ -1055,8 +1055,8 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attend_kernel(AttnA
       head = in8 >> 3;
       if (i >= a.max_few) return;
     } else if (CODES && (a.kv_heads & 7) == 0) {
-      // heads that are neighbours go to one XCD: they share the line of a page's powers (256 requests of 32 heads, pages of 2, 326 -> 321 us,
-      // 128 of 40 heads 213 -> 202; pages of 16 and of 1, and 16 heads, the same either way)
+      // heads that are neighbours go to one XCD, which then reads of a page what lies side by side (256 requests of 32 heads, pages of 2,
+      // 326 -> 321 us, 128 of 40 heads 213 -> 202; pages of 16 and of 1, and 16 heads, the same either way; the L2s ask for as many bytes)
       head = (head & 7) * (a.kv_heads >> 3) + (head >> 3);
     }
     few_tile<T, D, SUMS, CODES>(a, lds, i, head);
