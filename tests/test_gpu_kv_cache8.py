@@ -186,3 +186,70 @@ def test_another_stream(dev):
             cache.release(0)
         stream.synchronize()
     assert torch.equal(*results)
+
+
+@pytest.mark.parametrize("more", [False, True])
+def test_a_layer_over_codes_with_fused_norms(dev, more):
+    """Everything together: adapters and the 8-bit cache from one pool, norms fused with the sums at the blocks; a prompt whole and in parts,
+    against the layer in 64 bits over the values that the cache holds."""
+    import torch.nn.functional as F
+    from tests.test_gpu_norm import norm64
+    from valora_amd.infer_adapter import InferAdapter, LoraAdapterWeights
+    from valora_amd.layer import LayerPlans, LayerPools, LayerWeights, layer_forward
+    H, MLP, heads, dtype, r, n = 256, 512, 4, torch.float16, 16, 37
+    d = H // heads
+    g = torch.Generator().manual_seed(5)
+    mem = MemoryAllocator(300, 0, dtype, heads, d, 1, device=dev)
+    mem.key_buffer.fill_(math.nan), mem.value_buffer.fill_(math.nan)
+    adapters = InferAdapter.init(mem)
+    net = {"num_hidden_layers": 1, "hidden_size": H}
+    A = [[torch.randn(r, H, generator=g) * 0.05 for _ in range(4)]]
+    B = [[torch.randn(H, r, generator=g) * 0.05 for _ in range(4)]]
+    adapters.load_adapters([LoraAdapterWeights.from_dense("a", r, 2.0 * r, net, A, B, dtype=dtype, pin=False)])
+    mk = lambda i, o: (torch.randn(i, o, generator=g) / i ** 0.5).to(dtype)  # noqa: E731
+    vec = lambda: (1 + 0.1 * torch.randn(H, generator=g)).to(dtype)  # noqa: E731
+    plain = [mk(H, H), mk(H, H), mk(H, H), mk(H, H), mk(H, MLP), mk(H, MLP), mk(MLP, H), vec(), vec()]
+    extra = dict(post1=vec(), post2=vec(), gate1=vec(), gate2=vec(), residual_scale=1.5, block_scale=0.5) if more else {}
+    w = LayerWeights(*plain, **extra)
+    on = lambda t: t.to(dev) if isinstance(t, torch.Tensor) else t  # noqa: E731
+    wd = LayerWeights(*[on(t) for t in plain], **{k: on(t) for k, t in extra.items()})
+    x = torch.randn(n, H, generator=g).to(dtype)
+    zero_up = (torch.zeros(64, heads, d, dtype=dtype, device=dev), torch.zeros(64, heads, MLP // heads, dtype=dtype, device=dev))
+
+    def forward(cache, rows, slot):
+        step = cache.step([slot], [rows.shape[0]])
+        ids = torch.zeros(rows.shape[0], dtype=torch.long, device=dev)
+        pools = LayerPools((mem.key_buffer[0], mem.value_buffer[0]), zero_up, (zero_up[1], zero_up[0]), adapters.a_start, adapters.a_len,
+                           adapters.a_loc, adapters.a_scaling)
+        plans = LayerPlans(ids, adapters.a_start, adapters.a_len, r, H, MLP)
+        return layer_forward(rows, wd, pools, plans, step.attention(0), heads, fused=True)
+
+    assert int(adapters.a_loc.max()) < 64                # (the rows the zero buffers are indexed with)
+    before = mem.key_buffer[0][adapters.a_loc].clone()
+    cache = KVCache(mem, max_requests=2, max_len=63, q_heads=heads, rotary=Rotary(d, device=dev), codes=True)
+    whole = forward(cache, x.to(dev), 0)
+    parts = torch.cat([forward(cache, x[a:b].to(dev), 1) for a, b in ((0, 19), (19, 20), (20, 36), (36, 37))])
+    torch.cuda.synchronize()
+    assert torch.equal(mem.key_buffer[0][adapters.a_loc], before)
+
+    eff = lambda base, s: base.double() + 2.0 * A[0][s].to(dtype).double().T @ B[0][s].to(dtype).double().T  # noqa: E731
+    n64 = lambda z, wt: z if wt is None else norm64(z, wt, None, 1e-6, "rms", 0.0)  # noqa: E731
+    one = lambda t: 1.0 if t is None else t.double()  # noqa: E731
+    h = n64(x.double(), w.ln1)
+    q, k, v = ((h @ eff(m, s)).view(n, heads, d) for s, m in enumerate((w.wq, w.wk, w.wv)))
+    q, k = rotate(q, torch.arange(n), d), rotate(k, torch.arange(n), d)
+    for slot, got in ((0, whole), (1, parts)):
+        kc, vc = (t.cpu().double() for t in cache.read(slot, 0))
+        # half a step of a code, of a value that is off by some roundings of 2^-11 of its sums: 2^-8 of the largest
+        for mine, exact in ((kc, k), (vc, v)):
+            assert bool(((mine - exact).abs() <= exact.abs() * 2.0 ** -4 + 2.0 ** -8 * exact.abs().amax(-1, keepdim=True)).all())
+        a = torch.empty(n, heads, d, dtype=torch.float64)
+        for i in range(heads):
+            s = (q[:, i] @ kc[:, i].T * d ** -0.5).masked_fill(torch.ones(n, n).tril() == 0, -math.inf)
+            a[:, i] = torch.softmax(s, -1) @ vc[:, i]
+        y = w.residual_scale * x.double() + w.block_scale * one(w.gate1) * n64(a.view(n, H) @ eff(w.wo, 3), w.post1)
+        h2 = n64(y, w.ln2)
+        want = w.residual_scale * y + w.block_scale * one(w.gate2) * n64((F.silu(h2 @ w.w_gate.double()) * (h2 @ w.w_up.double())) @ w.w_down.double(), w.post2)
+        # about a dozen roundings of 2^-12 of the values on the way, of which few reach the output whole
+        err = float((got.cpu().double() - want).norm() / want.norm())
+        assert err <= 12 * 2.0 ** -12, (slot, err)

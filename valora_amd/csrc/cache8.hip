@@ -30,8 +30,8 @@ struct StoreArgs {
 
 constexpr int ST_THREADS = 256;
 // A round is what a workgroup's threads take at once, some heads of a token.  From MANY on a workgroup has four tokens, whose heads are cut in pieces
-// while there are fewer than FULL tokens; below it a round of one token (us of either, 32 query heads of 128: 1024 and 2048 tokens of 8 key
-// heads, 1536 and 3072 rounds, 14.4 / 12.7 and 16.8 / 19.3; 512 and 1024 of 32 key heads 15.0 / 12.8 and 17.6 / 20.1).
+// while there are fewer than FULL tokens; below it a round of one token (us of either with the read, 32 query heads of 128: 1024 and 2048 tokens of 8
+// key heads 14.4 / 12.7 and 16.8 / 19.3; 512 and 1024 of 32 key heads 15.0 / 12.8 and 17.6 / 20.1).
 constexpr int MANY = 2048, FULL = 4096;
 
 // A lane's part of a head: n elements from a0 on and, where they are the first halves of pairs, as many from a1 on
