@@ -121,6 +121,23 @@ def test_what_a_row_does_not_see_does_not_show(dev, dtype, n, length, value):
         check(dev, c, 16, window)
 
 
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(F16, 16, 16, 128), (BF16, 32, 16, 128), (BF16, 16, 16, 64), (F16, 16, 8, 256)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, "max"])
+def test_many_requests_that_decode(dev, dtype, hq, hkv, d, value):
+    """More requests times key heads than a list is cut for, each several tiles of a wave long; some see values that are no numbers, or the
+    largest, early and late."""
+    value = torch.finfo(dtype).max if value == "max" else value
+    reqs = [(1, 1 + 37 * i % 701) for i in range(130 if hkv == 8 else 70)]
+    c = make(dev, dtype, hq, hkv, d, 2, reqs, seed=13)
+    for b in range(0, len(reqs), 5):
+        for j in (reqs[b][1] // 7, reqs[b][1] - 1):
+            row = int(c["table"][b, j // 2]) * 2 + j % 2
+            c["vb"][row, b % hkv, j % d] = value
+            c["vb"][row, (b + 1) % hkv, :] = value
+    c["key_codes"], c["value_codes"], c["powers"], c["kb"], c["vb"] = cache_of(c["kb"], c["vb"], 2, dtype)
+    check(dev, c, 2)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("byte", [0, 255])
 def test_powers_that_were_never_written(dev, dtype, byte):

@@ -462,7 +462,7 @@ __device__ __forceinline__ float not_finite(float code) {
 // group 4: 5 of 30000 to 70000 tokens in pages of 16, 225 us, 5.2 TB/s.  One of 517 tokens 8.3 us: the launch, five round trips,
 // the join.)
 // Over codes K and V of a tile come into registers together, those of the next as soon as these have been used; V alone goes through LDS.  (The
-// same requests, pages of 2 and of 16: 321 us, 5.3 TB/s; 117, 5.1, of which the loads alone take 112; 8.2.)
+// same requests, pages of 2 and of 16: 313 us, 5.4 TB/s; 117, 5.1, of which the loads alone take 112; 8.2.)
 constexpr int FEW_TOKENS = 32, THREADS = 256;
 template <int D, bool CODES>
 struct Few {
@@ -580,8 +580,12 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     const bool more = k + 1 < mine;
     const int base = base_of(k);
     // K has come; V and the page numbers of a later tile are on their way
-    if constexpr (CODES) codes.keys_arrived();
-    else wait_vmcnt<EACH + 1>();
+    if constexpr (CODES) {
+      if constexpr (CAREFUL) load_codes(k);                     // (none ahead: the registers of this loop, the rare one, decide how many workgroups a CU holds)
+      codes.keys_arrived();
+    } else {
+      wait_vmcnt<EACH + 1>();
+    }
     f32x4 s[2];
     [[maybe_unused]] uint32_t powers[2];
     if constexpr (CODES)
@@ -598,7 +602,7 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     const uint32_t bad = (uint32_t)__ballot(bad_page(c, lds_word(slices + (k & 3) * 256 + (lane & 31) * 4)));
     if constexpr (CODES) {
       codes.template write_values<T>(vt, lane);
-      if (more) load_codes(k + 1);
+      if (!CAREFUL && more) load_codes(k + 1);
     } else {
       wait_lgkmcnt0();
       if (more) load_k(k + 1);
@@ -679,7 +683,7 @@ __device__ __forceinline__ void few_tile(const AttnArgs &a, char *lds, int rec_i
     load_pages(c, base_of(1), slices + 256, lane & 31);
     wait_vmcnt<0>();
     if constexpr (CODES) {
-      load_codes(0);
+      if constexpr (!decltype(careful)::value) load_codes(0);
     } else {
       load_k(0);
       load_v();
@@ -1097,7 +1101,15 @@ int launch_lists(hipStream_t st, const AttnLayout &L, AttnArgs a) {
   }
   if constexpr (D > 128 || CODES) {
     a.tall_blocks = 0;
-    hipLaunchKernelGGL((attend_kernel<T, D, SUMS, FEW_LIST, CODES>), dim3((unsigned)few), dim3(THREADS), 0, st, a);
+    // Over codes of 128 three workgroups have the registers of a CU, and where requests are whole and a page's heads no long run the third
+    // helps.  A cut list fills two a CU to the end, and of three it leaves a third idle in its last round; of long runs more at once
+    // part more from each other.  There room that nobody uses keeps the third out.  (us with two / three.  Whole: 256 requests of 32 heads,
+    // pages of 2, 322 / 313, 400 of 8, pages of 16, 131 / 128; 200 of 32, pages of 8 and 64, 230 / 234 and 223 / 231.  Cut: 5 long 117 / 127,
+    // 64 of 8 heads 62 / 65, and a list cut for three 119 and 65.)
+    constexpr uint32_t HALF = 80 << 10;
+    const bool third = (int64_t)a.n_req * a.kv_heads >= L.few_items && (int64_t)a.kv_heads << a.page_shift <= 128;
+    const uint32_t unused = CODES && D == 128 && !third ? HALF - Few<D, CODES>::TOTAL : 0;
+    hipLaunchKernelGGL((attend_kernel<T, D, SUMS, FEW_LIST, CODES>), dim3((unsigned)few), dim3(THREADS), unused, st, a);
     return check_launch("attend_kernel");
   }
   return MLORA_OK;
