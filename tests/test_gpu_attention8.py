@@ -231,3 +231,28 @@ def test_weights_where_the_scores_have_no_room(dev):
         check_out(out[b:b + 1], want, bound)
         assert bool(((w[b].cpu().double() - weights[0, :length]).abs() <= w_bound[0, :length] + 2.0 ** -22).all())
     assert float((w.sum(1) - hq).abs().max()) <= 1e-3 * hq
+
+
+def test_captured_with_room_that_nobody_uses(dev):
+    """Heads of 128, a list that is cut and one that is not: in one graph, replayed between eager calls, against the eager results."""
+    cases = [coded(dev, 2, F16, 4, 2, 128, [(1, 900), (1, 33)], seed=14), coded(dev, 2, F16, 16, 16, 128, [(1, 1 + i) for i in range(66)], seed=15)]
+    calls = []
+    for c in cases:
+        hq, d, hkv = c["q"].shape[1], c["q"].shape[2], c["kb"].shape[1]
+        plan = AttentionPlan(*c["lengths"], n_tokens=c["T"], max_seq_len=1, max_kv_len=max(c["lens"]), q_heads=hq, kv_heads=hkv, head_dim=d,
+                             page_size=2, window=0)
+        args = [c[n].to(dev) for n in ("q", "key_codes", "value_codes", "powers", "table")]
+        calls.append((plan, torch.zeros_like(args[0]), args))
+    want = [run(dev, c, 2) for c in cases]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for plan, out, args in calls:
+            plan.attend8(out, *args)
+    for _ in range(4):
+        for _, out, _ in calls:
+            out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        for (_, out, _), w, c in zip(calls, want, cases):
+            assert torch.equal(out, w)
+            assert torch.equal(run(dev, c, 2), w)
