@@ -491,7 +491,7 @@ int mlora_rotary_store_codes(void *stream, const mlora_rotary_part *q, const voi
                         const int64_t *positions, const int64_t *loc, int64_t T, int32_t rotary_dim, int32_t interleaved,
                         const double *freqs, float gain, mlora_dtype dtype);
 /* k[i], v[i] = what slot loc[i] holds ([n][kv_heads][head_dim] of dtype, strides in elements between tokens, rows of 16-byte
- * multiples); zeros where it is outside the cache.  k and v must not overlap each other or the cache.                */
+ * multiples); zeros where it is outside the cache.  k and v that overlap each other, the cache or loc are refused.    */
 int mlora_cache_read_codes(void *stream, const mlora_cache8 *cache, const int64_t *loc, int64_t n, void *k, int64_t k_stride, void *v,
                       int64_t v_stride, mlora_dtype dtype);
 /* mlora_paged_attention over that cache, with a plan of its kv_heads, head_dim and page_size; table: its pages.          */

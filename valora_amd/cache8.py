@@ -40,5 +40,6 @@ def new_powers(shape: Sequence[int], device) -> torch.Tensor:
 def read(key_codes: torch.Tensor, value_codes: torch.Tensor, powers: torch.Tensor, loc: torch.Tensor, dtype: torch.dtype,
          k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(k, v)``, ``[n, kv_heads, head_dim]`` of ``dtype``: what the slots ``loc`` (int64 ``[n]``) hold; zeros for one outside the cache.
-    Exact in the type that the cache was written from; as another type values are rounded to the nearest, beyond its largest to infinities."""
+    Exact in the type that the cache was written from; as another type values are rounded to the nearest, beyond its largest to infinities.
+    ``k_out`` and ``v_out`` may lie side by side in one tensor; they must not overlap each other, ``loc`` or the cache's pages, read or not."""
     return _b.cache8_read(key_codes, value_codes, powers, loc, dtype, k_out, v_out)

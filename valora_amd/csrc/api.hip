@@ -5,6 +5,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <utility>
 
 #include "mlora_internal.h"
 #include "one_call_tiles.h"
@@ -25,6 +26,70 @@ int check_launch(const char *what) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(MLORA_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));
   return MLORA_OK;
+}
+
+namespace {
+
+// Runs as n[0] times n[1] of them, the larger distance first; dimensions of one element are last
+struct Lattice {
+  int64_t lo, n[2], step[2], bytes;
+  // of the dimensions from d on
+  int64_t extent(int d) const {
+    int64_t e = bytes;
+    for (; d < 2; ++d) e += (n[d] - 1) * step[d];
+    return e;
+  }
+};
+
+Lattice lattice_of(const Runs &r) {
+  Lattice l{(int64_t)reinterpret_cast<intptr_t>(r.p), {r.rows, r.heads}, {r.row_stride, r.head_stride}, r.bytes};
+  for (int d = 0; d < 2; ++d) {
+    if (l.step[d] < 0) {
+      l.lo += l.step[d] * (l.n[d] - 1);
+      l.step[d] = -l.step[d];
+    }
+    if (l.n[d] == 1 || l.step[d] == 0) l.n[d] = 1, l.step[d] = 0;
+  }
+  const auto smaller_last = [&] {
+    if (l.step[0] >= l.step[1]) return;
+    std::swap(l.n[0], l.n[1]);
+    std::swap(l.step[0], l.step[1]);
+  };
+  smaller_last();
+  for (int d = 1; d >= 0; --d)
+    if (l.n[d] > 1 && l.step[d] == l.bytes) {                  // side by side: one longer run
+      l.bytes *= l.n[d];
+      l.n[d] = 1;
+      l.step[d] = 0;
+    }
+  smaller_last();
+  return l;
+}
+
+// b begins `off` bytes behind a
+bool meet(const Lattice &a, const Lattice &b, int64_t off, int d) {
+  if (off >= a.extent(d) || off + b.extent(d) <= 0) return false;
+  if (d == 2) return true;
+  if (a.n[d] == 1 && b.n[d] == 1) return meet(a, b, off, d + 1);
+  const int64_t step = a.n[d] > 1 ? a.step[d] : b.step[d];
+  if ((b.n[d] > 1 && b.step[d] != step) || a.extent(d + 1) > step || b.extent(d + 1) > step) return true;
+  // element i of b lies between elements i + k and i + k + 1 of a
+  int64_t k = off / step;
+  if (off % step < 0) --k;
+  for (int next = 0; next < 2; ++next, ++k) {
+    const int64_t first = k < 0 ? -k : 0, last = b.n[d] < a.n[d] - k ? b.n[d] : a.n[d] - k;
+    if (first < last && meet(a, b, off - k * step, d + 1)) return true;
+  }
+  return false;
+}
+
+}  // namespace
+
+bool share_memory(const Runs &a, const Runs &b) {
+  for (const Runs *r : {&a, &b})
+    if (!r->p || r->rows < 1 || r->heads < 1 || r->bytes < 1) return false;
+  const Lattice x = lattice_of(a), y = lattice_of(b);
+  return meet(x, y, y.lo - x.lo, 0);
 }
 
 int expand_bn();

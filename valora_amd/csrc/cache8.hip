@@ -299,6 +299,11 @@ int log2_of(int n) {
   return s;
 }
 
+// What the cache's pages take
+Runs key_pages(const mlora_cache8 &c) { return {c.key_codes, c.n_pages, c.key_stride, 1, 0, (int64_t)c.kv_heads * c.page_size * c.head_dim}; }
+Runs value_pages(const mlora_cache8 &c) { return {c.value_codes, c.n_pages, c.value_stride, 1, 0, (int64_t)c.kv_heads * c.page_size * c.head_dim}; }
+Runs power_pages(const mlora_cache8 &c) { return {c.powers, c.n_pages, c.powers_stride, 1, 0, (int64_t)c.kv_heads * c.page_size * 2}; }
+
 }  // namespace
 
 int check_cache8(const mlora_cache8 *c, int kv_heads, int head_dim, int page_size, const char *who) {
@@ -408,9 +413,16 @@ extern "C" int mlora_cache_read_codes(void *stream, const mlora_cache8 *cache, c
     return fail(MLORA_ERR_INVALID, "%s: rows of k and v must be multiples of 16 bytes and 16-byte aligned", who);
   const int pieces = (int)(w / 8), tokens = pieces >= READ_THREADS ? 1 : READ_THREADS / pieces;
   if (n > 0x7fffffffll * tokens) return fail(MLORA_ERR_NO_KERNEL, "%s: n=%lld too large", who, (long long)n);
+  const Runs to_k{k, n, k_stride * 2, 1, 0, w * 2}, to_v{v, n, v_stride * 2, 1, 0, w * 2};
+  if (share_memory(to_k, to_v)) return fail(MLORA_ERR_INVALID, "%s: k and v overlap", who);
   if (n == 0) return MLORA_OK;
   if (!loc || !k || !v) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
   if (cache->n_pages > 0 && (!cache->key_codes || !cache->value_codes || !cache->powers)) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
+  for (const Runs &to : {to_k, to_v}) {
+    if (share_memory(to, key_pages(*cache)) || share_memory(to, value_pages(*cache)) || share_memory(to, power_pages(*cache)))
+      return fail(MLORA_ERR_INVALID, "%s: k or v overlaps the cache", who);
+    if (share_memory(to, {loc, 1, 0, 1, 0, n * 8})) return fail(MLORA_ERR_INVALID, "%s: k or v overlaps loc", who);
+  }
   ReadArgs a{*cache, loc, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v), n, k_stride, v_stride, log2_of(cache->page_size), pieces, tokens,
              1.0f / (float)pieces, 8.0f / (float)cache->head_dim};
   const dim3 grid((unsigned)((n + tokens - 1) / tokens), (unsigned)((pieces + READ_THREADS - 1) / READ_THREADS));

@@ -83,6 +83,14 @@ static inline int64_t partial_stride_lines(int64_t max_rank) { return align_up(m
 // ---- error reporting (api.hip) ---------------------------------------------------------------
 int fail(int code, const char *fmt, ...);
 int check_launch(const char *what);
+// A call's operand in memory: `rows` times `heads` runs of `bytes`, at row * row_stride + head * head_stride from p on (strides in bytes)
+struct Runs {
+  const void *p;
+  int64_t rows, row_stride, heads, head_stride, bytes;
+};
+// Whether two of them share any.  Exact where rows (or heads, whichever are further apart) are as far apart in both and do not interleave, as those of
+// tensors cut out of one are; others share where one begins before the other ends.
+bool share_memory(const Runs &a, const Runs &b);
 bool share_elements(int64_t rows, int64_t row_stride, int64_t heads, int64_t head_stride, int64_t dim);   // rotary.hip
 int check_cache8(const mlora_cache8 *c, int kv_heads, int head_dim, int page_size, const char *who);       // cache8.hip
 
