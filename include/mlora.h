@@ -485,7 +485,8 @@ typedef struct {
 } mlora_cache8;
 /* mlora_rotary into that cache: q (may be null) is rotated from q->src to q->dst, the rotated k and the v of token t become codes
  * in slot loc[t] (device int64 [T], each at most once; those outside the cache are not stored).  k, v: [T][kv_heads][head_dim],
- * elements of a head contiguous, strides in elements.  k is rotated, and the nearest code found, in 64 bits.             */
+ * elements of a head contiguous, strides in elements, outside the slots that are written.  k is rotated, and the nearest code found,
+ * in 64 bits.  q->dst is q->src with its strides or apart from it; one over k, v, positions or loc is refused.            */
 int mlora_rotary_store_codes(void *stream, const mlora_rotary_part *q, const void *k, int64_t k_token_stride, int64_t k_head_stride,
                         const void *v, int64_t v_token_stride, int64_t v_head_stride, const mlora_cache8 *cache,
                         const int64_t *positions, const int64_t *loc, int64_t T, int32_t rotary_dim, int32_t interleaved,

@@ -1,8 +1,10 @@
 """Operands that share memory are refused where that would let one write over another; those cut out of one tensor side by side are not.  Through the C
 ABI with addresses that nothing is read from: calls that are accepted here stop at a null pointer behind the checks."""
+import random
+
 import pytest
 
-from tests.test_cache8_refusals import A, cache, read
+from tests.test_cache8_refusals import A, cache, read, store
 from valora_amd import _lib
 
 B = A + (1 << 27)      # away from the cache of those tests
@@ -33,3 +35,65 @@ def test_read_results_over_the_cache():
             assert read(cache(), **kw, loc=A - (1 << 16)) == -1 and b"overlaps the cache" in message(), kw
     for kw in (dict(k=B, loc=B + 16), dict(k=B, v=B + (1 << 16), loc=B + (1 << 16) - 8)):
         assert read(cache(), **dict(dict(v=B + (1 << 12)), **kw)) == -1 and b"overlaps loc" in message(), kw
+
+
+def part(**kw):
+    p = dict(src=B, dst=B, src_token_stride=512, src_head_stride=128, dst_token_stride=512, dst_head_stride=128, heads=4, flags=1)
+    p.update(kw)
+    return _lib.RotaryPart(*[p[n] for n, _ in _lib.RotaryPart._fields_])
+
+
+def stored(q, k, v, T, k_strides=(256, 128), v_strides=(256, 128), positions=A - (1 << 20), loc=A - (1 << 19)):
+    """Whether the call gets as far as the missing frequencies, or what it says."""
+    rc = _lib.lib().mlora_rotary_store_codes(None, q, k, *k_strides, v, *v_strides, cache(), positions, loc, T, 128, 0, None, 1.0, 0)
+    assert rc == -1
+    return b"null pointer" in message() or message()
+
+
+def test_q_out_over_what_the_call_reads():
+    far, wide = B + (1 << 20), dict(src_token_stride=1024, dst_token_stride=1024)
+    # in place, in a tensor of q, k and v side by side or head by head, or elsewhere
+    assert stored(part(), far, far + (1 << 16), 3) is True
+    assert stored(part(**wide), B + 1024, B + 1536, 3, (1024, 128), (1024, 128)) is True
+    by_head = dict(src_token_stride=1536, dst_token_stride=1536, src_head_stride=384, dst_head_stride=384)
+    assert stored(part(**by_head, heads=2), B + 256, B + 512, 3, (1536, 384), (1536, 384)) is True
+    assert stored(part(dst=far), B + (1 << 16), B + (1 << 17), 3) is True
+    # a token's or a head's place off, or in other strides
+    for kw in (dict(dst=B + 1024), dict(dst=B - 1024), dict(dst=B + 256), dict(dst_token_stride=520), dict(dst=B + 16)):
+        assert b"other heads of q" in stored(part(**kw), far, far + (1 << 16), 3), kw
+    # k or v
+    for at in (B, B + 256, B + 2 * 1024, B - 512, B + 3 * 1024 - 16):
+        assert b"overlaps k or v" in stored(part(), at, far, 3) and b"overlaps k or v" in stored(part(), far, at, 3), at
+    assert b"overlaps k or v" in stored(part(**wide), B + 1008, B + 1536, 3, (1024, 128), (1024, 128))
+    for kw in (dict(positions=B + 8), dict(loc=B - 16)):
+        assert b"positions or loc" in stored(part(), far, far + (1 << 16), 3, **kw)
+
+
+def test_powers_over_codes():
+    for kw in (dict(powers=A), dict(powers=A + 10 * 4096 - 2), dict(powers=A + (1 << 24) + 64), dict(key_stride=4160, powers=A + 4094, powers_stride=4160)):
+        assert store(cache(**kw)) == -1 and b"powers overlap codes" in message(), kw
+    page = dict(key_stride=4160, powers=A + 4096, powers_stride=4160)       # behind the keys' codes of each page
+    assert store(cache(**page), T=0) == 0
+
+
+def test_heads_of_any_strides_against_every_element():
+    """Nothing that overlaps gets through, and where the two have the same strides, and rows do not interleave, nothing else is refused."""
+    rng = random.Random(3)
+    seen = {True: 0, False: 0}
+    for _ in range(2000):
+        T, hq, extra = rng.randint(1, 4), rng.randint(1, 4), 8 * rng.randint(0, 40)
+        head = 128 + 8 * rng.randint(0, 40)
+        token = max(head * max(hq, 2), 128) + extra
+        other = rng.random() < 0.3
+        k_head, k_token = (8 * rng.randint(0, 60), 8 * rng.randint(0, 200)) if other else (head, token)
+        k = B + 16 * rng.randint(-token * T // 8, token * T // 8)
+        taken = lambda at, n, t, h: {(at - B) // 16 + (i * t + j * h) // 8 + e for i in range(T) for j in range(n) for e in range(16)}  # noqa: E731
+        q = part(heads=hq, src_token_stride=token, dst_token_stride=token, src_head_stride=head, dst_head_stride=head)
+        meets = bool(taken(B, hq, token, head) & taken(k, 2, k_token, k_head))
+        said = stored(q, k, A - (1 << 24), T, (k_token, k_head))
+        seen[meets] += 1
+        if meets:
+            assert said is not True and b"overlaps k or v" in said
+        elif not other:
+            assert said is True, (T, hq, token, head, (k - B) // 2)
+    assert min(seen.values()) > 200

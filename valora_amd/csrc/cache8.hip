@@ -351,19 +351,27 @@ extern "C" int mlora_rotary_store_codes(void *stream, const mlora_rotary_part *q
   if (q_heads < 0 || q_heads > 65536) return fail(MLORA_ERR_INVALID, "%s: heads=%d out of range", who, q_heads);
   if (q_heads > 0 && share_elements(T, q->dst_token_stride, q_heads, q->dst_head_stride, d))
     return fail(MLORA_ERR_INVALID, "%s: heads of a destination overlap", who);
-  // k's codes and v's: apart, or each page's side by side
-  const char *kc = static_cast<const char *>(cache->key_codes), *vc = static_cast<const char *>(cache->value_codes);
-  const int64_t w = (int64_t)cache->kv_heads * cache->page_size * d;
-  if (kc && vc && cache->n_pages > 0) {
-    const int64_t apart = vc > kc ? vc - kc : kc - vc;
-    const int64_t lower = (cache->n_pages - 1) * (vc > kc ? cache->key_stride : cache->value_stride) + w;
-    const int64_t in_page = apart % cache->key_stride;
-    if (apart < lower && (cache->key_stride != cache->value_stride || in_page < w || cache->key_stride - in_page < w))
-      return fail(MLORA_ERR_INVALID, "%s: codes of keys and values overlap", who);
-  }
+  // k's codes, v's and powers: apart, or each page's side by side
+  if (share_memory(key_pages(*cache), value_pages(*cache))) return fail(MLORA_ERR_INVALID, "%s: codes of keys and values overlap", who);
+  if (share_memory(power_pages(*cache), key_pages(*cache)) || share_memory(power_pages(*cache), value_pages(*cache)))
+    return fail(MLORA_ERR_INVALID, "%s: powers overlap codes", who);
   if (T == 0) return MLORA_OK;
-  if (!k || !v || !positions || !loc || !freqs || (q_heads > 0 && (!q->src || !q->dst))) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
-  if (cache->n_pages > 0 && (!kc || !vc || !cache->powers)) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
+  if (q_heads > 0 && (!q->src || !q->dst)) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
+  // what other workgroups read may not be where q goes; q itself only in its own place
+  if (q_heads > 0) {
+    const auto heads = [&](const void *p, int n, int64_t token, int64_t head) { return Runs{p, T, token * 2, n, head * 2, (int64_t)d * 2}; };
+    const Runs to = heads(q->dst, q_heads, q->dst_token_stride, q->dst_head_stride);
+    const bool in_place = q->src == q->dst && (T == 1 || q->src_token_stride == q->dst_token_stride) &&
+                          (q_heads == 1 || q->src_head_stride == q->dst_head_stride);
+    if (!in_place && share_memory(to, heads(q->src, q_heads, q->src_token_stride, q->src_head_stride)))
+      return fail(MLORA_ERR_INVALID, "%s: q's destination overlaps other heads of q", who);
+    if (share_memory(to, heads(k, cache->kv_heads, k_token_stride, k_head_stride)) || share_memory(to, heads(v, cache->kv_heads, v_token_stride, v_head_stride)))
+      return fail(MLORA_ERR_INVALID, "%s: q's destination overlaps k or v", who);
+    if (share_memory(to, {positions, 1, 0, 1, 0, T * 8}) || share_memory(to, {loc, 1, 0, 1, 0, T * 8}))
+      return fail(MLORA_ERR_INVALID, "%s: q's destination overlaps positions or loc", who);
+  }
+  if (!k || !v || !positions || !loc || !freqs) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
+  if (cache->n_pages > 0 && (!cache->key_codes || !cache->value_codes || !cache->powers)) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
   StoreArgs a{};
   bool vec = rotary_dim % 16 == 0 && ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0 &&
              ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;

@@ -116,5 +116,6 @@ class Rotary:
                value_codes: torch.Tensor, powers: torch.Tensor, loc: torch.Tensor, q_out: Optional[torch.Tensor] = None) -> None:
         """``store`` into the cache of 8-bit codes (``valora_amd.cache8``): token t's rotated k and its v go to slot ``loc[t]`` (int64, page
         times page size plus the place in the page; each at most once, those outside the cache are not stored).  ``head_dim`` is one that
-        attention takes.  k is rotated in 64 bits and rounded once, to the nearest code; q as ``store`` does, up to the last bit."""
+        attention takes.  k is rotated in 64 bits and rounded once, to the nearest code; q as ``store`` does, up to the last bit.  q, k and v may be
+        parts of one tensor; ``q_out`` is q itself or apart from all three, and k and v lie outside the slots that are written."""
         self._native.store8(positions, q, k, v, key_codes, value_codes, powers, loc, q_out)
