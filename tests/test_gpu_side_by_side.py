@@ -4,6 +4,7 @@ import torch
 
 from tests.test_gpu_cache8 import empty
 from valora_amd import cache8
+from valora_amd.norm import block_norm
 from valora_amd.rotary import Rotary
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +31,24 @@ def test_q_in_place_beside_k_and_v(dev, by_head, T):
     cache8.read(*got, loc, BF16, both[:, 0], both[:, 1])
     rk, rv = cache8.read(*got, loc, BF16)
     assert torch.equal(both[:, 0], rk) and torch.equal(both[:, 1], rv)
+
+
+@pytest.mark.parametrize("gate_width", [1, 520])
+@pytest.mark.parametrize("T,H", [(1, 520), (33, 520), (40, 96)])
+def test_norm_of_columns(dev, T, H, gate_width):
+    """A block's output, a gate and both results in columns of one tensor.  (Where rows are no whole accesses it is another kernel, whose result may be
+    the neighbour in 16 bits: a step, 2^-10 of the value, 2^-24 at least.)"""
+    near = lambda a, b: bool(((a.double() - b.double()).abs() <= b.double().abs() * 2.0 ** -10 + 2.0 ** -24).all())  # noqa: E731
+    gate_width = min(gate_width, H)
+    g = torch.Generator(device=dev).manual_seed(T)
+    wide = torch.randn(T, 4 * H + gate_width, generator=g, device=dev).to(F16)
+    x, block, r, h, gate = wide.split([H, H, H, H, gate_width], 1)
+    w = torch.randn(H, generator=g, device=dev).to(F16)
+    want_r, want_h = block_norm(x.clone(), w, block=block.clone(), block_weight=w, gate=gate.clone())
+    keep = wide.clone()
+    block_norm(x, w, block=block, block_weight=w, gate=gate, residual_out=r, out=h)
+    assert near(r, want_r) and near(h, want_h)
+    keep[:, 2 * H:4 * H] = wide[:, 2 * H:4 * H]
+    assert torch.equal(wide, keep)
+    block_norm(x, w, block=block, block_weight=w, gate=gate, residual_out=x, out=block)
+    assert torch.equal(x, r) and torch.equal(block, h)

@@ -4,7 +4,7 @@ import random
 
 import pytest
 
-from tests.test_cache8_refusals import A, cache, read, store
+from tests.test_cache8_refusals import A, cache, norm, read, store
 from valora_amd import _lib
 
 B = A + (1 << 27)      # away from the cache of those tests
@@ -97,3 +97,28 @@ def test_heads_of_any_strides_against_every_element():
         elif not other:
             assert said is True, (T, hq, token, head, (k - B) // 2)
     assert min(seen.values()) > 200
+
+
+def test_norm_results_beside_operands_in_one_tensor():
+    """Columns of one tensor are apart where their rows are; a shift by part of a row is not.  (x is missing: what is accepted gets as far as that.)"""
+    L = _lib.lib()
+    wide = dict(block_stride=256, residual_stride=256, out_stride=256)
+
+    def call(**kw):
+        assert L.mlora_block_norm(None, norm(**dict(dict(x=None, x_stride=64), **kw)), 0) == -1
+        return b"null pointer" in message() or message()
+
+    assert call(block=B, residual_out=B + 128, out=B + 256, **wide) is True
+    assert call(block=B + 256, residual_out=B + 128, out=B, **wide) is True
+    assert call(block=B, residual_out=B + 384, gate=B + 128, gate_row_stride=256, **wide) is True
+    assert call(block=B, residual_out=B + 384, gate=B + 128, gate_row_stride=256, gate_column_stride=0, **wide) is True
+    assert call(block=B, residual_out=B + 128, weight=B + 256, **wide) is True                         # between the first row and the second
+    assert call(block=B, out=B + 128, bias=B + 384, f32=2, **wide) is True
+    assert call(block=B, residual_out=B + 256, gate=B + 384, gate_row_stride=128, gate_column_stride=0, f32=16, **wide) is True
+    for kw, said in ((dict(residual_out=B + 126), b"other rows"), (dict(residual_out=B + 512 - 126), b"other rows"), (dict(out=B + 512), b"other rows"),
+                     (dict(residual_out=B + 128, out=B + 130), b"results overlap"), (dict(residual_out=B + 128, out=B + 640), b"results overlap"),
+                     (dict(residual_out=B + 128, gate=B + 254, gate_row_stride=256, gate_column_stride=0), b"gate"),
+                     (dict(residual_out=B + 128, weight=B + 638), b"vector"), (dict(out=B + 128, bias=B + 388, f32=2), b"vector"),
+                     (dict(residual_out=B + 256, gate=B + 380, gate_row_stride=128, gate_column_stride=0, f32=16), b"gate")):
+        got = call(**dict(dict(block=B), **wide), **kw)
+        assert got is not True and said in got, (kw, got)

@@ -257,13 +257,12 @@ int launch(hipStream_t st, const mlora_norm &n) {
 
 using namespace mlora;
 
-static bool meet(const char *a, int64_t a_bytes, const char *b, int64_t b_bytes) { return a && b && a < b + b_bytes && b < a + a_bytes; }
+// Rows of n's width in a tensor of the call
+static Runs rows_of(const mlora_norm &n, const void *p, int64_t stride) { return {p, n.T, stride * 2, 1, 0, n.H * 2}; }
 
 // Whether rows written at `d` can touch what other rows read at `s`: not where the two are the same rows
-static bool overlap(const void *d, int64_t d_stride, const void *s, int64_t s_stride, int64_t T, int64_t H) {
-  const char *a = static_cast<const char *>(d), *b = static_cast<const char *>(s);
-  if (a == b && (d_stride == s_stride || T == 1)) return false;
-  return meet(a, ((T - 1) * d_stride + H) * 2, b, ((T - 1) * s_stride + H) * 2);
+static bool overlap(const mlora_norm &n, const void *d, int64_t d_stride, const void *s, int64_t s_stride) {
+  return !(d == s && (d_stride == s_stride || n.T == 1)) && share_memory(rows_of(n, d, d_stride), rows_of(n, s, s_stride));
 }
 
 extern "C" int mlora_block_norm(void *stream, const mlora_norm *norm, mlora_dtype dtype) {
@@ -281,24 +280,23 @@ extern "C" int mlora_block_norm(void *stream, const mlora_norm *norm, mlora_dtyp
     return fail(MLORA_ERR_INVALID, "%s: elements of a row of the gate must be contiguous, or one, its rows in order", who);
   if (n.T > 1 && (n.x_stride < 0 || (n.block && n.block_stride < 0))) return fail(MLORA_ERR_INVALID, "%s: negative strides", who);
   if (n.T == 0) return MLORA_OK;
-  if (!n.x || (n.weight && !n.out) || (!n.weight && !n.residual_out)) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
   void *out = n.weight ? n.out : nullptr;
+  const int64_t gate_bytes = n.f32 & MLORA_NORM_F32_GATE ? 4 : 2;
+  const Runs gate{n.gate, n.T, n.gate_row_stride * gate_bytes, 1, 0, (n.gate_column_stride ? n.H : 1) * gate_bytes};
   for (const auto &d : {std::make_pair((void *)n.residual_out, n.residual_stride), std::make_pair(out, n.out_stride)}) {
     if (d.first && n.T > 1 && d.second < n.H) return fail(MLORA_ERR_INVALID, "%s: rows of a result overlap", who);
-    if (overlap(d.first, d.second, n.x, n.x_stride, n.T, n.H) || overlap(d.first, d.second, n.block, n.block_stride, n.T, n.H))
+    if (overlap(n, d.first, d.second, n.x, n.x_stride) || overlap(n, d.first, d.second, n.block, n.block_stride))
       return fail(MLORA_ERR_INVALID, "%s: a result overlaps other rows of an operand", who);
-    const char *to = static_cast<const char *>(d.first);
-    const int64_t bytes = ((n.T - 1) * d.second + n.H) * 2;
-    if (meet(to, bytes, static_cast<const char *>(n.gate),
-             ((n.T - 1) * n.gate_row_stride + (n.gate_column_stride ? n.H : 1)) * (n.f32 & MLORA_NORM_F32_GATE ? 4 : 2)))
-      return fail(MLORA_ERR_INVALID, "%s: a result overlaps the gate", who);
+    const Runs to = rows_of(n, d.first, d.second);
+    if (share_memory(to, gate)) return fail(MLORA_ERR_INVALID, "%s: a result overlaps the gate", who);
     const void *vectors[] = {n.weight, n.bias, n.block_weight, n.block_bias};
     for (int i = 0; i < 4; ++i)
-      if (meet(to, bytes, static_cast<const char *>(vectors[i]), n.H * (n.f32 >> i & 1 ? 4 : 2)))
+      if (share_memory(to, {vectors[i], 1, 0, 1, 0, n.H * (n.f32 >> i & 1 ? 4 : 2)}))
         return fail(MLORA_ERR_INVALID, "%s: a result overlaps a vector", who);
   }
-  if (out && n.residual_out && (out == n.residual_out || overlap(out, n.out_stride, n.residual_out, n.residual_stride, n.T, n.H)))
+  if (out && n.residual_out && (out == n.residual_out || overlap(n, out, n.out_stride, n.residual_out, n.residual_stride)))
     return fail(MLORA_ERR_INVALID, "%s: the results overlap", who);
+  if (!n.x || (n.weight && !n.out) || (!n.weight && !n.residual_out)) return fail(MLORA_ERR_INVALID, "%s: null pointer", who);
   // rows that are whole runs of eight, at 16 bytes
   bool vec = n.H % 8 == 0;
   const auto row = [&](const void *p, int64_t stride) { vec = vec && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (!p || n.T == 1 || stride % 8 == 0); };
