@@ -1,6 +1,9 @@
 // Torch binding of the norms around a layer's blocks (include/mlora.h).
+#include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+
+#include <utility>
 
 #include "binding_common.h"
 
@@ -11,6 +14,17 @@ using Maybe = c10::optional<at::Tensor>;
 py::tuple block_norm(const at::Tensor &x, const Maybe &weight, const Maybe &bias, const Maybe &block, const Maybe &block_weight, const Maybe &block_bias,
                      const Maybe &gate, double residual_scale, double block_scale, double eps, bool layer, double offset, const Maybe &residual_out,
                      const Maybe &out) {
+  // (a result without a history would drop the gradient without a word)
+  const auto no_gradient = [](const at::Tensor &t, const char *name) {
+    if (t.requires_grad()) raise(std::string("block_norm has no backward pass: ") + name + " requires a gradient (call it under torch.no_grad())");
+  };
+  if (at::GradMode::is_enabled()) {
+    no_gradient(x, "x");
+    const std::pair<const Maybe &, const char *> others[] = {{weight, "weight"}, {bias, "bias"}, {block, "block"}, {block_weight, "block_weight"},
+                                                             {block_bias, "block_bias"}, {gate, "gate"}, {residual_out, "residual_out"}, {out, "out"}};
+    for (const auto &[t, name] : others)
+      if (t.has_value()) no_gradient(*t, name);
+  }
   if (!x.is_cuda()) raise("x must be a CUDA tensor");
   const c10::Device dev = x.device();
   const mlora_dtype code = dtype_code(x);

@@ -105,7 +105,7 @@ def layer_forward(x: torch.Tensor, w: LayerWeights, pools: Optional[LayerPools],
     rotates q and k itself (``cos`` / ``sin`` None).
 
     ``fused``: norms and residual sums by ``valora_amd.norm.block_norm``, in 32 bits to each result's one rounding (results differ from the
-    others' in the last bit); the weights' ``post1`` ... ``block_scale`` need it."""
+    others' in the last bit), without a backward pass; the weights' ``post1`` ... ``block_scale`` need it."""
     if w.around_blocks() and not fused:
         raise RuntimeError("norms after blocks, gates and scales need layer_forward(..., fused=True)")
 

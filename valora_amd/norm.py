@@ -28,7 +28,8 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     ``[tokens, 1]`` or ``[tokens, width]``) are of that type or float32.  Without ``block`` r is ``x`` itself; without ``block_weight`` the block
     joins as it is; without ``weight`` h is None.  Everything is in 32 bits; r and h are rounded once each, h from the unrounded r.  Widths go up
     to 32768.  ``residual_out`` and ``out`` may be ``x`` or ``block`` themselves, or other columns of one tensor; results that overlap anything
-    else that the call reads, or each other, are refused."""
+    else that the call reads, or each other, are refused.  There is no backward pass: operands that require a gradient are refused where one
+    would be recorded."""
     if kind not in ("rms", "layer"):
         raise RuntimeError(f"unknown norm {kind!r} (rms or layer)")
     return _b.block_norm(x, weight, bias, block, block_weight, block_bias, gate, residual_scale, block_scale, eps, kind == "layer", offset,
