@@ -402,9 +402,21 @@ extern "C" int mlora_rotary_store_codes(void *stream, const mlora_rotary_part *q
   a.many = T * a.heads >= (int64_t)MANY * per_round;
   const int64_t pieces = !a.many ? rounds : T >= FULL ? 1 : FULL / T < rounds ? FULL / T : rounds;
   a.per_piece = (int)((rounds + pieces - 1) / pieces) * per_round;
-  const dim3 grid((unsigned)T, (unsigned)((a.heads + a.per_piece - 1) / a.per_piece));
-  if (dtype == MLORA_F16) launch_store<_Float16>((hipStream_t)stream, grid, a, interleaved != 0, vec);
-  else launch_store<__bf16>((hipStream_t)stream, grid, a, interleaved != 0, vec);
+  for (int64_t at = 0; at < T; at += most_blocks(ST_THREADS)) {
+    StoreArgs part = a;
+    part.T = T - at < most_blocks(ST_THREADS) ? T - at : most_blocks(ST_THREADS);
+    if (q_heads > 0) {
+      part.q.src = static_cast<const uint16_t *>(a.q.src) + at * a.q.src_token_stride;
+      part.q.dst = static_cast<uint16_t *>(a.q.dst) + at * a.q.dst_token_stride;
+    }
+    part.k += at * a.k_token;
+    part.v += at * a.v_token;
+    part.positions += at;
+    part.loc += at;
+    const dim3 grid((unsigned)part.T, (unsigned)((a.heads + a.per_piece - 1) / a.per_piece));
+    if (dtype == MLORA_F16) launch_store<_Float16>((hipStream_t)stream, grid, part, interleaved != 0, vec);
+    else launch_store<__bf16>((hipStream_t)stream, grid, part, interleaved != 0, vec);
+  }
   return check_launch("store8_kernel");
 }
 
@@ -433,8 +445,16 @@ extern "C" int mlora_cache_read_codes(void *stream, const mlora_cache8 *cache, c
   }
   ReadArgs a{*cache, loc, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v), n, k_stride, v_stride, log2_of(cache->page_size), pieces, tokens,
              1.0f / (float)pieces, 8.0f / (float)cache->head_dim};
-  const dim3 grid((unsigned)((n + tokens - 1) / tokens), (unsigned)((pieces + READ_THREADS - 1) / READ_THREADS));
-  if (dtype == MLORA_F16) hipLaunchKernelGGL((read8_kernel<_Float16>), grid, dim3(READ_THREADS), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL((read8_kernel<__bf16>), grid, dim3(READ_THREADS), 0, (hipStream_t)stream, a);
+  const int64_t most = most_blocks(READ_THREADS) * tokens;
+  for (int64_t at = 0; at < n; at += most) {
+    ReadArgs part = a;
+    part.n = n - at < most ? n - at : most;
+    part.loc += at;
+    part.k += at * k_stride;
+    part.v += at * v_stride;
+    const dim3 grid((unsigned)((part.n + tokens - 1) / tokens), (unsigned)((pieces + READ_THREADS - 1) / READ_THREADS));
+    if (dtype == MLORA_F16) hipLaunchKernelGGL((read8_kernel<_Float16>), grid, dim3(READ_THREADS), 0, (hipStream_t)stream, part);
+    else hipLaunchKernelGGL((read8_kernel<__bf16>), grid, dim3(READ_THREADS), 0, (hipStream_t)stream, part);
+  }
   return check_launch("read8_kernel");
 }

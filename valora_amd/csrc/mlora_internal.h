@@ -83,6 +83,8 @@ static inline int64_t partial_stride_lines(int64_t max_rank) { return align_up(m
 // ---- error reporting (api.hip) ---------------------------------------------------------------
 int fail(int code, const char *fmt, ...);
 int check_launch(const char *what);
+// Workgroups that a launch may have along a dimension: its threads are counted in 32 bits, and what is beyond them is left out without an error
+constexpr int64_t most_blocks(int threads) { return 0xffffffffll / threads; }
 // A call's operand in memory: `rows` times `heads` runs of `bytes`, at row * row_stride + head * head_stride from p on (strides in bytes)
 struct Runs {
   const void *p;

@@ -232,15 +232,33 @@ __global__ __launch_bounds__(MANY ? 1024 : 256) void block_norm_kernel(mlora_nor
   }
 }
 
+// `rows` rows from `at` on
+mlora_norm rows_from(mlora_norm n, int64_t at, int64_t rows) {
+  const auto read = [&](const void *&p, int64_t stride, int bytes) { p = p ? static_cast<const char *>(p) + at * stride * bytes : nullptr; };
+  const auto written = [&](void *&p, int64_t stride) { p = p ? static_cast<char *>(p) + at * stride * 2 : nullptr; };
+  read(n.x, n.x_stride, 2);
+  read(n.block, n.block_stride, 2);
+  read(n.gate, n.gate_row_stride, n.f32 & MLORA_NORM_F32_GATE ? 4 : 2);
+  written(n.residual_out, n.residual_stride);
+  written(n.out, n.out_stride);
+  n.T = rows;
+  return n;
+}
+
 template <typename T, bool VEC, bool EARLY>
 int launch(hipStream_t st, const mlora_norm &n) {
   const int units = (int)((n.H + 7) / 8);
   const auto go = [&](auto many, auto v) {
     constexpr bool MANY = decltype(many)::value;
     constexpr int V = decltype(v)::value;
-    const int64_t blocks = MANY ? n.T : (n.T + 3) / 4;
     const int threads = MANY ? ((units + V - 1) / V + 63) / 64 * 64 : 256;
-    hipLaunchKernelGGL((block_norm_kernel<T, VEC, MANY, V, EARLY && V == 1>), dim3((unsigned)blocks), dim3((unsigned)threads), 0, st, n);
+    constexpr int ROWS = MANY ? 1 : 4;
+    const int64_t most = most_blocks(threads) * ROWS;
+    for (int64_t at = 0; at < n.T; at += most) {
+      const mlora_norm part = rows_from(n, at, n.T - at < most ? n.T - at : most);
+      hipLaunchKernelGGL((block_norm_kernel<T, VEC, MANY, V, EARLY && V == 1>), dim3((unsigned)((part.T + ROWS - 1) / ROWS)), dim3((unsigned)threads), 0,
+                         st, part);
+    }
     return check_launch("block_norm_kernel");
   };
   using std::integral_constant;
