@@ -71,3 +71,17 @@ def test_tokens_read(dev):
         for at in (0, 1 << 29, (1 << 30) - 1000):
             assert bool((got[at:at + 100] == its[1]).all())
         assert alike(got[:-70], its[1])
+
+
+def test_tokens_rotated(dev):
+    """q elsewhere, k and v into rows: a token a workgroup of 256 threads."""
+    T, d = (1 << 24) + 3, 32
+    one = torch.randn(3, 1, d, device=dev).to(F16)
+    rotary = Rotary(d, device=dev)
+    positions, loc = torch.full((T,), 7, device=dev), torch.arange(T, device=dev).flip(0)
+    q_out, kb, vb = (torch.full((T + extra, 1, d), 9.0, dtype=F16, device=dev) for extra in (0, 1, 1))
+    rotary.store(positions, one[:1].expand(T, 1, d), one[1:2].expand(T, 1, d), one[2:].expand(T, 1, d), kb, vb, loc, q_out=q_out)
+    turned = one.clone()
+    rotary.apply(torch.full((3,), 7, device=dev), turned)
+    for rows, want in ((q_out, turned[0]), (kb, turned[1]), (vb, one[2])):
+        assert alike(rows[:T], want) and alike(rows[T:], torch.full_like(want, 9.0))

@@ -1082,7 +1082,7 @@ int launch_lists(hipStream_t st, const AttnLayout &L, AttnArgs a) {
   // whole lines: 32 heads of 128, 256 requests 343 / 358, as a page is then read by one XCD alone.)
   a.heads_together = CODES && ((D << a.page_shift) & 127) != 0;
   const int64_t few = (a.heads_together ? align_up(L.max_few, 8) : L.max_few) * a.kv_heads, tall = L.max_shares * a.kv_heads;
-  if (few + tall > 0x7fffffff) return fail(MLORA_ERR_NO_KERNEL, "paged_attention: too many tiles");
+  if (few + tall > most_blocks(THREADS)) return fail(MLORA_ERR_NO_KERNEL, "paged_attention: too many tiles");
   a.tall_blocks = (int)tall;
   a.max_few = (int)L.max_few;
   // both lists in one kernel do not fit the scalar registers at 256; decoding over codes has a kernel without the room that tall tiles take

@@ -236,6 +236,7 @@ extern "C" int mlora_cache_evict(void *stream, const int32_t *table, int64_t tab
                                  int64_t budget, int64_t recent, int64_t sinks, int32_t *new_table, int32_t *new_kv_len,
                                  float *new_weights, int32_t *freed) {
   if (n_req < 0 || width < 0 || n_req > 0x7fffffff) return fail(MLORA_ERR_INVALID, "cache_evict: negative size");
+  if (n_req > most_blocks(EV_THREADS)) return fail(MLORA_ERR_NO_KERNEL, "cache_evict: more than %lld requests", (long long)most_blocks(EV_THREADS));
   int shift = 0;
   while (shift < 8 && (1 << shift) < page_size) ++shift;
   if (page_size < 1 || (1 << shift) != page_size)

@@ -306,7 +306,7 @@ int rows_call(bool scatter, hipStream_t st, void *pool, int64_t pool_rows, int64
     return fail(MLORA_ERR_INVALID, "%s: rows and layer strides must be multiples of 16 bytes and 16-byte aligned", who);
   if (n_layers > 65535) return fail(MLORA_ERR_INVALID, "%s: more than 65535 layers", who);
   const int64_t blocks = (n + RPW - 1) / RPW;
-  if (blocks > 0x7fffffff) return fail(MLORA_ERR_INVALID, "%s: too many rows", who);
+  if (blocks > most_blocks(256)) return fail(MLORA_ERR_INVALID, "%s: too many rows", who);
   dim3 grid((unsigned)blocks, (unsigned)n_layers);
   if (scatter)
     hipLaunchKernelGGL(pool_rows_kernel<true>, grid, dim3(256), 0, st, static_cast<unsigned char *>(pool), pool_rows,

@@ -224,8 +224,18 @@ extern "C" int mlora_rotary(void *stream, const mlora_rotary_part *parts, int32_
   const int64_t rounds = (units + RO_THREADS - 1) / RO_THREADS;
   const int64_t pieces = T >= 512 ? 1 : rounds < 65535 ? rounds : 65535;
   a.per_piece = (int)((rounds + pieces - 1) / pieces * RO_THREADS);
-  const dim3 grid((unsigned)T, (unsigned)((units + a.per_piece - 1) / a.per_piece));
-  if (dtype == MLORA_F16) launch<_Float16>((hipStream_t)stream, grid, a, interleaved != 0, vec);
-  else launch<__bf16>((hipStream_t)stream, grid, a, interleaved != 0, vec);
+  for (int64_t at = 0; at < T; at += most_blocks(RO_THREADS)) {
+    RotaryArgs some = a;
+    for (int i = 0; i < n_parts; ++i) {
+      mlora_rotary_part &p = some.part[i];
+      p.src = p.src ? static_cast<const uint16_t *>(p.src) + at * p.src_token_stride : nullptr;
+      if (p.dst && !(p.flags & MLORA_ROTARY_TO_ROWS)) p.dst = static_cast<uint16_t *>(p.dst) + at * p.dst_token_stride;
+    }
+    some.positions += at;
+    if (loc) some.loc += at;
+    const dim3 grid((unsigned)(T - at < most_blocks(RO_THREADS) ? T - at : most_blocks(RO_THREADS)), (unsigned)((units + a.per_piece - 1) / a.per_piece));
+    if (dtype == MLORA_F16) launch<_Float16>((hipStream_t)stream, grid, some, interleaved != 0, vec);
+    else launch<__bf16>((hipStream_t)stream, grid, some, interleaved != 0, vec);
+  }
   return check_launch("rotary_kernel");
 }
