@@ -45,6 +45,7 @@ struct AttnLayout {
   int off_few, off_tall, off_joins, off_requests, off_shares, off_arrive;      // (words is checked to fit)
   int64_t words;
   int few_items;                             // (piece, key head) pairs the list is cut for
+  bool few_whole;                            // as many requests with new tokens times key heads, or more: of like lengths, none is cut
   bool tall_each;                            // a share a tall tile: none is long enough to be cut
   int few_least, tall_least;                 // spans up to these are not cut
 };

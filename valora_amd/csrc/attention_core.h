@@ -1105,9 +1105,10 @@ int launch_lists(hipStream_t st, const AttnLayout &L, AttnArgs a) {
     // helps.  A cut list fills two a CU to the end, and of three it leaves a third idle in its last round; of long runs more at once
     // part more from each other.  There room that nobody uses keeps the third out.  (us with two / three.  Whole: 256 requests of 32 heads,
     // pages of 2, 322 / 313, 400 of 8, pages of 16, 131 / 128; 200 of 32, pages of 8 and 64, 230 / 234 and 223 / 231.  Cut: 5 long 117 / 127,
-    // 64 of 8 heads 62 / 65, and a list cut for three 119 and 65.)
+    // 64 of 8 heads 62 / 65, and a list cut for three 119 and 65.)  Lengths are not known here: that requests are whole goes by how many have new
+    // tokens, as if they were alike, and slots of the plan that have none do not count.
     constexpr uint32_t THIRD = 56 << 10;                       // more than a third of a CU's room, less than half
-    const bool third = (int64_t)a.n_req * a.kv_heads >= L.few_items && (int64_t)a.kv_heads << a.page_shift <= 128;
+    const bool third = L.few_whole && (int64_t)a.kv_heads << a.page_shift <= 128;
     const uint32_t unused = CODES && D == 128 && !third ? THIRD - Few<D, CODES>::TOTAL : 0;
     hipLaunchKernelGGL((attend_kernel<T, D, SUMS, FEW_LIST, CODES>), dim3((unsigned)few), dim3(THREADS), unused, st, a);
     return check_launch("attend_kernel");

@@ -328,6 +328,7 @@ AttnLayout attention_layout(const mlora_attention_plan &p) {
   const auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
   // few rows: sum of ceil(span / piece) <= tiles + sum of spans / piece, and a tile of k > 1 pieces has a span above (k - 1) pieces
   const int64_t few_more = ceil_div(L.few_items, p.kv_heads), few_cut = ceil_div(p.max_kv_len, L.few_least);
+  L.few_whole = n * p.kv_heads >= L.few_items;
   L.max_few = least(n + few_more, n * (few_cut > 1 ? few_cut : 1));
   L.slots_few = few_cut > 1 ? least(2 * few_more, n * few_cut) : 0;
   // tall: a share's beginning cuts one tile at most; k pieces of a tile are k - 1 cuts, and a cut tile has two pieces at least
