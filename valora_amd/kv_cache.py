@@ -148,53 +148,58 @@ class KVCache:
         total = sum(seq_lens)
         lens, seen = list(self.lens), list(self.seen)
         start, new = [0] * len(lens), [0] * len(lens)
-        rows, columns, positions, at = [], [], [], 0
+        positions, at = [], 0
         new_rows, new_columns = [], []                      # where in the table the pool's rows go
-        old_rows, old_columns = [], []                      # rows that have room for a token
-        source = []                                         # of each token's row: among the new ones, or behind them among the old
+        old_rows, old_columns = [], []                      # rows of the table that have room for a token
+        source, place = [], []                              # of each token: its row, among the old ones or behind them the new; where in it
+        page = self.page
+        n_old = sum(lens[s] % page > 0 for s in slots) if page > 1 else 0
         for s, n in zip(slots, seq_lens):
             start[s], new[s] = at, n
-            if self.page > 1:
-                full = self._rows(lens[s])
-                source += [len(new_rows) + c // self.page - full if c // self.page >= full else -1 - len(old_rows)
-                           for c in range(lens[s], lens[s] + n)]
-                if lens[s] % self.page:
+            first = lens[s]
+            if page > 1:
+                room = min(-first % page, n)                # tokens that go into the last row
+                if room:
+                    source += [len(old_rows)] * room
                     old_rows.append(s)
-                    old_columns.append(full - 1)
-            fresh = range(self._rows(lens[s]), self._rows(lens[s] + n))
-            new_rows += [s] * len(fresh)
-            new_columns += fresh
-            rows += [s] * n
-            columns += range(lens[s], lens[s] + n)
+                    old_columns.append(first // page)
+                fresh = n_old + len(new_rows)
+                source += [fresh + i // page for i in range(n - room)]
+                place += [c % page for c in range(first, first + n)]
+                columns = range(self._rows(first), self._rows(first + n))
+            else:
+                columns = range(first, first + n)
+            new_rows += [s] * len(columns)
+            new_columns += columns
             positions += range(seen[s], seen[s] + n)
             at += n
             lens[s] += n
             seen[s] += n
         dev = self.mem.device
-        index = torch.tensor([rows, columns, positions], dtype=torch.long).to(dev)
-        fresh = index
-        if self.page > 1:
-            fresh = torch.tensor([new_rows, new_columns], dtype=torch.long).to(dev)
-            old = torch.tensor([old_rows, old_columns], dtype=torch.long).to(dev)
-            source = torch.tensor([i if i >= 0 else len(new_rows) - 1 - i for i in source], dtype=torch.long).to(dev)
+        # (one copy to the device: each costs as much as a launch or more)
+        if page > 1:
+            lists = [positions, new_rows, new_columns, old_rows, old_columns, source, place]
+            positions, new_rows, new_columns, old_rows, old_columns, source, place = \
+                torch.tensor(sum(lists, []), dtype=torch.long).to(dev).split([len(l) for l in lists])
+        else:
+            positions, new_rows, new_columns = torch.tensor([positions, new_rows, new_columns], dtype=torch.long).to(dev)
         lengths = torch.tensor([start, new, lens], dtype=torch.int32).to(dev)
         plan = AttentionPlan(lengths[0], lengths[1], lengths[2], n_tokens=total, max_seq_len=max(seq_lens, default=0),
                              max_kv_len=max((lens[s] for s in slots), default=0), q_heads=self.q_heads,
                              kv_heads=self.mem.head_num, head_dim=self.mem.head_dim, page_size=self.page, window=self.window)
         with _on(dev):
-            got = self.mem.alloc(len(new_rows))
+            got = self.mem.alloc(new_rows.numel())
             try:
                 loc = got
-                if self.page > 1:
-                    its = torch.cat([got, self.table[old[0], old[1]].to(torch.long)])
-                    loc = its[source] * self.page + index[1] % self.page
-                self.table[fresh[0], fresh[1]] = got.to(torch.int32)
+                if page > 1:
+                    loc = torch.cat([self.table[old_rows, old_columns].to(torch.long), got])[source] * page + place
+                self.table[new_rows, new_columns] = got.to(torch.int32)
             except BaseException:
                 self.mem.free(got)
                 raise
         self.lens, self.seen = lens, seen
         self._changes += 1
-        return CacheStep(self, index[2], loc, plan)
+        return CacheStep(self, positions, loc, plan)
 
     def evict(self, budget: int, recent: int, sinks: int = 0) -> int:
         """Every slot with more than ``budget`` cached tokens gives up those that got the least attention (see the function
