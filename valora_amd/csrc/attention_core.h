@@ -1148,125 +1148,9 @@ __global__ __launch_bounds__(THREADS) void attend_join_kernel(AttnArgs a) {
 //     weights[b][j] += sum over the call's rows of exp(scale q.k_j - log sum)
 // The sum of a row is not known before its last token.  Decoding tiles therefore leave their scores, 4 bytes for the 512 of a token's
 // K and V that each query head of a group shares, and a thread sums those of a token.  (K read a second time: 64 requests of
-// 1000 to 4100 tokens, 8 key heads, 68 us of 194.)  For tall tiles, and where the scores have no room, a wave owns 64 cached
-// tokens and goes over all key heads and rows again.  A weight is one sum in a fixed order either way.  (The same requests now: 14 us
-// for leaving the scores, 15 for this launch, 152 in all.)
-constexpr int WEIGHT_WAVES = WEIGHT_TOKENS / 64;
-
-template <typename T, int D>
-__global__ __launch_bounds__(WEIGHT_WAVES * 64, 2) void attend_weights_kernel(AttnArgs a) {
-  constexpr int CH = D / 32;
-  using vec8 = typename Traits<T>::vec8;
-  __shared__ int found;
-  const int32_t *requests = a.plan + a.off_requests;
-  const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6), lrow = lane & 15, kg = lane >> 4;
-  const int total = a.plan[AH_BLOCKS];
-  for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    // the request whose run of blocks holds the item
-    __syncthreads();
-    for (int b = threadIdx.x; b < a.n_req; b += WEIGHT_WAVES * 64)
-      if (requests[(int64_t)b * AT_REC] <= item && (b + 1 == a.n_req || item < requests[(int64_t)(b + 1) * AT_REC])) found = b;
-    __syncthreads();
-    const int b = (int)uniform((uint32_t)found);
-    const int32_t *rq = requests + (int64_t)b * AT_REC;
-    const int tok0 = rq[1], n = rq[2], kv = rq[3], pos0 = kv - n, rows = n * a.group;
-    const int begin = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
-    if (rows <= FEW_ROWS && a.plan[AH_SCORES]) {
-      // the scores are there: a thread a token
-      const int j = begin + (item - rq[0]) * WEIGHT_TOKENS + (int)threadIdx.x;
-      if (j >= kv) continue;
-      const float *sc = a.scores + (int64_t)((uint64_t)(uint32_t)rq[5] | (uint64_t)(uint32_t)rq[6] << 32) + (j - begin);
-      const int stride = rq[7], n_rows = rows * a.kv_heads;
-      auto share = [&](int r, int &tok) {
-        const int head = r / rows, row = r - head * rows;
-        tok = row / a.group;
-        const float lse = a.lse[(int64_t)(tok0 + tok) * a.q_heads + head * a.group + row - tok * a.group];
-        const float e = exp2_(fmaf(sc[(int64_t)r * stride], a.c, -lse));
-        return lse == -INFINITY ? 0.0f : e;
-      };
-      float x = 0.0f;
-      int tok;
-#pragma unroll 8
-      for (int r = 0; r < n_rows; ++r) x += share(r, tok);
-      if (x != x) {
-        // A row whose own sum is no number makes that of all tokens, where one that does not see this token (its score is -infinity)
-        // would have added 0: once more, over the rows of the tokens [j - pos0, behind), which see it.
-        const int32_t page = a.table[(int64_t)b * a.table_stride + (j >> a.page_shift)];
-        const int behind = (uint32_t)page >= (uint32_t)a.n_pages ? 0 : a.window > 0 ? j - pos0 + a.window : n;
-        x = 0.0f;
-#pragma unroll 1
-        for (int r = 0; r < n_rows; ++r) {
-          const float e = share(r, tok);
-          x += tok >= j - pos0 && tok < behind ? e : 0.0f;
-        }
-      }
-      a.weights[(int64_t)b * a.weights_stride + j] += x;
-      continue;
-    }
-    const int base = begin + (item - rq[0]) * WEIGHT_TOKENS + wave * 64;
-    if (base >= kv) continue;
-    // rows that see any of the tokens
-    const int row_lo = base > pos0 ? (base - pos0) * a.group & ~15 : 0;
-    const int64_t hi = a.window > 0 ? ((int64_t)base + 63 - pos0 + a.window) * a.group : rows;
-    const int row_hi = hi < rows ? (int)hi : rows;
-
-    const int32_t *table = a.table + (int64_t)b * a.table_stride;
-    int64_t at[4];                                              // this lane's token of each 16: pool row
-    uint64_t bad = 0;                                           // tokens whose page is none of the pool
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      const int j = min(base + tt * 16 + lrow, kv - 1);
-      const int32_t page = table[j >> a.page_shift];
-      const bool none = (uint32_t)page >= (uint32_t)a.n_pages;
-      at[tt] = none ? 0 : ((int64_t)page << a.page_shift) + (j & ((1 << a.page_shift) - 1));
-      bad |= (uint64_t)(__ballot(none) & 0xffffu) << tt * 16;
-    }
-    float w[4][4] = {};
-    for (int head = 0; head < a.kv_heads; ++head) {
-      const char *kp = reinterpret_cast<const char *>(a.k) + head * D * 2 + kg * 16;
-      vec8 kf[4][CH];
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int i = 0; i < CH; ++i) kf[tt][i] = as<vec8>(*reinterpret_cast<const u32x4 *>(kp + at[tt] * a.k_stride + i * 64));
-      for (int r0 = row_lo; r0 < row_hi; r0 += 16) {
-        const int row = r0 + lrow < rows ? r0 + lrow : rows - 1;
-        const int tok = row / a.group, h = head * a.group + row - tok * a.group;
-        const float lse = r0 + lrow < rows ? a.lse[(int64_t)(tok0 + tok) * a.q_heads + h] : -INFINITY;
-        const uint16_t *qp = a.q + (int64_t)(tok0 + tok) * a.q_stride + h * D + kg * 8;
-        vec8 q[CH];
-#pragma unroll
-        for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 32));
-        const int last = pos0 + tok, from = a.window > 0 ? last - a.window + 1 : 0;
-        const uint64_t sees = lse == -INFINITY ? 0 : (run(from - base, last - base) & ~bad) >> kg * 4;
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          f32x4 s{0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < CH; ++i) s = Traits<T>::mfma(kf[tt][i], q[i], s);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[tt][i] += as<float>(as<uint32_t>(exp2_(fmaf(s[i], a.c, -lse))) & bit((uint32_t)(sees >> (tt >> 1) * 32), (tt & 1) * 16 + i));
-        }
-      }
-    }
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = w[tt][i];
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
-        const int j = base + tt * 16 + kg * 4 + i;
-        if (lrow == 0 && j < kv) a.weights[(int64_t)b * a.weights_stride + j] += x;
-      }
-  }
-}
-
-// Over codes the same sums are two kernels.  Where the scores are there, a thread sums a token's, as above; where they are not, 64 tokens are a
-// workgroup's, whose waves share out heads, and their rows where heads are few, and add up their parts in order.  (A wave alone with 64
-// tokens leaves most of the device idle where few are cached.  us in all, alone / shared: a prompt of 2048, 32 heads of 128, 3070 / 633;
-// 500 tokens over 11500 among 31 decoding requests, 8 key heads, 900 / 286.  64 decoding requests of 1000 to 4100: 99 either way.)
+// 1000 to 4100 tokens, 8 key heads, 68 us of 194.)  For tall tiles, and where the scores have no room, the keys are read again, for 64
+// cached tokens at a time.  A weight is one sum in a fixed order either way.  (The same requests over 16 bits now: 14 us for leaving the
+// scores, 15 for this launch, 149 in all.)
 
 // The request whose run of blocks of WEIGHT_TOKENS holds the block, for everyone
 __device__ __forceinline__ int request_of(const AttnArgs &a, int block, int *found) {
@@ -1277,135 +1161,106 @@ __device__ __forceinline__ int request_of(const AttnArgs &a, int block, int *fou
   __syncthreads();
   return (int)uniform((uint32_t)*found);
 }
-__device__ __forceinline__ bool has_scores(const AttnArgs &a, const int32_t *rq) { return rq[2] * a.group <= FEW_ROWS && a.plan[AH_SCORES]; }
 
-template <bool CODES>
-__global__ __launch_bounds__(WEIGHT_TOKENS) void attend_scores_kernel(AttnArgs a) {
-  __shared__ int found;
-  const int total = a.plan[AH_BLOCKS];
-  for (int block = blockIdx.x; block < total; block += gridDim.x) {
-    const int b = request_of(a, block, &found);
-    const int32_t *rq = a.plan + a.off_requests + (int64_t)b * AT_REC;
-    if (!has_scores(a, rq)) continue;
-    const int tok0 = rq[1], n = rq[2], kv = rq[3], pos0 = kv - n, rows = n * a.group, stride = rq[7], n_rows = rows * a.kv_heads;
-    const int begin = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
-    const int j = begin + (block - rq[0]) * WEIGHT_TOKENS + (int)threadIdx.x;
-    if (j >= kv) continue;
-    const float *sc = a.scores + (int64_t)((uint64_t)(uint32_t)rq[5] | (uint64_t)(uint32_t)rq[6] << 32) + (j - begin);
-    auto share = [&](int r, int &tok) {
-      const int head = r / rows, row = r - head * rows;
-      tok = row / a.group;
-      const float lse = a.lse[(int64_t)(tok0 + tok) * a.q_heads + head * a.group + row - tok * a.group];
-      const float e = exp2_(fmaf(sc[(int64_t)r * stride], a.c, -lse));
-      return lse == -INFINITY ? 0.0f : e;
-    };
-    float x = 0.0f;
-    int tok;
+// What the kernels below take of a request's record
+struct Weighed {
+  int first_block, tok0, n, kv, pos0, rows, begin;
+  __device__ __forceinline__ Weighed(const AttnArgs &a, const int32_t *rq)
+      : first_block(rq[0]), tok0(rq[1]), n(rq[2]), kv(rq[3]), pos0(kv - n), rows(n * a.group),
+        begin(a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0) {}
+  __device__ __forceinline__ bool has_scores(const AttnArgs &a) const { return rows <= FEW_ROWS && a.plan[AH_SCORES]; }
+};
+
+// Where the scores are there: a thread a token of request b's block
+__device__ __forceinline__ void sum_scores(const AttnArgs &a, const int32_t *rq, const Weighed &w, int b, int block) {
+  const int j = w.begin + (block - w.first_block) * WEIGHT_TOKENS + (int)threadIdx.x;
+  if (j >= w.kv) return;
+  const float *sc = a.scores + (int64_t)((uint64_t)(uint32_t)rq[5] | (uint64_t)(uint32_t)rq[6] << 32) + (j - w.begin);
+  const int stride = rq[7], n_rows = w.rows * a.kv_heads;
+  auto share = [&](int r, int &tok) {
+    const int head = r / w.rows, row = r - head * w.rows;
+    tok = row / a.group;
+    const float lse = a.lse[(int64_t)(w.tok0 + tok) * a.q_heads + head * a.group + row - tok * a.group];
+    const float e = exp2_(fmaf(sc[(int64_t)r * stride], a.c, -lse));
+    return lse == -INFINITY ? 0.0f : e;
+  };
+  float x = 0.0f;
+  int tok;
 #pragma unroll 8
-    for (int r = 0; r < n_rows; ++r) x += share(r, tok);
-    if (x != x) {
-      // (as above: rows that are no numbers count where they see the token)
-      const int32_t page = a.table[(int64_t)b * a.table_stride + (j >> a.page_shift)];
-      const int behind = (uint32_t)page >= (uint32_t)a.n_pages ? 0 : a.window > 0 ? j - pos0 + a.window : n;
-      x = 0.0f;
+  for (int r = 0; r < n_rows; ++r) x += share(r, tok);
+  if (x != x) {
+    // A row whose own sum is no number makes that of all tokens, where one that does not see this token (its score is -infinity)
+    // would have added 0: once more, over the rows of the tokens [j - pos0, behind), which see it.
+    const int32_t page = a.table[(int64_t)b * a.table_stride + (j >> a.page_shift)];
+    const int behind = (uint32_t)page >= (uint32_t)a.n_pages ? 0 : a.window > 0 ? j - w.pos0 + a.window : w.n;
+    x = 0.0f;
 #pragma unroll 1
-      for (int r = 0; r < n_rows; ++r) {
-        const float e = share(r, tok);
-        x += tok >= j - pos0 && tok < behind ? e : 0.0f;
-      }
+    for (int r = 0; r < n_rows; ++r) {
+      const float e = share(r, tok);
+      x += tok >= j - w.pos0 && tok < behind ? e : 0.0f;
     }
-    a.weights[(int64_t)b * a.weights_stride + j] += x;
   }
+  a.weights[(int64_t)b * a.weights_stride + j] += x;
 }
 
-constexpr int SHARED_WAVES = 8;
+// Where they are not: 64 cached tokens from `base` on, whose keys of a head are in kf, and that head's rows [first, last_row) of those that see any
 template <typename T, int D>
-__global__ __launch_bounds__(SHARED_WAVES * 64) void attend_weights_codes_kernel(AttnArgs a) {
-  constexpr int CH = D / 32, PARTS = WEIGHT_TOKENS / 64;
+__device__ __forceinline__ void sum_rows(const AttnArgs &a, const Weighed &rq, const typename Traits<T>::vec8 (&kf)[4][D / 32], int head, int first,
+                                         int last_row, int base, uint64_t bad, float (&w)[4][4]) {
+  constexpr int CH = D / 32;
   using vec8 = typename Traits<T>::vec8;
-  __shared__ int found;
-  __shared__ float parts[SHARED_WAVES][64];
-  const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6), lrow = lane & 15, kg = lane >> 4;
-  const int total = a.plan[AH_BLOCKS] * PARTS;
-  for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    const int b = request_of(a, item / PARTS, &found);
-    const int32_t *rq = a.plan + a.off_requests + (int64_t)b * AT_REC;
-    if (has_scores(a, rq)) continue;
-    const int tok0 = rq[1], n = rq[2], kv = rq[3], pos0 = kv - n, rows = n * a.group;
-    const int begin = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
-    const int base = begin + (item - rq[0] * PARTS) * 64;
-    if (base >= kv) continue;
-    // rows that see any of the tokens
-    const int row_lo = base > pos0 ? (base - pos0) * a.group & ~15 : 0;
-    const int64_t hi = a.window > 0 ? ((int64_t)base + 63 - pos0 + a.window) * a.group : rows;
-    const int row_hi = hi < rows ? (int)hi : rows;
-    const int32_t *table = a.table + (int64_t)b * a.table_stride;
-    const char *kc[4], *ke[4];                                  // this lane's token of each 16: where its codes and powers are
-    uint64_t bad = 0;                                           // tokens whose page is none of the pool
+  const int lane = threadIdx.x & 63, lrow = lane & 15, kg = lane >> 4;
+  for (int r0 = first; r0 < last_row; r0 += 16) {
+    const int row = r0 + lrow < rq.rows ? r0 + lrow : rq.rows - 1;
+    const int tok = row / a.group, h = head * a.group + row - tok * a.group;
+    const float lse = r0 + lrow < rq.rows ? a.lse[(int64_t)(rq.tok0 + tok) * a.q_heads + h] : -INFINITY;
+    const uint16_t *qp = a.q + (int64_t)(rq.tok0 + tok) * a.q_stride + h * D + kg * 8;
+    vec8 q[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 32));
+    const int last = rq.pos0 + tok, from = a.window > 0 ? last - a.window + 1 : 0;
+    const uint64_t sees = lse == -INFINITY ? 0 : (run(from - base, last - base) & ~bad) >> kg * 4;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
-      const int j = min(base + tt * 16 + lrow, kv - 1);
-      const int32_t page = table[j >> a.page_shift];
-      const bool none = (uint32_t)page >= (uint32_t)a.n_pages;
-      const int64_t at = none ? 0 : page, off = j & ((1 << a.page_shift) - 1);
-      kc[tt] = reinterpret_cast<const char *>(a.k) + at * a.k_stride + off * D + kg * 8;
-      ke[tt] = reinterpret_cast<const char *>(a.e) + at * a.e_stride + off * 2;
-      bad |= (uint64_t)(__ballot(none) & 0xffffu) << tt * 16;
-    }
-    // heads, and where they are fewer than waves runs of their rows
-    const int runs = (SHARED_WAVES + a.kv_heads - 1) / a.kv_heads;
-    const int each = ((row_hi - row_lo + 15) / 16 + runs - 1) / runs * 16;
-    float w[4][4] = {};
-    for (int pair = wave; pair < a.kv_heads * runs; pair += SHARED_WAVES) {
-      const int head = pair / runs, first = row_lo + (pair - head * runs) * each, last_row = min(first + each, row_hi);
-      if (first >= last_row) continue;
-      vec8 kf[4][CH];
+      f32x4 s{0, 0, 0, 0};
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const int64_t slots = (int64_t)head << a.page_shift;
-        const float power = k_power(*reinterpret_cast<const uint8_t *>(ke[tt] + slots * 2));
+      for (int i = 0; i < CH; ++i) s = Traits<T>::mfma(kf[tt][i], q[i], s);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) kf[tt][i] = values_of<T>(*reinterpret_cast<const u32x2 *>(kc[tt] + slots * D + i * 32), power);
-      }
-      for (int r0 = first; r0 < last_row; r0 += 16) {
-        const int row = r0 + lrow < rows ? r0 + lrow : rows - 1;
-        const int tok = row / a.group, h = head * a.group + row - tok * a.group;
-        const float lse = r0 + lrow < rows ? a.lse[(int64_t)(tok0 + tok) * a.q_heads + h] : -INFINITY;
-        const uint16_t *qp = a.q + (int64_t)(tok0 + tok) * a.q_stride + h * D + kg * 8;
-        vec8 q[CH];
-#pragma unroll
-        for (int i = 0; i < CH; ++i) q[i] = as<vec8>(load16(qp + i * 32));
-        const int last = pos0 + tok, from = a.window > 0 ? last - a.window + 1 : 0;
-        const uint64_t sees = lse == -INFINITY ? 0 : (run(from - base, last - base) & ~bad) >> kg * 4;
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          f32x4 s{0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < CH; ++i) s = Traits<T>::mfma(kf[tt][i], q[i], s);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[tt][i] += as<float>(as<uint32_t>(exp2_(fmaf(s[i], a.c, -lse))) & bit((uint32_t)(sees >> (tt >> 1) * 32), (tt & 1) * 16 + i));
-        }
-      }
-    }
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = w[tt][i];
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
-        if (lrow == 0) parts[wave][tt * 16 + kg * 4 + i] = x;
-      }
-    __syncthreads();
-    if (threadIdx.x < 64 && base + lane < kv) {
-      float x = 0.0f;
-#pragma unroll
-      for (int i = 0; i < SHARED_WAVES; ++i) x += parts[i][lane];
-      a.weights[(int64_t)b * a.weights_stride + base + lane] += x;
+      for (int i = 0; i < 4; ++i)
+        w[tt][i] += as<float>(as<uint32_t>(exp2_(fmaf(s[i], a.c, -lse))) & bit((uint32_t)(sees >> (tt >> 1) * 32), (tt & 1) * 16 + i));
     }
   }
 }
+
+// Rows that see any of 64 tokens from `base` on
+struct Seeing {
+  int lo, hi;
+  __device__ __forceinline__ Seeing(const AttnArgs &a, const Weighed &rq, int base) {
+    lo = base > rq.pos0 ? (base - rq.pos0) * a.group & ~15 : 0;
+    const int64_t end = a.window > 0 ? ((int64_t)base + 63 - rq.pos0 + a.window) * a.group : rq.rows;
+    hi = end < rq.rows ? (int)end : rq.rows;
+  }
+};
+
+// What a lane's sixteen rows gave its tokens, for each of the tokens
+template <typename F>
+__device__ __forceinline__ void over_rows(const float (&w)[4][4], F take) {
+  const int lane = threadIdx.x & 63, lrow = lane & 15, kg = lane >> 4;
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = w[tt][i];
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
+      if (lrow == 0) take(tt * 16 + kg * 4 + i, x);
+    }
+}
+
+// ... which the two kinds of cache do by kernels of their own (csrc/attention.hip, csrc/attention8.hip); `most`: blocks of WEIGHT_TOKENS that there
+// can be.  As many workgroups as the device holds at once: how many there are it knows.
+template <typename T, int D>
+int sum_weights(hipStream_t st, const AttnLayout &L, const AttnArgs &a, int64_t most);
 
 template <typename T, int D, bool CODES>
 int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, const AttnArgs &a) {
@@ -1415,20 +1270,8 @@ int launch(hipStream_t st, const mlora_attention_plan &p, const AttnLayout &L, c
     if (int rc = check_launch("attend_join_kernel")) return rc;
   }
   if (a.weights && p.max_kv_len > 0) {
-    // as many workgroups as the device holds at once: how many blocks there are it knows
     const int64_t most = p.n_req * ((p.max_kv_len + WEIGHT_TOKENS - 1) / WEIGHT_TOKENS);
-    if constexpr (CODES) {
-      hipLaunchKernelGGL(attend_scores_kernel<CODES>, dim3((unsigned)(most < 1024 ? most : 1024)), dim3(WEIGHT_TOKENS), 0, st, a);
-      if (int rc = check_launch("attend_scores_kernel")) return rc;
-      // requests without scores: those of more rows, and all where their room is bounded and may not do
-      if (L.max_shares > 0 || L.scores >= MAX_SCORES) {
-        const int64_t items = most * (WEIGHT_TOKENS / 64);
-        hipLaunchKernelGGL((attend_weights_codes_kernel<T, D>), dim3((unsigned)(items < 1024 ? items : 1024)), dim3(SHARED_WAVES * 64), 0, st, a);
-      }
-    } else {
-      hipLaunchKernelGGL((attend_weights_kernel<T, D>), dim3((unsigned)(most < 1024 ? most : 1024)), dim3(WEIGHT_WAVES * 64), 0, st, a);
-    }
-    if (int rc = check_launch("attend_weights_kernel")) return rc;
+    if (int rc = sum_weights<T, D>(st, L, a, most)) return rc;
   }
   return MLORA_OK;
 }
