@@ -309,9 +309,9 @@ struct TileCodes {
 // A wave's tile of 32 tokens.  K goes into the first product as it comes: lane (row, kg) holds, of tokens `row` and 16 + row, the 16 elements
 // from 16 kg on of each 64, and the 8 from 8 kg on of 32 that are left; q is read in that order too.  Powers are loaded once a token,
 // by lane token and token + 32, and go round by ds_bpermute: loaded by each lane that needs one, they were 40 % of the look-ups
-// in the L1 (256 requests of 200 to 2000 tokens, 32 heads, 344 us; then 326).  What is left of their cost is lines: 13 us of those 326 for the ones
-// that hold the powers of a page of 2 tokens, which every XCD reads.  The loads of this loop without its work take 319, of 1.70 GB; with
-// codes of two tiles on their way (at 234 registers) it is no faster.
+// in the L1 (256 requests of 200 to 2000 tokens, 32 heads, 344 us; then 326).  What was left of their cost is lines: 13 us of those 326 for the ones
+// that hold the powers of a page of 2 tokens, which every XCD reads.  At that step, with two workgroups a CU, the loads of this loop took 319
+// without its work, of 1.70 GB; with codes of two tiles on their way (at 234 registers) it was no faster.
 template <int D>
 struct WaveCodes {
   static constexpr int B = D / 64, REST = D % 64 / 32, P = D / 16, EACH = D / 32;
@@ -1060,7 +1060,8 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attend_kernel(AttnA
       if (i >= a.max_few) return;
     } else if (CODES && (a.kv_heads & 7) == 0) {
       // heads that are neighbours go to one XCD, which then reads of a page what lies side by side (256 requests of 32 heads, pages of 2,
-      // 326 -> 321 us, 128 of 40 heads 213 -> 202; pages of 16 and of 1, and 16 heads, the same either way; the L2s ask for as many bytes)
+      // 326 -> 321 us, 128 of 40 heads 213 -> 202; pages of 16 and of 1, and 16 heads, the same either way.  The L2s ask for as many bytes,
+      // so it is not a line that they share; what it is was not found.)
       head = (head & 7) * (a.kv_heads >> 3) + (head >> 3);
     }
     few_tile<T, D, SUMS, CODES>(a, lds, i, head);
@@ -1105,7 +1106,8 @@ int launch_lists(hipStream_t st, const AttnLayout &L, AttnArgs a) {
     // helps.  A cut list fills two a CU to the end, and of three it leaves a third idle in its last round; of long runs more at once
     // part more from each other.  There room that nobody uses keeps the third out.  (us with two / three.  Whole: 256 requests of 32 heads,
     // pages of 2, 322 / 313, 400 of 8, pages of 16, 131 / 128; 200 of 32, pages of 8 and 64, 230 / 234 and 223 / 231.  Cut: 5 long 117 / 127,
-    // 64 of 8 heads 62 / 65, and a list cut for three 119 and 65.)  Lengths are not known here: that requests are whole goes by how many have new
+    // 64 of 8 heads 62 / 65, and a list cut for three 119 and 65.  Heads of 32, 64 and 96 have the registers of five, four and three, and take
+    // them: 64 requests of 2000, 8 key heads, with two / so 23.9 / 19.6, 34.2 / 32.0, 39.2 / 38.8.)  Lengths are not known here: that requests are whole goes by how many have new
     // tokens, as if they were alike, and slots of the plan that have none do not count.
     constexpr uint32_t THIRD = 56 << 10;                       // more than a third of a CU's room, less than half
     const bool third = L.few_whole && (int64_t)a.kv_heads << a.page_shift <= 128;

@@ -7,7 +7,9 @@
 //
 // Bound by bytes (8191 tokens, 32 query and 8 key heads of 128, bf16: 185 MB in 40 us, 4.6 TB/s; a copy of as much takes 36).  Where tokens are many, four a
 // workgroup share one wait for positions, frequencies and sines (a token a workgroup: 49 us; two and eight: 41), and a lane that owned eight
-// elements and loaded their partners a second time took 55: half of it were the vector units.
+// elements and loaded their partners a second time took 55: half of it were the vector units.  Where rows or what is rotated of them are no whole runs
+// of 16 bytes it goes by elements, a token a workgroup (120 of 128 rotated: 2048 tokens 30 us, 12.5 by runs, 8191 96 and 31 with part of it in the
+// memory-side cache).
 #include "codes8.h"
 
 namespace mlora {
@@ -30,8 +32,10 @@ struct StoreArgs {
 
 constexpr int ST_THREADS = 256;
 // A round is what a workgroup's threads take at once, some heads of a token.  From MANY on a workgroup has four tokens, whose heads are cut in pieces
-// while there are fewer than FULL tokens; below it a round of one token (us of either with the read, 32 query heads of 128: 1024 and 2048 tokens of 8
-// key heads 14.4 / 12.7 and 16.8 / 19.3; 512 and 1024 of 32 key heads 15.0 / 12.8 and 17.6 / 20.1).
+// while there are fewer than FULL tokens; below it a round of one token, each of which works out the token's sines again (us of four tokens / of one,
+// 32 query heads.  Heads of 128: 1024 and 2048 tokens of 8 key heads 9.7 / 8.3 and 12.5 / 14.8, 512 and 1024 of 32 9.8 / 7.6 and 11.1 / 13.5.  Of 256:
+// 512 and 1024 of 8 10.1 / 7.7 and 11.4 / 12.9, 256 and 512 of 32 10.3 / 7.8 and 12.2 / 14.0.  Of 64: 1024, 1536 and 2048 of 8 6.3 / 6.0, 7.3 / 8.4 and
+// 7.7 / 10.1, 1024 and 1536 of 32 9.5 / 8.7 and 11.4 / 12.1; the border of 8 key heads of 64 is set at 2731 tokens and lies near 1100).
 constexpr int MANY = 2048, FULL = 4096;
 
 // A lane's part of a head: n elements from a0 on and, where they are the first halves of pairs, as many from a1 on

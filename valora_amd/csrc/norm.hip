@@ -17,8 +17,9 @@ namespace mlora {
 namespace {
 
 // Runs of eight: a thread has one of up to NORM_ONE, which keeps its registers few and loads all it needs at once; rows of more would be workgroups
-// of many waves that wait for each other (8191 of 5120, one / two runs a thread: 63.4 / 62.5 us, 2048 of 7168 32.9 / 29.2), unless they are few
-// and the chain counts (256 of 5120 4.7 / 5.3 us).
+// of many waves that wait for each other, unless they are few and the chain counts (one / two runs a thread, rows of 5120 and of 7168 with two norms,
+// us: 256 rows 4.8 / 5.2 and 5.4 / 5.5; 400 6.2 / 5.9 and 7.4 / 6.9; 512 6.6 / 6.2 and 7.9 / 7.5; 700 8.3 / 7.5 and 10.0 / 9.4; 2048 18.4 / 17.7
+// and 26.2 / 22.1.  So the border lies near 300 rows, and 300 to 512 lose a twentieth.)
 constexpr int NORM_ONE = 512, NORM_FEW_ROWS = 512;
 constexpr int NORM_MAX = 32768;
 
