@@ -1107,8 +1107,9 @@ int launch_lists(hipStream_t st, const AttnLayout &L, AttnArgs a) {
     // part more from each other.  There room that nobody uses keeps the third out.  (us with two / three.  Whole: 256 requests of 32 heads,
     // pages of 2, 322 / 313, 400 of 8, pages of 16, 131 / 128; 200 of 32, pages of 8 and 64, 230 / 234 and 223 / 231.  Cut: 5 long 117 / 127,
     // 64 of 8 heads 62 / 65, and a list cut for three 119 and 65.  Heads of 32, 64 and 96 have the registers of five, four and three, and take
-    // them: 64 requests of 2000, 8 key heads, with two / so 23.9 / 19.6, 34.2 / 32.0, 39.2 / 38.8.)  Lengths are not known here: that requests are whole goes by how many have new
-    // tokens, as if they were alike, and slots of the plan that have none do not count.
+    // them: 64 requests of 2000, 8 key heads, with two / so 23.9 / 19.6, 34.2 / 32.0, 39.2 / 38.8.)  Lengths are not known here: that requests are
+    // whole goes by how many can have new tokens, as if their lengths were alike; slots of the plan that have none do not count (5 long ones in 256 slots,
+    // pages of 2 and of 16, 125.5 and 116.1, and 134.3 and 127.6 as if each slot had some).
     constexpr uint32_t THIRD = 56 << 10;                       // more than a third of a CU's room, less than half
     const bool third = L.few_whole && (int64_t)a.kv_heads << a.page_shift <= 128;
     const uint32_t unused = CODES && D == 128 && !third ? THIRD - Few<D, CODES>::TOTAL : 0;

@@ -35,7 +35,9 @@ constexpr int ST_THREADS = 256;
 // while there are fewer than FULL tokens; below it a round of one token, each of which works out the token's sines again (us of four tokens / of one,
 // 32 query heads.  Heads of 128: 1024 and 2048 tokens of 8 key heads 9.7 / 8.3 and 12.5 / 14.8, 512 and 1024 of 32 9.8 / 7.6 and 11.1 / 13.5.  Of 256:
 // 512 and 1024 of 8 10.1 / 7.7 and 11.4 / 12.9, 256 and 512 of 32 10.3 / 7.8 and 12.2 / 14.0.  Of 64: 1024, 1536 and 2048 of 8 6.3 / 6.0, 7.3 / 8.4 and
-// 7.7 / 10.1, 1024 and 1536 of 32 9.5 / 8.7 and 11.4 / 12.1; the border of 8 key heads of 64 is set at 2731 tokens and lies near 1100).
+// 7.7 / 10.1, 1024 and 1536 of 32 9.5 / 8.7 and 11.4 / 12.1; the border of 8 key heads of 64 is set at 2731 tokens and lies near 1100).  FULL: 2048
+// tokens of 32 key heads in pieces / whole 12.1 / 12.9 (heads of 64), 19.8 / 22.9 (128), 31.4 / 41.9 (256); 4096 in a piece a round / whole 19.5 / 18.2,
+// 34.3 / 32.2, 84 / 77; 3000 the same within 4 % but for 32 heads of 256 (55 / 60).
 constexpr int MANY = 2048, FULL = 4096;
 
 // A lane's part of a head: n elements from a0 on and, where they are the first halves of pairs, as many from a1 on
